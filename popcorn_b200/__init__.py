@@ -63,6 +63,16 @@ EXT_SYMBOLS = (
     "popcornDequantizeMatmulRowParallel_i8f32",
     "popcornGetLastNcclError",
 )
+# Every symbol declared in include/popcorn_serve.h.
+SERVE_SYMBOLS = (
+    "popcornKvAppend",
+    "popcornKvRead",
+    "popcornKvAttention",
+)
+
+TYPE_F32 = 0
+TYPE_F16 = 1
+TYPE_BF16 = 2
 
 TP_MAX_RANKS = 8
 
@@ -77,6 +87,22 @@ class TpGroup(ctypes.Structure):
         ("rank", ctypes.c_int),
         ("world", ctypes.c_int),
     ]
+
+
+class KvCacheStruct(ctypes.Structure):
+    """popcornKvCache_t (include/popcorn_serve.h)."""
+
+    _fields_ = [
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("k_scale", ctypes.c_void_p),
+        ("v_scale", ctypes.c_void_p),
+        ("pages", ctypes.c_int64),
+        ("heads", ctypes.c_int64),
+        ("page_size", ctypes.c_int64),
+        ("dim", ctypes.c_int64),
+    ]
+
 
 _vp = ctypes.c_void_p
 _i64 = ctypes.c_int64
@@ -109,6 +135,11 @@ _SIGNATURES = {
     "popcornDequantizeMatmulColumnParallel_i8f32": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp]),
     "popcornDequantizeMatmulRowParallel_i8f32": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp]),
     "popcornGetLastNcclError": (_int, []),
+    "popcornKvAppend": (_int, [_vp, _vp, _i64, _i64, _vp, _i64, _i64, _int, _vp, _i64, _vp, _vp, _i64, _i64, _vp, _vp,
+                               _i64, _i64, _i64, _vp, _vp, _i64, _i64, _int, _vp]),
+    "popcornKvRead": (_int, [_vp, _vp, _int, _vp, _vp, _i64, _vp]),
+    "popcornKvAttention": (_int, [_vp, _vp, _vp, _i64, _i64, _int, _vp, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _i64,
+                                  _int, _i64, ctypes.c_float, _vp]),
 }
 
 _lib = None
@@ -401,4 +432,189 @@ def dequantize(qweight, scale, out=None, stream=None, dtype=None):
     else:
         _check(popcornDequantize_i8f32(out.data_ptr(), qweight.data_ptr(), scale.data_ptr(), N, K, st),
                "popcornDequantize_i8f32")
+    return out
+
+
+# ---------------------------------------------------------------------------
+# Serving operators (include/popcorn_serve.h).
+# ---------------------------------------------------------------------------
+_TYPES = {}  # torch dtype -> popcornType_t, filled on first use
+
+
+def _type_of(dtype, where: str) -> int:
+    if not _TYPES:
+        import torch
+
+        _TYPES.update({torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16})
+    try:
+        return _TYPES[dtype]
+    except KeyError:
+        raise ValueError(f"{where}: float32, float16 or bfloat16 wanted, got {dtype}") from None
+
+
+def _want(ok: bool, where: str, what: str) -> None:
+    if not ok:
+        raise ValueError(f"{where}: {what}")
+
+
+def _whole(t, shape, where: str, name: str):
+    """Device pointer of a contiguous int32 tensor of this shape."""
+    import torch
+
+    if t.dtype is not torch.int32 or t.shape != shape or not t.is_contiguous() or not t.is_cuda:
+        raise ValueError(f"{where}: {name}: a contiguous int32 CUDA tensor {tuple(shape)} wanted, "
+                         f"got {t.dtype} {tuple(t.shape)}")
+    return t.data_ptr()
+
+
+class KvCache:
+    """A paged key/value cache in 8 bits: codes int8 [pages, heads, page_size, dim] and one f32 scale per page and
+    head [pages, heads], keys and values apart (a cached value is code * scale). ``page_size`` is a power of two from
+    16 to 256, ``dim`` a multiple of 16 up to 256. Wraps the caller's tensors; :meth:`empty` makes them."""
+
+    __slots__ = ("k", "v", "k_scale", "v_scale", "pages", "heads", "page_size", "dim", "_struct", "_ref")
+
+    def __init__(self, k, v, k_scale, v_scale):
+        import torch
+
+        _want(k.dim() == 4 and k.shape == v.shape and k.dtype is v.dtype is torch.int8, "KvCache",
+              "k and v: int8 [pages, heads, page_size, dim]")
+        self.pages, self.heads, self.page_size, self.dim = k.shape
+        for s in (k_scale, v_scale):
+            _want(s.shape == k.shape[:2] and s.dtype is torch.float32, "KvCache",
+                  "k_scale and v_scale: float32 [pages, heads]")
+        for t in (k, v, k_scale, v_scale):
+            _want(t.is_contiguous() and t.is_cuda and t.device == k.device, "KvCache",
+                  "contiguous CUDA tensors on one device")
+        _want(self.page_size in (16, 32, 64, 128, 256), "KvCache", "page_size: a power of two from 16 to 256")
+        _want(self.dim % 16 == 0 and 16 <= self.dim <= 256, "KvCache", "dim: a multiple of 16 from 16 to 256")
+        _want(self.pages > 0 and self.heads > 0, "KvCache", "at least one page and one head")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self._struct = KvCacheStruct(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), self.pages,
+                                     self.heads, self.page_size, self.dim)
+        self._ref = ctypes.addressof(self._struct)
+
+    @classmethod
+    def empty(cls, pages: int, heads: int, dim: int, page_size: int = 16, device="cuda"):
+        """A cache of zeros."""
+        import torch
+
+        codes = [torch.zeros((pages, heads, page_size, dim), dtype=torch.int8, device=device) for _ in range(2)]
+        scales = [torch.zeros((pages, heads), dtype=torch.float32, device=device) for _ in range(2)]
+        return cls(*codes, *scales)
+
+
+def _rows(t, tokens, heads, dim, kind, where, name):
+    """Checks [tokens, heads, dim] with dim contiguous."""
+    if t.shape != (tokens, heads, dim) or t.dtype is not kind or not t.is_cuda:
+        raise ValueError(f"{where}: {name}: {kind} CUDA tensor {(tokens, heads, dim)} wanted, "
+                         f"got {t.dtype} {tuple(t.shape)}")
+    a, b, c = t.stride()
+    if c != 1:
+        raise ValueError(f"{where}: {name}: the last dimension must be contiguous")
+    return a, b
+
+
+def _batch(table, first, tokens, where):
+    seqs, width = table.shape
+    if first is not None:
+        return seqs, _whole(table, (seqs, width), where, "table"), width, _whole(first, (seqs + 1,), where, "first")
+    _want(tokens == seqs, where, f"{tokens} tokens for {seqs} sequences need `first`")
+    return seqs, _whole(table, (seqs, width), where, "table"), width, None
+
+
+def kv_append(cache: KvCache, k, v, table, start, first=None, q=None, cos=None, sin=None, interleaved: bool = False,
+              q_out=None, stream=None):
+    """Append keys and values [tokens, heads, dim] to the sequences of ``table`` int32 [seqs, pages] behind the
+    ``start`` int32 [seqs] tokens that they hold, rotating keys (and queries ``q`` [tokens, q_heads, dim]) by the
+    tables ``cos``, ``sin`` f32 [positions, rot_dim / 2]. ``first`` int32 [seqs + 1]: each sequence's run of tokens
+    (None: one token each). Returns the rotated queries (``q_out``, or a new tensor), None without ``q``."""
+    where = "kv_append"
+    import torch
+
+    tokens = k.shape[0]
+    kind = k.dtype
+    kt, kh = _rows(k, tokens, cache.heads, cache.dim, kind, where, "k")
+    vt, vh = _rows(v, tokens, cache.heads, cache.dim, kind, where, "v")
+    seqs, tp, width, fp = _batch(table, first, tokens, where)
+    sp = _whole(start, (seqs,), where, "start")
+    qp = op = None
+    qt = qh = q_heads = 0
+    if q is not None:
+        q_heads = q.shape[1]
+        qt, qh = _rows(q, tokens, q_heads, cache.dim, kind, where, "q")
+        if q_out is None:
+            q_out = torch.empty((tokens, q_heads, cache.dim), dtype=kind, device=q.device)
+        else:
+            _rows(q_out, tokens, q_heads, cache.dim, kind, where, "q_out")
+            _want(q_out.is_contiguous(), where, "q_out must be contiguous")
+        qp, op = q.data_ptr(), q_out.data_ptr()
+    cp = np_ = None
+    positions = rot = 0
+    if cos is not None:
+        positions, rot = cos.shape
+        for t in (cos, sin):
+            _want(t.shape == cos.shape and t.dtype is torch.float32 and t.is_contiguous() and t.is_cuda, where,
+                  "cos and sin: contiguous float32 CUDA tensors [positions, rot_dim / 2]")
+        cp, np_, rot = cos.data_ptr(), sin.data_ptr(), 2 * rot
+    _check(load_library().popcornKvAppend(cache._ref, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh,
+                                          _type_of(kind, where), tp, width, fp, sp, seqs, tokens, op, qp, qt, qh,
+                                          q_heads, cp, np_, positions, rot, interleaved, _stream_handle(stream)),
+           "popcornKvAppend")
+    return q_out
+
+
+def kv_read(cache: KvCache, pages, dtype=None, k_out=None, v_out=None, stream=None):
+    """The values (code * scale) of the pages listed in ``pages`` int32 [n]: (keys, values), each
+    [n, heads, page_size, dim] in ``dtype`` (float32)."""
+    import torch
+
+    where = "kv_read"
+    dtype = dtype or (k_out.dtype if k_out is not None else torch.float32)
+    n = pages.shape[0]
+    shape = (n, cache.heads, cache.page_size, cache.dim)
+    if k_out is None:
+        k_out = torch.empty(shape, dtype=dtype, device=cache.k.device)
+    if v_out is None:
+        v_out = torch.empty(shape, dtype=dtype, device=cache.k.device)
+    for t in (k_out, v_out):
+        _want(t.shape == shape and t.dtype is dtype and t.is_contiguous() and t.is_cuda, where,
+              f"outputs: contiguous {dtype} CUDA tensors {shape}")
+    lp = _whole(pages, (n,), where, "pages")
+    if n:
+        _check(load_library().popcornKvRead(k_out.data_ptr(), v_out.data_ptr(), _type_of(dtype, where), cache._ref,
+                                            lp, n, _stream_handle(stream)), "popcornKvRead")
+    return k_out, v_out
+
+
+def kv_attention(cache: KvCache, q, table, length, first=None, max_tokens: int | None = None, causal: bool = True,
+                 window: int = 0, scale: float | None = None, out=None, lse=None, stream=None):
+    """Attention of queries ``q`` [tokens, q_heads, dim] over the cached tokens of their sequences: ``length`` int32
+    [seqs] counts them, the queries' own included; sequence b's queries (``first`` as in :func:`kv_append`, at most
+    ``max_tokens`` each) are its last positions. ``window`` > 0 limits a query to that many last positions, ``scale``
+    is 1 / sqrt(dim) unless given, ``lse`` f32 [tokens, q_heads] takes the log of the softmax denominators."""
+    import torch
+
+    where = "kv_attention"
+    tokens, q_heads, dim = q.shape
+    qt, qh = _rows(q, tokens, q_heads, cache.dim, q.dtype, where, "q")
+    _want(q_heads % cache.heads == 0, where, f"{q_heads} query heads over {cache.heads} cache heads")
+    seqs, tp, width, fp = _batch(table, first, tokens, where)
+    lp = _whole(length, (seqs,), where, "length")
+    if out is None:
+        out = torch.empty((tokens, q_heads, dim), dtype=q.dtype, device=q.device)
+    else:
+        _rows(out, tokens, q_heads, dim, q.dtype, where, "out")
+        _want(out.is_contiguous(), where, "out must be contiguous")
+    ep = None
+    if lse is not None:
+        _want(lse.shape == (tokens, q_heads) and lse.dtype is torch.float32 and lse.is_contiguous() and lse.is_cuda,
+              where, "lse: a contiguous float32 CUDA tensor [tokens, q_heads]")
+        ep = lse.data_ptr()
+    if max_tokens is None:
+        max_tokens = 1 if first is None else tokens
+    _check(load_library().popcornKvAttention(out.data_ptr(), ep, q.data_ptr(), qt, qh, _type_of(q.dtype, where),
+                                             cache._ref, tp, width, fp, lp, seqs, tokens, max_tokens, q_heads, causal,
+                                             window, dim ** -0.5 if scale is None else scale,
+                                             _stream_handle(stream)), "popcornKvAttention")
     return out

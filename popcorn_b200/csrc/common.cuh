@@ -143,6 +143,8 @@ cudaError_t tc_take_errors(unsigned int* bits);
 cudaError_t gemv_take_errors(unsigned int* bits);
 cudaError_t i4_take_errors(unsigned int* bits);
 cudaError_t grouped_take_errors(unsigned int* bits);
+cudaError_t kv_take_errors(unsigned int* bits);
+cudaError_t kv_attention_take_errors(unsigned int* bits);
 
 }  // namespace pcb
 

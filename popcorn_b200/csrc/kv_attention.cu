@@ -1,0 +1,808 @@
+// Attention over the paged 8-bit key/value cache.
+//
+// out = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q . k_j - max),  with
+// k_j = ck_j ks, v_j = cv_j vs: codes ck, cv and one scale for each block of
+// a page's tokens and a head. The block scales leave the inner products:
+// q . k_j = (q . ck_j) ks, and vs joins p_j.
+//
+// Few query rows (kv_rows_kernel). What it cannot do without is one read of
+// the visible codes, 2 dim bytes a token and head; it is bound by HBM. Layout:
+//  * A warp takes 16 tokens at a time. Tokens are the M side of the matrix
+//    instructions and up to 8 NT query rows (the heads that share a key head,
+//    times the sequence's tokens) their N side, so that a few rows fill the
+//    instruction better than with queries as M. The operands of both products
+//    come straight from global memory in 16-byte loads: the sums over dim and
+//    over tokens may run in any order, so each lane takes whole 16-byte pieces
+//    and the other operand is permuted to match. No shared memory, no barrier.
+//  * Scores: mma s8 x s8 -> s32 on the raw key codes; each query row is fixed
+//    point in signed base-256 digits (2 for f16 / bf16, 3 for f32), each
+//    digit one product, so the sums are exact integers. The accumulators
+//    start at the bits of 1.5 2^23, which makes them floats at no cost.
+//  * Softmax: running maximum m of log2-domain scores plus the exponent of vs
+//    (so that p vs stays in range whatever the scales are); it moves only when
+//    a score exceeds it by 2^8, which is rare after the first tiles, so most
+//    tiles pay one vote instead of a reduction. Probabilities are scaled by
+//    2^6 to keep small ones out of f16's subnormals (largest 2^15).
+//  * Values: codes become f16 exactly (byte permutes), probabilities f16 for
+//    16-bit outputs and f16 high + f16 rest for f32, products accumulate in
+//    f32. For f32 each tile's product starts from zero and is added to the
+//    running sum by an ordinary f32 add: the tensor cores' accumulation
+//    truncates, which over hundreds of tiles costs more than f32 should lose.
+//  * Work is the list of (sequence, row tile, key head) tasks, cut into equal
+//    runs of 16-token tiles over all blocks whatever the lengths are (lengths
+//    are on the device; every block finds its run by a scan over them). A task
+//    that spans blocks leaves partial (m, l, sum) triples, joined in a fixed
+//    order by kv_join_kernel.
+#include <cmath>
+
+#include "kv.cuh"
+#include "mma_frag.cuh"
+
+namespace pcb {
+namespace {
+
+__device__ unsigned int g_attn_err = 0;
+
+constexpr int kWarps = 4;
+constexpr int kThreads = 32 * kWarps;
+constexpr float kMagic = 12582912.0f;       // 1.5 2^23
+constexpr int kMagicBits = 0x4B400000;
+constexpr float kLift = 6.0f;               // probabilities are scaled by 2^6
+constexpr float kSlack = 8.0f;              // and may exceed the running maximum by 2^8
+
+struct AttnArgs {
+    void* out;
+    float* lse;
+    const void* q;
+    int64_t q_tok, q_head;
+    const int8_t* k;
+    const int8_t* v;
+    const float* ks;
+    const float* vs;
+    const int32_t* table;
+    const int32_t* first;
+    const int32_t* length;
+    int64_t table_pages, pages, window;
+    int seqs, tokens, heads, group, dim, page_shift, causal;
+    float scale_log2;   // scale * log2(e)
+    int q_vec;          // query rows start on four-element boundaries
+    int by_task;        // join entries are indexed by task (else by block)
+    int entries;
+    int4* entry;        // [0]: number of entries; then one per task or block
+    float2* ml;         // [2 blocks][rows]: maximum, denominator
+    float* part;        // [2 blocks][rows][DP]
+};
+
+struct Seq {  // one sequence's share of the work
+    int row0, rows;     // first query token, number of them
+    int len;            // visible length
+    int lo;             // first token of the first tile
+    int tiles;          // 16-token tiles that some query may see
+};
+
+__device__ __forceinline__ Seq sequence(const AttnArgs& a, int b) {
+    Seq s;
+    s.row0 = a.first ? a.first[b] : b;
+    s.rows = a.first ? a.first[b + 1] - s.row0 : 1;
+    if (s.row0 < 0 || s.rows < 0 || s.rows > a.tokens - s.row0) s.rows = 0;
+    const int64_t most = a.table_pages << a.page_shift;
+    int64_t len = a.length[b];
+    if (len > most) {
+        atomicOr(&g_attn_err, kKvErrAttention);
+        len = most;
+    }
+    s.len = static_cast<int>(max(len, int64_t{0}));
+    int64_t lo = 0;
+    if (a.window > 0) lo = max(int64_t{0}, static_cast<int64_t>(s.len) - s.rows + 1 - a.window);
+    lo = min(lo, static_cast<int64_t>(s.len));
+    s.lo = static_cast<int>(lo) & ~15;
+    s.tiles = (s.len - s.lo + 15) >> 4;
+    return s;
+}
+
+__device__ __forceinline__ void mma_f16_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Transposes the warp's 8 x 8 matrix of 16-bit elements.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Cache codes are read once: no allocation in L1.
+__device__ __forceinline__ void load_codes(uint32_t (&w)[4], const int8_t* p, bool ok) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %5, 0;\n\t"
+        "mov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\tmov.b32 %3, 0;\n\t"
+        "@p ld.global.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];\n\t}"
+        : "=&r"(w[0]), "=&r"(w[1]), "=&r"(w[2]), "=&r"(w[3])
+        : "l"(p), "r"(static_cast<int>(ok)));
+}
+__device__ __forceinline__ void load_codes(uint32_t (&w)[2], const int8_t* p, bool ok) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %3, 0;\n\t"
+        "mov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\t"
+        "@p ld.global.L1::no_allocate.v2.b32 {%0, %1}, [%2];\n\t}"
+        : "=&r"(w[0]), "=&r"(w[1])
+        : "l"(p), "r"(static_cast<int>(ok)));
+}
+
+// Two f16 of signed codes from the biased bytes (code + 128) that `sel` picks
+// out of w: byte u in the low mantissa byte of 1024 is 1024 + u.
+template <uint32_t SEL>
+__device__ __forceinline__ uint32_t codes_f16(uint32_t w) {
+    const uint32_t x = __byte_perm(w, 0x64646464u, SEL);
+    const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&x), __half2{__float2half_rn(1152.0f), __float2half_rn(1152.0f)});
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Query rows as the B operand of the score products: DIGITS words for each
+// 32-wide step's two halves, and each row's factor. Lane (g, t) = (lane / 4,
+// lane % 4) holds row g; its pieces are the 16-byte pieces t, t + 4, ... of
+// dim, the same ones that lane (., t) loads of a key.
+template <typename T, int DP, int DIGITS>
+__device__ __forceinline__ float query_digits(uint32_t (&qd)[DIGITS][DP / 16], const T* row, bool valid, int dim,
+                                              bool vec, int t) {
+    constexpr int PIECES = DP / 64;
+    float m = 0.0f;
+    bool bad = false;
+    #pragma unroll
+    for (int c = 0; c < PIECES; ++c) {
+        const int d0 = 16 * (t + 4 * c);
+        #pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (valid && d0 < dim) load4(row + d0 + 4 * w, vec, v);
+            #pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                m = fmaxf(m, fabsf(v[j]));
+                bad = bad || !(fabsf(v[j]) <= 3.4028234663852886e38f);
+            }
+        }
+    }
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    int nan = bad;
+    nan |= __shfl_xor_sync(0xffffffffu, nan, 1);
+    nan |= __shfl_xor_sync(0xffffffffu, nan, 2);
+    // Three digits: a power of two that brings the largest element to
+    // [2^21, 2^22), exact and inside the balanced digits' range. Two digits:
+    // the largest element becomes 32512 = 127 * 256, since with a power of two
+    // the 15 bits could be too few for f16 queries' 11.
+    float up, down;
+    if constexpr (DIGITS == 3) {
+        const int e = max(-126, min(120, 21 + 127 - static_cast<int>(__float_as_uint(m) >> 23)));
+        up = __int_as_float((127 + e) << 23);
+        down = __int_as_float((127 - e) << 23);
+    } else {
+        const float most = fmaxf(m, 1e-30f);
+        up = 32512.0f / most;
+        down = most / 32512.0f;
+    }
+    constexpr uint32_t BIAS = DIGITS == 2 ? 0x8080u : 0x808080u;
+    #pragma unroll
+    for (int c = 0; c < PIECES; ++c) {
+        const int d0 = 16 * (t + 4 * c);
+        #pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (valid && !nan && d0 < dim) load4(row + d0 + 4 * w, vec, v);
+            uint32_t y[4];
+            #pragma unroll
+            for (int j = 0; j < 4; ++j) y[j] = static_cast<uint32_t>(__float2int_rn(v[j] * up)) + BIAS;
+            #pragma unroll
+            for (int i = 0; i < DIGITS; ++i) {
+                const uint32_t sel = static_cast<uint32_t>(i | ((i + 4) << 4));
+                qd[i][4 * c + w] =
+                    __byte_perm(__byte_perm(y[0], y[1], sel), __byte_perm(y[2], y[3], sel), 0x5410) ^ 0x80808080u;
+            }
+        }
+    }
+    return nan ? __int_as_float(0x7fffffff) : down;
+}
+
+template <typename T>
+struct Traits {
+    static constexpr int kDigits = 2;
+    static constexpr bool kExact = false;
+};
+template <>
+struct Traits<float> {
+    static constexpr int kDigits = 3;
+    static constexpr bool kExact = true;
+};
+
+// Joins W partial results of one row: element d of sums at stride `pitch`.
+// factor(w) scales partial w to the joint maximum.
+__device__ __forceinline__ float join_factor(float m, float top) { return m == -INFINITY ? 0.0f : exp2_fast(m - top); }
+
+template <typename T>
+__device__ __forceinline__ void store_row(const AttnArgs& a, int64_t t, int head, int d, const float (&o)[4], float l,
+                                          float top, bool lead) {
+    T* out = static_cast<T*>(a.out) + (t * (a.heads * a.group) + head) * a.dim;
+    const float inv = l != 0.0f ? 1.0f / l : 0.0f;  // l = 0: the row sees nothing (a NaN l stays NaN)
+    if (d < a.dim) {
+        const float r[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
+        store4(out + d, true, r);
+    }
+    if (lead && a.lse) {
+        a.lse[t * (a.heads * a.group) + head] =
+            l != 0.0f ? (top - kLift + log2f(l)) * 0.69314718055994531f : -INFINITY;
+    }
+}
+
+template <typename T, int DP, int NT>
+__global__ void __launch_bounds__(kThreads, Traits<T>::kExact || NT == 2 || DP == 256 ? (DP == 256 ? 2 : 3) : 4)
+kv_rows_kernel(const AttnArgs a) {
+    constexpr int DIGITS = Traits<T>::kDigits;
+    constexpr bool EXACT = Traits<T>::kExact;
+    constexpr int ROWS = 8 * NT;
+    constexpr int KP = DP / 64;                // 16-byte pieces of a key row per lane
+    constexpr int VW = DP == 64 ? 2 : 4;       // words per piece of a value row
+    constexpr int VP = DP == 256 ? 2 : 1;      // pieces of a value row per lane
+    constexpr int NJ = DP / 16;                // 16-wide steps of dim in the value product
+    __shared__ float s_ml[kWarps][ROWS][2];
+    __shared__ __align__(16) float s_o[kWarps][ROWS][DP];
+    __shared__ int64_t s_scan[kWarps], s_tasks[kWarps], s_from, s_task0;
+    __shared__ int s_b;
+
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int g = lane >> 2, t = lane & 3;
+    pdl_launch_dependents();
+    pdl_wait();
+
+    // --- this block's run of tiles ------------------------------------------
+    int64_t total = 0, all_tasks = 0, run0 = 0, run1 = 0, blocks = 1;
+    for (int pass = 0; pass < 2; ++pass) {
+        int64_t seen = 0, tasks = 0;
+        for (int base = 0; base < a.seqs; base += kThreads) {
+            int64_t mine = 0, mine_tasks = 0;
+            if (base + tid < a.seqs) {
+                const Seq s = sequence(a, base + tid);
+                mine_tasks = static_cast<int64_t>((static_cast<int64_t>(s.rows) * a.group + ROWS - 1) / ROWS) * a.heads;
+                mine = mine_tasks * max(s.tiles, 1);
+            }
+            int64_t x = mine, y = mine_tasks;
+            #pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int64_t u = __shfl_up_sync(0xffffffffu, x, o), w = __shfl_up_sync(0xffffffffu, y, o);
+                if (lane >= o) x += u, y += w;
+            }
+            __syncthreads();
+            if (lane == 31) s_scan[warp] = x, s_tasks[warp] = y;
+            __syncthreads();
+            int64_t before = seen, before_tasks = tasks;
+            #pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                if (w < warp) before += s_scan[w], before_tasks += s_tasks[w];
+                seen += s_scan[w], tasks += s_tasks[w];
+            }
+            const int64_t from = before + x - mine;
+            // One chunk holds every sequence: its scan serves both passes.
+            if (a.seqs <= kThreads) {
+                total = seen;
+                blocks = max(int64_t{1}, min(static_cast<int64_t>(gridDim.x), total / kWarps));
+                if (blockIdx.x < blocks) {
+                    run0 = blockIdx.x * total / blocks;
+                    run1 = (blockIdx.x + 1) * total / blocks;
+                }
+            }
+            if ((pass == 1 || a.seqs <= kThreads) && run0 >= from && run0 < from + mine) {
+                s_b = base + tid;
+                s_from = from;
+                s_task0 = before_tasks + y - mine_tasks;
+            }
+        }
+        total = seen;
+        all_tasks = tasks;
+        if (pass == 0) {
+            blocks = max(int64_t{1}, min(static_cast<int64_t>(gridDim.x), total / kWarps));
+            if (blockIdx.x < blocks) {
+                run0 = blockIdx.x * total / blocks;
+                run1 = (blockIdx.x + 1) * total / blocks;
+            }
+            if (a.seqs <= kThreads) break;
+        }
+    }
+    __syncthreads();
+    if (tid == 0) {
+        if (a.by_task) {
+            if (blockIdx.x == 0) a.entry[0] = make_int4(static_cast<int>(all_tasks), 0, 0, 0);
+        } else {
+            if (blockIdx.x == 0) a.entry[0] = make_int4(static_cast<int>(gridDim.x), 0, 0, 0);
+            a.entry[1 + blockIdx.x] = make_int4(0, 0, 0, 0);
+        }
+    }
+    if (run0 >= run1) return;
+    int b = s_b;
+    int64_t from = s_from, task0 = s_task0;
+
+    while (run0 < run1) {
+        const Seq s = sequence(a, b);
+        const int tiles = max(s.tiles, 1);
+        const int row_tiles = (s.rows * a.group + ROWS - 1) / ROWS;
+        const int64_t units = static_cast<int64_t>(row_tiles) * a.heads * tiles;
+        if (run0 >= from + units) {
+            from += units;
+            task0 += static_cast<int64_t>(row_tiles) * a.heads;
+            ++b;
+            continue;
+        }
+        const int task = static_cast<int>((run0 - from) / tiles);
+        const int u0 = static_cast<int>((run0 - from) % tiles);
+        const int u1 = static_cast<int>(min(static_cast<int64_t>(tiles), u0 + (run1 - run0)));
+        const int h = task % a.heads, rt = task / a.heads;
+        const int row_end = s.rows * a.group;
+
+        // --- query rows ------------------------------------------------------
+        uint32_t qd[NT][DIGITS][DP / 16];
+        float fac[NT][2];
+        int see0[NT][2], see1[NT][2];  // visible tokens of rows 2 t, 2 t + 1
+        #pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const int r = rt * ROWS + 8 * n + g;
+            const int tok = r / a.group, hd = r - tok * a.group;
+            const T* row = static_cast<const T*>(a.q) + (s.row0 + tok) * a.q_tok +
+                           static_cast<int64_t>(h * a.group + hd) * a.q_head;
+            const float f = query_digits<T, DP, DIGITS>(qd[n], row, r < row_end, a.dim, a.q_vec != 0, t) * a.scale_log2;
+            #pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                fac[n][c] = __shfl_sync(0xffffffffu, f, 4 * (2 * t + c));
+                const int rc = rt * ROWS + 8 * n + 2 * t + c;
+                const int64_t pos = static_cast<int64_t>(s.len) - s.rows + rc / a.group;
+                see1[n][c] = a.causal ? static_cast<int>(max(pos + 1, int64_t{0})) : s.len;
+                see0[n][c] = a.window > 0 ? static_cast<int>(max(pos + 1 - a.window, int64_t{0})) : 0;
+            }
+        }
+        // Tokens that every row of the tile sees: no mask inside.
+        const int tok_lo = rt * ROWS / a.group, tok_hi = min(s.rows - 1, (rt * ROWS + ROWS - 1) / a.group);
+        const int all1 = a.causal ? s.len - s.rows + tok_lo + 1 : s.len;
+        const int64_t all0 = a.window > 0 ? static_cast<int64_t>(s.len) - s.rows + tok_hi + 1 - a.window : 0;
+
+        float o[NT][NJ][4] = {};
+        float m[NT][2], l[NT][2];
+        #pragma unroll
+        for (int n = 0; n < NT; ++n) m[n][0] = m[n][1] = -INFINITY, l[n][0] = l[n][1] = 0.0f;
+
+        const int32_t* table = a.table + static_cast<int64_t>(b) * a.table_pages;
+        const int last = min(u1, s.tiles);
+        const int page_mask = (1 << a.page_shift) - 1;
+        const auto page_of = [&](int tile) {
+            return tile < last ? table[(s.lo + 16 * tile) >> a.page_shift] : 0;
+        };
+        uint32_t kr[2][KP][4], vr[4][VP][VW];
+        float ks = 0.0f, vs = 0.0f;
+        const auto load_k = [&](int tile, int page) {
+            const int64_t at = static_cast<int64_t>(page) * a.heads + h;
+            const int8_t* p = a.k + ((at << a.page_shift) + ((s.lo + 16 * tile) & page_mask)) * a.dim;
+            #pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                #pragma unroll
+                for (int c = 0; c < KP; ++c) {
+                    load_codes(kr[r][c], p + (g + 8 * r) * a.dim + 16 * (t + 4 * c), 16 * (t + 4 * c) < a.dim);
+                }
+            }
+            ks = a.ks[at];
+        };
+        const auto load_v = [&](int tile, int page) {
+            const int64_t at = static_cast<int64_t>(page) * a.heads + h;
+            const int8_t* p = a.v + ((at << a.page_shift) + ((s.lo + 16 * tile) & page_mask)) * a.dim;
+            #pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int row = 2 * t + (i & 1) + 8 * (i >> 1);
+                #pragma unroll
+                for (int c = 0; c < VP; ++c) {
+                    const int d = 4 * VW * (g + 8 * c);
+                    load_codes(vr[i][c], p + row * a.dim + d, d < a.dim);
+                }
+            }
+            vs = a.vs[at];
+        };
+        const auto checked = [&](int page, bool& ok) {
+            ok = page >= 0 && page < a.pages;
+            return ok ? page : 0;
+        };
+
+        int tile = u0 + warp;
+        bool ok = true, ok_next = true;
+        int page = checked(page_of(tile), ok);
+        int page_next = page_of(tile + kWarps);
+        if (tile < last) {
+            load_k(tile, page);
+            load_v(tile, page);
+        }
+        for (; tile < last; tile += kWarps) {
+            page_next = checked(page_next, ok_next);
+            const bool more = tile + kWarps < last;
+
+            int sc[NT][DIGITS][4];
+            #pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                #pragma unroll
+                for (int i = 0; i < DIGITS; ++i) {
+                    sc[n][i][0] = sc[n][i][1] = sc[n][i][2] = sc[n][i][3] = kMagicBits;
+                }
+            }
+            #pragma unroll
+            for (int step = 0; step < DP / 32; ++step) {
+                // Words of the step's two halves: pieces 2 i and 2 i + 1, or two
+                // words of the only piece.
+                constexpr bool ONE = DP == 64;
+                const int p0 = ONE ? 0 : 2 * (step / 4), p1 = ONE ? 0 : p0 + 1;
+                const int w0 = ONE ? step : step % 4, w1 = ONE ? step + 2 : w0;
+                const uint32_t ka[4] = {kr[0][p0][w0], kr[1][p0][w0], kr[0][p1][w1], kr[1][p1][w1]};
+                #pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    #pragma unroll
+                    for (int i = 0; i < DIGITS; ++i) {
+                        mma_s8_16832(sc[n][i], ka, qd[n][i][4 * p0 + w0], qd[n][i][4 * p1 + w1]);
+                    }
+                }
+            }
+            const float ks_now = ks;
+            const bool ok_now = ok;
+            const int page_after = page_of(tile + 2 * kWarps);
+            if (more) load_k(tile + kWarps, page_next);
+
+            // vs = 2^ve vf with vf in [1, 2); scales below 2^-80 belong to
+            // all-zero codes, non-finite ones pass through vf.
+            const uint32_t vbits = __float_as_uint(vs);
+            int ve = static_cast<int>((vbits >> 23) & 0xffu) - 127;
+            float vf = __uint_as_float((vbits & 0x807fffffu) | 0x3f800000u);
+            if (ve == 128) ve = 0, vf = vs;
+            if (ve < -80) ve = -80, vf = 0.0f;
+            if (!ok_now) ve = 0, vf = 0.0f;
+            const float vexp = static_cast<float>(ve), vinv = __int_as_float((127 - ve) << 23);
+
+            const int tok = s.lo + 16 * tile;
+            const bool whole = ok_now && tok >= all0 && tok + 16 <= all1;
+            float p[NT][4];
+            bool grow = false;
+            #pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                #pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    float x = __int_as_float(sc[n][DIGITS - 1][c]) - kMagic;
+                    #pragma unroll
+                    for (int i = DIGITS - 2; i >= 0; --i) {
+                        x = fmaf(x, 256.0f, __int_as_float(sc[n][i][c]) - kMagic);
+                    }
+                    p[n][c] = fmaf(x, fac[n][c & 1] * ks_now, vexp);
+                }
+                if (!whole) {
+                    #pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const int j = tok + g + 8 * (c >> 1);
+                        if (!ok_now || j < see0[n][c & 1] || j >= see1[n][c & 1] || j >= s.len) p[n][c] = -INFINITY;
+                    }
+                }
+                #pragma unroll
+                for (int c = 0; c < 4; ++c) grow = grow || p[n][c] > m[n][c & 1] + kSlack;
+            }
+            if (__any_sync(0xffffffffu, grow)) {
+                #pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    #pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        float top = fmaxf(p[n][c], p[n][c + 2]);
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                        top = fmaxf(top, m[n][c]);
+                        const float by = join_factor(m[n][c], top);
+                        m[n][c] = top;
+                        l[n][c] *= by;
+                        #pragma unroll
+                        for (int j = 0; j < NJ; ++j) o[n][j][c] *= by, o[n][j][c + 2] *= by;
+                    }
+                }
+            }
+            uint32_t hi[NT][2], lo[NT][2];
+            #pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                float e[4];
+                #pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const float base = m[n][c & 1] == -INFINITY ? 0.0f : m[n][c & 1];
+                    const float x = exp2_fast(p[n][c] + (kLift - base));
+                    l[n][c & 1] = fmaf(x, vinv, l[n][c & 1]);
+                    e[c] = x * vf;
+                    if (!whole && p[n][c] == -INFINITY) e[c] = 0.0f;  // hidden from this row: vf may be NaN
+                }
+                #pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const uint32_t top = pack_f16(e[2 * r], e[2 * r + 1]);
+                    hi[n][r] = transpose8(top);
+                    if (EXACT) {
+                        const __half2 th = *reinterpret_cast<const __half2*>(&top);
+                        lo[n][r] = transpose8(pack_f16(e[2 * r] - __low2float(th), e[2 * r + 1] - __high2float(th)));
+                    }
+                }
+            }
+            #pragma unroll
+            for (int c = 0; c < VP; ++c) {
+                #pragma unroll
+                for (int w = 0; w < VW; ++w) {
+                    // Bytes 0, 1 and 2, 3 of this word, of the token pairs
+                    // (2 t, 2 t + 1) and (2 t + 8, 2 t + 9).
+                    const uint32_t bias = 0x80808080u;
+                    const uint32_t x0 = __byte_perm(vr[0][c][w], vr[1][c][w], 0x5140) ^ bias;
+                    const uint32_t y0 = __byte_perm(vr[0][c][w], vr[1][c][w], 0x7362) ^ bias;
+                    const uint32_t x1 = __byte_perm(vr[2][c][w], vr[3][c][w], 0x5140) ^ bias;
+                    const uint32_t y1 = __byte_perm(vr[2][c][w], vr[3][c][w], 0x7362) ^ bias;
+                    const uint32_t va[2][4] = {
+                        {codes_f16<0x4140>(x0), codes_f16<0x4342>(x0), codes_f16<0x4140>(x1), codes_f16<0x4342>(x1)},
+                        {codes_f16<0x4140>(y0), codes_f16<0x4342>(y0), codes_f16<0x4140>(y1), codes_f16<0x4342>(y1)}};
+                    #pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int j = 2 * (VW * c + w) + i;
+                        #pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            if (EXACT) {
+                                float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                                mma_f16_16816(d, va[i], lo[n][0], lo[n][1]);
+                                mma_f16_16816(d, va[i], hi[n][0], hi[n][1]);
+                                #pragma unroll
+                                for (int c4 = 0; c4 < 4; ++c4) o[n][j][c4] += d[c4];
+                            } else {
+                                mma_f16_16816(o[n][j], va[i], hi[n][0], hi[n][1]);
+                            }
+                        }
+                    }
+                }
+            }
+            if (more) load_v(tile + kWarps, page_next);
+            if (!ok_now && lane == 0) atomicOr(&g_attn_err, kKvErrAttention);
+            page = page_next;
+            ok = ok_next;
+            page_next = page_after;
+        }
+
+        // --- join the warps --------------------------------------------------
+        __syncthreads();  // the previous task's results have been read
+        #pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            #pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                float x = l[n][c];
+                x += __shfl_xor_sync(0xffffffffu, x, 4);
+                x += __shfl_xor_sync(0xffffffffu, x, 8);
+                x += __shfl_xor_sync(0xffffffffu, x, 16);
+                const int r = 8 * n + 2 * t + c;
+                if (g == 0) s_ml[warp][r][0] = m[n][c], s_ml[warp][r][1] = x;
+                // Elements 2 j, 2 j + 1 of the lane's run of dim.
+                #pragma unroll
+                for (int j = 0; j < NJ; j += 2) {
+                    const int run = DP == 64 ? 8 * g : 16 * (g + 8 * (j / 8));
+                    *reinterpret_cast<float4*>(&s_o[warp][r][run + 2 * (j % 8)]) =
+                        make_float4(o[n][j][c], o[n][j][c + 2], o[n][j + 1][c], o[n][j + 1][c + 2]);
+                }
+            }
+        }
+        __syncthreads();
+        const bool complete = u0 == 0 && u1 == tiles;
+        const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (u0 > 0 ? 0 : 1);
+        for (int i = tid; i < ROWS * (DP / 4); i += kThreads) {
+            const int r = i / (DP / 4), d = 4 * (i % (DP / 4));
+            const int row = rt * ROWS + r;
+            if (row >= row_end) continue;
+            float top = -INFINITY, den = 0.0f, sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            #pragma unroll
+            for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_ml[w][r][0]);
+            #pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                const float f = join_factor(s_ml[w][r][0], top);
+                const float4 x = *reinterpret_cast<const float4*>(&s_o[w][r][d]);
+                den = fmaf(s_ml[w][r][1], f, den);
+                sum[0] = fmaf(x.x, f, sum[0]), sum[1] = fmaf(x.y, f, sum[1]);
+                sum[2] = fmaf(x.z, f, sum[2]), sum[3] = fmaf(x.w, f, sum[3]);
+            }
+            if (complete) {
+                const int tk = row / a.group;
+                store_row<T>(a, s.row0 + tk, h * a.group + row - tk * a.group, d, sum, den, top, d == 0);
+            } else {
+                if (d == 0) a.ml[slot * ROWS + r] = make_float2(top, den);
+                *reinterpret_cast<float4*>(a.part + (slot * ROWS + r) * DP + d) =
+                    make_float4(sum[0], sum[1], sum[2], sum[3]);
+            }
+        }
+        if (tid == 0 && u0 == 0 && (a.by_task || !complete)) {
+            // Blocks that hold the rest of the task: the last one owns its last
+            // tile (block c owns tiles [c total / blocks, (c + 1) total / blocks)).
+            const int64_t end = from + static_cast<int64_t>(task + 1) * tiles;
+            const int64_t owner = complete ? blockIdx.x : (end * blocks - 1) / total;
+            const int more = static_cast<int>(owner - blockIdx.x);
+            const int64_t e = a.by_task ? task0 + task : blockIdx.x;
+            // (A `first` that does not ascend can make more tasks than there are.)
+            if (e < a.entries) a.entry[1 + e] = make_int4(more, b, task, blockIdx.x);
+        }
+        run0 += u1 - u0;
+    }
+}
+
+// Joins the partial results of one row of one task: block 0's second slot,
+// then the first slots of the blocks after it, in that order. Four warps take
+// every fourth partial; bound by the latency of their loads.
+template <typename T, int DP, int ROWS>
+__global__ void __launch_bounds__(kThreads) kv_join_kernel(const AttnArgs a) {
+    __shared__ float s_top[kWarps], s_den[kWarps];
+    __shared__ __align__(16) float s_o[kWarps][DP];
+    pdl_launch_dependents();
+    pdl_wait();
+    if (static_cast<int>(blockIdx.x) >= a.entry[0].x) return;
+    const int4 e = a.entry[1 + blockIdx.x];
+    if (e.x == 0) return;
+    const Seq s = sequence(a, e.y);
+    const int r = blockIdx.y, h = e.z % a.heads, row = e.z / a.heads * ROWS + r;
+    if (row >= s.rows * a.group) return;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int count = e.x + 1;
+    const auto slot = [&](int i) { return static_cast<int64_t>(2 * (e.w + i) + (i == 0 ? 1 : 0)) * ROWS + r; };
+
+    float top = -INFINITY;
+    for (int i = tid; i < count; i += kThreads) top = fmaxf(top, a.ml[slot(i)].x);
+    #pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (lane == 0) s_top[warp] = top;
+    __syncthreads();
+    #pragma unroll
+    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_top[w]);
+
+    constexpr int PER = DP >= 128 ? DP / 128 : 1;  // float4 pieces per lane
+    float den = 0.0f, sum[PER][4] = {};
+    #pragma unroll 4
+    for (int i = warp; i < count; i += kWarps) {
+        const float2 ml = a.ml[slot(i)];
+        const float f = join_factor(ml.x, top);
+        den = fmaf(ml.y, f, den);
+        #pragma unroll
+        for (int k = 0; k < PER; ++k) {
+            const int d = 4 * (lane + 32 * k);
+            if (d < DP) {
+                const float4 x = *reinterpret_cast<const float4*>(a.part + slot(i) * DP + d);
+                sum[k][0] = fmaf(x.x, f, sum[k][0]), sum[k][1] = fmaf(x.y, f, sum[k][1]);
+                sum[k][2] = fmaf(x.z, f, sum[k][2]), sum[k][3] = fmaf(x.w, f, sum[k][3]);
+            }
+        }
+    }
+    if (lane == 0) s_den[warp] = den;
+    #pragma unroll
+    for (int k = 0; k < PER; ++k) {
+        const int d = 4 * (lane + 32 * k);
+        if (d < DP) *reinterpret_cast<float4*>(&s_o[warp][d]) = make_float4(sum[k][0], sum[k][1], sum[k][2], sum[k][3]);
+    }
+    __syncthreads();
+    const int d = 4 * tid;
+    if (d >= DP) return;
+    float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    den = 0.0f;
+    #pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        den += s_den[w];
+        #pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] += s_o[w][d + j];
+    }
+    const int tk = row / a.group;
+    store_row<T>(a, s.row0 + tk, h * a.group + row - tk * a.group, d, o, den, top, d == 0);
+}
+
+template <typename T, int DP, int NT>
+cudaError_t launch_rows(AttnArgs a, int64_t tasks, cudaStream_t stream) {
+    constexpr int ROWS = 8 * NT;
+    // One wave: as many blocks as are resident at once.
+    static int resident = 0;
+    int per_sm = __atomic_load_n(&resident, __ATOMIC_RELAXED);
+    if (per_sm == 0) {
+        cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kv_rows_kernel<T, DP, NT>, kThreads, 0);
+        if (e != cudaSuccess) return e;
+        if (per_sm < 1) return cudaErrorInvalidConfiguration;
+        __atomic_store_n(&resident, per_sm, __ATOMIC_RELAXED);
+    }
+    const int64_t grid = static_cast<int64_t>(per_sm) * device_sm_count();
+    a.by_task = tasks <= grid ? 1 : 0;
+    a.entries = static_cast<int>(a.by_task ? tasks : grid);
+    const size_t entry_bytes = (1 + grid) * sizeof(int4);
+    const size_t ml_bytes = ((2 * grid * ROWS * sizeof(float2)) + 15) / 16 * 16;
+    char* ws = nullptr;
+    cudaError_t e = scratch_alloc(reinterpret_cast<void**>(&ws),
+                                  entry_bytes + ml_bytes + 2 * grid * ROWS * DP * sizeof(float), stream);
+    if (e != cudaSuccess) return e;
+    a.entry = reinterpret_cast<int4*>(ws);
+    a.ml = reinterpret_cast<float2*>(ws + entry_bytes);
+    a.part = reinterpret_cast<float*>(ws + entry_bytes + ml_bytes);
+    cudaLaunchAttribute attr[1];
+    cudaLaunchConfig_t cfg = pdl_config(dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, stream, attr);
+    e = cudaLaunchKernelEx(&cfg, kv_rows_kernel<T, DP, NT>, a);
+    if (e == cudaSuccess) {
+        cfg.gridDim = dim3(static_cast<unsigned>(a.entries), ROWS);
+        e = cudaLaunchKernelEx(&cfg, kv_join_kernel<T, DP, ROWS>, a);
+    }
+    const cudaError_t f = scratch_free(ws, stream);
+    return e != cudaSuccess ? e : f;
+}
+
+template <typename T>
+cudaError_t launch_attention(const AttnArgs& a, int64_t max_tokens, cudaStream_t stream) {
+    // Tasks of at most 8 or 16 query rows; an upper bound of their number.
+    const bool two = !Traits<T>::kExact && a.dim <= 128 && max_tokens * a.group > 8;
+    const int rows = two ? 16 : 8;
+    const int64_t tasks = a.heads * (static_cast<int64_t>(a.tokens) * a.group / rows + a.seqs);
+    if (two) {
+        if constexpr (!Traits<T>::kExact) {
+            return a.dim <= 64 ? launch_rows<T, 64, 2>(a, tasks, stream) : launch_rows<T, 128, 2>(a, tasks, stream);
+        }
+    }
+    if (a.dim <= 64) return launch_rows<T, 64, 1>(a, tasks, stream);
+    if (a.dim <= 128) return launch_rows<T, 128, 1>(a, tasks, stream);
+    return launch_rows<T, 256, 1>(a, tasks, stream);
+}
+
+}  // namespace
+
+cudaError_t kv_attention_take_errors(unsigned int* bits) {
+    const unsigned int zero = 0;
+    cudaError_t e = cudaMemcpyFromSymbol(bits, g_attn_err, sizeof(unsigned int));
+    if (e == cudaSuccess && *bits != 0) e = cudaMemcpyToSymbol(g_attn_err, &zero, sizeof(unsigned int));
+    return e;
+}
+
+}  // namespace pcb
+
+extern "C" popcornStatus_t popcornKvAttention(void* out, float* lse, const void* q, int64_t q_token_stride,
+                                              int64_t q_head_stride, popcornType_t type, const popcornKvCache_t* cache,
+                                              const int32_t* table, int64_t table_pages, const int32_t* first,
+                                              const int32_t* length, int64_t seqs, int64_t tokens, int64_t max_tokens,
+                                              int64_t q_heads, int causal, int64_t window, float scale,
+                                              cudaStream_t stream) {
+    if (out == nullptr || q == nullptr || cache == nullptr || cache->k == nullptr || cache->v == nullptr ||
+        cache->k_scale == nullptr || cache->v_scale == nullptr || table == nullptr || length == nullptr) {
+        return POPCORN_ERROR_INVALID_VALUE;
+    }
+    if (seqs <= 0 || tokens <= 0) return POPCORN_SUCCESS;
+    if (!pcb::kv_cache_supported(*cache) || !pcb::kv_type_supported(type) || table_pages <= 0 || q_heads <= 0 ||
+        q_heads % cache->heads != 0 || q_heads > 65535 || max_tokens <= 0 || !pcb::aligned16(out)) {
+        return POPCORN_ERROR_INVALID_VALUE;
+    }
+    // Positions and row counts are 32-bit inside a sequence.
+    if ((first == nullptr && tokens != seqs) || seqs > INT32_MAX / 2 || tokens > INT32_MAX / q_heads ||
+        table_pages > (INT32_MAX - 64) / cache->page_size) {
+        return POPCORN_ERROR_INVALID_VALUE;
+    }
+    pcb::AttnArgs a = {};
+    a.out = out, a.lse = lse, a.q = q, a.q_tok = q_token_stride, a.q_head = q_head_stride;
+    a.k = cache->k, a.v = cache->v, a.ks = cache->k_scale, a.vs = cache->v_scale;
+    a.table = table, a.first = first, a.length = length;
+    a.table_pages = table_pages, a.pages = cache->pages, a.window = window;
+    a.seqs = static_cast<int>(seqs), a.tokens = static_cast<int>(tokens);
+    a.heads = static_cast<int>(cache->heads), a.group = static_cast<int>(q_heads / cache->heads);
+    a.dim = static_cast<int>(cache->dim), a.page_shift = pcb::log2_of(cache->page_size);
+    a.causal = causal;
+    a.scale_log2 = scale * 1.4426950408889634f;
+    const int64_t four = 4 * pcb::kv_type_size(type);
+    a.q_vec = reinterpret_cast<uintptr_t>(q) % four == 0 && q_token_stride % 4 == 0 && q_head_stride % 4 == 0;
+    cudaError_t e;
+    switch (type) {
+        case POPCORN_TYPE_F32: e = pcb::launch_attention<float>(a, max_tokens, stream); break;
+        case POPCORN_TYPE_F16: e = pcb::launch_attention<__half>(a, max_tokens, stream); break;
+        default: e = pcb::launch_attention<__nv_bfloat16>(a, max_tokens, stream); break;
+    }
+    if (e != cudaSuccess) return pcb::record_cuda(e);
+    return pcb::check_launch();
+}

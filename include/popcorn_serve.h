@@ -147,6 +147,9 @@ popcornStatus_t popcornKvRead(
  *             (0 or less: no window)
  *   lse       optional f32 [tokens, q_heads]: the natural logarithm of the
  *             softmax's denominator, -inf where a query sees nothing
+ *   workspace  optional, 16-byte aligned, popcornKvAttentionWorkspace bytes
+ *             (independent of lengths; nothing in it needs to start at zero
+ *             and nothing is kept in it); NULL: from the library's pool
  *
  * A query that sees nothing gives zeros. Scores, statistics and sums are
  * f32 or exact integers; f32 queries keep 23 bits relative to their row's
@@ -174,7 +177,80 @@ popcornStatus_t popcornKvAttention(
     int causal,
     int64_t window,
     float scale,
+    void* workspace,
+    int64_t workspace_bytes,
     cudaStream_t stream
+);
+
+/* Bytes of workspace that popcornKvAttention takes for these sizes (0 where
+ * the call would be refused or has no work). Launches nothing. */
+int64_t popcornKvAttentionWorkspace(
+    const popcornKvCache_t* cache,
+    popcornType_t type,
+    int64_t seqs,
+    int64_t tokens,
+    int64_t max_tokens,
+    int64_t q_heads
+);
+
+/*
+ * A mixture-of-experts layer for a few tokens, experts in popcorn's
+ * per-channel int8 (W[n, k] = q[n, k] * s[n]):
+ *   z = x @ router^T                       [M, E]
+ *   p = softmax(z); each token picks the top_k experts of largest z, the
+ *       lowest index first among equals; with renormalize their p are
+ *       divided by their sum
+ *   out[m] = sum over its picks e of p_e *
+ *            (silu(x W_gate[e]^T) * (x W_up[e]^T)) W_down[e]^T
+ *
+ *   x [M, K], out [M, K], router [E, K] f32
+ *   q_gate, q_up int8 [E, F, K], s_gate, s_up f32 [E, F]
+ *   q_down int8 [E, K, F], s_down f32 [E, K]
+ *   experts int32 [M, top_k], weights f32 [M, top_k]: optional (both or
+ *             neither), the picks, largest first
+ *   workspace optional, 256-byte aligned, popcornMoeWorkspace bytes; NULL:
+ *             from the library's pool
+ *
+ * Limits (else POPCORN_ERROR_INVALID_VALUE): E <= 256, 1 <= top_k <=
+ * min(E, 16), K and F <= 65536. Any M, meant for up to a few tens: 64 tokens
+ * are one pass over the chosen experts. K and F that are multiples of 16 with
+ * 16-byte aligned codes run on the warp-level tensor path: activations and
+ * hidden values as 30-bit fixed point, exact integer dot products (of 32
+ * columns for the down product, joined in f32). Other sizes and alignments
+ * sum in f32. A token with a NaN or an infinity gives NaN for that token.
+ * Results do not depend on the order in which blocks of the GPU run.
+ */
+popcornStatus_t popcornMoe_i8f32(
+    float* out,
+    int32_t* experts,
+    float* weights,
+    const float* x,
+    const float* router,
+    const int8_t* q_gate,
+    const float* s_gate,
+    const int8_t* q_up,
+    const float* s_up,
+    const int8_t* q_down,
+    const float* s_down,
+    int64_t M,
+    int64_t K,
+    int64_t F,
+    int64_t E,
+    int64_t top_k,
+    int renormalize,
+    void* workspace,
+    int64_t workspace_bytes,
+    cudaStream_t stream
+);
+
+/* Bytes of workspace that popcornMoe_i8f32 takes for these sizes (0 where the
+ * call would be refused or has no work). Launches nothing. */
+int64_t popcornMoeWorkspace(
+    int64_t M,
+    int64_t K,
+    int64_t F,
+    int64_t E,
+    int64_t top_k
 );
 
 #ifdef __cplusplus

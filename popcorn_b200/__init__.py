@@ -68,6 +68,9 @@ SERVE_SYMBOLS = (
     "popcornKvAppend",
     "popcornKvRead",
     "popcornKvAttention",
+    "popcornKvAttentionWorkspace",
+    "popcornMoe_i8f32",
+    "popcornMoeWorkspace",
 )
 
 TYPE_F32 = 0
@@ -139,7 +142,10 @@ _SIGNATURES = {
                                _i64, _i64, _i64, _vp, _vp, _i64, _i64, _int, _vp]),
     "popcornKvRead": (_int, [_vp, _vp, _int, _vp, _vp, _i64, _vp]),
     "popcornKvAttention": (_int, [_vp, _vp, _vp, _i64, _i64, _int, _vp, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _i64,
-                                  _int, _i64, ctypes.c_float, _vp]),
+                                  _int, _i64, ctypes.c_float, _vp, _i64, _vp]),
+    "popcornKvAttentionWorkspace": (_i64, [_vp, _int, _i64, _i64, _i64, _i64]),
+    "popcornMoe_i8f32": (_int, [_vp] * 11 + [_i64] * 5 + [_int, _vp, _i64, _vp]),
+    "popcornMoeWorkspace": (_i64, [_i64] * 5),
 }
 
 _lib = None
@@ -457,13 +463,23 @@ def _want(ok: bool, where: str, what: str) -> None:
         raise ValueError(f"{where}: {what}")
 
 
-def _whole(t, shape, where: str, name: str):
+def _stream_on(stream, device):
+    """The handle of `stream`, by default the current one of `device`. (torch.cuda.current_stream builds an object
+    for it, 3 us of a decode step's 8.)"""
+    if stream is None:
+        import torch
+
+        return torch._C._cuda_getCurrentRawStream(device.index)
+    return stream if isinstance(stream, int) else stream.cuda_stream
+
+
+def _whole(t, shape, device, where: str, name: str):
     """Device pointer of a contiguous int32 tensor of this shape."""
     import torch
 
-    if t.dtype is not torch.int32 or t.shape != shape or not t.is_contiguous() or not t.is_cuda:
-        raise ValueError(f"{where}: {name}: a contiguous int32 CUDA tensor {tuple(shape)} wanted, "
-                         f"got {t.dtype} {tuple(t.shape)}")
+    if t.dtype is not torch.int32 or t.shape != shape or not t.is_contiguous() or t.device != device:
+        raise ValueError(f"{where}: {name}: a contiguous int32 tensor {tuple(shape)} on {device} wanted, "
+                         f"got {t.dtype} {tuple(t.shape)} on {t.device}")
     return t.data_ptr()
 
 
@@ -472,7 +488,8 @@ class KvCache:
     head [pages, heads], keys and values apart (a cached value is code * scale). ``page_size`` is a power of two from
     16 to 256, ``dim`` a multiple of 16 up to 256. Wraps the caller's tensors; :meth:`empty` makes them."""
 
-    __slots__ = ("k", "v", "k_scale", "v_scale", "pages", "heads", "page_size", "dim", "_struct", "_ref")
+    __slots__ = ("k", "v", "k_scale", "v_scale", "pages", "heads", "page_size", "dim", "device", "_struct", "_ref",
+                 "_workspaces")
 
     def __init__(self, k, v, k_scale, v_scale):
         import torch
@@ -493,6 +510,8 @@ class KvCache:
         self._struct = KvCacheStruct(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), self.pages,
                                      self.heads, self.page_size, self.dim)
         self._ref = ctypes.addressof(self._struct)
+        self.device = k.device
+        self._workspaces = {}  # sizes -> bytes of an attention call's workspace
 
     @classmethod
     def empty(cls, pages: int, heads: int, dim: int, page_size: int = 16, device="cuda"):
@@ -504,23 +523,26 @@ class KvCache:
         return cls(*codes, *scales)
 
 
-def _rows(t, tokens, heads, dim, kind, where, name):
-    """Checks [tokens, heads, dim] with dim contiguous."""
-    if t.shape != (tokens, heads, dim) or t.dtype is not kind or not t.is_cuda:
-        raise ValueError(f"{where}: {name}: {kind} CUDA tensor {(tokens, heads, dim)} wanted, "
-                         f"got {t.dtype} {tuple(t.shape)}")
+def _rows(t, shape, kind, device, where, name):
+    """Strides of the first two dimensions of [tokens, heads, dim] with dim contiguous."""
+    if t.shape != shape or t.dtype is not kind or t.device != device:
+        raise ValueError(f"{where}: {name}: {kind} {tuple(shape)} on {device} wanted, "
+                         f"got {t.dtype} {tuple(t.shape)} on {t.device}")
     a, b, c = t.stride()
     if c != 1:
         raise ValueError(f"{where}: {name}: the last dimension must be contiguous")
     return a, b
 
 
-def _batch(table, first, tokens, where):
-    seqs, width = table.shape
+def _batch(table, first, tokens, device, where):
+    if table.dim() != 2:
+        raise ValueError(f"{where}: table: [seqs, pages] wanted")
+    seqs, width = shape = table.shape
+    tp = _whole(table, shape, device, where, "table")
     if first is not None:
-        return seqs, _whole(table, (seqs, width), where, "table"), width, _whole(first, (seqs + 1,), where, "first")
+        return seqs, tp, width, _whole(first, (seqs + 1,), device, where, "first")
     _want(tokens == seqs, where, f"{tokens} tokens for {seqs} sequences need `first`")
-    return seqs, _whole(table, (seqs, width), where, "table"), width, None
+    return seqs, tp, width, None
 
 
 def kv_append(cache: KvCache, k, v, table, start, first=None, q=None, cos=None, sin=None, interleaved: bool = False,
@@ -529,38 +551,41 @@ def kv_append(cache: KvCache, k, v, table, start, first=None, q=None, cos=None, 
     ``start`` int32 [seqs] tokens that they hold, rotating keys (and queries ``q`` [tokens, q_heads, dim]) by the
     tables ``cos``, ``sin`` f32 [positions, rot_dim / 2]. ``first`` int32 [seqs + 1]: each sequence's run of tokens
     (None: one token each). Returns the rotated queries (``q_out``, or a new tensor), None without ``q``."""
-    where = "kv_append"
     import torch
 
-    tokens = k.shape[0]
-    kind = k.dtype
-    kt, kh = _rows(k, tokens, cache.heads, cache.dim, kind, where, "k")
-    vt, vh = _rows(v, tokens, cache.heads, cache.dim, kind, where, "v")
-    seqs, tp, width, fp = _batch(table, first, tokens, where)
-    sp = _whole(start, (seqs,), where, "start")
+    where = "kv_append"
+    device, kind, dim = cache.device, k.dtype, cache.dim
+    shape = k.shape
+    tokens = shape[0]
+    _want(shape == (tokens, cache.heads, dim), where, f"k: [tokens, {cache.heads}, {dim}] wanted")
+    kt, kh = _rows(k, shape, kind, device, where, "k")
+    vt, vh = _rows(v, shape, kind, device, where, "v")
+    seqs, tp, width, fp = _batch(table, first, tokens, device, where)
+    sp = _whole(start, (seqs,), device, where, "start")
     qp = op = None
     qt = qh = q_heads = 0
     if q is not None:
         q_heads = q.shape[1]
-        qt, qh = _rows(q, tokens, q_heads, cache.dim, kind, where, "q")
+        shape = (tokens, q_heads, dim)
+        qt, qh = _rows(q, shape, kind, device, where, "q")
         if q_out is None:
-            q_out = torch.empty((tokens, q_heads, cache.dim), dtype=kind, device=q.device)
+            q_out = q.new_empty(shape)
         else:
-            _rows(q_out, tokens, q_heads, cache.dim, kind, where, "q_out")
+            _rows(q_out, shape, kind, device, where, "q_out")
             _want(q_out.is_contiguous(), where, "q_out must be contiguous")
         qp, op = q.data_ptr(), q_out.data_ptr()
     cp = np_ = None
     positions = rot = 0
     if cos is not None:
-        positions, rot = cos.shape
+        positions, rot = shape = cos.shape
         for t in (cos, sin):
-            _want(t.shape == cos.shape and t.dtype is torch.float32 and t.is_contiguous() and t.is_cuda, where,
-                  "cos and sin: contiguous float32 CUDA tensors [positions, rot_dim / 2]")
+            if t.shape != shape or t.dtype is not torch.float32 or not t.is_contiguous() or t.device != device:
+                raise ValueError(f"{where}: cos and sin: contiguous float32 [positions, rot_dim / 2] on {device}")
         cp, np_, rot = cos.data_ptr(), sin.data_ptr(), 2 * rot
-    _check(load_library().popcornKvAppend(cache._ref, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh,
-                                          _type_of(kind, where), tp, width, fp, sp, seqs, tokens, op, qp, qt, qh,
-                                          q_heads, cp, np_, positions, rot, interleaved, _stream_handle(stream)),
-           "popcornKvAppend")
+    st = load_library().popcornKvAppend(cache._ref, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, _type_of(kind, where),
+                                        tp, width, fp, sp, seqs, tokens, op, qp, qt, qh, q_heads, cp, np_, positions,
+                                        rot, interleaved, _stream_on(stream, device))
+    _check(st, "popcornKvAppend")
     return q_out
 
 
@@ -572,18 +597,18 @@ def kv_read(cache: KvCache, pages, dtype=None, k_out=None, v_out=None, stream=No
     where = "kv_read"
     dtype = dtype or (k_out.dtype if k_out is not None else torch.float32)
     n = pages.shape[0]
+    device = cache.device
     shape = (n, cache.heads, cache.page_size, cache.dim)
     if k_out is None:
-        k_out = torch.empty(shape, dtype=dtype, device=cache.k.device)
+        k_out = cache.k_scale.new_empty(shape, dtype=dtype)
     if v_out is None:
-        v_out = torch.empty(shape, dtype=dtype, device=cache.k.device)
+        v_out = torch.empty_like(k_out)
     for t in (k_out, v_out):
-        _want(t.shape == shape and t.dtype is dtype and t.is_contiguous() and t.is_cuda, where,
-              f"outputs: contiguous {dtype} CUDA tensors {shape}")
-    lp = _whole(pages, (n,), where, "pages")
-    if n:
-        _check(load_library().popcornKvRead(k_out.data_ptr(), v_out.data_ptr(), _type_of(dtype, where), cache._ref,
-                                            lp, n, _stream_handle(stream)), "popcornKvRead")
+        if t.shape != shape or t.dtype is not dtype or not t.is_contiguous() or t.device != device:
+            raise ValueError(f"{where}: outputs: contiguous {dtype} {shape} on {device}")
+    st = load_library().popcornKvRead(k_out.data_ptr(), v_out.data_ptr(), _type_of(dtype, where), cache._ref,
+                                      _whole(pages, (n,), device, where, "pages"), n, _stream_on(stream, device))
+    _check(st if n else POPCORN_SUCCESS, "popcornKvRead")
     return k_out, v_out
 
 
@@ -596,25 +621,76 @@ def kv_attention(cache: KvCache, q, table, length, first=None, max_tokens: int |
     import torch
 
     where = "kv_attention"
-    tokens, q_heads, dim = q.shape
-    qt, qh = _rows(q, tokens, q_heads, cache.dim, q.dtype, where, "q")
-    _want(q_heads % cache.heads == 0, where, f"{q_heads} query heads over {cache.heads} cache heads")
-    seqs, tp, width, fp = _batch(table, first, tokens, where)
-    lp = _whole(length, (seqs,), where, "length")
+    device, kind = cache.device, q.dtype
+    tokens, q_heads, dim = shape = q.shape
+    _want(dim == cache.dim and q_heads % cache.heads == 0, where,
+          f"q: {q_heads} heads of {dim} over a cache of {cache.heads} heads of {cache.dim}")
+    qt, qh = _rows(q, shape, kind, device, where, "q")
+    seqs, tp, width, fp = _batch(table, first, tokens, device, where)
+    lp = _whole(length, (seqs,), device, where, "length")
     if out is None:
-        out = torch.empty((tokens, q_heads, dim), dtype=q.dtype, device=q.device)
+        out = q.new_empty(shape)
     else:
-        _rows(out, tokens, q_heads, dim, q.dtype, where, "out")
+        _rows(out, shape, kind, device, where, "out")
         _want(out.is_contiguous(), where, "out must be contiguous")
     ep = None
     if lse is not None:
-        _want(lse.shape == (tokens, q_heads) and lse.dtype is torch.float32 and lse.is_contiguous() and lse.is_cuda,
-              where, "lse: a contiguous float32 CUDA tensor [tokens, q_heads]")
+        _want(lse.shape == (tokens, q_heads) and lse.dtype is torch.float32 and lse.is_contiguous() and
+              lse.device == device, where, f"lse: contiguous float32 [tokens, q_heads] on {device}")
         ep = lse.data_ptr()
     if max_tokens is None:
         max_tokens = 1 if first is None else tokens
-    _check(load_library().popcornKvAttention(out.data_ptr(), ep, q.data_ptr(), qt, qh, _type_of(q.dtype, where),
-                                             cache._ref, tp, width, fp, lp, seqs, tokens, max_tokens, q_heads, causal,
-                                             window, dim ** -0.5 if scale is None else scale,
-                                             _stream_handle(stream)), "popcornKvAttention")
+    lib = load_library()
+    code = _type_of(kind, where)
+    sizes = (code, seqs, tokens, max_tokens, q_heads)
+    need = cache._workspaces.get(sizes)
+    if need is None:
+        need = lib.popcornKvAttentionWorkspace(cache._ref, *sizes)
+        if len(cache._workspaces) < 4096:
+            cache._workspaces[sizes] = need
+    ws = cache.k.new_empty(need)  # on the current stream, like the output
+    st = lib.popcornKvAttention(out.data_ptr(), ep, q.data_ptr(), qt, qh, code, cache._ref, tp, width, fp, lp, seqs,
+                                tokens, max_tokens, q_heads, causal, window, dim ** -0.5 if scale is None else scale,
+                                ws.data_ptr() if need else None, need, _stream_on(stream, device))
+    _check(st, "popcornKvAttention")
     return out
+
+
+def moe(x, router, q_gate, s_gate, q_up, s_up, q_down, s_down, top_k: int, renormalize: bool = True, out=None,
+        routing: bool = False, stream=None):
+    """Mixture-of-experts layer for a few tokens x f32 [M, K] on int8 experts (q_gate, q_up [E, F, K], q_down
+    [E, K, F], f32 scales per output channel): each token's ``top_k`` experts by router f32 [E, K], weighted with
+    their softmax probabilities (``renormalize``: divided by their sum). Returns out [M, K]; with ``routing``
+    (out, experts int32 [M, top_k], weights f32 [M, top_k])."""
+    import torch
+
+    where = "moe"
+    device = x.device
+    (M, K), (E, F) = x.shape, s_gate.shape
+    f32, i8 = torch.float32, torch.int8
+    for name, t, shape, kind in (("x", x, (M, K), f32), ("router", router, (E, K), f32),
+                                 ("q_gate", q_gate, (E, F, K), i8), ("s_gate", s_gate, (E, F), f32),
+                                 ("q_up", q_up, (E, F, K), i8), ("s_up", s_up, (E, F), f32),
+                                 ("q_down", q_down, (E, K, F), i8), ("s_down", s_down, (E, K), f32)):
+        if t.shape != shape or t.dtype is not kind or not t.is_contiguous() or t.device != device:
+            raise ValueError(f"{where}: {name}: a contiguous {kind} {shape} on {device} wanted, "
+                             f"got {t.dtype} {tuple(t.shape)} on {t.device}")
+    _want(x.is_cuda, where, "CUDA tensors wanted")
+    if out is None:
+        out = torch.empty_like(x)
+    else:
+        _want(out.shape == (M, K) and out.dtype is f32 and out.is_contiguous() and out.device == device, where,
+              "out: contiguous float32 [M, K]")
+    experts = weights = None
+    if routing:
+        experts = x.new_empty((M, top_k), dtype=torch.int32)
+        weights = x.new_empty((M, top_k))
+    lib = load_library()
+    need = lib.popcornMoeWorkspace(M, K, F, E, top_k)
+    ws = q_gate.new_empty(need) if need else None  # on the current stream, like the output
+    st = lib.popcornMoe_i8f32(out.data_ptr(), _ptr_or_null(experts), _ptr_or_null(weights), x.data_ptr(),
+                              router.data_ptr(), q_gate.data_ptr(), s_gate.data_ptr(), q_up.data_ptr(),
+                              s_up.data_ptr(), q_down.data_ptr(), s_down.data_ptr(), M, K, F, E, top_k, renormalize,
+                              _ptr_or_null(ws), need, _stream_on(stream, device))
+    _check(st, "popcornMoe_i8f32")
+    return (out, experts, weights) if routing else out

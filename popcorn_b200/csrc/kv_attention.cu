@@ -24,8 +24,8 @@
 //    tiles pay one vote instead of a reduction. Probabilities are scaled by
 //    2^6 to keep small ones out of f16's subnormals (largest 2^15).
 //  * Values: codes become f16 exactly (byte permutes), probabilities f16 for
-//    16-bit outputs and f16 high + f16 rest for f32, products accumulate in
-//    f32. For f32 each tile's product starts from zero and is added to the
+//    bf16 outputs and f16 high + f16 rest for f16 and f32, products accumulate
+//    in f32. For f32 each tile's product starts from zero and is added to the
 //    running sum by an ordinary f32 add: the tensor cores' accumulation
 //    truncates, which over hundreds of tiles costs more than f32 should lose.
 //  * Work is the list of (sequence, row tile, key head) tasks, cut into equal
@@ -68,7 +68,7 @@ struct AttnArgs {
     int q_vec;          // query rows start on four-element boundaries
     int by_task;        // join entries are indexed by task (else by block)
     int entries;
-    int4* entry;        // [0]: number of entries; then one per task or block
+    int4* entry;        // [0]: number of entries; then two words each, per task or block
     float2* ml;         // [2 blocks][rows]: maximum, denominator
     float* part;        // [2 blocks][rows][DP]
 };
@@ -220,13 +220,21 @@ __device__ __forceinline__ float query_digits(uint32_t (&qd)[DIGITS][DP / 16], c
 
 template <typename T>
 struct Traits {
+    static constexpr int kDigits = 2;     // of a query element
+    static constexpr bool kSplit = false; // probabilities as two f16
+    static constexpr bool kFresh = false; // each tile's product summed on its own
+};
+template <>
+struct Traits<__half> {
     static constexpr int kDigits = 2;
-    static constexpr bool kExact = false;
+    static constexpr bool kSplit = true;  // one f16 would add as much error as f16 outputs have
+    static constexpr bool kFresh = false;
 };
 template <>
 struct Traits<float> {
     static constexpr int kDigits = 3;
-    static constexpr bool kExact = true;
+    static constexpr bool kSplit = true;
+    static constexpr bool kFresh = true;
 };
 
 // Joins W partial results of one row: element d of sums at stride `pitch`.
@@ -249,10 +257,10 @@ __device__ __forceinline__ void store_row(const AttnArgs& a, int64_t t, int head
 }
 
 template <typename T, int DP, int NT>
-__global__ void __launch_bounds__(kThreads, Traits<T>::kExact || NT == 2 || DP == 256 ? (DP == 256 ? 2 : 3) : 4)
+__global__ void __launch_bounds__(kThreads, Traits<T>::kFresh || NT == 2 || DP == 256 ? (DP == 256 ? 2 : 3) : 4)
 kv_rows_kernel(const AttnArgs a) {
     constexpr int DIGITS = Traits<T>::kDigits;
-    constexpr bool EXACT = Traits<T>::kExact;
+    constexpr bool SPLIT = Traits<T>::kSplit, FRESH = Traits<T>::kFresh;
     constexpr int ROWS = 8 * NT;
     constexpr int KP = DP / 64;                // 16-byte pieces of a key row per lane
     constexpr int VW = DP == 64 ? 2 : 4;       // words per piece of a value row
@@ -327,7 +335,7 @@ kv_rows_kernel(const AttnArgs a) {
             if (blockIdx.x == 0) a.entry[0] = make_int4(static_cast<int>(all_tasks), 0, 0, 0);
         } else {
             if (blockIdx.x == 0) a.entry[0] = make_int4(static_cast<int>(gridDim.x), 0, 0, 0);
-            a.entry[1 + blockIdx.x] = make_int4(0, 0, 0, 0);
+            a.entry[1 + 2 * blockIdx.x] = make_int4(0, 0, 0, 0);
         }
     }
     if (run0 >= run1) return;
@@ -351,35 +359,10 @@ kv_rows_kernel(const AttnArgs a) {
         const int h = task % a.heads, rt = task / a.heads;
         const int row_end = s.rows * a.group;
 
-        // --- query rows ------------------------------------------------------
-        uint32_t qd[NT][DIGITS][DP / 16];
-        float fac[NT][2];
-        int see0[NT][2], see1[NT][2];  // visible tokens of rows 2 t, 2 t + 1
-        #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            const int r = rt * ROWS + 8 * n + g;
-            const int tok = r / a.group, hd = r - tok * a.group;
-            const T* row = static_cast<const T*>(a.q) + (s.row0 + tok) * a.q_tok +
-                           static_cast<int64_t>(h * a.group + hd) * a.q_head;
-            const float f = query_digits<T, DP, DIGITS>(qd[n], row, r < row_end, a.dim, a.q_vec != 0, t) * a.scale_log2;
-            #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                fac[n][c] = __shfl_sync(0xffffffffu, f, 4 * (2 * t + c));
-                const int rc = rt * ROWS + 8 * n + 2 * t + c;
-                const int64_t pos = static_cast<int64_t>(s.len) - s.rows + rc / a.group;
-                see1[n][c] = a.causal ? static_cast<int>(max(pos + 1, int64_t{0})) : s.len;
-                see0[n][c] = a.window > 0 ? static_cast<int>(max(pos + 1 - a.window, int64_t{0})) : 0;
-            }
-        }
         // Tokens that every row of the tile sees: no mask inside.
         const int tok_lo = rt * ROWS / a.group, tok_hi = min(s.rows - 1, (rt * ROWS + ROWS - 1) / a.group);
         const int all1 = a.causal ? s.len - s.rows + tok_lo + 1 : s.len;
         const int64_t all0 = a.window > 0 ? static_cast<int64_t>(s.len) - s.rows + tok_hi + 1 - a.window : 0;
-
-        float o[NT][NJ][4] = {};
-        float m[NT][2], l[NT][2];
-        #pragma unroll
-        for (int n = 0; n < NT; ++n) m[n][0] = m[n][1] = -INFINITY, l[n][0] = l[n][1] = 0.0f;
 
         const int32_t* table = a.table + static_cast<int64_t>(b) * a.table_pages;
         const int last = min(u1, s.tiles);
@@ -428,6 +411,31 @@ kv_rows_kernel(const AttnArgs a) {
             load_k(tile, page);
             load_v(tile, page);
         }
+        // --- query rows ------------------------------------------------------
+        uint32_t qd[NT][DIGITS][DP / 16];
+        float fac[NT][2];
+        int see0[NT][2], see1[NT][2];  // visible tokens of rows 2 t, 2 t + 1
+        #pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const int r = rt * ROWS + 8 * n + g;
+            const int tok = r / a.group, hd = r - tok * a.group;
+            const T* row = static_cast<const T*>(a.q) + (s.row0 + tok) * a.q_tok +
+                           static_cast<int64_t>(h * a.group + hd) * a.q_head;
+            const float f = query_digits<T, DP, DIGITS>(qd[n], row, r < row_end, a.dim, a.q_vec != 0, t) * a.scale_log2;
+            #pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                fac[n][c] = __shfl_sync(0xffffffffu, f, 4 * (2 * t + c));
+                const int rc = rt * ROWS + 8 * n + 2 * t + c;
+                const int64_t pos = static_cast<int64_t>(s.len) - s.rows + rc / a.group;
+                see1[n][c] = a.causal ? static_cast<int>(max(pos + 1, int64_t{0})) : s.len;
+                see0[n][c] = a.window > 0 ? static_cast<int>(max(pos + 1 - a.window, int64_t{0})) : 0;
+            }
+        }
+        float o[NT][NJ][4] = {};
+        float m[NT][2], l[NT][2];
+        #pragma unroll
+        for (int n = 0; n < NT; ++n) m[n][0] = m[n][1] = -INFINITY, l[n][0] = l[n][1] = 0.0f;
+
         for (; tile < last; tile += kWarps) {
             page_next = checked(page_next, ok_next);
             const bool more = tile + kWarps < last;
@@ -530,7 +538,7 @@ kv_rows_kernel(const AttnArgs a) {
                 for (int r = 0; r < 2; ++r) {
                     const uint32_t top = pack_f16(e[2 * r], e[2 * r + 1]);
                     hi[n][r] = transpose8(top);
-                    if (EXACT) {
+                    if (SPLIT) {
                         const __half2 th = *reinterpret_cast<const __half2*>(&top);
                         lo[n][r] = transpose8(pack_f16(e[2 * r] - __low2float(th), e[2 * r + 1] - __high2float(th)));
                     }
@@ -555,13 +563,14 @@ kv_rows_kernel(const AttnArgs a) {
                         const int j = 2 * (VW * c + w) + i;
                         #pragma unroll
                         for (int n = 0; n < NT; ++n) {
-                            if (EXACT) {
+                            if (FRESH) {
                                 float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
                                 mma_f16_16816(d, va[i], lo[n][0], lo[n][1]);
                                 mma_f16_16816(d, va[i], hi[n][0], hi[n][1]);
                                 #pragma unroll
                                 for (int c4 = 0; c4 < 4; ++c4) o[n][j][c4] += d[c4];
                             } else {
+                                if (SPLIT) mma_f16_16816(o[n][j], va[i], lo[n][0], lo[n][1]);
                                 mma_f16_16816(o[n][j], va[i], hi[n][0], hi[n][1]);
                             }
                         }
@@ -631,31 +640,51 @@ kv_rows_kernel(const AttnArgs a) {
             const int more = static_cast<int>(owner - blockIdx.x);
             const int64_t e = a.by_task ? task0 + task : blockIdx.x;
             // (A `first` that does not ascend can make more tasks than there are.)
-            if (e < a.entries) a.entry[1 + e] = make_int4(more, b, task, blockIdx.x);
+            if (e < a.entries) {
+                a.entry[1 + 2 * e] = make_int4(more, blockIdx.x, s.row0, s.rows);
+                a.entry[2 + 2 * e] = make_int4(task, 0, 0, 0);
+            }
         }
         run0 += u1 - u0;
     }
 }
 
-// Joins the partial results of one row of one task: block 0's second slot,
+// Joins the partial results of one row of one task: block c's second slot,
 // then the first slots of the blocks after it, in that order. Four warps take
-// every fourth partial; bound by the latency of their loads.
+// every fourth partial. Bound by latency: the entry, then maxima and the first
+// four sums of each warp at once, then the output.
 template <typename T, int DP, int ROWS>
 __global__ void __launch_bounds__(kThreads) kv_join_kernel(const AttnArgs a) {
+    constexpr int PER = DP >= 128 ? DP / 128 : 1;  // float4 pieces of a sum per lane
+    constexpr int AHEAD = 4;
     __shared__ float s_top[kWarps], s_den[kWarps];
     __shared__ __align__(16) float s_o[kWarps][DP];
     pdl_launch_dependents();
     pdl_wait();
-    if (static_cast<int>(blockIdx.x) >= a.entry[0].x) return;
-    const int4 e = a.entry[1 + blockIdx.x];
-    if (e.x == 0) return;
-    const Seq s = sequence(a, e.y);
-    const int r = blockIdx.y, h = e.z % a.heads, row = e.z / a.heads * ROWS + r;
-    if (row >= s.rows * a.group) return;
+    const int entries = a.entry[0].x;
+    const int4 e = a.entry[1 + 2 * blockIdx.x];
+    const int task = a.entry[2 + 2 * blockIdx.x].x;
+    if (static_cast<int>(blockIdx.x) >= entries || e.x == 0) return;
+    const int r = blockIdx.y, h = task % a.heads, row = task / a.heads * ROWS + r;
+    if (row >= e.w * a.group) return;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int count = e.x + 1;
-    const auto slot = [&](int i) { return static_cast<int64_t>(2 * (e.w + i) + (i == 0 ? 1 : 0)) * ROWS + r; };
-
+    const auto slot = [&](int i) { return static_cast<int64_t>(2 * (e.y + i) + (i == 0 ? 1 : 0)) * ROWS + r; };
+    const auto load = [&](int i, float2& ml, float4 (&x)[PER]) {
+        ml = a.ml[slot(i)];
+        #pragma unroll
+        for (int k = 0; k < PER; ++k) {
+            const int d = 4 * (lane + 32 * k);
+            if (d < DP) x[k] = *reinterpret_cast<const float4*>(a.part + slot(i) * DP + d);
+        }
+    };
+    float2 ml[AHEAD];
+    float4 x[AHEAD][PER] = {};
+    #pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+        ml[j] = make_float2(-INFINITY, 0.0f);
+        if (warp + j * kWarps < count) load(warp + j * kWarps, ml[j], x[j]);
+    }
     float top = -INFINITY;
     for (int i = tid; i < count; i += kThreads) top = fmaxf(top, a.ml[slot(i)].x);
     #pragma unroll
@@ -665,22 +694,22 @@ __global__ void __launch_bounds__(kThreads) kv_join_kernel(const AttnArgs a) {
     #pragma unroll
     for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_top[w]);
 
-    constexpr int PER = DP >= 128 ? DP / 128 : 1;  // float4 pieces per lane
     float den = 0.0f, sum[PER][4] = {};
-    #pragma unroll 4
-    for (int i = warp; i < count; i += kWarps) {
-        const float2 ml = a.ml[slot(i)];
-        const float f = join_factor(ml.x, top);
-        den = fmaf(ml.y, f, den);
+    const auto add = [&](const float2& m, const float4 (&v)[PER]) {
+        const float f = join_factor(m.x, top);
+        den = fmaf(m.y, f, den);
         #pragma unroll
         for (int k = 0; k < PER; ++k) {
-            const int d = 4 * (lane + 32 * k);
-            if (d < DP) {
-                const float4 x = *reinterpret_cast<const float4*>(a.part + slot(i) * DP + d);
-                sum[k][0] = fmaf(x.x, f, sum[k][0]), sum[k][1] = fmaf(x.y, f, sum[k][1]);
-                sum[k][2] = fmaf(x.z, f, sum[k][2]), sum[k][3] = fmaf(x.w, f, sum[k][3]);
-            }
+            sum[k][0] = fmaf(v[k].x, f, sum[k][0]), sum[k][1] = fmaf(v[k].y, f, sum[k][1]);
+            sum[k][2] = fmaf(v[k].z, f, sum[k][2]), sum[k][3] = fmaf(v[k].w, f, sum[k][3]);
         }
+    };
+    #pragma unroll
+    for (int j = 0; j < AHEAD; ++j) add(ml[j], x[j]);
+    #pragma unroll 4
+    for (int i = warp + AHEAD * kWarps; i < count; i += kWarps) {
+        load(i, ml[0], x[0]);
+        add(ml[0], x[0]);
     }
     if (lane == 0) s_den[warp] = den;
     #pragma unroll
@@ -700,58 +729,90 @@ __global__ void __launch_bounds__(kThreads) kv_join_kernel(const AttnArgs a) {
         for (int j = 0; j < 4; ++j) o[j] += s_o[w][d + j];
     }
     const int tk = row / a.group;
-    store_row<T>(a, s.row0 + tk, h * a.group + row - tk * a.group, d, o, den, top, d == 0);
+    store_row<T>(a, e.z + tk, h * a.group + row - tk * a.group, d, o, den, top, d == 0);
 }
 
+// Work blocks of kv_rows_kernel: one wave, as many as are resident at once.
 template <typename T, int DP, int NT>
-cudaError_t launch_rows(AttnArgs a, int64_t tasks, cudaStream_t stream) {
-    constexpr int ROWS = 8 * NT;
-    // One wave: as many blocks as are resident at once.
+cudaError_t rows_grid(int64_t* grid) {
     static int resident = 0;
     int per_sm = __atomic_load_n(&resident, __ATOMIC_RELAXED);
     if (per_sm == 0) {
-        cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kv_rows_kernel<T, DP, NT>, kThreads, 0);
+        const cudaError_t e =
+            cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kv_rows_kernel<T, DP, NT>, kThreads, 0);
         if (e != cudaSuccess) return e;
         if (per_sm < 1) return cudaErrorInvalidConfiguration;
         __atomic_store_n(&resident, per_sm, __ATOMIC_RELAXED);
     }
-    const int64_t grid = static_cast<int64_t>(per_sm) * device_sm_count();
+    *grid = static_cast<int64_t>(per_sm) * device_sm_count();
+    return cudaSuccess;
+}
+
+// Launches with the caller's workspace, or only says how many bytes it takes
+// (ws_bytes != nullptr).
+template <typename T, int DP, int NT>
+cudaError_t run_rows(AttnArgs a, int64_t tasks, void* ws, int64_t* ws_bytes, cudaStream_t stream) {
+    constexpr int ROWS = 8 * NT;
+    int64_t grid = 0;
+    cudaError_t e = rows_grid<T, DP, NT>(&grid);
+    if (e != cudaSuccess) return e;
+    const int64_t entry_bytes = (1 + 2 * grid) * sizeof(int4);
+    const int64_t ml_bytes = 2 * grid * ROWS * sizeof(float2);
+    if (ws_bytes != nullptr) {
+        *ws_bytes = entry_bytes + ml_bytes + 2 * grid * ROWS * DP * sizeof(float);
+        return cudaSuccess;
+    }
     a.by_task = tasks <= grid ? 1 : 0;
     a.entries = static_cast<int>(a.by_task ? tasks : grid);
-    const size_t entry_bytes = (1 + grid) * sizeof(int4);
-    const size_t ml_bytes = ((2 * grid * ROWS * sizeof(float2)) + 15) / 16 * 16;
-    char* ws = nullptr;
-    cudaError_t e = scratch_alloc(reinterpret_cast<void**>(&ws),
-                                  entry_bytes + ml_bytes + 2 * grid * ROWS * DP * sizeof(float), stream);
-    if (e != cudaSuccess) return e;
-    a.entry = reinterpret_cast<int4*>(ws);
-    a.ml = reinterpret_cast<float2*>(ws + entry_bytes);
-    a.part = reinterpret_cast<float*>(ws + entry_bytes + ml_bytes);
+    a.entry = static_cast<int4*>(ws);
+    a.ml = reinterpret_cast<float2*>(static_cast<char*>(ws) + entry_bytes);
+    a.part = reinterpret_cast<float*>(static_cast<char*>(ws) + entry_bytes + ml_bytes);
     cudaLaunchAttribute attr[1];
     cudaLaunchConfig_t cfg = pdl_config(dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, stream, attr);
     e = cudaLaunchKernelEx(&cfg, kv_rows_kernel<T, DP, NT>, a);
-    if (e == cudaSuccess) {
-        cfg.gridDim = dim3(static_cast<unsigned>(a.entries), ROWS);
-        e = cudaLaunchKernelEx(&cfg, kv_join_kernel<T, DP, ROWS>, a);
-    }
-    const cudaError_t f = scratch_free(ws, stream);
-    return e != cudaSuccess ? e : f;
+    if (e != cudaSuccess) return e;
+    cfg.gridDim = dim3(static_cast<unsigned>(a.entries), ROWS);
+    return cudaLaunchKernelEx(&cfg, kv_join_kernel<T, DP, ROWS>, a);
 }
 
 template <typename T>
-cudaError_t launch_attention(const AttnArgs& a, int64_t max_tokens, cudaStream_t stream) {
+cudaError_t run_attention(const AttnArgs& a, int64_t max_tokens, void* ws, int64_t* ws_bytes, cudaStream_t stream) {
     // Tasks of at most 8 or 16 query rows; an upper bound of their number.
-    const bool two = !Traits<T>::kExact && a.dim <= 128 && max_tokens * a.group > 8;
+    const bool two = !Traits<T>::kFresh && a.dim <= 128 && max_tokens * a.group > 8;
     const int rows = two ? 16 : 8;
     const int64_t tasks = a.heads * (static_cast<int64_t>(a.tokens) * a.group / rows + a.seqs);
-    if (two) {
-        if constexpr (!Traits<T>::kExact) {
-            return a.dim <= 64 ? launch_rows<T, 64, 2>(a, tasks, stream) : launch_rows<T, 128, 2>(a, tasks, stream);
-        }
+    if constexpr (!Traits<T>::kFresh) {
+        if (two && a.dim <= 64) return run_rows<T, 64, 2>(a, tasks, ws, ws_bytes, stream);
+        if (two) return run_rows<T, 128, 2>(a, tasks, ws, ws_bytes, stream);
     }
-    if (a.dim <= 64) return launch_rows<T, 64, 1>(a, tasks, stream);
-    if (a.dim <= 128) return launch_rows<T, 128, 1>(a, tasks, stream);
-    return launch_rows<T, 256, 1>(a, tasks, stream);
+    if (a.dim <= 64) return run_rows<T, 64, 1>(a, tasks, ws, ws_bytes, stream);
+    if (a.dim <= 128) return run_rows<T, 128, 1>(a, tasks, ws, ws_bytes, stream);
+    return run_rows<T, 256, 1>(a, tasks, ws, ws_bytes, stream);
+}
+
+cudaError_t run_typed(popcornType_t type, const AttnArgs& a, int64_t max_tokens, void* ws, int64_t* ws_bytes,
+                      cudaStream_t stream) {
+    switch (type) {
+        case POPCORN_TYPE_F32: return run_attention<float>(a, max_tokens, ws, ws_bytes, stream);
+        case POPCORN_TYPE_F16: return run_attention<__half>(a, max_tokens, ws, ws_bytes, stream);
+        default: return run_attention<__nv_bfloat16>(a, max_tokens, ws, ws_bytes, stream);
+    }
+}
+
+// Argument checks that the workspace query shares with the call.
+bool attention_supported(const popcornKvCache_t& c, popcornType_t type, int64_t seqs, int64_t tokens,
+                         int64_t max_tokens, int64_t q_heads) {
+    return kv_cache_supported(c) && kv_type_supported(type) && q_heads > 0 && q_heads <= 65535 &&
+           q_heads % c.heads == 0 && max_tokens > 0 && seqs <= INT32_MAX / 2 && tokens <= INT32_MAX / q_heads;
+}
+
+AttnArgs attention_sizes(const popcornKvCache_t& c, int64_t seqs, int64_t tokens, int64_t q_heads) {
+    AttnArgs a = {};
+    a.pages = c.pages;
+    a.seqs = static_cast<int>(seqs), a.tokens = static_cast<int>(tokens);
+    a.heads = static_cast<int>(c.heads), a.group = static_cast<int>(q_heads / c.heads);
+    a.dim = static_cast<int>(c.dim), a.page_shift = log2_of(c.page_size);
+    return a;
 }
 
 }  // namespace
@@ -765,43 +826,58 @@ cudaError_t kv_attention_take_errors(unsigned int* bits) {
 
 }  // namespace pcb
 
+extern "C" int64_t popcornKvAttentionWorkspace(const popcornKvCache_t* cache, popcornType_t type, int64_t seqs,
+                                               int64_t tokens, int64_t max_tokens, int64_t q_heads) {
+    if (cache == nullptr || seqs <= 0 || tokens <= 0 ||
+        !pcb::attention_supported(*cache, type, seqs, tokens, max_tokens, q_heads)) {
+        return 0;
+    }
+    int64_t bytes = 0;
+    const pcb::AttnArgs a = pcb::attention_sizes(*cache, seqs, tokens, q_heads);
+    const cudaError_t e = pcb::run_typed(type, a, max_tokens, nullptr, &bytes, nullptr);
+    return pcb::record_cuda(e) == POPCORN_SUCCESS ? bytes : 0;
+}
+
 extern "C" popcornStatus_t popcornKvAttention(void* out, float* lse, const void* q, int64_t q_token_stride,
                                               int64_t q_head_stride, popcornType_t type, const popcornKvCache_t* cache,
                                               const int32_t* table, int64_t table_pages, const int32_t* first,
                                               const int32_t* length, int64_t seqs, int64_t tokens, int64_t max_tokens,
                                               int64_t q_heads, int causal, int64_t window, float scale,
-                                              cudaStream_t stream) {
+                                              void* workspace, int64_t workspace_bytes, cudaStream_t stream) {
     if (out == nullptr || q == nullptr || cache == nullptr || cache->k == nullptr || cache->v == nullptr ||
         cache->k_scale == nullptr || cache->v_scale == nullptr || table == nullptr || length == nullptr) {
         return POPCORN_ERROR_INVALID_VALUE;
     }
     if (seqs <= 0 || tokens <= 0) return POPCORN_SUCCESS;
-    if (!pcb::kv_cache_supported(*cache) || !pcb::kv_type_supported(type) || table_pages <= 0 || q_heads <= 0 ||
-        q_heads % cache->heads != 0 || q_heads > 65535 || max_tokens <= 0 || !pcb::aligned16(out)) {
-        return POPCORN_ERROR_INVALID_VALUE;
-    }
     // Positions and row counts are 32-bit inside a sequence.
-    if ((first == nullptr && tokens != seqs) || seqs > INT32_MAX / 2 || tokens > INT32_MAX / q_heads ||
-        table_pages > (INT32_MAX - 64) / cache->page_size) {
+    if (!pcb::attention_supported(*cache, type, seqs, tokens, max_tokens, q_heads) || table_pages <= 0 ||
+        table_pages > (INT32_MAX - 64) / cache->page_size || !pcb::aligned16(out) ||
+        (first == nullptr && tokens != seqs)) {
         return POPCORN_ERROR_INVALID_VALUE;
     }
-    pcb::AttnArgs a = {};
+    pcb::AttnArgs a = pcb::attention_sizes(*cache, seqs, tokens, q_heads);
     a.out = out, a.lse = lse, a.q = q, a.q_tok = q_token_stride, a.q_head = q_head_stride;
     a.k = cache->k, a.v = cache->v, a.ks = cache->k_scale, a.vs = cache->v_scale;
     a.table = table, a.first = first, a.length = length;
-    a.table_pages = table_pages, a.pages = cache->pages, a.window = window;
-    a.seqs = static_cast<int>(seqs), a.tokens = static_cast<int>(tokens);
-    a.heads = static_cast<int>(cache->heads), a.group = static_cast<int>(q_heads / cache->heads);
-    a.dim = static_cast<int>(cache->dim), a.page_shift = pcb::log2_of(cache->page_size);
-    a.causal = causal;
+    a.table_pages = table_pages, a.window = window, a.causal = causal;
     a.scale_log2 = scale * 1.4426950408889634f;
     const int64_t four = 4 * pcb::kv_type_size(type);
     a.q_vec = reinterpret_cast<uintptr_t>(q) % four == 0 && q_token_stride % 4 == 0 && q_head_stride % 4 == 0;
-    cudaError_t e;
-    switch (type) {
-        case POPCORN_TYPE_F32: e = pcb::launch_attention<float>(a, max_tokens, stream); break;
-        case POPCORN_TYPE_F16: e = pcb::launch_attention<__half>(a, max_tokens, stream); break;
-        default: e = pcb::launch_attention<__nv_bfloat16>(a, max_tokens, stream); break;
+
+    int64_t need = 0;
+    cudaError_t e = pcb::run_typed(type, a, max_tokens, nullptr, &need, stream);
+    if (e != cudaSuccess) return pcb::record_cuda(e);
+    void* ws = workspace;
+    if (workspace == nullptr) {
+        e = pcb::scratch_alloc(&ws, static_cast<size_t>(need), stream);
+        if (e != cudaSuccess) return pcb::record_cuda(e);
+    } else if (workspace_bytes < need || !pcb::aligned16(workspace)) {
+        return POPCORN_ERROR_INVALID_VALUE;
+    }
+    e = pcb::run_typed(type, a, max_tokens, ws, nullptr, stream);
+    if (workspace == nullptr) {
+        const cudaError_t f = pcb::scratch_free(ws, stream);
+        if (e == cudaSuccess) e = f;
     }
     if (e != cudaSuccess) return pcb::record_cuda(e);
     return pcb::check_launch();

@@ -41,36 +41,51 @@ struct AppendArgs {
     int q_parts;         // blocks per query token
 };
 
-// Elements 4 i .. 4 i + 3 of a row, rotated (rot > 0) by the row's cos / sin.
-// Products and sums are rounded one by one so that a restatement in separate
-// f32 operations gives the same bits.
+// A row of dim elements in units that rotate by themselves: with the halves
+// paired, unit u < rot / 8 is the two groups of four 4 u and 4 u + rot / 2,
+// the units after it are single groups; with neighbours paired (or without
+// rotation) every unit is a single group. Element index of a unit's first
+// group, and whether it has a second one (at + rot / 2).
+struct Unit {
+    int at;
+    bool pair;
+};
+__device__ __forceinline__ Unit unit_of(int u, int rot, bool interleaved) {
+    if (interleaved || u >= (rot >> 3)) return {4 * (interleaved ? u : u + (rot >> 3)), false};
+    return {4 * u, true};
+}
+
+// A unit's elements, rotated by the row's cos / sin. Products and sums are
+// rounded one by one so that a restatement in separate f32 operations gives
+// the same bits.
 template <typename T>
-__device__ __forceinline__ void rotated4(const T* row, int i, int rot, bool interleaved, const float* cos,
-                                         const float* sin, bool vec, float (&v)[4]) {
-    const int d = 4 * i;
-    load4(row + d, vec, v);
-    if (d >= rot) return;
-    const int half = rot >> 1;
-    if (interleaved) {
+__device__ __forceinline__ void load_unit(const T* row, Unit u, int rot, bool vec, float (&v)[8]) {
+    float lo[4], hi[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    load4(row + u.at, vec, lo);
+    if (u.pair) load4(row + u.at + (rot >> 1), vec, hi);
+    #pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = lo[j], v[4 + j] = hi[j];
+}
+__device__ __forceinline__ void turn_unit(Unit u, int rot, const float* cos, const float* sin, bool vec,
+                                          float (&v)[8]) {
+    if (u.pair) {
+        float c[4], s[4];
+        load4(cos + u.at, vec, c);
+        load4(sin + u.at, vec, s);
+        #pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float a = v[j], b = v[4 + j];
+            v[j] = __fsub_rn(__fmul_rn(a, c[j]), __fmul_rn(b, s[j]));
+            v[4 + j] = __fadd_rn(__fmul_rn(b, c[j]), __fmul_rn(a, s[j]));
+        }
+    } else if (u.at < rot) {  // neighbours paired
         #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            const float c = cos[2 * i + j], s = sin[2 * i + j];
+            const float c = cos[(u.at >> 1) + j], s = sin[(u.at >> 1) + j];
             const float a = v[2 * j], b = v[2 * j + 1];
             v[2 * j] = __fsub_rn(__fmul_rn(a, c), __fmul_rn(b, s));
             v[2 * j + 1] = __fadd_rn(__fmul_rn(b, c), __fmul_rn(a, s));
         }
-        return;
-    }
-    const bool low = d < half;
-    const int k = low ? d : d - half;
-    float p[4], c[4], s[4];
-    load4(row + (low ? d + half : d - half), vec, p);
-    load4(cos + k, vec, c);
-    load4(sin + k, vec, s);
-    #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const float own = __fmul_rn(v[j], c[j]), other = __fmul_rn(p[j], s[j]);
-        v[j] = low ? __fsub_rn(own, other) : __fadd_rn(own, other);
     }
 }
 
@@ -78,25 +93,41 @@ __device__ __forceinline__ int encode(float x, float s) {
     // rint of the quotient, clamped; NaN (0 / 0, inf / inf) becomes 0.
     return s > 0.0f ? max(-128, min(127, __float2int_rn(__fdiv_rn(x, s)))) : 0;
 }
+__device__ __forceinline__ uint32_t encode4(const float* v, float s) {
+    uint32_t r = 0;
+    #pragma unroll
+    for (int j = 0; j < 4; ++j) r |= (static_cast<uint32_t>(encode(v[j], s)) & 0xffu) << (8 * j);
+    return r;
+}
 
 // THREADS threads per block: the first half works on keys, the second on
-// values. CQ: 4-element groups of the new rows that a thread keeps in
-// registers between the maximum and the encoding; what does not fit is read
-// (from L1 or L2) and rotated again. Decode (few new rows a block) runs one
-// warp for each half, prompts four.
-template <typename T, int THREADS, int CQ>
-__global__ void __launch_bounds__(THREADS) append_kernel(const AppendArgs a) {
+// values. CU: units of the new rows that a thread keeps in registers between
+// the maximum and the encoding; what does not fit is read (from L1 or L2) and
+// rotated again. Decode (few new rows a block) runs one warp for each half,
+// prompts four.
+template <typename T, int THREADS, int CU>
+__global__ void __launch_bounds__(THREADS, THREADS == 64 ? 12 : 4) append_kernel(const AppendArgs a) {
     constexpr int H = THREADS / 2;
     __shared__ float part[THREADS / 32];
     pdl_launch_dependents();
     pdl_wait();
     const int tid = threadIdx.x, lane = tid & 31;
-    const bool vec = a.vec != 0;
-    const int quads = a.dim >> 2;
+    const bool vec = a.vec != 0, inter = a.interleaved != 0;
+    const int q_units = a.dim / 4 - (inter ? 0 : a.rot >> 3);
 
     if (blockIdx.x >= a.blocks) {  // queries: one token's heads, split over q_parts blocks
         const int64_t qb = blockIdx.x - a.blocks;
         const int64_t t = qb / a.q_parts;
+        const int part_i = static_cast<int>(qb % a.q_parts);
+        const int total = a.q_heads * q_units;
+        const T* q = static_cast<const T*>(a.q) + t * a.q_tok;
+        T* o = static_cast<T*>(a.q_out) + t * a.q_heads * a.dim;
+        float v[2][8];
+        #pragma unroll
+        for (int u = 0; u < 2; ++u) {  // the rows first: their loads need no position
+            const int i = (part_i * 2 + u) * THREADS + tid, h = i / q_units;
+            if (i < total) load_unit(q + h * a.q_head, unit_of(i - h * q_units, a.rot, inter), a.rot, vec, v[u]);
+        }
         const int64_t b = a.first ? sequence_of(a.first, a.seqs, t, lane) : t;
         if (b >= a.seqs) return;
         const int64_t pos = a.start[b] + (a.first ? t - a.first[b] : 0);
@@ -104,34 +135,15 @@ __global__ void __launch_bounds__(THREADS) append_kernel(const AppendArgs a) {
             if (tid == 0) atomicOr(&g_kv_err, kKvErrAppend);
             return;
         }
-        const float* cos = a.cos + pos * (a.rot >> 1);
-        const float* sin = a.sin + pos * (a.rot >> 1);
-        const int total = a.q_heads * quads;
-        const T* q = static_cast<const T*>(a.q) + t * a.q_tok;
-        T* o = static_cast<T*>(a.q_out) + t * a.q_heads * a.dim;
-        // A rotated pair's two halves may lie in different threads, and q_out
-        // may be q: each batch of heads is read whole, then written.
-        const int part_i = static_cast<int>(qb % a.q_parts);
-        const int heads_each = (a.q_heads + a.q_parts - 1) / a.q_parts;
-        const int lo = part_i * heads_each * quads, hi = min(total, lo + heads_each * quads);
-        const int step = max(1, (THREADS * 4) / quads) * quads;  // whole heads
-        for (int base = lo; base < hi; base += step) {
-            const int end = min(hi, base + step);
-            float v[4][4];
-            #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const int i = base + tid + u * THREADS;
-                if (i < end) {
-                    const int h = i / quads;
-                    rotated4(q + h * a.q_head, i - h * quads, a.rot, a.interleaved != 0, cos, sin, vec, v[u]);
-                }
-            }
-            __syncthreads();
-            #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const int i = base + tid + u * THREADS;
-                if (i < end) store4(o + 4 * i, a.q_vec != 0, v[u]);
-            }
+        #pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int i = (part_i * 2 + u) * THREADS + tid, h = i / q_units;
+            if (i >= total) break;
+            const Unit un = unit_of(i - h * q_units, a.rot, inter);
+            turn_unit(un, a.rot, a.cos + pos * (a.rot >> 1), a.sin + pos * (a.rot >> 1), vec, v[u]);
+            const float lo[4] = {v[u][0], v[u][1], v[u][2], v[u][3]}, hi[4] = {v[u][4], v[u][5], v[u][6], v[u][7]};
+            store4(o + h * a.dim + un.at, a.q_vec != 0, lo);
+            if (un.pair) store4(o + h * a.dim + un.at + (a.rot >> 1), a.q_vec != 0, hi);
         }
         return;
     }
@@ -142,6 +154,7 @@ __global__ void __launch_bounds__(THREADS) append_kernel(const AppendArgs a) {
     const int64_t t_end = min(a.tokens, (slot + 1) * a.chunk);
     const T* x = static_cast<const T*>(a.x[kv]) + h * a.head[kv];
     const int rot = kv == 0 ? a.rot : 0;
+    const int units = kv == 0 ? q_units : a.dim >> 2;
     const int page_size = 1 << a.page_shift;
 
     for (int64_t t = slot * a.chunk; t < t_end;) {
@@ -171,28 +184,36 @@ __global__ void __launch_bounds__(THREADS) append_kernel(const AppendArgs a) {
         const int64_t block = page * a.heads + h;
         int8_t* codes = a.codes[kv] + (block << a.page_shift) * a.dim;
         const float old = row == 0 ? 0.0f : a.scale[kv][block];
-        const int total = n * quads;
+        const int total = n * units;
 
-        float v[CQ][4];
+        const auto rotated = [&](int i, Unit& un, float (&v)[8]) {  // returns the element index in the block
+            const int r = i / units;
+            un = unit_of(i - r * units, rot, inter);
+            load_unit(x + (t + r) * a.tok[kv], un, rot, vec, v);
+            if (rot > 0) turn_unit(un, rot, a.cos + (pos + r) * (rot >> 1), a.sin + (pos + r) * (rot >> 1), vec, v);
+            return (row + r) * a.dim + un.at;
+        };
+        const auto put = [&](int e, Unit un, const float (&v)[8], float s) {
+            *reinterpret_cast<uint32_t*>(codes + e) = encode4(v, s);
+            if (un.pair) *reinterpret_cast<uint32_t*>(codes + e + (rot >> 1)) = encode4(v + 4, s);
+        };
+        float v[CU][8];
         float m = 0.0f;
         #pragma unroll
-        for (int u = 0; u < CQ; ++u) {
-            const int i = ht + u * H;
-            if (i < total) {
-                const int r = i / quads;
-                rotated4(x + (t + r) * a.tok[kv], i - r * quads, rot, a.interleaved != 0,
-                         a.cos + (pos + r) * (a.rot >> 1), a.sin + (pos + r) * (a.rot >> 1), vec, v[u]);
+        for (int u = 0; u < CU; ++u) {
+            Unit un;
+            if (ht + u * H < total) {
+                rotated(ht + u * H, un, v[u]);
                 #pragma unroll
-                for (int j = 0; j < 4; ++j) m = fmaxf(m, fabsf(v[u][j]));
+                for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(v[u][j]));  // (a single group's rest is zero)
             }
         }
-        for (int i = ht + CQ * H; i < total; i += H) {
-            const int r = i / quads;
-            float w[4];
-            rotated4(x + (t + r) * a.tok[kv], i - r * quads, rot, a.interleaved != 0,
-                     a.cos + (pos + r) * (a.rot >> 1), a.sin + (pos + r) * (a.rot >> 1), vec, w);
+        for (int i = ht + CU * H; i < total; i += H) {
+            Unit un;
+            float w[8];
+            rotated(i, un, w);
             #pragma unroll
-            for (int j = 0; j < 4; ++j) m = fmaxf(m, fabsf(w[j]));
+            for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(w[j]));
         }
         // |x| as an unsigned integer keeps its order (no NaN: fmaxf dropped them).
         m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));
@@ -226,26 +247,20 @@ __global__ void __launch_bounds__(THREADS) append_kernel(const AppendArgs a) {
                 w[i] = c;
             }
         }
-        uint32_t* w = reinterpret_cast<uint32_t*>(codes + row * a.dim);
         #pragma unroll
-        for (int u = 0; u < CQ; ++u) {
+        for (int u = 0; u < CU; ++u) {
             const int i = ht + u * H;
             if (i < total) {
-                uint32_t r = 0;
-                #pragma unroll
-                for (int j = 0; j < 4; ++j) r |= (static_cast<uint32_t>(encode(v[u][j], s)) & 0xffu) << (8 * j);
-                w[i] = r;
+                const int r = i / units;
+                const Unit un = unit_of(i - r * units, rot, inter);
+                put((row + r) * a.dim + un.at, un, v[u], s);
             }
         }
-        for (int i = ht + CQ * H; i < total; i += H) {
-            const int r = i / quads;
-            float f[4];
-            rotated4(x + (t + r) * a.tok[kv], i - r * quads, rot, a.interleaved != 0,
-                     a.cos + (pos + r) * (a.rot >> 1), a.sin + (pos + r) * (a.rot >> 1), vec, f);
-            uint32_t c = 0;
-            #pragma unroll
-            for (int j = 0; j < 4; ++j) c |= (static_cast<uint32_t>(encode(f[j], s)) & 0xffu) << (8 * j);
-            w[i] = c;
+        for (int i = ht + CU * H; i < total; i += H) {
+            Unit un;
+            float w[8];
+            const int e = rotated(i, un, w);
+            put(e, un, w, s);
         }
         __syncwarp();  // every lane has read the old scale
         if (ht == 0 && (row == 0 || s != old)) a.scale[kv][block] = s;
@@ -297,8 +312,8 @@ cudaError_t launch_append(const AppendArgs& a, bool few, cudaStream_t stream) {
     if (grid > INT32_MAX) return cudaErrorInvalidConfiguration;
     cudaLaunchAttribute attr[1];
     const cudaLaunchConfig_t cfg = pdl_config(dim3(static_cast<unsigned>(grid)), dim3(threads), 0, stream, attr);
-    return few ? cudaLaunchKernelEx(&cfg, append_kernel<T, 64, 4>, a)
-               : cudaLaunchKernelEx(&cfg, append_kernel<T, 256, 16>, a);
+    return few ? cudaLaunchKernelEx(&cfg, append_kernel<T, 64, 2>, a)
+               : cudaLaunchKernelEx(&cfg, append_kernel<T, 256, 4>, a);
 }
 
 template <typename T>
@@ -380,15 +395,17 @@ extern "C" popcornStatus_t popcornKvAppend(const popcornKvCache_t* cache, const 
     a.vec = vec ? 1 : 0;
     a.q_vec = pcb::aligned_to(q_out, four) ? 1 : 0;
 
-    // A slot covers as many tokens as a sequence brings on average, up to a
-    // page: at decode every token is its own slot, so that blocks of different
-    // sequences run side by side; at prompts a slot holds about one block.
+    // A slot's blocks are worked on one after the other. At prompts (a page of
+    // tokens a sequence and more) a slot of a page's length holds about one
+    // block; below, slots of a quarter of a sequence's tokens keep blocks of
+    // different sequences side by side, at decode each token is its own slot.
     const int64_t each = tokens / seqs;
-    a.chunk = static_cast<int>(each < 1 ? 1 : each > cache->page_size ? cache->page_size : each);
+    a.chunk = static_cast<int>(each >= cache->page_size ? cache->page_size : each < 8 ? 1 : each / 4);
     const bool few = each < 8;
     a.blocks = pcb::ceil_div(tokens, a.chunk) * cache->heads;
     const int threads = few ? 64 : 256;
-    a.q_parts = static_cast<int>(q != nullptr ? pcb::ceil_div(q_heads * (cache->dim / 4), threads * 4) : 1);
+    const int64_t units = cache->dim / 4 - (interleaved ? 0 : a.rot / 8);
+    a.q_parts = static_cast<int>(q != nullptr ? pcb::ceil_div(q_heads * units, threads * 2) : 1);
 
     cudaError_t e;
     switch (type) {

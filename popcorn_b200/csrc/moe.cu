@@ -1,0 +1,691 @@
+// A mixture-of-experts layer for a few tokens on per-channel int8 experts:
+//   z = x Wr^T,  p = softmax(z),  the top_k largest p of each token,
+//   out[m] = sum over its experts e of p'_e * (silu(x Wg_e^T) * (x Wu_e^T)) Wd_e^T.
+// What it cannot do without is one read of the chosen experts' codes, 3 K F
+// bytes each; it is bound by HBM. Three launches, overlapped by programmatic
+// dependent launch:
+//  1. route_kernel: the logits, one block per expert and eight tokens, and the
+//     activations as fixed point.
+//  2. up_kernel: every block picks the experts itself from the logits (a few
+//     KB, cheaper than a launch), then walks over (chosen expert, 32 rows of
+//     gate and of up) items and writes silu(g) u as fixed point.
+//  3. down_kernel: a block owns 16 output channels and goes through all chosen
+//     experts, so that a token's sum over its experts needs no other block.
+//
+// Products. mma s8 x s8 -> s32 with the codes as they are: 16 weight rows are
+// the M side; the eight columns of the N side are two tokens times the four
+// balanced base-256 digits of 30-bit fixed point. Sums are exact integers and
+// join in double or f32, so the result's error is f32 rounding. The operands
+// come from global memory in 16-byte loads without shared memory: columns of
+// the product may be taken in any order, so lane (g, t) = (lane / 4, lane % 4)
+// takes piece t of each 64-column window, the words of which feed two 32-deep
+// steps. The activations' fixed point has one power of two per token, the
+// hidden values' one for each 32 rows that an item covers: columns
+// 64 w + 16 t + 8 s + i (t < 4, i < 8), which are the columns of step s of
+// window w in the next product.
+#include <cmath>
+
+#include "common.cuh"
+#include "mma_frag.cuh"
+#include "popcorn_serve.h"
+
+namespace pcb {
+namespace {
+
+constexpr int kMoeThreads = 256;
+constexpr int kMoeWarps = kMoeThreads / 32;
+constexpr int kMoeTokens = 64;    // tokens of one pass
+constexpr int kMoeExperts = 256;
+constexpr int kMoeTop = 16;
+constexpr int kMagicBits = 0x4B400000;   // 1.5 2^23 as f32
+constexpr float kMagic = 12582912.0f;
+
+struct MoeArgs {
+    float* out;
+    int* experts;      // [M, top]
+    float* weights;    // [M, top]
+    const float* x;
+    const float* router;
+    const int8_t* qg;
+    const float* sg;
+    const int8_t* qu;
+    const float* su;
+    const int8_t* qd;
+    const float* sd;
+    float* logits;     // [M, E]
+    int8_t* xd;        // [M][4][kp] digits of x
+    float* xs;         // [M] its unit
+    int8_t* hd;        // [M top][4][fp] digits of the hidden values
+    float* hs;         // [M top][fp / 32] their units
+    float* h;          // [M top][F] hidden values (plain kernels only)
+    int M, K, F, E, top, renorm, kp, fp;
+};
+
+__device__ __forceinline__ uint4 load_stream(const int8_t* p, bool ok) {
+    uint4 v;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %5, 0;\n\t"
+        "mov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\tmov.b32 %3, 0;\n\t"
+        "@p ld.global.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];\n\t}"
+        : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w)
+        : "l"(p), "r"(static_cast<int>(ok)));
+    return v;
+}
+
+// Fixed point of values up to m in magnitude: 2^s brings m to [2^29, 2^30)
+// (as two factors, since s goes up to 149, where the unit 2^-s is f32's
+// smallest number). Zero gives digits 0; a non-finite m digits 0 and unit NaN.
+struct Fixed {
+    float up, more, unit;
+};
+__device__ __forceinline__ Fixed fixed_for(float m, bool bad) {
+    if (bad) return {0.0f, 0.0f, __int_as_float(0x7fffffff)};
+    const int s = max(-98, min(149, 29 + 127 - static_cast<int>(__float_as_uint(m) >> 23)));
+    const int s0 = min(s, 126);
+    return {__int_as_float((127 + s0) << 23), __int_as_float((127 + s - s0) << 23), ldexpf(1.0f, -s)};
+}
+// The four balanced digits of v, lowest byte first.
+__device__ __forceinline__ uint32_t digits_of(float v, const Fixed& f) {
+    return (static_cast<uint32_t>(__float2int_rn(v * f.up * f.more)) + 0x80808080u) ^ 0x80808080u;
+}
+__device__ __forceinline__ bool not_finite(float v) { return !(fabsf(v) <= 3.4028234663852886e38f); }
+
+// ------------------------------------------------------------------ routing
+// Block e < E: logits of expert e for tokens 8 y .. 8 y + 7. Blocks behind
+// them (y = 0): the digits of one token each.
+__global__ void __launch_bounds__(128) route_kernel(const MoeArgs a) {
+    __shared__ float part[4][8];
+    __shared__ int s_bad;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    pdl_launch_dependents();
+    const int e = blockIdx.x;
+    if (e < a.E && blockIdx.y == 0 && tid < 4) {
+        prefetch_l2_range(a.router + static_cast<int64_t>(e) * a.K, 4LL * a.K, tid, 4);
+    }
+    pdl_wait();
+    if (e >= a.E) {
+        const int m = e - a.E;
+        if (blockIdx.y != 0 || a.xd == nullptr) return;
+        const float* x = a.x + static_cast<int64_t>(m) * a.K;
+        float top = 0.0f;
+        bool bad = false;
+        for (int k = tid; k < a.K; k += 128) {
+            const float v = x[k];
+            top = fmaxf(top, fabsf(v));
+            bad = bad || not_finite(v);
+        }
+        if (tid == 0) s_bad = 0;
+        top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+        if (lane == 0) part[warp][0] = top;
+        __syncthreads();
+        if (bad) s_bad = 1;
+        __syncthreads();
+        #pragma unroll
+        for (int w = 0; w < 4; ++w) top = fmaxf(top, part[w][0]);
+        const Fixed f = fixed_for(top, s_bad != 0);
+        int8_t* d = a.xd + static_cast<int64_t>(m) * 4 * a.kp;
+        for (int k = 4 * tid; k < a.kp; k += 512) {
+            uint32_t y[4];
+            #pragma unroll
+            for (int j = 0; j < 4; ++j) y[j] = k < a.K && f.up != 0.0f ? digits_of(x[k + j], f) : 0u;
+            #pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t sel = static_cast<uint32_t>(i | ((i + 4) << 4));
+                *reinterpret_cast<uint32_t*>(d + static_cast<int64_t>(i) * a.kp + k) =
+                    __byte_perm(__byte_perm(y[0], y[1], sel), __byte_perm(y[2], y[3], sel), 0x5410);
+            }
+        }
+        if (tid == 0) a.xs[m] = f.unit;
+        return;
+    }
+    const float* w = a.router + static_cast<int64_t>(e) * a.K;
+    const int m0 = blockIdx.y * 8;
+    const int n = min(8, a.M - m0);
+    const float* x = a.x + static_cast<int64_t>(m0) * a.K;
+    float acc[8] = {};
+    if (a.K % 4 == 0 && ((reinterpret_cast<uintptr_t>(a.router) | reinterpret_cast<uintptr_t>(a.x)) & 15u) == 0) {
+        #pragma unroll 4
+        for (int k = 4 * tid; k < a.K; k += 512) {
+            const float4 r = *reinterpret_cast<const float4*>(w + k);
+            #pragma unroll
+            for (int m = 0; m < 8; ++m) {
+                if (m < n) {
+                    const float4 v = *reinterpret_cast<const float4*>(x + static_cast<int64_t>(m) * a.K + k);
+                    acc[m] = fmaf(r.x, v.x, fmaf(r.y, v.y, fmaf(r.z, v.z, fmaf(r.w, v.w, acc[m]))));
+                }
+            }
+        }
+    } else {
+        for (int k = tid; k < a.K; k += 128) {
+            #pragma unroll
+            for (int m = 0; m < 8; ++m) {
+                if (m < n) acc[m] = fmaf(w[k], x[static_cast<int64_t>(m) * a.K + k], acc[m]);
+            }
+        }
+    }
+    #pragma unroll
+    for (int m = 0; m < 8; ++m) {
+        #pragma unroll
+        for (int o = 16; o > 0; o >>= 1) acc[m] += __shfl_xor_sync(0xffffffffu, acc[m], o);
+        if (lane == 0) part[warp][m] = acc[m];
+    }
+    __syncthreads();
+    if (tid < n) {
+        a.logits[static_cast<int64_t>(m0 + tid) * a.E + e] = part[0][tid] + part[1][tid] + part[2][tid] + part[3][tid];
+    }
+}
+
+// What a block knows of the routing: for each chosen expert the tokens that
+// picked it, as bits.
+struct Routing {
+    unsigned int tokens[kMoeExperts][2];
+    short active[kMoeExperts];
+    int count;
+    short pick[kMoeTokens * kMoeTop];
+    float weight[kMoeTokens * kMoeTop];
+};
+
+// One warp: token m's experts. Softmax over all logits; the top ones by
+// repeated maxima, the lowest index first among equals. NaN logits count as
+// -inf. Writes pick and weight.
+__device__ void pick_experts(const MoeArgs& a, int m, Routing& r, int lane) {
+    constexpr int PER = kMoeExperts / 32;
+    float z[PER];
+    float top = -INFINITY;
+    #pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int e = lane + 32 * i;
+        z[i] = e < a.E ? a.logits[static_cast<int64_t>(m) * a.E + e] : -INFINITY;
+        top = fmaxf(top, z[i]);
+    }
+    #pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    float sum = 0.0f;
+    #pragma unroll
+    for (int i = 0; i < PER; ++i) sum += lane + 32 * i < a.E ? expf(z[i] - top) : 0.0f;
+    #pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    unsigned int taken = 0;  // bit i: z[i] has been picked
+    float mine = 0.0f;       // lane j: probability of pick j
+    int mine_e = 0;
+    float picked = 0.0f;
+    for (int j = 0; j < a.top; ++j) {
+        float best = -INFINITY;
+        int at = kMoeExperts;
+        #pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int e = lane + 32 * i;
+            const bool open = e < a.E && !(taken >> i & 1u);
+            if (open && (at == kMoeExperts || z[i] > best)) best = z[i] == z[i] ? z[i] : -INFINITY, at = e;
+        }
+        #pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            const float ob = __shfl_xor_sync(0xffffffffu, best, o);
+            const int oa = __shfl_xor_sync(0xffffffffu, at, o);
+            if (ob > best || (ob == best && oa < at)) best = ob, at = oa;
+        }
+        if ((at & 31) == lane) taken |= 1u << (at >> 5);
+        const float p = expf(best - top) / sum;
+        picked += p;
+        if (lane == j) mine = p, mine_e = at;
+    }
+    if (lane < a.top) {
+        r.pick[m * a.top + lane] = static_cast<short>(mine_e);
+        r.weight[m * a.top + lane] = a.renorm ? mine / picked : mine;
+    }
+}
+
+// The block's view of picks already in r.pick: token bits and active experts.
+__device__ void list_experts(const MoeArgs& a, Routing& r) {
+    const int tid = threadIdx.x;
+    if (tid < kMoeExperts) r.tokens[tid][0] = r.tokens[tid][1] = 0;
+    __syncthreads();
+    for (int i = tid; i < a.M * a.top; i += kMoeThreads) {
+        const int m = i / a.top;
+        atomicOr(&r.tokens[r.pick[i]][m >> 5], 1u << (m & 31));
+    }
+    __syncthreads();
+    if (tid < 32) {
+        int count = 0;
+        for (int e0 = 0; e0 < a.E; e0 += 32) {
+            const int e = e0 + tid;
+            const bool on = e < a.E && (r.tokens[e][0] | r.tokens[e][1]) != 0;
+            const unsigned int b = __ballot_sync(0xffffffffu, on);
+            if (on) r.active[count + __popc(b & ((1u << tid) - 1u))] = static_cast<short>(e);
+            count += __popc(b);
+        }
+        if (tid == 0) r.count = count;
+    }
+    __syncthreads();
+}
+
+// Token number j (from 0) of an expert, in ascending order; -1 past the last.
+__device__ __forceinline__ int token_of(const unsigned int (&bits)[2], int j) {
+    const int low = __popc(bits[0]);
+    const bool hi = j >= low;
+    unsigned int b = bits[hi];
+    for (int i = hi ? j - low : j; i > 0; --i) b &= b - 1;
+    return b ? __ffs(b) - 1 + (hi ? 32 : 0) : -1;
+}
+
+// Which of its picks token m made with expert e.
+__device__ __forceinline__ int pair_of(const MoeArgs& a, const Routing& r, int m, int e) {
+    for (int j = 0; j < a.top; ++j) {
+        if (r.pick[m * a.top + j] == e) return m * a.top + j;
+    }
+    return m * a.top;
+}
+
+__device__ void route_tokens(const MoeArgs& a, Routing& r) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    for (int m = warp; m < a.M; m += kMoeWarps) pick_experts(a, m, r, lane);
+    __syncthreads();
+    if (blockIdx.x == 0) {
+        for (int i = threadIdx.x; i < a.M * a.top; i += kMoeThreads) {
+            a.experts[i] = r.pick[i];
+            a.weights[i] = r.weight[i];
+        }
+    }
+}
+
+// ------------------------------------------------------------- gate and up
+// NP pairs of tokens at a time. An item is 32 rows of both matrices: two tiles
+// of 16 rows each, of which rows 0-7 and 8-15 are runs of eight (the columns
+// that share a unit in the next product). Warps take every eighth window.
+template <int NP>
+__global__ void __launch_bounds__(kMoeThreads, NP == 1 ? 3 : 2) up_kernel(const MoeArgs a) {
+    __shared__ Routing r;
+    __shared__ int sums[4][16][8 * NP + 1];  // [gate 0, gate 1, up 0, up 1][row][token, digit]
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int g = lane >> 2, t = lane & 3;
+    pdl_launch_dependents();
+    pdl_wait();
+    route_tokens(a, r);
+    list_experts(a, r);
+
+    const int halves = a.fp / 32, windows = (a.K + 63) / 64;
+    const int items = r.count * halves;
+    for (int i = tid; i < 4 * 16 * (8 * NP + 1); i += kMoeThreads) (&sums[0][0][0])[i] = 0;
+    __syncthreads();
+    for (int item = blockIdx.x; item < items; item += gridDim.x) {
+        const int e = r.active[item / halves];
+        const int f0 = (item % halves) / 2 * 64, half = item % halves & 1;
+        const int tokens = __popc(r.tokens[e][0]) + __popc(r.tokens[e][1]);
+        const int8_t* rows[4][2];
+        #pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            #pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int f = min(f0 + 16 * (2 * i + j) + 8 * half + g, a.F - 1);
+                const int64_t at = (static_cast<int64_t>(e) * a.F + f) * a.K + 16 * t;
+                rows[i][j] = a.qg + at;
+                rows[2 + i][j] = a.qu + at;
+            }
+        }
+        for (int j0 = 0; j0 < tokens; j0 += 2 * NP) {
+            const int8_t* xd[NP];
+            bool on[NP];
+            #pragma unroll
+            for (int n = 0; n < NP; ++n) {
+                const int m = token_of(r.tokens[e], j0 + 2 * n + (g >> 2));
+                on[n] = m >= 0;
+                xd[n] = a.xd + (static_cast<int64_t>(max(m, 0)) * 4 + (g & 3)) * a.kp + 16 * t;
+            }
+            int acc[NP][4][4] = {};
+            for (int w = warp; w < windows; w += kMoeWarps) {
+                const bool in = 64 * w + 16 * t < a.K;
+                uint4 q[4][2], b[NP];
+                #pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    #pragma unroll
+                    for (int j = 0; j < 2; ++j) q[i][j] = load_stream(rows[i][j] + 64 * w, in);
+                }
+                #pragma unroll
+                for (int n = 0; n < NP; ++n) {
+                    b[n] = make_uint4(0u, 0u, 0u, 0u);
+                    if (on[n]) b[n] = *reinterpret_cast<const uint4*>(xd[n] + 64 * w);
+                }
+                #pragma unroll
+                for (int n = 0; n < NP; ++n) {
+                    #pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t lo[4] = {q[i][0].x, q[i][1].x, q[i][0].y, q[i][1].y};
+                        const uint32_t hi[4] = {q[i][0].z, q[i][1].z, q[i][0].w, q[i][1].w};
+                        mma_s8_16832(acc[n][i], lo, b[n].x, b[n].y);
+                        mma_s8_16832(acc[n][i], hi, b[n].z, b[n].w);
+                    }
+                }
+            }
+            #pragma unroll
+            for (int n = 0; n < NP; ++n) {
+                #pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    #pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        atomicAdd(&sums[i][g + 8 * (c >> 1)][8 * n + 2 * t + (c & 1)], acc[n][i][c]);
+                    }
+                }
+            }
+            __syncthreads();
+            // Warp j: token j0 + j, lane: one of the 32 rows.
+            if (warp < 2 * NP && j0 + warp < tokens) {
+                const int m = token_of(r.tokens[e], j0 + warp);
+                const int run = lane >> 3, f = f0 + 16 * run + 8 * half + (lane & 7);
+                const int tile = run >> 1, row = 8 * (run & 1) + (lane & 7);
+                const float unit = a.xs[m];
+                const auto dot = [&](const int (&s)[16][8 * NP + 1]) {
+                    const int* d = &s[row][4 * warp];
+                    return static_cast<float>(((static_cast<double>(d[3]) * 256.0 + d[2]) * 256.0 + d[1]) * 256.0 + d[0]);
+                };
+                float h = 0.0f;
+                if (f < a.F) {
+                    const int64_t at = static_cast<int64_t>(e) * a.F + f;
+                    const float gate = dot(sums[tile]) * unit * a.sg[at], up = dot(sums[2 + tile]) * unit * a.su[at];
+                    h = gate / (1.0f + expf(-gate)) * up;
+                }
+                const bool bad = __any_sync(0xffffffffu, not_finite(h));
+                const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(h))));
+                const Fixed fx = fixed_for(top, bad);
+                const uint32_t y = bad ? 0u : digits_of(h, fx);
+                const int64_t pair = pair_of(a, r, m, e);
+                int8_t* hd = a.hd + pair * 4 * a.fp + f;
+                #pragma unroll
+                for (int i = 0; i < 4; ++i) hd[static_cast<int64_t>(i) * a.fp] = static_cast<int8_t>(y >> (8 * i));
+                if (lane == 0) a.hs[pair * halves + (f0 / 32 + half)] = fx.unit;
+            }
+            __syncthreads();
+            for (int i = tid; i < 4 * 16 * (8 * NP + 1); i += kMoeThreads) (&sums[0][0][0])[i] = 0;
+            __syncthreads();
+        }
+    }
+}
+
+// -------------------------------------------------------------------- down
+// A block owns output channels 16 x .. 16 x + 15. Warps take every eighth
+// window of each chosen expert, four windows' loads at once; a step's exact
+// integer sums join in f32 with the step's unit. Each warp adds its experts'
+// results, weighted, to its own sums per token, and the warps' sums are added
+// in order at the end.
+template <int NP>
+__global__ void __launch_bounds__(kMoeThreads, 2) down_kernel(const MoeArgs a) {
+    extern __shared__ float outs[];  // [warp][token][16]
+    __shared__ Routing r;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int g = lane >> 2, t = lane & 3;
+    pdl_launch_dependents();
+    for (int i = tid; i < kMoeWarps * a.M * 16; i += kMoeThreads) outs[i] = 0.0f;
+    pdl_wait();
+    for (int i = tid; i < a.M * a.top; i += kMoeThreads) {
+        r.pick[i] = static_cast<short>(a.experts[i]);
+        r.weight[i] = a.weights[i];
+    }
+    __syncthreads();
+    list_experts(a, r);
+
+    const int n0 = blockIdx.x * 16;
+    const int windows = a.fp / 64;
+    float* mine = outs + warp * a.M * 16;
+    for (int i = 0; i < r.count; ++i) {
+        const int e = r.active[i];
+        const int tokens = __popc(r.tokens[e][0]) + __popc(r.tokens[e][1]);
+        const int8_t* rows[2];
+        float scale[2];
+        #pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int n = min(n0 + 8 * j + g, a.K - 1);
+            rows[j] = a.qd + (static_cast<int64_t>(e) * a.K + n) * a.F + 16 * t;
+            scale[j] = a.sd[static_cast<int64_t>(e) * a.K + n];
+        }
+        for (int j0 = 0; j0 < tokens; j0 += 2 * NP) {
+            const int8_t* hd[NP];
+            const float* hs[NP];
+            bool on[NP];
+            #pragma unroll
+            for (int n = 0; n < NP; ++n) {
+                // This lane's column of the B operand, and the token of its result columns.
+                const int m = token_of(r.tokens[e], j0 + 2 * n + (g >> 2));
+                on[n] = m >= 0;
+                const int64_t pair = on[n] ? pair_of(a, r, m, e) : 0;
+                hd[n] = a.hd + (pair * 4 + (g & 3)) * a.fp + 16 * t;
+                const int mr = token_of(r.tokens[e], j0 + 2 * n + (t >> 1));
+                hs[n] = a.hs + (mr >= 0 ? pair_of(a, r, mr, e) : 0) * static_cast<int64_t>(2 * windows);
+            }
+            float acc[NP][4] = {};
+            constexpr int AHEAD = NP == 4 ? 2 : 4;
+            for (int w0 = warp; w0 < windows; w0 += AHEAD * kMoeWarps) {
+                uint4 q[AHEAD][2], b[AHEAD][NP];
+                float2 unit[AHEAD][NP];
+                #pragma unroll
+                for (int k = 0; k < AHEAD; ++k) {
+                    const int w = w0 + k * kMoeWarps;
+                    const bool in = 64 * w + 16 * t < a.F;
+                    #pragma unroll
+                    for (int j = 0; j < 2; ++j) q[k][j] = load_stream(rows[j] + 64 * w, in);
+                    #pragma unroll
+                    for (int n = 0; n < NP; ++n) {
+                        b[k][n] = make_uint4(0u, 0u, 0u, 0u);
+                        unit[k][n] = make_float2(0.0f, 0.0f);
+                        if (w < windows) {
+                            if (on[n]) b[k][n] = *reinterpret_cast<const uint4*>(hd[n] + 64 * w);
+                            unit[k][n] = *reinterpret_cast<const float2*>(hs[n] + 2 * w);
+                        }
+                    }
+                }
+                #pragma unroll
+                for (int k = 0; k < AHEAD; ++k) {
+                    const uint32_t lo[4] = {q[k][0].x, q[k][1].x, q[k][0].y, q[k][1].y};
+                    const uint32_t hi[4] = {q[k][0].z, q[k][1].z, q[k][0].w, q[k][1].w};
+                    #pragma unroll
+                    for (int n = 0; n < NP; ++n) {
+                        int d[2][4];
+                        #pragma unroll
+                        for (int c = 0; c < 4; ++c) d[0][c] = d[1][c] = kMagicBits;
+                        mma_s8_16832(d[0], lo, b[k][n].x, b[k][n].y);
+                        mma_s8_16832(d[1], hi, b[k][n].z, b[k][n].w);
+                        #pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            acc[n][c] = fmaf(__int_as_float(d[0][c]) - kMagic, unit[k][n].x, acc[n][c]);
+                            acc[n][c] = fmaf(__int_as_float(d[1][c]) - kMagic, unit[k][n].y, acc[n][c]);
+                        }
+                    }
+                }
+            }
+            #pragma unroll
+            for (int n = 0; n < NP; ++n) {
+                // Lane (g, t) has digits 2 (t % 2) and 2 (t % 2) + 1 of token t / 2.
+                const int m = token_of(r.tokens[e], j0 + 2 * n + (t >> 1));
+                const float weight = m >= 0 ? r.weight[pair_of(a, r, m, e)] : 0.0f;
+                #pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    float v = fmaf(acc[n][2 * j + 1], 256.0f, acc[n][2 * j]);
+                    v = fmaf(__shfl_xor_sync(0xffffffffu, v, 1), (t & 1) ? 0.0f : 65536.0f, v);
+                    if (m >= 0 && !(t & 1)) mine[m * 16 + 8 * j + g] += v * scale[j] * weight;
+                }
+            }
+        }
+    }
+    __syncthreads();
+    for (int i = tid; i < a.M * 16; i += kMoeThreads) {
+        const int m = i / 16, n = n0 + i % 16;
+        float v = 0.0f;
+        #pragma unroll
+        for (int w = 0; w < kMoeWarps; ++w) v += outs[w * a.M * 16 + i];
+        if (n < a.K) a.out[static_cast<int64_t>(m) * a.K + n] = v;
+    }
+}
+
+// --------------------------------------------------- any sizes and alignment
+// Sizes that are not multiples of 16 and unaligned codes: one warp per value.
+__global__ void __launch_bounds__(kMoeThreads) plain_up_kernel(const MoeArgs a) {
+    __shared__ Routing r;
+    pdl_launch_dependents();
+    pdl_wait();
+    route_tokens(a, r);
+    const int lane = threadIdx.x & 31;
+    const int64_t total = static_cast<int64_t>(a.M) * a.top * a.F;
+    for (int64_t i = blockIdx.x * kMoeWarps + (threadIdx.x >> 5); i < total; i += gridDim.x * kMoeWarps) {
+        const int pair = static_cast<int>(i / a.F), f = static_cast<int>(i % a.F);
+        const int64_t at = static_cast<int64_t>(r.pick[pair]) * a.F + f;
+        const float* x = a.x + static_cast<int64_t>(pair / a.top) * a.K;
+        float g = 0.0f, u = 0.0f;
+        for (int k = lane; k < a.K; k += 32) {
+            g = fmaf(x[k], static_cast<float>(a.qg[at * a.K + k]), g);
+            u = fmaf(x[k], static_cast<float>(a.qu[at * a.K + k]), u);
+        }
+        #pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            g += __shfl_xor_sync(0xffffffffu, g, o);
+            u += __shfl_xor_sync(0xffffffffu, u, o);
+        }
+        g *= a.sg[at];
+        if (lane == 0) a.h[i] = g / (1.0f + expf(-g)) * (u * a.su[at]);
+    }
+}
+
+__global__ void __launch_bounds__(kMoeThreads) plain_down_kernel(const MoeArgs a) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int lane = threadIdx.x & 31;
+    const int64_t total = static_cast<int64_t>(a.M) * a.K;
+    for (int64_t i = blockIdx.x * kMoeWarps + (threadIdx.x >> 5); i < total; i += gridDim.x * kMoeWarps) {
+        const int m = static_cast<int>(i / a.K), n = static_cast<int>(i % a.K);
+        float out = 0.0f;
+        for (int j = 0; j < a.top; ++j) {
+            const int pair = m * a.top + j;
+            const int64_t at = static_cast<int64_t>(a.experts[pair]) * a.K + n;
+            float v = 0.0f;
+            for (int f = lane; f < a.F; f += 32) {
+                v = fmaf(a.h[static_cast<int64_t>(pair) * a.F + f], static_cast<float>(a.qd[at * a.F + f]), v);
+            }
+            #pragma unroll
+            for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+            out = fmaf(v * a.sd[at], a.weights[pair], out);
+        }
+        if (lane == 0) a.out[i] = out;
+    }
+}
+
+int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+
+bool sizes_supported(int64_t M, int64_t K, int64_t F, int64_t E, int64_t top) {
+    // 65536 columns keep a digit's sum inside 31 bits.
+    return K <= 65536 && F <= 65536 && E <= kMoeExperts && top <= kMoeTop && top <= E && M <= (int64_t{1} << 30);
+}
+
+// Whether the tensor kernels take these sizes (alignment aside).
+bool tensor_sizes(int64_t K, int64_t F) { return K % 16 == 0 && F % 16 == 0; }
+
+// Places of the scratch buffers; returns the bytes they take.
+int64_t lay_out(MoeArgs& a, char* ws, int64_t M, bool tensor, bool own_picks) {
+    int64_t at = 0;
+    const auto take = [&](int64_t bytes) {
+        char* p = ws + at;
+        at += round_up(bytes, 256);
+        return p;
+    };
+    const int64_t pairs = M * a.top;
+    a.logits = reinterpret_cast<float*>(take(4 * M * a.E));
+    int* const experts = reinterpret_cast<int*>(take(4 * pairs));
+    float* const weights = reinterpret_cast<float*>(take(4 * pairs));
+    if (own_picks) a.experts = experts, a.weights = weights;
+    if (tensor) {
+        a.xd = reinterpret_cast<int8_t*>(take(M * 4 * a.kp));
+        a.xs = reinterpret_cast<float*>(take(4 * M));
+        a.hd = reinterpret_cast<int8_t*>(take(pairs * 4 * a.fp));
+        a.hs = reinterpret_cast<float*>(take(pairs * (a.fp / 32) * 4));
+    } else {
+        a.h = reinterpret_cast<float*>(take(4 * pairs * a.F));
+    }
+    return at;
+}
+
+template <int NP>
+cudaError_t run_tensor(const MoeArgs& a, cudaStream_t stream) {
+    const int sms = device_sm_count();
+    cudaLaunchAttribute attr[1];
+    // Items of the chosen experts are dealt out to one wave of blocks.
+    const int per_sm = NP == 1 ? 3 : 2;
+    const int64_t items = static_cast<int64_t>(a.E < a.M * a.top ? a.E : a.M * a.top) * (a.fp / 32);
+    const int64_t grid = items < static_cast<int64_t>(per_sm) * sms ? items : static_cast<int64_t>(per_sm) * sms;
+    cudaLaunchConfig_t cfg = pdl_config(dim3(static_cast<unsigned>(grid)), dim3(kMoeThreads), 0, stream, attr);
+    cudaError_t e = cudaLaunchKernelEx(&cfg, up_kernel<NP>, a);
+    if (e != cudaSuccess) return e;
+    cfg.gridDim = dim3(static_cast<unsigned>(ceil_div(a.K, 16)));
+    cfg.dynamicSmemBytes = static_cast<size_t>(kMoeWarps) * a.M * 16 * sizeof(float);
+    return cudaLaunchKernelEx(&cfg, down_kernel<NP>, a);
+}
+
+cudaError_t run_pass(const MoeArgs& a, bool tensor, cudaStream_t stream) {
+    cudaLaunchAttribute attr[1];
+    cudaLaunchConfig_t cfg = pdl_config(dim3(a.E + (tensor ? a.M : 0), (a.M + 7) / 8), dim3(128), 0, stream, attr);
+    cudaError_t e = cudaLaunchKernelEx(&cfg, route_kernel, a);
+    if (e != cudaSuccess) return e;
+    if (!tensor) {
+        cfg.gridDim = dim3(4 * device_sm_count());
+        cfg.blockDim = dim3(kMoeThreads);
+        e = cudaLaunchKernelEx(&cfg, plain_up_kernel, a);
+        return e != cudaSuccess ? e : cudaLaunchKernelEx(&cfg, plain_down_kernel, a);
+    }
+    // Tokens an expert has to take at a time: by how many pick it on average.
+    if (a.M <= 2) return run_tensor<1>(a, stream);
+    if (a.M <= 4 || a.M * a.top <= 2 * a.E) return run_tensor<2>(a, stream);
+    return run_tensor<4>(a, stream);
+}
+
+}  // namespace
+}  // namespace pcb
+
+extern "C" int64_t popcornMoeWorkspace(int64_t M, int64_t K, int64_t F, int64_t E, int64_t top_k) {
+    if (M <= 0 || K <= 0 || F <= 0 || E <= 0 || top_k <= 0 || !pcb::sizes_supported(M, K, F, E, top_k)) return 0;
+    pcb::MoeArgs a = {};
+    a.K = static_cast<int>(K), a.F = static_cast<int>(F), a.E = static_cast<int>(E), a.top = static_cast<int>(top_k);
+    a.kp = static_cast<int>(pcb::round_up(K, 64)), a.fp = static_cast<int>(pcb::round_up(F, 64));
+    const int64_t m = M < pcb::kMoeTokens ? M : pcb::kMoeTokens;
+    // (Either kind of kernel: the sizes do not say how the codes are aligned.)
+    const int64_t plain = pcb::lay_out(a, nullptr, m, false, true);
+    const int64_t tensor = pcb::tensor_sizes(K, F) ? pcb::lay_out(a, nullptr, m, true, true) : 0;
+    return plain > tensor ? plain : tensor;
+}
+
+extern "C" popcornStatus_t popcornMoe_i8f32(float* out, int32_t* experts, float* weights, const float* x,
+                                            const float* router, const int8_t* q_gate, const float* s_gate,
+                                            const int8_t* q_up, const float* s_up, const int8_t* q_down,
+                                            const float* s_down, int64_t M, int64_t K, int64_t F, int64_t E,
+                                            int64_t top_k, int renormalize, void* workspace, int64_t workspace_bytes,
+                                            cudaStream_t stream) {
+    if (out == nullptr || x == nullptr || router == nullptr || q_gate == nullptr || s_gate == nullptr ||
+        q_up == nullptr || s_up == nullptr || q_down == nullptr || s_down == nullptr ||
+        (experts == nullptr) != (weights == nullptr)) {
+        return POPCORN_ERROR_INVALID_VALUE;
+    }
+    if (M <= 0 || K <= 0 || F <= 0 || E <= 0) return POPCORN_SUCCESS;
+    if (top_k <= 0 || !pcb::sizes_supported(M, K, F, E, top_k)) return POPCORN_ERROR_INVALID_VALUE;
+    const int64_t need = popcornMoeWorkspace(M, K, F, E, top_k);
+    void* ws = workspace;
+    if (workspace == nullptr) {
+        const cudaError_t e = pcb::scratch_alloc(&ws, static_cast<size_t>(need), stream);
+        if (e != cudaSuccess) return pcb::record_cuda(e);
+    } else if (workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0) {
+        return POPCORN_ERROR_INVALID_VALUE;
+    }
+    const bool tensor = pcb::tensor_sizes(K, F) && pcb::aligned16(q_gate) && pcb::aligned16(q_up) && pcb::aligned16(q_down);
+    pcb::MoeArgs a = {};
+    a.router = router, a.qg = q_gate, a.sg = s_gate, a.qu = q_up, a.su = s_up, a.qd = q_down, a.sd = s_down;
+    a.K = static_cast<int>(K), a.F = static_cast<int>(F), a.E = static_cast<int>(E), a.top = static_cast<int>(top_k);
+    a.renorm = renormalize;
+    a.kp = static_cast<int>(pcb::round_up(K, 64)), a.fp = static_cast<int>(pcb::round_up(F, 64));
+    cudaError_t e = cudaSuccess;
+    for (int64_t m = 0; m < M && e == cudaSuccess; m += pcb::kMoeTokens) {
+        a.M = static_cast<int>(M - m < pcb::kMoeTokens ? M - m : pcb::kMoeTokens);
+        a.out = out + m * K, a.x = x + m * K;
+        if (experts != nullptr) a.experts = experts + m * top_k, a.weights = weights + m * top_k;
+        pcb::lay_out(a, static_cast<char*>(ws), M < pcb::kMoeTokens ? M : pcb::kMoeTokens, tensor, experts == nullptr);
+        e = pcb::run_pass(a, tensor, stream);
+    }
+    if (workspace == nullptr) {
+        const cudaError_t f = pcb::scratch_free(ws, stream);
+        if (e == cudaSuccess) e = f;
+    }
+    if (e != cudaSuccess) return pcb::record_cuda(e);
+    return pcb::check_launch();
+}

@@ -34,6 +34,7 @@
 //    that spans blocks leaves partial (m, l, sum) triples, joined in a fixed
 //    order by kv_join_kernel.
 #include <cmath>
+#include <type_traits>
 
 #include "kv.cuh"
 #include "mma_frag.cuh"
@@ -49,6 +50,7 @@ constexpr float kMagic = 12582912.0f;       // 1.5 2^23
 constexpr int kMagicBits = 0x4B400000;
 constexpr float kLift = 6.0f;               // probabilities are scaled by 2^6
 constexpr float kSlack = 8.0f;              // and may exceed the running maximum by 2^8
+constexpr int kTaskUnits = 8;               // a task's fixed cost in tiles (its queries, its join)
 
 struct AttnArgs {
     void* out;
@@ -126,22 +128,34 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Cache codes are read once: no allocation in L1.
+// Cache codes are read once: no allocation in L1. CHECK: zeros unless ok.
+template <bool CHECK>
 __device__ __forceinline__ void load_codes(uint32_t (&w)[4], const int8_t* p, bool ok) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %5, 0;\n\t"
-        "mov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\tmov.b32 %3, 0;\n\t"
-        "@p ld.global.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];\n\t}"
-        : "=&r"(w[0]), "=&r"(w[1]), "=&r"(w[2]), "=&r"(w[3])
-        : "l"(p), "r"(static_cast<int>(ok)));
+    if constexpr (CHECK) {
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %5, 0;\n\t"
+            "mov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\tmov.b32 %3, 0;\n\t"
+            "@p ld.global.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];\n\t}"
+            : "=&r"(w[0]), "=&r"(w[1]), "=&r"(w[2]), "=&r"(w[3])
+            : "l"(p), "r"(static_cast<int>(ok)));
+    } else {
+        asm volatile("ld.global.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                     : "l"(p));
+    }
 }
+template <bool CHECK>
 __device__ __forceinline__ void load_codes(uint32_t (&w)[2], const int8_t* p, bool ok) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %3, 0;\n\t"
-        "mov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\t"
-        "@p ld.global.L1::no_allocate.v2.b32 {%0, %1}, [%2];\n\t}"
-        : "=&r"(w[0]), "=&r"(w[1])
-        : "l"(p), "r"(static_cast<int>(ok)));
+    if constexpr (CHECK) {
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %3, 0;\n\t"
+            "mov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\t"
+            "@p ld.global.L1::no_allocate.v2.b32 {%0, %1}, [%2];\n\t}"
+            : "=&r"(w[0]), "=&r"(w[1])
+            : "l"(p), "r"(static_cast<int>(ok)));
+    } else {
+        asm volatile("ld.global.L1::no_allocate.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p));
+    }
 }
 
 // Two f16 of signed codes from the biased bytes (code + 128) that `sel` picks
@@ -256,7 +270,8 @@ __device__ __forceinline__ void store_row(const AttnArgs& a, int64_t t, int head
     }
 }
 
-template <typename T, int DP, int NT>
+// DP: dim rounded up to 64, 128 or 256; FULL: dim is DP.
+template <typename T, int DP, int NT, bool FULL>
 __global__ void __launch_bounds__(kThreads, Traits<T>::kFresh || NT == 2 || DP == 256 ? (DP == 256 ? 2 : 3) : 4)
 kv_rows_kernel(const AttnArgs a) {
     constexpr int DIGITS = Traits<T>::kDigits;
@@ -271,6 +286,7 @@ kv_rows_kernel(const AttnArgs a) {
     __shared__ int64_t s_scan[kWarps], s_tasks[kWarps], s_from, s_task0;
     __shared__ int s_b;
 
+    const int dim = FULL ? DP : a.dim;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = lane >> 2, t = lane & 3;
     pdl_launch_dependents();
@@ -285,7 +301,7 @@ kv_rows_kernel(const AttnArgs a) {
             if (base + tid < a.seqs) {
                 const Seq s = sequence(a, base + tid);
                 mine_tasks = static_cast<int64_t>((static_cast<int64_t>(s.rows) * a.group + ROWS - 1) / ROWS) * a.heads;
-                mine = mine_tasks * max(s.tiles, 1);
+                mine = mine_tasks * (kTaskUnits + max(s.tiles, 1));
             }
             int64_t x = mine, y = mine_tasks;
             #pragma unroll
@@ -306,7 +322,7 @@ kv_rows_kernel(const AttnArgs a) {
             // One chunk holds every sequence: its scan serves both passes.
             if (a.seqs <= kThreads) {
                 total = seen;
-                blocks = max(int64_t{1}, min(static_cast<int64_t>(gridDim.x), total / kWarps));
+                blocks = max(int64_t{1}, min(static_cast<int64_t>(gridDim.x), total / (kTaskUnits + kWarps)));
                 if (blockIdx.x < blocks) {
                     run0 = blockIdx.x * total / blocks;
                     run1 = (blockIdx.x + 1) * total / blocks;
@@ -321,7 +337,7 @@ kv_rows_kernel(const AttnArgs a) {
         total = seen;
         all_tasks = tasks;
         if (pass == 0) {
-            blocks = max(int64_t{1}, min(static_cast<int64_t>(gridDim.x), total / kWarps));
+            blocks = max(int64_t{1}, min(static_cast<int64_t>(gridDim.x), total / (kTaskUnits + kWarps)));
             if (blockIdx.x < blocks) {
                 run0 = blockIdx.x * total / blocks;
                 run1 = (blockIdx.x + 1) * total / blocks;
@@ -346,16 +362,20 @@ kv_rows_kernel(const AttnArgs a) {
         const Seq s = sequence(a, b);
         const int tiles = max(s.tiles, 1);
         const int row_tiles = (s.rows * a.group + ROWS - 1) / ROWS;
-        const int64_t units = static_cast<int64_t>(row_tiles) * a.heads * tiles;
+        const int each = kTaskUnits + tiles;
+        const int64_t units = static_cast<int64_t>(row_tiles) * a.heads * each;
         if (run0 >= from + units) {
             from += units;
             task0 += static_cast<int64_t>(row_tiles) * a.heads;
             ++b;
             continue;
         }
-        const int task = static_cast<int>((run0 - from) / tiles);
-        const int u0 = static_cast<int>((run0 - from) % tiles);
-        const int u1 = static_cast<int>(min(static_cast<int64_t>(tiles), u0 + (run1 - run0)));
+        const int task = static_cast<int>((run0 - from) / each);
+        const int c0 = static_cast<int>((run0 - from) % each);
+        const int c1 = static_cast<int>(min(static_cast<int64_t>(each), c0 + (run1 - run0)));
+        run0 += c1 - c0;
+        const int u0 = max(0, c0 - kTaskUnits), u1 = c1 - kTaskUnits;
+        if (u1 <= 0) continue;  // only the fixed cost fell into this run: the next block has it all
         const int h = task % a.heads, rt = task / a.heads;
         const int row_end = s.rows * a.group;
 
@@ -370,30 +390,33 @@ kv_rows_kernel(const AttnArgs a) {
         const auto page_of = [&](int tile) {
             return tile < last ? table[(s.lo + 16 * tile) >> a.page_shift] : 0;
         };
+        // This lane's pieces: keys of rows g, g + 8, values of rows 2 t, 2 t + 1
+        // and those eight further.
+        const int8_t* k_lane = a.k + g * dim + 16 * t;
+        const int8_t* v_lane = a.v + 2 * t * dim + 4 * VW * g;
         uint32_t kr[2][KP][4], vr[4][VP][VW];
         float ks = 0.0f, vs = 0.0f;
         const auto load_k = [&](int tile, int page) {
             const int64_t at = static_cast<int64_t>(page) * a.heads + h;
-            const int8_t* p = a.k + ((at << a.page_shift) + ((s.lo + 16 * tile) & page_mask)) * a.dim;
+            const int8_t* p = k_lane + ((at << a.page_shift) + ((s.lo + 16 * tile) & page_mask)) * dim;
             #pragma unroll
             for (int r = 0; r < 2; ++r) {
                 #pragma unroll
                 for (int c = 0; c < KP; ++c) {
-                    load_codes(kr[r][c], p + (g + 8 * r) * a.dim + 16 * (t + 4 * c), 16 * (t + 4 * c) < a.dim);
+                    load_codes<!FULL>(kr[r][c], p + 8 * r * dim + 64 * c, 16 * (t + 4 * c) < dim);
                 }
             }
             ks = a.ks[at];
         };
         const auto load_v = [&](int tile, int page) {
             const int64_t at = static_cast<int64_t>(page) * a.heads + h;
-            const int8_t* p = a.v + ((at << a.page_shift) + ((s.lo + 16 * tile) & page_mask)) * a.dim;
+            const int8_t* p = v_lane + ((at << a.page_shift) + ((s.lo + 16 * tile) & page_mask)) * dim;
             #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int row = 2 * t + (i & 1) + 8 * (i >> 1);
                 #pragma unroll
                 for (int c = 0; c < VP; ++c) {
-                    const int d = 4 * VW * (g + 8 * c);
-                    load_codes(vr[i][c], p + row * a.dim + d, d < a.dim);
+                    load_codes<!FULL>(vr[i][c], p + ((i & 1) + 8 * (i >> 1)) * dim + 32 * VW * c,
+                                      4 * VW * (g + 8 * c) < dim);
                 }
             }
             vs = a.vs[at];
@@ -421,7 +444,7 @@ kv_rows_kernel(const AttnArgs a) {
             const int tok = r / a.group, hd = r - tok * a.group;
             const T* row = static_cast<const T*>(a.q) + (s.row0 + tok) * a.q_tok +
                            static_cast<int64_t>(h * a.group + hd) * a.q_head;
-            const float f = query_digits<T, DP, DIGITS>(qd[n], row, r < row_end, a.dim, a.q_vec != 0, t) * a.scale_log2;
+            const float f = query_digits<T, DP, DIGITS>(qd[n], row, r < row_end, dim, a.q_vec != 0, t) * a.scale_log2;
             #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 fac[n][c] = __shfl_sync(0xffffffffu, f, 4 * (2 * t + c));
@@ -634,8 +657,8 @@ kv_rows_kernel(const AttnArgs a) {
         }
         if (tid == 0 && u0 == 0 && (a.by_task || !complete)) {
             // Blocks that hold the rest of the task: the last one owns its last
-            // tile (block c owns tiles [c total / blocks, (c + 1) total / blocks)).
-            const int64_t end = from + static_cast<int64_t>(task + 1) * tiles;
+            // unit (block c owns units [c total / blocks, (c + 1) total / blocks)).
+            const int64_t end = from + static_cast<int64_t>(task + 1) * each;
             const int64_t owner = complete ? blockIdx.x : (end * blocks - 1) / total;
             const int more = static_cast<int>(owner - blockIdx.x);
             const int64_t e = a.by_task ? task0 + task : blockIdx.x;
@@ -645,7 +668,6 @@ kv_rows_kernel(const AttnArgs a) {
                 a.entry[2 + 2 * e] = make_int4(task, 0, 0, 0);
             }
         }
-        run0 += u1 - u0;
     }
 }
 
@@ -733,13 +755,13 @@ __global__ void __launch_bounds__(kThreads) kv_join_kernel(const AttnArgs a) {
 }
 
 // Work blocks of kv_rows_kernel: one wave, as many as are resident at once.
-template <typename T, int DP, int NT>
+template <typename T, int DP, int NT, bool FULL>
 cudaError_t rows_grid(int64_t* grid) {
     static int resident = 0;
     int per_sm = __atomic_load_n(&resident, __ATOMIC_RELAXED);
     if (per_sm == 0) {
         const cudaError_t e =
-            cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kv_rows_kernel<T, DP, NT>, kThreads, 0);
+            cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kv_rows_kernel<T, DP, NT, FULL>, kThreads, 0);
         if (e != cudaSuccess) return e;
         if (per_sm < 1) return cudaErrorInvalidConfiguration;
         __atomic_store_n(&resident, per_sm, __ATOMIC_RELAXED);
@@ -750,11 +772,11 @@ cudaError_t rows_grid(int64_t* grid) {
 
 // Launches with the caller's workspace, or only says how many bytes it takes
 // (ws_bytes != nullptr).
-template <typename T, int DP, int NT>
+template <typename T, int DP, int NT, bool FULL>
 cudaError_t run_rows(AttnArgs a, int64_t tasks, void* ws, int64_t* ws_bytes, cudaStream_t stream) {
     constexpr int ROWS = 8 * NT;
     int64_t grid = 0;
-    cudaError_t e = rows_grid<T, DP, NT>(&grid);
+    cudaError_t e = rows_grid<T, DP, NT, FULL>(&grid);
     if (e != cudaSuccess) return e;
     const int64_t entry_bytes = (1 + 2 * grid) * sizeof(int4);
     const int64_t ml_bytes = 2 * grid * ROWS * sizeof(float2);
@@ -769,7 +791,7 @@ cudaError_t run_rows(AttnArgs a, int64_t tasks, void* ws, int64_t* ws_bytes, cud
     a.part = reinterpret_cast<float*>(static_cast<char*>(ws) + entry_bytes + ml_bytes);
     cudaLaunchAttribute attr[1];
     cudaLaunchConfig_t cfg = pdl_config(dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, stream, attr);
-    e = cudaLaunchKernelEx(&cfg, kv_rows_kernel<T, DP, NT>, a);
+    e = cudaLaunchKernelEx(&cfg, kv_rows_kernel<T, DP, NT, FULL>, a);
     if (e != cudaSuccess) return e;
     cfg.gridDim = dim3(static_cast<unsigned>(a.entries), ROWS);
     return cudaLaunchKernelEx(&cfg, kv_join_kernel<T, DP, ROWS>, a);
@@ -781,13 +803,20 @@ cudaError_t run_attention(const AttnArgs& a, int64_t max_tokens, void* ws, int64
     const bool two = !Traits<T>::kFresh && a.dim <= 128 && max_tokens * a.group > 8;
     const int rows = two ? 16 : 8;
     const int64_t tasks = a.heads * (static_cast<int64_t>(a.tokens) * a.group / rows + a.seqs);
+    const auto run = [&](auto dp, auto nt) {
+        constexpr int DP = decltype(dp)::value, NT = decltype(nt)::value;
+        return a.dim == DP ? run_rows<T, DP, NT, true>(a, tasks, ws, ws_bytes, stream)
+                           : run_rows<T, DP, NT, false>(a, tasks, ws, ws_bytes, stream);
+    };
+    const std::integral_constant<int, 1> one;
     if constexpr (!Traits<T>::kFresh) {
-        if (two && a.dim <= 64) return run_rows<T, 64, 2>(a, tasks, ws, ws_bytes, stream);
-        if (two) return run_rows<T, 128, 2>(a, tasks, ws, ws_bytes, stream);
+        const std::integral_constant<int, 2> pair;
+        if (two && a.dim <= 64) return run(std::integral_constant<int, 64>{}, pair);
+        if (two) return run(std::integral_constant<int, 128>{}, pair);
     }
-    if (a.dim <= 64) return run_rows<T, 64, 1>(a, tasks, ws, ws_bytes, stream);
-    if (a.dim <= 128) return run_rows<T, 128, 1>(a, tasks, ws, ws_bytes, stream);
-    return run_rows<T, 256, 1>(a, tasks, ws, ws_bytes, stream);
+    if (a.dim <= 64) return run(std::integral_constant<int, 64>{}, one);
+    if (a.dim <= 128) return run(std::integral_constant<int, 128>{}, one);
+    return run(std::integral_constant<int, 256>{}, one);
 }
 
 cudaError_t run_typed(popcornType_t type, const AttnArgs& a, int64_t max_tokens, void* ws, int64_t* ws_bytes,

@@ -28,6 +28,7 @@
 #include "common.cuh"
 #include "mma_frag.cuh"
 #include "popcorn_serve.h"
+#include "sm100.cuh"
 
 namespace pcb {
 namespace {
@@ -59,6 +60,7 @@ struct MoeArgs {
     float* hs;         // [M top][fp / 32] their units
     float* h;          // [M top][F] hidden values (plain kernels only)
     int M, K, F, E, top, renorm, kp, fp;
+    int split;         // blocks that share 16 output channels of the down product
 };
 
 __device__ __forceinline__ uint4 load_stream(const int8_t* p, bool ok) {
@@ -175,15 +177,26 @@ __global__ void __launch_bounds__(128) route_kernel(const MoeArgs a) {
     }
 }
 
-// What a block knows of the routing: for each chosen expert the tokens that
-// picked it, as bits.
+// What a block knows of the routing. A job is up to 2 NP tokens of one
+// expert; the list of positions holds the chosen experts' (token, pick) pairs
+// expert by expert, tokens ascending.
 struct Routing {
-    unsigned int tokens[kMoeExperts][2];
-    short active[kMoeExperts];
-    int count;
-    short pick[kMoeTokens * kMoeTop];
-    float weight[kMoeTokens * kMoeTop];
+    unsigned int tokens[kMoeExperts][2];            // an expert's tokens, as bits
+    short base[kMoeExperts];                        // its first position
+    short pair[kMoeTokens * kMoeTop];               // position -> token * top + pick
+    unsigned char token[kMoeTokens * kMoeTop];      // position -> token
+    unsigned int job[kMoeTokens * kMoeTop];         // expert | position << 8 | tokens << 24
+    int jobs;
+    short pick[kMoeTokens * kMoeTop];               // pair -> expert
+    float weight[kMoeTokens * kMoeTop];             // pair -> weight
 };
+struct Job {
+    int expert, pos, count;
+};
+__device__ __forceinline__ Job job_of(const Routing& r, int j) {
+    const unsigned int x = r.job[j];
+    return {static_cast<int>(x & 0xffu), static_cast<int>(x >> 8 & 0xffffu), static_cast<int>(x >> 24)};
+}
 
 // One warp: token m's experts. Softmax over all logits; the top ones by
 // repeated maxima, the lowest index first among equals. NaN logits count as
@@ -235,8 +248,9 @@ __device__ void pick_experts(const MoeArgs& a, int m, Routing& r, int lane) {
     }
 }
 
-// The block's view of picks already in r.pick: token bits and active experts.
-__device__ void list_experts(const MoeArgs& a, Routing& r) {
+// The block's lists from the picks in r.pick.
+template <int NP>
+__device__ void list_jobs(const MoeArgs& a, Routing& r) {
     const int tid = threadIdx.x;
     if (tid < kMoeExperts) r.tokens[tid][0] = r.tokens[tid][1] = 0;
     __syncthreads();
@@ -246,34 +260,38 @@ __device__ void list_experts(const MoeArgs& a, Routing& r) {
     }
     __syncthreads();
     if (tid < 32) {
-        int count = 0;
+        int jobs = 0, pos = 0;
         for (int e0 = 0; e0 < a.E; e0 += 32) {
             const int e = e0 + tid;
-            const bool on = e < a.E && (r.tokens[e][0] | r.tokens[e][1]) != 0;
-            const unsigned int b = __ballot_sync(0xffffffffu, on);
-            if (on) r.active[count + __popc(b & ((1u << tid) - 1u))] = static_cast<short>(e);
-            count += __popc(b);
+            const int n = e < a.E ? __popc(r.tokens[e][0]) + __popc(r.tokens[e][1]) : 0;
+            const int j = (n + 2 * NP - 1) / (2 * NP);
+            int sum = n | j << 16;  // both totals stay under 2^11
+            #pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int u = __shfl_up_sync(0xffffffffu, sum, o);
+                if (tid >= o) sum += u;
+            }
+            const int from = pos + (sum & 0xffff) - n, job = jobs + (sum >> 16) - j;
+            if (n) r.base[e] = static_cast<short>(from);
+            for (int k = 0; k < j; ++k) {
+                r.job[job + k] = static_cast<unsigned int>(e) | static_cast<unsigned int>(from + 2 * NP * k) << 8 |
+                                 static_cast<unsigned int>(min(2 * NP, n - 2 * NP * k)) << 24;
+            }
+            sum = __shfl_sync(0xffffffffu, sum, 31);
+            pos += sum & 0xffff;
+            jobs += sum >> 16;
         }
-        if (tid == 0) r.count = count;
+        if (tid == 0) r.jobs = jobs;
     }
     __syncthreads();
-}
-
-// Token number j (from 0) of an expert, in ascending order; -1 past the last.
-__device__ __forceinline__ int token_of(const unsigned int (&bits)[2], int j) {
-    const int low = __popc(bits[0]);
-    const bool hi = j >= low;
-    unsigned int b = bits[hi];
-    for (int i = hi ? j - low : j; i > 0; --i) b &= b - 1;
-    return b ? __ffs(b) - 1 + (hi ? 32 : 0) : -1;
-}
-
-// Which of its picks token m made with expert e.
-__device__ __forceinline__ int pair_of(const MoeArgs& a, const Routing& r, int m, int e) {
-    for (int j = 0; j < a.top; ++j) {
-        if (r.pick[m * a.top + j] == e) return m * a.top + j;
+    for (int i = tid; i < a.M * a.top; i += kMoeThreads) {
+        const int m = i / a.top, e = r.pick[i];
+        const unsigned int below = (1u << (m & 31)) - 1u;
+        const int rank = m < 32 ? __popc(r.tokens[e][0] & below) : __popc(r.tokens[e][0]) + __popc(r.tokens[e][1] & below);
+        r.pair[r.base[e] + rank] = static_cast<short>(i);
+        r.token[r.base[e] + rank] = static_cast<unsigned char>(m);
     }
-    return m * a.top;
+    __syncthreads();
 }
 
 __device__ void route_tokens(const MoeArgs& a, Routing& r) {
@@ -289,123 +307,134 @@ __device__ void route_tokens(const MoeArgs& a, Routing& r) {
 }
 
 // ------------------------------------------------------------- gate and up
-// NP pairs of tokens at a time. An item is 32 rows of both matrices: two tiles
-// of 16 rows each, of which rows 0-7 and 8-15 are runs of eight (the columns
-// that share a unit in the next product). Warps take every eighth window.
+// An item is a job's 32 rows of both matrices: two tiles of 16 rows each, of
+// which rows 0-7 and 8-15 are runs of eight (the columns that share a unit in
+// the next product). Warps take every eighth window; a window's loads are
+// issued as soon as the one before has been multiplied, across items too, so
+// that they are in flight while the item's sums are joined.
 template <int NP>
 __global__ void __launch_bounds__(kMoeThreads, NP == 1 ? 3 : 2) up_kernel(const MoeArgs a) {
     __shared__ Routing r;
-    __shared__ int sums[4][16][8 * NP + 1];  // [gate 0, gate 1, up 0, up 1][row][token, digit]
+    __shared__ int sums[2][4][16][8 * NP + 1];  // item parity; [gate 0, gate 1, up 0, up 1][row][token, digit]
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = lane >> 2, t = lane & 3;
     pdl_launch_dependents();
+    for (int i = tid; i < 2 * 4 * 16 * (8 * NP + 1); i += kMoeThreads) (&sums[0][0][0][0])[i] = 0;
     pdl_wait();
     route_tokens(a, r);
-    list_experts(a, r);
+    list_jobs<NP>(a, r);
 
     const int halves = a.fp / 32, windows = (a.K + 63) / 64;
-    const int items = r.count * halves;
-    for (int i = tid; i < 4 * 16 * (8 * NP + 1); i += kMoeThreads) (&sums[0][0][0])[i] = 0;
-    __syncthreads();
-    for (int item = blockIdx.x; item < items; item += gridDim.x) {
-        const int e = r.active[item / halves];
-        const int f0 = (item % halves) / 2 * 64, half = item % halves & 1;
-        const int tokens = __popc(r.tokens[e][0]) + __popc(r.tokens[e][1]);
-        const int8_t* rows[4][2];
+    const int items = r.jobs * halves;
+    const int8_t *gate[4], *up[4], *xd[NP];
+    bool on[NP];
+    uint4 q[4][2], b[NP];
+    const auto setup = [&](int item) {
+        const Job job = job_of(r, item / halves);
+        const int h = item % halves;
         #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < 4; ++i) {
+            const int f = min(h / 2 * 64 + 16 * i + 8 * (h & 1) + g, a.F - 1);
+            const int64_t at = (static_cast<int64_t>(job.expert) * a.F + f) * a.K + 16 * t;
+            gate[i] = a.qg + at;
+            up[i] = a.qu + at;
+        }
+        #pragma unroll
+        for (int n = 0; n < NP; ++n) {
+            const int j = 2 * n + (g >> 2);
+            on[n] = j < job.count;
+            const int m = on[n] ? r.token[job.pos + j] : 0;
+            xd[n] = a.xd + (static_cast<int64_t>(m) * 4 + (g & 3)) * a.kp + 16 * t;
+        }
+    };
+    const auto load = [&](int w) {
+        const bool in = 64 * w + 16 * t < a.K;
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            q[i >> 1][i & 1] = load_stream(gate[i] + 64 * w, in);
+            q[2 + (i >> 1)][i & 1] = load_stream(up[i] + 64 * w, in);
+        }
+        #pragma unroll
+        for (int n = 0; n < NP; ++n) {
+            b[n] = make_uint4(0u, 0u, 0u, 0u);
+            if (on[n]) b[n] = *reinterpret_cast<const uint4*>(xd[n] + 64 * w);
+        }
+    };
+    int parity = 0;
+    if (static_cast<int>(blockIdx.x) < items) {
+        setup(blockIdx.x);
+        if (warp < windows) load(warp);
+    }
+    for (int item = blockIdx.x; item < items; item += gridDim.x, parity ^= 1) {
+        int acc[NP][4][4] = {};
+        for (int w = warp; w < windows; w += kMoeWarps) {
             #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int f = min(f0 + 16 * (2 * i + j) + 8 * half + g, a.F - 1);
-                const int64_t at = (static_cast<int64_t>(e) * a.F + f) * a.K + 16 * t;
-                rows[i][j] = a.qg + at;
-                rows[2 + i][j] = a.qu + at;
+            for (int n = 0; n < NP; ++n) {
+                #pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t lo[4] = {q[i][0].x, q[i][1].x, q[i][0].y, q[i][1].y};
+                    const uint32_t hi[4] = {q[i][0].z, q[i][1].z, q[i][0].w, q[i][1].w};
+                    mma_s8_16832(acc[n][i], lo, b[n].x, b[n].y);
+                    mma_s8_16832(acc[n][i], hi, b[n].z, b[n].w);
+                }
+            }
+            if (w + kMoeWarps < windows) load(w + kMoeWarps);
+        }
+        const int next = item + gridDim.x;
+        if (next < items) {
+            setup(next);
+            if (warp < windows) load(warp);
+        }
+        #pragma unroll
+        for (int n = 0; n < NP; ++n) {
+            #pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                #pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    atomicAdd(&sums[parity][i][g + 8 * (c >> 1)][8 * n + 2 * t + (c & 1)], acc[n][i][c]);
+                }
             }
         }
-        for (int j0 = 0; j0 < tokens; j0 += 2 * NP) {
-            const int8_t* xd[NP];
-            bool on[NP];
+        __syncthreads();
+        // Warp j: the job's token j; lane: one of the 32 rows. Sums are set back
+        // to zero as they are read; the other parity's barrier comes before the
+        // next use of this one's.
+        const Job job = job_of(r, item / halves);
+        if (warp < job.count) {
+            const int m = r.token[job.pos + warp];
+            const int h2 = item % halves;
+            const int run = lane >> 3, f = h2 / 2 * 64 + 16 * run + 8 * (h2 & 1) + (lane & 7);
+            const int tile = run >> 1, row = 8 * (run & 1) + (lane & 7);
+            const float unit = a.xs[m];
+            const int64_t at = static_cast<int64_t>(job.expert) * a.F + min(f, a.F - 1);
+            const float sg = a.sg[at], su = a.su[at];
+            const auto dot = [&](int (&s)[16][8 * NP + 1]) {
+                int* d = &s[row][4 * warp];
+                const double v = ((static_cast<double>(d[3]) * 256.0 + d[2]) * 256.0 + d[1]) * 256.0 + d[0];
+                d[0] = d[1] = d[2] = d[3] = 0;
+                return static_cast<float>(v);
+            };
+            const float gv = dot(sums[parity][tile]) * unit * sg, uv = dot(sums[parity][2 + tile]) * unit * su;
+            const float h = f < a.F ? gv / (1.0f + expf(-gv)) * uv : 0.0f;
+            const bool bad = __any_sync(0xffffffffu, not_finite(h));
+            const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(h))));
+            const Fixed fx = fixed_for(top, bad);
+            const uint32_t y = bad ? 0u : digits_of(h, fx);
+            const int64_t pair = r.pair[job.pos + warp];
+            int8_t* hd = a.hd + pair * 4 * a.fp + f;
             #pragma unroll
-            for (int n = 0; n < NP; ++n) {
-                const int m = token_of(r.tokens[e], j0 + 2 * n + (g >> 2));
-                on[n] = m >= 0;
-                xd[n] = a.xd + (static_cast<int64_t>(max(m, 0)) * 4 + (g & 3)) * a.kp + 16 * t;
-            }
-            int acc[NP][4][4] = {};
-            for (int w = warp; w < windows; w += kMoeWarps) {
-                const bool in = 64 * w + 16 * t < a.K;
-                uint4 q[4][2], b[NP];
-                #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    #pragma unroll
-                    for (int j = 0; j < 2; ++j) q[i][j] = load_stream(rows[i][j] + 64 * w, in);
-                }
-                #pragma unroll
-                for (int n = 0; n < NP; ++n) {
-                    b[n] = make_uint4(0u, 0u, 0u, 0u);
-                    if (on[n]) b[n] = *reinterpret_cast<const uint4*>(xd[n] + 64 * w);
-                }
-                #pragma unroll
-                for (int n = 0; n < NP; ++n) {
-                    #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const uint32_t lo[4] = {q[i][0].x, q[i][1].x, q[i][0].y, q[i][1].y};
-                        const uint32_t hi[4] = {q[i][0].z, q[i][1].z, q[i][0].w, q[i][1].w};
-                        mma_s8_16832(acc[n][i], lo, b[n].x, b[n].y);
-                        mma_s8_16832(acc[n][i], hi, b[n].z, b[n].w);
-                    }
-                }
-            }
-            #pragma unroll
-            for (int n = 0; n < NP; ++n) {
-                #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        atomicAdd(&sums[i][g + 8 * (c >> 1)][8 * n + 2 * t + (c & 1)], acc[n][i][c]);
-                    }
-                }
-            }
-            __syncthreads();
-            // Warp j: token j0 + j, lane: one of the 32 rows.
-            if (warp < 2 * NP && j0 + warp < tokens) {
-                const int m = token_of(r.tokens[e], j0 + warp);
-                const int run = lane >> 3, f = f0 + 16 * run + 8 * half + (lane & 7);
-                const int tile = run >> 1, row = 8 * (run & 1) + (lane & 7);
-                const float unit = a.xs[m];
-                const auto dot = [&](const int (&s)[16][8 * NP + 1]) {
-                    const int* d = &s[row][4 * warp];
-                    return static_cast<float>(((static_cast<double>(d[3]) * 256.0 + d[2]) * 256.0 + d[1]) * 256.0 + d[0]);
-                };
-                float h = 0.0f;
-                if (f < a.F) {
-                    const int64_t at = static_cast<int64_t>(e) * a.F + f;
-                    const float gate = dot(sums[tile]) * unit * a.sg[at], up = dot(sums[2 + tile]) * unit * a.su[at];
-                    h = gate / (1.0f + expf(-gate)) * up;
-                }
-                const bool bad = __any_sync(0xffffffffu, not_finite(h));
-                const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(h))));
-                const Fixed fx = fixed_for(top, bad);
-                const uint32_t y = bad ? 0u : digits_of(h, fx);
-                const int64_t pair = pair_of(a, r, m, e);
-                int8_t* hd = a.hd + pair * 4 * a.fp + f;
-                #pragma unroll
-                for (int i = 0; i < 4; ++i) hd[static_cast<int64_t>(i) * a.fp] = static_cast<int8_t>(y >> (8 * i));
-                if (lane == 0) a.hs[pair * halves + (f0 / 32 + half)] = fx.unit;
-            }
-            __syncthreads();
-            for (int i = tid; i < 4 * 16 * (8 * NP + 1); i += kMoeThreads) (&sums[0][0][0])[i] = 0;
-            __syncthreads();
+            for (int i = 0; i < 4; ++i) hd[static_cast<int64_t>(i) * a.fp] = static_cast<int8_t>(y >> (8 * i));
+            if (lane == 0) a.hs[pair * halves + h2] = fx.unit;
         }
     }
 }
 
 // -------------------------------------------------------------------- down
-// A block owns output channels 16 x .. 16 x + 15. Warps take every eighth
-// window of each chosen expert, four windows' loads at once; a step's exact
-// integer sums join in f32 with the step's unit. Each warp adds its experts'
-// results, weighted, to its own sums per token, and the warps' sums are added
-// in order at the end.
+// A cluster of blocks owns output channels 16 x .. 16 x + 15 and its warps
+// share the (job, window) list in equal runs. Four windows' loads go out at
+// once; a step's exact integer sums join in f32 with the step's unit. At the
+// end of a job a warp adds its result, weighted, to its own sums per token;
+// warps, then blocks, are added in order at the end.
 template <int NP>
 __global__ void __launch_bounds__(kMoeThreads, 2) down_kernel(const MoeArgs a) {
     extern __shared__ float outs[];  // [warp][token][16]
@@ -420,98 +449,116 @@ __global__ void __launch_bounds__(kMoeThreads, 2) down_kernel(const MoeArgs a) {
         r.weight[i] = a.weights[i];
     }
     __syncthreads();
-    list_experts(a, r);
+    list_jobs<NP>(a, r);
 
-    const int n0 = blockIdx.x * 16;
+    const int rank = blockIdx.x % a.split;
+    const int n0 = blockIdx.x / a.split * 16;
     const int windows = a.fp / 64;
+    const int64_t units = static_cast<int64_t>(r.jobs) * windows;
+    const int who = rank * kMoeWarps + warp, all = a.split * kMoeWarps;
+    int u = static_cast<int>(units * who / all);
+    const int u_end = static_cast<int>(units * (who + 1) / all);
     float* mine = outs + warp * a.M * 16;
-    for (int i = 0; i < r.count; ++i) {
-        const int e = r.active[i];
-        const int tokens = __popc(r.tokens[e][0]) + __popc(r.tokens[e][1]);
+    while (u < u_end) {
+        const int w_begin = u % windows;
+        const Job job = job_of(r, u / windows);
+        const int w_end = min(windows, w_begin + (u_end - u));
+        u += w_end - w_begin;
         const int8_t* rows[2];
         float scale[2];
         #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            const int n = min(n0 + 8 * j + g, a.K - 1);
-            rows[j] = a.qd + (static_cast<int64_t>(e) * a.K + n) * a.F + 16 * t;
-            scale[j] = a.sd[static_cast<int64_t>(e) * a.K + n];
+            const int64_t n = static_cast<int64_t>(job.expert) * a.K + min(n0 + 8 * j + g, a.K - 1);
+            rows[j] = a.qd + n * a.F + 16 * t;
+            scale[j] = a.sd[n];
         }
-        for (int j0 = 0; j0 < tokens; j0 += 2 * NP) {
-            const int8_t* hd[NP];
-            const float* hs[NP];
-            bool on[NP];
+        const int8_t* hd[NP];
+        const float* hs[NP];
+        bool on[NP];
+        #pragma unroll
+        for (int n = 0; n < NP; ++n) {
+            // This lane's column of the B operand, and the token of its result columns.
+            const int j = 2 * n + (g >> 2), jr = min(2 * n + (t >> 1), job.count - 1);
+            on[n] = j < job.count;
+            hd[n] = a.hd + (static_cast<int64_t>(r.pair[job.pos + (on[n] ? j : 0)]) * 4 + (g & 3)) * a.fp + 16 * t;
+            hs[n] = a.hs + static_cast<int64_t>(r.pair[job.pos + jr]) * (2 * windows);
+        }
+        float acc[NP][4] = {};
+        constexpr int AHEAD = NP == 4 ? 2 : 4;
+        for (int w0 = w_begin; w0 < w_end; w0 += AHEAD) {
+            uint4 q[AHEAD][2], b[AHEAD][NP];
+            float2 unit[AHEAD][NP];
             #pragma unroll
-            for (int n = 0; n < NP; ++n) {
-                // This lane's column of the B operand, and the token of its result columns.
-                const int m = token_of(r.tokens[e], j0 + 2 * n + (g >> 2));
-                on[n] = m >= 0;
-                const int64_t pair = on[n] ? pair_of(a, r, m, e) : 0;
-                hd[n] = a.hd + (pair * 4 + (g & 3)) * a.fp + 16 * t;
-                const int mr = token_of(r.tokens[e], j0 + 2 * n + (t >> 1));
-                hs[n] = a.hs + (mr >= 0 ? pair_of(a, r, mr, e) : 0) * static_cast<int64_t>(2 * windows);
-            }
-            float acc[NP][4] = {};
-            constexpr int AHEAD = NP == 4 ? 2 : 4;
-            for (int w0 = warp; w0 < windows; w0 += AHEAD * kMoeWarps) {
-                uint4 q[AHEAD][2], b[AHEAD][NP];
-                float2 unit[AHEAD][NP];
+            for (int k = 0; k < AHEAD; ++k) {
+                const int w = w0 + k;
+                const bool in = w < w_end && 64 * w + 16 * t < a.F;
                 #pragma unroll
-                for (int k = 0; k < AHEAD; ++k) {
-                    const int w = w0 + k * kMoeWarps;
-                    const bool in = 64 * w + 16 * t < a.F;
-                    #pragma unroll
-                    for (int j = 0; j < 2; ++j) q[k][j] = load_stream(rows[j] + 64 * w, in);
-                    #pragma unroll
-                    for (int n = 0; n < NP; ++n) {
-                        b[k][n] = make_uint4(0u, 0u, 0u, 0u);
-                        unit[k][n] = make_float2(0.0f, 0.0f);
-                        if (w < windows) {
-                            if (on[n]) b[k][n] = *reinterpret_cast<const uint4*>(hd[n] + 64 * w);
-                            unit[k][n] = *reinterpret_cast<const float2*>(hs[n] + 2 * w);
-                        }
-                    }
-                }
+                for (int j = 0; j < 2; ++j) q[k][j] = load_stream(rows[j] + 64 * w, in);
                 #pragma unroll
-                for (int k = 0; k < AHEAD; ++k) {
-                    const uint32_t lo[4] = {q[k][0].x, q[k][1].x, q[k][0].y, q[k][1].y};
-                    const uint32_t hi[4] = {q[k][0].z, q[k][1].z, q[k][0].w, q[k][1].w};
-                    #pragma unroll
-                    for (int n = 0; n < NP; ++n) {
-                        int d[2][4];
-                        #pragma unroll
-                        for (int c = 0; c < 4; ++c) d[0][c] = d[1][c] = kMagicBits;
-                        mma_s8_16832(d[0], lo, b[k][n].x, b[k][n].y);
-                        mma_s8_16832(d[1], hi, b[k][n].z, b[k][n].w);
-                        #pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            acc[n][c] = fmaf(__int_as_float(d[0][c]) - kMagic, unit[k][n].x, acc[n][c]);
-                            acc[n][c] = fmaf(__int_as_float(d[1][c]) - kMagic, unit[k][n].y, acc[n][c]);
-                        }
+                for (int n = 0; n < NP; ++n) {
+                    b[k][n] = make_uint4(0u, 0u, 0u, 0u);
+                    unit[k][n] = make_float2(0.0f, 0.0f);
+                    if (w < w_end) {
+                        if (on[n]) b[k][n] = *reinterpret_cast<const uint4*>(hd[n] + 64 * w);
+                        unit[k][n] = *reinterpret_cast<const float2*>(hs[n] + 2 * w);
                     }
                 }
             }
             #pragma unroll
-            for (int n = 0; n < NP; ++n) {
-                // Lane (g, t) has digits 2 (t % 2) and 2 (t % 2) + 1 of token t / 2.
-                const int m = token_of(r.tokens[e], j0 + 2 * n + (t >> 1));
-                const float weight = m >= 0 ? r.weight[pair_of(a, r, m, e)] : 0.0f;
+            for (int k = 0; k < AHEAD; ++k) {
+                const uint32_t lo[4] = {q[k][0].x, q[k][1].x, q[k][0].y, q[k][1].y};
+                const uint32_t hi[4] = {q[k][0].z, q[k][1].z, q[k][0].w, q[k][1].w};
                 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    float v = fmaf(acc[n][2 * j + 1], 256.0f, acc[n][2 * j]);
-                    v = fmaf(__shfl_xor_sync(0xffffffffu, v, 1), (t & 1) ? 0.0f : 65536.0f, v);
-                    if (m >= 0 && !(t & 1)) mine[m * 16 + 8 * j + g] += v * scale[j] * weight;
+                for (int n = 0; n < NP; ++n) {
+                    int d[2][4];
+                    #pragma unroll
+                    for (int c = 0; c < 4; ++c) d[0][c] = d[1][c] = kMagicBits;
+                    mma_s8_16832(d[0], lo, b[k][n].x, b[k][n].y);
+                    mma_s8_16832(d[1], hi, b[k][n].z, b[k][n].w);
+                    #pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        acc[n][c] = fmaf(__int_as_float(d[0][c]) - kMagic, unit[k][n].x, acc[n][c]);
+                        acc[n][c] = fmaf(__int_as_float(d[1][c]) - kMagic, unit[k][n].y, acc[n][c]);
+                    }
+                }
+            }
+        }
+        #pragma unroll
+        for (int n = 0; n < NP; ++n) {
+            // Lane (g, t) has digits 2 (t % 2) and 2 (t % 2) + 1 of token t / 2.
+            const int j = 2 * n + (t >> 1);
+            #pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                float v = fmaf(acc[n][2 * i + 1], 256.0f, acc[n][2 * i]);
+                v = fmaf(__shfl_xor_sync(0xffffffffu, v, 1), (t & 1) ? 0.0f : 65536.0f, v);
+                if (j < job.count && !(t & 1)) {
+                    mine[r.token[job.pos + j] * 16 + 8 * i + g] += v * scale[i] * r.weight[r.pair[job.pos + j]];
                 }
             }
         }
     }
     __syncthreads();
     for (int i = tid; i < a.M * 16; i += kMoeThreads) {
-        const int m = i / 16, n = n0 + i % 16;
         float v = 0.0f;
         #pragma unroll
         for (int w = 0; w < kMoeWarps; ++w) v += outs[w * a.M * 16 + i];
+        outs[i] = v;  // (only this thread reads or writes place i of any warp)
+    }
+    sm100::cluster_sync();
+    for (int i = rank * kMoeThreads + tid; i < a.M * 16; i += a.split * kMoeThreads) {
+        const int m = i / 16, n = n0 + i % 16;
+        float v = 0.0f;
+        for (int c = 0; c < a.split; ++c) {
+            float x;
+            asm volatile("ld.shared::cluster.f32 %0, [%1];"
+                         : "=f"(x)
+                         : "r"(sm100::mapa_shared(sm100::smem_addr(outs + i), c))
+                         : "memory");
+            v += x;
+        }
         if (n < a.K) a.out[static_cast<int64_t>(m) * a.K + n] = v;
     }
+    sm100::cluster_sync();  // no block leaves while another reads its sums
 }
 
 // --------------------------------------------------- any sizes and alignment
@@ -600,18 +647,26 @@ int64_t lay_out(MoeArgs& a, char* ws, int64_t M, bool tensor, bool own_picks) {
 }
 
 template <int NP>
-cudaError_t run_tensor(const MoeArgs& a, cudaStream_t stream) {
-    const int sms = device_sm_count();
-    cudaLaunchAttribute attr[1];
+cudaError_t run_tensor(MoeArgs a, cudaStream_t stream) {
+    const int64_t sms = device_sm_count();
+    cudaLaunchAttribute attr[2];
     // Items of the chosen experts are dealt out to one wave of blocks.
-    const int per_sm = NP == 1 ? 3 : 2;
-    const int64_t items = static_cast<int64_t>(a.E < a.M * a.top ? a.E : a.M * a.top) * (a.fp / 32);
-    const int64_t grid = items < static_cast<int64_t>(per_sm) * sms ? items : static_cast<int64_t>(per_sm) * sms;
-    cudaLaunchConfig_t cfg = pdl_config(dim3(static_cast<unsigned>(grid)), dim3(kMoeThreads), 0, stream, attr);
+    const int64_t jobs = a.M * a.top;  // at most
+    const int64_t items = jobs * (a.fp / 32), wave = (NP == 1 ? 3 : 2) * sms;
+    cudaLaunchConfig_t cfg =
+        pdl_config(dim3(static_cast<unsigned>(items < wave ? items : wave)), dim3(kMoeThreads), 0, stream, attr);
     cudaError_t e = cudaLaunchKernelEx(&cfg, up_kernel<NP>, a);
     if (e != cudaSuccess) return e;
-    cfg.gridDim = dim3(static_cast<unsigned>(ceil_div(a.K, 16)));
+    // Enough blocks for three on every SM, at most a cluster of eight.
+    const int64_t tiles = ceil_div(a.K, 16);
+    a.split = 1;
+    while (a.split < 8 && tiles * a.split < 3 * sms) a.split *= 2;
+    cfg.gridDim = dim3(static_cast<unsigned>(tiles * a.split));
     cfg.dynamicSmemBytes = static_cast<size_t>(kMoeWarps) * a.M * 16 * sizeof(float);
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = a.split;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.numAttrs = 2;
     return cudaLaunchKernelEx(&cfg, down_kernel<NP>, a);
 }
 

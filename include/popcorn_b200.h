@@ -148,7 +148,8 @@ popcornStatus_t popcornDequantizeMatmulNoAlloc_i8f32(
  * likewise, 0x1000 the per-group int8 decode kernel likewise. Bits 0x2000 and
  * 0x4000 (shifted by 16) come from popcorn_serve.h: an append or read-back,
  * or an attention call, met a page index, position or length outside the
- * cache or its table and skipped it. */
+ * cache or its table and skipped it; 0x8000 from a bounded wait of the
+ * attention kernel for prompts. */
 int popcornB200DeviceErrors(unsigned int* flags);
 
 /*

@@ -28,15 +28,14 @@
 //    in f32. For f32 each tile's product starts from zero and is added to the
 //    running sum by an ordinary f32 add: the tensor cores' accumulation
 //    truncates, which over hundreds of tiles costs more than f32 should lose.
-//  * Work is the list of (sequence, row tile, key head) tasks, cut into equal
-//    runs of 16-token tiles over all blocks whatever the lengths are (lengths
-//    are on the device; every block finds its run by a scan over them). A task
-//    that spans blocks leaves partial (m, l, sum) triples, joined in a fixed
-//    order by kv_join_kernel.
-#include <cmath>
+//  * Tasks of 16-token tiles, cut into equal runs over one wave of blocks
+//    (kv_attention.cuh); split tasks are joined by kv_join_kernel.
+//
+// Sequences with more query rows than one tile of 16 go to the kernel of
+// kv_prompt.cu where it takes their type and dim.
 #include <type_traits>
 
-#include "kv.cuh"
+#include "kv_attention.cuh"
 #include "mma_frag.cuh"
 
 namespace pcb {
@@ -48,59 +47,7 @@ constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr float kMagic = 12582912.0f;       // 1.5 2^23
 constexpr int kMagicBits = 0x4B400000;
-constexpr float kLift = 6.0f;               // probabilities are scaled by 2^6
-constexpr float kSlack = 8.0f;              // and may exceed the running maximum by 2^8
 constexpr int kTaskUnits = 8;               // a task's fixed cost in tiles (its queries, its join)
-
-struct AttnArgs {
-    void* out;
-    float* lse;
-    const void* q;
-    int64_t q_tok, q_head;
-    const int8_t* k;
-    const int8_t* v;
-    const float* ks;
-    const float* vs;
-    const int32_t* table;
-    const int32_t* first;
-    const int32_t* length;
-    int64_t table_pages, pages, window;
-    int seqs, tokens, heads, group, dim, page_shift, causal;
-    float scale_log2;   // scale * log2(e)
-    int q_vec;          // query rows start on four-element boundaries
-    int by_task;        // join entries are indexed by task (else by block)
-    int entries;
-    int4* entry;        // [0]: number of entries; then two words each, per task or block
-    float2* ml;         // [2 blocks][rows]: maximum, denominator
-    float* part;        // [2 blocks][rows][DP]
-};
-
-struct Seq {  // one sequence's share of the work
-    int row0, rows;     // first query token, number of them
-    int len;            // visible length
-    int lo;             // first token of the first tile
-    int tiles;          // 16-token tiles that some query may see
-};
-
-__device__ __forceinline__ Seq sequence(const AttnArgs& a, int b) {
-    Seq s;
-    s.row0 = a.first ? a.first[b] : b;
-    s.rows = a.first ? a.first[b + 1] - s.row0 : 1;
-    if (s.row0 < 0 || s.rows < 0 || s.rows > a.tokens - s.row0) s.rows = 0;
-    const int64_t most = a.table_pages << a.page_shift;
-    int64_t len = a.length[b];
-    if (len > most) {
-        atomicOr(&g_attn_err, kKvErrAttention);
-        len = most;
-    }
-    s.len = static_cast<int>(max(len, int64_t{0}));
-    int64_t lo = 0;
-    if (a.window > 0) lo = max(int64_t{0}, static_cast<int64_t>(s.len) - s.rows + 1 - a.window);
-    lo = min(lo, static_cast<int64_t>(s.len));
-    s.lo = static_cast<int>(lo) & ~15;
-    s.tiles = (s.len - s.lo + 15) >> 4;
-    return s;
-}
 
 __device__ __forceinline__ void mma_f16_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile(
@@ -114,12 +61,6 @@ __device__ __forceinline__ void mma_f16_16816(float (&d)[4], const uint32_t (&a)
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     uint32_t y;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
-    return y;
-}
-
-__device__ __forceinline__ float exp2_fast(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
 
@@ -251,25 +192,6 @@ struct Traits<float> {
     static constexpr bool kFresh = true;
 };
 
-// Joins W partial results of one row: element d of sums at stride `pitch`.
-// factor(w) scales partial w to the joint maximum.
-__device__ __forceinline__ float join_factor(float m, float top) { return m == -INFINITY ? 0.0f : exp2_fast(m - top); }
-
-template <typename T>
-__device__ __forceinline__ void store_row(const AttnArgs& a, int64_t t, int head, int d, const float (&o)[4], float l,
-                                          float top, bool lead) {
-    T* out = static_cast<T*>(a.out) + (t * (a.heads * a.group) + head) * a.dim;
-    const float inv = l != 0.0f ? 1.0f / l : 0.0f;  // l = 0: the row sees nothing (a NaN l stays NaN)
-    if (d < a.dim) {
-        const float r[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
-        store4(out + d, true, r);
-    }
-    if (lead && a.lse) {
-        a.lse[t * (a.heads * a.group) + head] =
-            l != 0.0f ? (top - kLift + log2f(l)) * 0.69314718055994531f : -INFINITY;
-    }
-}
-
 // DP: dim rounded up to 64, 128 or 256; FULL: dim is DP.
 template <typename T, int DP, int NT, bool FULL>
 __global__ void __launch_bounds__(kThreads, Traits<T>::kFresh || NT == 2 || DP == 256 ? (DP == 256 ? 2 : 3) : 4)
@@ -283,8 +205,6 @@ kv_rows_kernel(const AttnArgs a) {
     constexpr int NJ = DP / 16;                // 16-wide steps of dim in the value product
     __shared__ float s_ml[kWarps][ROWS][2];
     __shared__ __align__(16) float s_o[kWarps][ROWS][DP];
-    __shared__ int64_t s_scan[kWarps], s_tasks[kWarps], s_from, s_task0;
-    __shared__ int s_b;
 
     const int dim = FULL ? DP : a.dim;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -292,75 +212,25 @@ kv_rows_kernel(const AttnArgs a) {
     pdl_launch_dependents();
     pdl_wait();
 
-    // --- this block's run of tiles ------------------------------------------
-    int64_t total = 0, all_tasks = 0, run0 = 0, run1 = 0, blocks = 1;
-    for (int pass = 0; pass < 2; ++pass) {
-        int64_t seen = 0, tasks = 0;
-        for (int base = 0; base < a.seqs; base += kThreads) {
-            int64_t mine = 0, mine_tasks = 0;
-            if (base + tid < a.seqs) {
-                const Seq s = sequence(a, base + tid);
-                mine_tasks = static_cast<int64_t>((static_cast<int64_t>(s.rows) * a.group + ROWS - 1) / ROWS) * a.heads;
-                mine = mine_tasks * (kTaskUnits + max(s.tiles, 1));
-            }
-            int64_t x = mine, y = mine_tasks;
-            #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int64_t u = __shfl_up_sync(0xffffffffu, x, o), w = __shfl_up_sync(0xffffffffu, y, o);
-                if (lane >= o) x += u, y += w;
-            }
-            __syncthreads();
-            if (lane == 31) s_scan[warp] = x, s_tasks[warp] = y;
-            __syncthreads();
-            int64_t before = seen, before_tasks = tasks;
-            #pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                if (w < warp) before += s_scan[w], before_tasks += s_tasks[w];
-                seen += s_scan[w], tasks += s_tasks[w];
-            }
-            const int64_t from = before + x - mine;
-            // One chunk holds every sequence: its scan serves both passes.
-            if (a.seqs <= kThreads) {
-                total = seen;
-                blocks = max(int64_t{1}, min(static_cast<int64_t>(gridDim.x), total / (kTaskUnits + kWarps)));
-                if (blockIdx.x < blocks) {
-                    run0 = blockIdx.x * total / blocks;
-                    run1 = (blockIdx.x + 1) * total / blocks;
-                }
-            }
-            if ((pass == 1 || a.seqs <= kThreads) && run0 >= from && run0 < from + mine) {
-                s_b = base + tid;
-                s_from = from;
-                s_task0 = before_tasks + y - mine_tasks;
-            }
-        }
-        total = seen;
-        all_tasks = tasks;
-        if (pass == 0) {
-            blocks = max(int64_t{1}, min(static_cast<int64_t>(gridDim.x), total / (kTaskUnits + kWarps)));
-            if (blockIdx.x < blocks) {
-                run0 = blockIdx.x * total / blocks;
-                run1 = (blockIdx.x + 1) * total / blocks;
-            }
-            if (a.seqs <= kThreads) break;
-        }
-    }
-    __syncthreads();
-    if (tid == 0) {
-        if (a.by_task) {
-            if (blockIdx.x == 0) a.entry[0] = make_int4(static_cast<int>(all_tasks), 0, 0, 0);
-        } else {
-            if (blockIdx.x == 0) a.entry[0] = make_int4(static_cast<int>(gridDim.x), 0, 0, 0);
-            a.entry[1 + 2 * blockIdx.x] = make_int4(0, 0, 0, 0);
-        }
-    }
-    if (run0 >= run1) return;
-    int b = s_b;
-    int64_t from = s_from, task0 = s_task0;
+    // A sequence's tiles are those that its first and last query see together.
+    const auto tiles_of = [&](const Seq& s, Span& see) {
+        see = span_of(a, s, 0, s.rows - 1);
+        return (see.hi - see.lo + 15) >> 4;
+    };
+    const Run run = find_run<kThreads>(a.seqs, kTaskUnits + kWarps, [&](int b, int64_t& units, int64_t& tasks) {
+        const Seq s = sequence(a, b, &g_attn_err);
+        Span see;
+        tasks = static_cast<int64_t>((s.rows * a.group + ROWS - 1) / ROWS) * a.heads;
+        units = tasks * (kTaskUnits + max(tiles_of(s, see), 1));
+    });
+    if (tid == 0) clear_entries(a, run);
+    int64_t run0 = run.begin, from = run.from, task0 = run.task0;
+    int b = run.b;
 
-    while (run0 < run1) {
-        const Seq s = sequence(a, b);
-        const int tiles = max(s.tiles, 1);
+    while (run0 < run.end) {
+        const Seq s = sequence(a, b, &g_attn_err);
+        Span see;
+        const int seen_tiles = tiles_of(s, see), tiles = max(seen_tiles, 1);
         const int row_tiles = (s.rows * a.group + ROWS - 1) / ROWS;
         const int each = kTaskUnits + tiles;
         const int64_t units = static_cast<int64_t>(row_tiles) * a.heads * each;
@@ -372,7 +242,7 @@ kv_rows_kernel(const AttnArgs a) {
         }
         const int task = static_cast<int>((run0 - from) / each);
         const int c0 = static_cast<int>((run0 - from) % each);
-        const int c1 = static_cast<int>(min(static_cast<int64_t>(each), c0 + (run1 - run0)));
+        const int c1 = static_cast<int>(min(static_cast<int64_t>(each), c0 + (run.end - run0)));
         run0 += c1 - c0;
         const int u0 = max(0, c0 - kTaskUnits), u1 = c1 - kTaskUnits;
         if (u1 <= 0) continue;  // only the fixed cost fell into this run: the next block has it all
@@ -385,10 +255,10 @@ kv_rows_kernel(const AttnArgs a) {
         const int64_t all0 = a.window > 0 ? static_cast<int64_t>(s.len) - s.rows + tok_hi + 1 - a.window : 0;
 
         const int32_t* table = a.table + static_cast<int64_t>(b) * a.table_pages;
-        const int last = min(u1, s.tiles);
+        const int last = min(u1, seen_tiles);
         const int page_mask = (1 << a.page_shift) - 1;
         const auto page_of = [&](int tile) {
-            return tile < last ? table[(s.lo + 16 * tile) >> a.page_shift] : 0;
+            return tile < last ? table[(see.lo + 16 * tile) >> a.page_shift] : 0;
         };
         // This lane's pieces: keys of rows g, g + 8, values of rows 2 t, 2 t + 1
         // and those eight further.
@@ -398,7 +268,7 @@ kv_rows_kernel(const AttnArgs a) {
         float ks = 0.0f, vs = 0.0f;
         const auto load_k = [&](int tile, int page) {
             const int64_t at = static_cast<int64_t>(page) * a.heads + h;
-            const int8_t* p = k_lane + ((at << a.page_shift) + ((s.lo + 16 * tile) & page_mask)) * dim;
+            const int8_t* p = k_lane + ((at << a.page_shift) + ((see.lo + 16 * tile) & page_mask)) * dim;
             #pragma unroll
             for (int r = 0; r < 2; ++r) {
                 #pragma unroll
@@ -410,7 +280,7 @@ kv_rows_kernel(const AttnArgs a) {
         };
         const auto load_v = [&](int tile, int page) {
             const int64_t at = static_cast<int64_t>(page) * a.heads + h;
-            const int8_t* p = v_lane + ((at << a.page_shift) + ((s.lo + 16 * tile) & page_mask)) * dim;
+            const int8_t* p = v_lane + ((at << a.page_shift) + ((see.lo + 16 * tile) & page_mask)) * dim;
             #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 #pragma unroll
@@ -502,7 +372,7 @@ kv_rows_kernel(const AttnArgs a) {
             if (!ok_now) ve = 0, vf = 0.0f;
             const float vexp = static_cast<float>(ve), vinv = __int_as_float((127 - ve) << 23);
 
-            const int tok = s.lo + 16 * tile;
+            const int tok = see.lo + 16 * tile;
             const bool whole = ok_now && tok >= all0 && tok + 16 <= all1;
             float p[NT][4];
             bool grow = false;
@@ -656,17 +526,8 @@ kv_rows_kernel(const AttnArgs a) {
             }
         }
         if (tid == 0 && u0 == 0 && (a.by_task || !complete)) {
-            // Blocks that hold the rest of the task: the last one owns its last
-            // unit (block c owns units [c total / blocks, (c + 1) total / blocks)).
-            const int64_t end = from + static_cast<int64_t>(task + 1) * each;
-            const int64_t owner = complete ? blockIdx.x : (end * blocks - 1) / total;
-            const int more = static_cast<int>(owner - blockIdx.x);
-            const int64_t e = a.by_task ? task0 + task : blockIdx.x;
-            // (A `first` that does not ascend can make more tasks than there are.)
-            if (e < a.entries) {
-                a.entry[1 + 2 * e] = make_int4(more, blockIdx.x, s.row0, s.rows);
-                a.entry[2 + 2 * e] = make_int4(task, 0, 0, 0);
-            }
+            const int owner = complete ? blockIdx.x : owner_of_last(run, from + static_cast<int64_t>(task + 1) * each);
+            put_entry(a, task0 + task, owner - blockIdx.x, s, task);
         }
     }
 }
@@ -819,13 +680,41 @@ cudaError_t run_attention(const AttnArgs& a, int64_t max_tokens, void* ws, int64
     return run(std::integral_constant<int, 256>{}, one);
 }
 
-cudaError_t run_typed(popcornType_t type, const AttnArgs& a, int64_t max_tokens, void* ws, int64_t* ws_bytes,
-                      cudaStream_t stream) {
+cudaError_t run_rows_typed(popcornType_t type, const AttnArgs& a, int64_t max_tokens, void* ws, int64_t* ws_bytes,
+                           cudaStream_t stream) {
     switch (type) {
         case POPCORN_TYPE_F32: return run_attention<float>(a, max_tokens, ws, ws_bytes, stream);
         case POPCORN_TYPE_F16: return run_attention<__half>(a, max_tokens, ws, ws_bytes, stream);
         default: return run_attention<__nv_bfloat16>(a, max_tokens, ws, ws_bytes, stream);
     }
+}
+
+// Launches the kernel, or the two, that the sizes ask for; with ws_bytes only
+// says how much workspace they take. Sequences of up to 16 query rows go to
+// kv_rows_kernel and longer ones to the prompt kernel, each of which skips the
+// other's; where all sequences have max_tokens queries only one is launched.
+cudaError_t run_typed(popcornType_t type, AttnArgs a, int64_t max_tokens, void* ws, int64_t* ws_bytes,
+                      cudaStream_t stream) {
+    a.min_rows = 1, a.max_rows = INT32_MAX;
+    if (max_tokens * a.group < kPromptRows || !prompt_supported(type, a.dim)) {
+        return run_rows_typed(type, a, max_tokens, ws, ws_bytes, stream);
+    }
+    const bool both = a.tokens != max_tokens * a.seqs;
+    const int64_t few = (kPromptRows - 1) / a.group;  // queries of a sequence that kv_rows_kernel keeps
+    AttnArgs rows = a;
+    rows.max_rows = kPromptRows - 1;
+    a.min_rows = kPromptRows;
+    int64_t bytes = 0, more = 0;
+    cudaError_t e = cudaSuccess;
+    if (ws_bytes != nullptr) {
+        e = run_prompt(type, a, nullptr, &bytes, stream);
+        if (e == cudaSuccess && both && few > 0) e = run_rows_typed(type, rows, few, nullptr, &more, stream);
+        *ws_bytes = bytes > more ? bytes : more;
+        return e;
+    }
+    e = run_prompt(type, a, ws, nullptr, stream);
+    if (e == cudaSuccess && both && few > 0) e = run_rows_typed(type, rows, few, ws, nullptr, stream);
+    return e;
 }
 
 // Argument checks that the workspace query shares with the call.
@@ -848,8 +737,11 @@ AttnArgs attention_sizes(const popcornKvCache_t& c, int64_t seqs, int64_t tokens
 
 cudaError_t kv_attention_take_errors(unsigned int* bits) {
     const unsigned int zero = 0;
+    unsigned int prompt = 0;
     cudaError_t e = cudaMemcpyFromSymbol(bits, g_attn_err, sizeof(unsigned int));
     if (e == cudaSuccess && *bits != 0) e = cudaMemcpyToSymbol(g_attn_err, &zero, sizeof(unsigned int));
+    if (e == cudaSuccess) e = kv_prompt_take_errors(&prompt);
+    *bits |= prompt;
     return e;
 }
 

@@ -1,0 +1,715 @@
+// Attention over the paged 8-bit cache for many query rows of one sequence
+// (prompt chunks), f16 and bf16, dim 64 or 128: tcgen05 on f16 operands.
+//
+// Rows are a sequence's queries times the heads that share a key head. A task
+// is 256 of them, two tiles of 128 (the tensor instruction's M), against all
+// tokens they see in tiles of 128; what it has to do is 4 dim flops a
+// (row, token) pair, so it is bound by the tensor cores and, almost as
+// closely, by one exponential a pair (16 a cycle and SM: 2048 cycles for the
+// 256 x 128 pairs of a step, the same as its two products take).
+//
+//   scores S = Q K^T: Q as f16 in shared memory (each row scaled by a power
+//       of two, exact for f16, and for bf16 down to 2^-24 of the row's largest
+//       element), key codes as f16 (exact), f32 sums in tensor memory
+//   P = exp2(S ks f + log2(vs) - m): the block scales are constant over 16
+//       tokens at least; f16, written over S in tensor memory
+//   O += P V: value codes as f16 (exact), transposed on the way into shared
+//       memory, f32 sums in tensor memory
+//
+// Warps 0-3 and 4-7 are the softmax of the two tiles (a thread owns a row, so
+// maxima and sums need no exchange), 8-11 convert codes, one thread of warp 12
+// issues the products: while one tile's softmax runs, the tensor cores work on
+// the other's. The maximum moves only when a score exceeds it by 2^8 (then the
+// thread rescales O in tensor memory), as in kv_attention.cu, whose scaling
+// conventions, work split and partial results these are.
+//
+// Every wait is bounded (sm100.cuh); one that runs out sets error bit 0x8000
+// and ends the block.
+#include "kv_attention.cuh"
+#include "sm100.cuh"
+
+namespace pcb {
+namespace {
+
+using namespace sm100;
+
+__device__ unsigned int g_prompt_err = 0;
+constexpr unsigned int kErrWait = 0x8000u;
+
+constexpr int kTile = 128;          // rows of a tile, tokens of a step
+constexpr int kRows = 2 * kTile;    // rows of a task
+constexpr int kSoftWarps = 8, kConvWarps = 4;
+constexpr int kPThreads = 32 * (kSoftWarps + kConvWarps + 1);
+constexpr int kConvThreads = 32 * kConvWarps;
+constexpr int kStages = 2;
+constexpr int kScaleRing = 4;
+constexpr int kFixedUnits = 2;      // a task's fixed cost in steps
+
+// Barriers, 8 bytes each.
+enum Bar { kKFull = 0, kKEmpty = 2, kVFull = 4, kVEmpty = 6, kSFull = 8, kPReady = 10, kODone = 12, kQReady = 14, kDrain = 16, kBars = 17 };
+
+template <int DP>
+struct Lay {  // shared memory, bytes; operand tiles in 128-byte swizzled rows
+    static constexpr int kQTile = DP / 64 * kTile * 128;
+    static constexpr int kKStage = DP / 64 * kTile * 128;
+    static constexpr int kVStage = 2 * DP * 128;
+    static constexpr int kQ = 0;
+    static constexpr int kK = kQ + 2 * kQTile;
+    static constexpr int kV = kK + kStages * kKStage;
+    static constexpr int kScales = kV + kStages * kVStage;  // [ring][8] {ks, log2 vs, 1 / vs}
+    static constexpr int kBytes = kScales + kScaleRing * 8 * 16;
+    static constexpr int kAlloc = kBytes + 1024;            // the tiles start on 1024 bytes
+};
+
+struct GroupScale {
+    float ks, lv, iv, pad;
+};
+
+__device__ __forceinline__ void mma_f16_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                           uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+__device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+__device__ __forceinline__ void store_shared16(uint32_t addr, const uint32_t (&v)[4]) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3])
+                 : "memory");
+}
+
+__device__ __forceinline__ uint32_t as_f16(uint32_t biased) {  // halves 1024 + code + 128
+    const __half2 c = __half2{__float2half_rn(1152.0f), __float2half_rn(1152.0f)};
+    const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&biased), c);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Walks a block's run segment by segment; every role walks the same way.
+struct Walk {
+    const AttnArgs& a;
+    const Run& run;
+    int64_t at, from, task0;
+    int b, rt;
+    Seq s;
+    Span see;             // of the row tile
+    int each, steps;      // units and steps of a task of this row tile
+    int task_in_tile;     // key head
+    int u0, u1;           // the segment's steps
+    bool complete;
+    int more;             // blocks after this one that hold the rest
+    int64_t task_number;
+
+    __device__ Walk(const AttnArgs& args, const Run& r)
+        : a(args), run(r), at(r.begin), from(r.from), task0(r.task0), b(r.b), rt(0) {
+        if (at < run.end) s = sequence(a, b, &g_prompt_err), tile_sizes();
+    }
+    __device__ int row_tiles() const { return (s.rows * a.group + kRows - 1) / kRows; }
+    __device__ void tile_sizes() {
+        see = span_of(a, s, rt * kRows / a.group, min(s.rows - 1, (rt * kRows + kRows - 1) / a.group));
+        steps = max((see.hi - see.lo + kTile - 1) / kTile, 1);
+        each = kFixedUnits + steps;
+    }
+    __device__ bool next() {
+        while (at < run.end) {
+            if (s.rows == 0 || rt >= row_tiles()) {
+                ++b;
+                rt = 0;
+                s = sequence(a, b, &g_prompt_err);
+                if (s.rows > 0) tile_sizes();
+                continue;
+            }
+            const int64_t units = static_cast<int64_t>(each) * a.heads;
+            if (at >= from + units) {
+                from += units;
+                task0 += a.heads;
+                if (++rt < row_tiles()) tile_sizes();
+                continue;
+            }
+            task_in_tile = static_cast<int>((at - from) / each);
+            const int c0 = static_cast<int>((at - from) % each);
+            const int c1 = static_cast<int>(min(static_cast<int64_t>(each), c0 + (run.end - at)));
+            at += c1 - c0;
+            u0 = max(0, c0 - kFixedUnits);
+            u1 = c1 - kFixedUnits;
+            if (u1 <= 0) continue;
+            complete = u0 == 0 && u1 == steps;
+            more = complete ? 0 : owner_of_last(run, from + static_cast<int64_t>(task_in_tile + 1) * each) - static_cast<int>(blockIdx.x);
+            task_number = task0 + task_in_tile;
+            return true;
+        }
+        return false;
+    }
+    __device__ int tiles() const { return s.rows * a.group - rt * kRows > kTile ? 2 : 1; }
+};
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const AttnArgs a) {
+    using L = Lay<DP>;
+    extern __shared__ uint8_t raw[];
+    __shared__ __align__(8) uint64_t bars[kBars];
+    __shared__ uint32_t s_tmem;
+    const uint32_t smem = (smem_addr(raw) + 1023u) & ~1023u;
+    GroupScale* const ring = reinterpret_cast<GroupScale*>(raw + (smem - smem_addr(raw)) + L::kScales);
+    const uint32_t bar0 = smem_addr(bars);
+    const auto bar = [&](int which, int i) { return bar0 + 8u * (which + i); };
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    unsigned int* const err = &g_prompt_err;
+    // A warp's lanes go on together, or none does.
+    const auto wait = [&](int which, int i, int turn) {
+        return __all_sync(0xffffffffu, mbar_wait(bar(which, i), turn & 1, err, kErrWait)) != 0;
+    };
+
+    if (tid == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(bar(kKFull, i), kConvThreads);
+            mbar_init(bar(kKEmpty, i), 1);
+            mbar_init(bar(kVFull, i), kConvThreads);
+            mbar_init(bar(kVEmpty, i), 1);
+            mbar_init(bar(kSFull, i), 1);
+            mbar_init(bar(kPReady, i), kTile);
+            mbar_init(bar(kODone, i), 1);
+            mbar_init(bar(kQReady, i), kTile);
+        }
+        mbar_init(bar(kDrain, 0), 1);
+        fence_barrier_init();
+    }
+    // Tensor memory is taken only when the kernel before has ended, and the one
+    // after may start only when it has been taken: neither can hold columns
+    // that the other waits for.
+    pdl_wait();
+    if (warp == kSoftWarps + kConvWarps) {
+        tmem_alloc(smem_addr(&s_tmem), 512);
+        tmem_relinquish();
+    }
+    pdl_launch_dependents();
+    const Run run = find_run<kPThreads>(a.seqs, kFixedUnits + 1, [&](int b, int64_t& units, int64_t& tasks) {
+        const Seq s = sequence(a, b, &g_prompt_err);
+        for (int r = 0; r < s.rows * a.group; r += kRows) {
+            const Span see = span_of(a, s, r / a.group, min(s.rows - 1, (r + kRows - 1) / a.group));
+            units += static_cast<int64_t>(kFixedUnits + max((see.hi - see.lo + kTile - 1) / kTile, 1)) * a.heads;
+            tasks += a.heads;
+        }
+    });
+    if (tid == 0) clear_entries(a, run);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
+    // Columns: S and P of the two tiles at 0 and 128, O at 256 and 384.
+
+    Walk walk(a, run);
+    if (warp < kSoftWarps) {
+        // ----------------------------------------------------------- softmax
+        const int m = warp >> 2;                    // tile
+        const int row = tid & (kTile - 1);
+        const uint32_t lanes = tmem + (static_cast<uint32_t>(warp & 3) << 21);  // this warp's 32 lanes
+        const uint32_t s_col = lanes + 128 * m, o_col = lanes + 256 + 128 * m;
+        int steps_done = 0;                         // of this tile, over all segments
+        int ring_at = 0;                            // steps of the block, both tiles
+        bool good = true;
+        while (good && walk.next()) {
+            const int n = walk.u1 - walk.u0;
+            if (m >= walk.tiles()) {
+                ring_at += n;
+                continue;
+            }
+            const int r = walk.rt * kRows + m * kTile + row;
+            const int tok = r / a.group, hd = r - tok * a.group;
+            const bool valid = r < walk.s.rows * a.group;
+            const int head = walk.task_in_tile * a.group + hd;
+            // --- the query row: a power of two brings its largest element to [2^9, 2^10)
+            float fac;
+            {
+                const T* q = static_cast<const T*>(a.q) + (walk.s.row0 + tok) * a.q_tok + head * a.q_head;
+                float top = 0.0f;
+                bool bad = false;
+                #pragma unroll 4
+                for (int d = 0; d < DP; d += 4) {
+                    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    if (valid) load4(q + d, a.q_vec != 0, v);
+                    #pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        top = fmaxf(top, fabsf(v[j]));
+                        bad = bad || !(fabsf(v[j]) <= 3.4028234663852886e38f);
+                    }
+                }
+                const int e = max(-126, min(120, 9 + 127 - static_cast<int>(__float_as_uint(top) >> 23)));
+                const float up = bad ? 0.0f : __int_as_float((127 + e) << 23);
+                const uint32_t base = smem + L::kQ + m * L::kQTile + row * 128;
+                #pragma unroll 4
+                for (int d = 0; d < DP; d += 8) {
+                    float v[8] = {};
+                    if (valid && !bad) {
+                        load4(q + d, a.q_vec != 0, reinterpret_cast<float(&)[4]>(v[0]));
+                        load4(q + d + 4, a.q_vec != 0, reinterpret_cast<float(&)[4]>(v[4]));
+                    }
+                    uint32_t w[4];
+                    #pragma unroll
+                    for (int j = 0; j < 4; ++j) w[j] = pack_f16(v[2 * j] * up, v[2 * j + 1] * up);
+                    store_shared16(base + (d / 64) * (kTile * 128) + ((((d % 64) / 8) ^ (row & 7)) << 4), w);
+                }
+                fac = bad ? __int_as_float(0x7fffffff) : __int_as_float((127 - e) << 23) * a.scale_log2;
+            }
+            fence_async_shared();
+            mbar_arrive(bar(kQReady, m));
+
+            const int64_t pos = static_cast<int64_t>(walk.s.len) - walk.s.rows + tok;
+            int see1 = a.causal ? static_cast<int>(max(pos + 1, int64_t{0})) : walk.s.len;
+            int see0 = a.window > 0 ? static_cast<int>(max(pos + 1 - a.window, int64_t{0})) : 0;
+            see1 = min(see1, walk.s.len);
+            if (!valid) see0 = 0, see1 = INT32_MAX;  // (never stored: no reason to mask)
+            if (see1 <= see0) fac = 0.0f;
+            float top = -INFINITY, den = 0.0f;
+            for (int i = 0; i < n; ++i, ++steps_done, ++ring_at) {
+                if (!(good = wait(kSFull, m, steps_done))) break;
+                tc_fence_after();
+                const GroupScale* gs = ring + (ring_at % kScaleRing) * 8;
+                const int j0 = walk.see.lo + (walk.u0 + i) * kTile;
+                const bool whole = __all_sync(0xffffffffu, see0 <= j0 && j0 + kTile <= see1);
+                // --- maximum
+                float best = -INFINITY;
+                #pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t x[32];
+                    tmem_ld_32x32b_x32(s_col + 32 * c, x);
+                    tmem_wait_ld();
+                    #pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const float kf = gs[2 * c + h].ks * fac, lv = gs[2 * c + h].lv;
+                        if (whole) {
+                            #pragma unroll
+                            for (int j = 0; j < 16; ++j) best = fmaxf(best, fmaf(__uint_as_float(x[16 * h + j]), kf, lv));
+                        } else {
+                            #pragma unroll
+                            for (int j = 0; j < 16; ++j) {
+                                const int k = j0 + 32 * c + 16 * h + j;
+                                if (k >= see0 && k < see1) best = fmaxf(best, fmaf(__uint_as_float(x[16 * h + j]), kf, lv));
+                            }
+                        }
+                    }
+                }
+                const bool grow = best > top + kSlack;
+                if (__any_sync(0xffffffffu, grow)) {
+                    const float now = fmaxf(top, best);
+                    const float by = join_factor(top, now);
+                    top = now;
+                    den *= by;
+                    if (i > 0) {
+                        if (!(good = wait(kODone, m, steps_done - 1))) break;
+                        tc_fence_after();
+                        #pragma unroll
+                        for (int c = 0; c < DP / 32; ++c) {
+                            uint32_t x[32];
+                            tmem_ld_32x32b_x32(o_col + 32 * c, x);
+                            tmem_wait_ld();
+                            #pragma unroll
+                            for (int j = 0; j < 32; ++j) x[j] = __float_as_uint(__uint_as_float(x[j]) * by);
+                            tmem_st_32x32b_x32(o_col + 32 * c, x);
+                        }
+                    }
+                }
+                // --- probabilities, over the scores
+                const float shift = kLift - (top == -INFINITY ? 0.0f : top);
+                #pragma unroll
+                for (int c2 = 0; c2 < 2; ++c2) {
+                    uint32_t w[32];
+                    #pragma unroll
+                    for (int c1 = 0; c1 < 2; ++c1) {
+                        const int c = 2 * c2 + c1;
+                        uint32_t x[32];
+                        tmem_ld_32x32b_x32(s_col + 32 * c, x);
+                        tmem_wait_ld();
+                        #pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const GroupScale g = gs[2 * c + h];
+                            const float kf = g.ks * fac, lv = g.lv + shift;
+                            #pragma unroll
+                            for (int j = 0; j < 16; j += 2) {
+                                float p0 = exp2_fast(fmaf(__uint_as_float(x[16 * h + j]), kf, lv));
+                                float p1 = exp2_fast(fmaf(__uint_as_float(x[16 * h + j + 1]), kf, lv));
+                                if (!whole) {
+                                    const int k = j0 + 32 * c + 16 * h + j;
+                                    if (k < see0 || k >= see1) p0 = 0.0f;
+                                    if (k + 1 < see0 || k + 1 >= see1) p1 = 0.0f;
+                                }
+                                den = fmaf(p0, g.iv, den);
+                                den = fmaf(p1, g.iv, den);
+                                w[16 * c1 + 8 * h + j / 2] = pack_f16(p0, p1);
+                            }
+                        }
+                    }
+                    tmem_st_32x32b_x32(s_col + 32 * c2, w);
+                }
+                tmem_wait_st();
+                tc_fence_before();
+                mbar_arrive(bar(kPReady, m));
+            }
+            if (!good) break;
+            // --- the segment's result
+            if (!(good = wait(kODone, m, steps_done - 1))) break;
+            tc_fence_after();
+            const int64_t slot = (2 * static_cast<int64_t>(blockIdx.x) + (walk.u0 > 0 ? 0 : 1)) * kRows + m * kTile + row;
+            const float inv = inverse(den);
+            T* out = static_cast<T*>(a.out) + ((walk.s.row0 + tok) * static_cast<int64_t>(a.heads * a.group) + head) * DP;
+            #pragma unroll
+            for (int c = 0; c < DP / 32; ++c) {
+                uint32_t x[32];
+                tmem_ld_32x32b_x32(o_col + 32 * c, x);
+                tmem_wait_ld();
+                if (!valid) continue;
+                if (walk.complete) {
+                    #pragma unroll
+                    for (int j = 0; j < 32; j += 8) {
+                        uint4 o;
+                        T* e = reinterpret_cast<T*>(&o);
+                        #pragma unroll
+                        for (int k = 0; k < 8; ++k) e[k] = from_f32<T>(__uint_as_float(x[j + k]) * inv);
+                        *reinterpret_cast<uint4*>(out + 32 * c + j) = o;
+                    }
+                } else {
+                    #pragma unroll
+                    for (int j = 0; j < 32; j += 4) {
+                        *reinterpret_cast<uint4*>(a.part + slot * DP + 32 * c + j) =
+                            make_uint4(x[j], x[j + 1], x[j + 2], x[j + 3]);
+                    }
+                }
+            }
+            if (valid && walk.complete) store_lse(a, walk.s.row0 + tok, head, den, top);
+            if (valid && !walk.complete) a.ml[slot] = make_float2(top, den);
+            if (tid == 0 && walk.u0 == 0 && (a.by_task || !walk.complete)) {
+                put_entry(a, walk.task_number, walk.more, walk.s, walk.rt * a.heads + walk.task_in_tile);
+            }
+            tc_fence_before();  // O has been read: the next segment's products may follow
+        }
+    } else if (warp < kSoftWarps + kConvWarps) {
+        // ----------------------------------------------------------- convert
+        constexpr int CK = DP / 16;                      // 16-byte pieces of a key row
+        constexpr int KN = kTile * CK / kConvThreads;    // pieces per thread and step
+        constexpr int RK = kConvThreads / CK;            // rows between a thread's pieces
+        constexpr int WV = DP / 4;                       // words of a value row
+        constexpr int VO = 16 * WV / kConvThreads;       // runs of 8 tokens (of one word) per thread and step
+        const int ct = tid - 32 * kSoftWarps;
+        const int krow = ct / CK, kpiece = ct % CK;
+        const int vword = ct % WV, voct = ct / WV;       // run voct + i * (kConvThreads / WV)
+        const int page_mask = (1 << a.page_shift) - 1;
+        // The step's eight groups of 16 tokens: lane j < 8 of every warp looks up
+        // group j. -1: nothing there.
+        struct Step {
+            int h, j0, len;
+            int64_t seq;
+        };
+        const auto look_up = [&](const Step& st) {
+            const int j = st.j0 + 16 * (lane & 7);
+            if (j >= st.len) return -1;
+            const int p = a.table[st.seq * a.table_pages + (j >> a.page_shift)];
+            if (p < 0 || p >= a.pages) {
+                if (lane < 8 && warp == kSoftWarps) atomicOr(err, kKvErrAttention);
+                return -1;
+            }
+            return p;
+        };
+        const auto block_of = [&](const Step& st, int pages, int group) -> int64_t {
+            const int p = __shfl_sync(0xffffffffu, pages, group);
+            if (p < 0) return -1;
+            const int j = st.j0 + 16 * group;
+            return (((static_cast<int64_t>(p) * a.heads + st.h) << a.page_shift) + (j & page_mask)) * DP;
+        };
+        uint4 kq[KN];
+        uint32_t vq[VO][8];
+        const auto load_k = [&](const Step& st, int pages) {
+            #pragma unroll
+            for (int i = 0; i < KN; ++i) {
+                const int r = krow + i * RK;
+                const int64_t at = block_of(st, pages, r >> 4);
+                kq[i] = make_uint4(0u, 0u, 0u, 0u);
+                if (at >= 0) kq[i] = *reinterpret_cast<const uint4*>(a.k + at + (r & 15) * DP + 16 * kpiece);
+            }
+        };
+        const auto load_v = [&](const Step& st, int pages) {
+            #pragma unroll
+            for (int i = 0; i < VO; ++i) {
+                const int oct = voct + i * (kConvThreads / WV);
+                const int64_t at = block_of(st, pages, oct >> 1);
+                #pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    vq[i][j] = 0u;
+                    if (at >= 0) {
+                        vq[i][j] = *reinterpret_cast<const uint32_t*>(a.v + at + (8 * (oct & 1) + j) * DP + 4 * vword);
+                    }
+                }
+            }
+        };
+        int kt = 0;  // steps of the block
+        bool good = true;
+        int left = 0;  // steps left in the segment
+        Step cur = {0, 0, 0, 0}, nxt;
+        const auto advance = [&](Step& st) -> bool {
+            if (left == 0) {
+                if (!walk.next()) return false;
+                left = walk.u1 - walk.u0;
+                st.h = walk.task_in_tile;
+                st.seq = walk.b;
+                st.len = min(walk.see.hi, walk.s.len);
+                st.j0 = walk.see.lo + walk.u0 * kTile;
+            } else {
+                st.j0 += kTile;
+            }
+            --left;
+            return true;
+        };
+        bool have = advance(cur);
+        int pages = -1, pages_next = -1;
+        if (have) {
+            pages = look_up(cur);
+            load_k(cur, pages);
+        }
+        while (good && have) {
+            nxt = cur;
+            const bool have_next = advance(nxt);
+            const int stage = kt % kStages, turn = kt / kStages;
+            // Scales of the step's groups.
+            if (warp == kSoftWarps && lane < 8) {
+                GroupScale g = {0.0f, -INFINITY, 1.0f, 0.0f};
+                if (pages >= 0) {
+                    const int64_t at = static_cast<int64_t>(pages) * a.heads + cur.h;
+                    const float vs = a.vs[at];
+                    g.ks = a.ks[at];
+                    const bool tiny = fabsf(vs) < kKvSmallestScale;  // all-zero codes
+                    g.lv = tiny ? -80.0f : log2f(vs);
+                    g.iv = tiny ? 1.0f / kKvSmallestScale : fabsf(vs) <= 3.4028234663852886e38f ? 1.0f / vs : 1.0f;
+                }
+                ring[(kt % kScaleRing) * 8 + lane] = g;
+            }
+            load_v(cur, pages);
+            if (have_next) pages_next = look_up(nxt);
+            if (kt >= kStages && !(good = wait(kKEmpty, stage, turn - 1))) break;
+            #pragma unroll
+            for (int i = 0; i < KN; ++i) {
+                const int r = krow + i * RK;
+                const uint32_t in[4] = {kq[i].x ^ 0x80808080u, kq[i].y ^ 0x80808080u, kq[i].z ^ 0x80808080u,
+                                        kq[i].w ^ 0x80808080u};
+                uint32_t lo[4], hi[4];
+                #pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    lo[2 * j] = as_f16(__byte_perm(in[j], 0x64646464u, 0x4140));
+                    lo[2 * j + 1] = as_f16(__byte_perm(in[j], 0x64646464u, 0x4342));
+                    hi[2 * j] = as_f16(__byte_perm(in[2 + j], 0x64646464u, 0x4140));
+                    hi[2 * j + 1] = as_f16(__byte_perm(in[2 + j], 0x64646464u, 0x4342));
+                }
+                const uint32_t base = smem + L::kK + stage * L::kKStage + (kpiece / 4) * (kTile * 128) + r * 128;
+                const uint32_t unit = 2 * (kpiece % 4);
+                store_shared16(base + (((unit) ^ (r & 7)) << 4), lo);
+                store_shared16(base + (((unit + 1) ^ (r & 7)) << 4), hi);
+            }
+            fence_async_shared();
+            mbar_arrive(bar(kKFull, stage));
+            if (have_next) load_k(nxt, pages_next);
+            if (kt >= kStages && !(good = wait(kVEmpty, stage, turn - 1))) break;
+            #pragma unroll
+            for (int i = 0; i < VO; ++i) {
+                const int oct = voct + i * (kConvThreads / WV);
+                // V transposed: row d, 64 tokens to a 128-byte row. Lanes take the
+                // word's four bytes in different orders, so that eight lanes'
+                // stores fall into eight different 16-byte banks.
+                #pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t byte = (j + (vword >> 1)) & 3;
+                    const uint32_t sel = byte | (byte + 4) << 8;
+                    uint32_t w[4];
+                    #pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const uint32_t x = __byte_perm(vq[i][2 * k], vq[i][2 * k + 1], sel);
+                        w[k] = as_f16((x & 0x00ff00ffu) ^ 0x64806480u);
+                    }
+                    const uint32_t d = 4 * vword + byte;
+                    store_shared16(smem + L::kV + stage * L::kVStage + (oct >> 3) * (DP * 128) + d * 128 +
+                                       (((oct & 7) ^ (d & 7)) << 4),
+                                   w);
+                }
+            }
+            fence_async_shared();
+            mbar_arrive(bar(kVFull, stage));
+            cur = nxt;
+            pages = pages_next;
+            have = have_next;
+            ++kt;
+        }
+    } else if (lane == 0) {
+        // ------------------------------------------------------------- issue
+        constexpr uint32_t id_qk = idesc_f16_f32(kTile, kTile), id_pv = idesc_f16_f32(kTile, DP);
+        int kt = 0, segs[2] = {0, 0}, done[2] = {0, 0};
+        bool good = true;
+        const auto scores = [&](int m, int stage) {
+            #pragma unroll
+            for (int j = 0; j < DP / 16; ++j) {
+                const uint32_t off = (j / 4) * (kTile * 128);
+                mma_f16_ss(tmem + 128 * m,
+                           smem_desc_sw128_kmajor(smem + L::kQ + m * L::kQTile + off) + (j % 4) * 2,
+                           smem_desc_sw128_kmajor(smem + L::kK + stage * L::kKStage + off) + (j % 4) * 2, id_qk, j > 0);
+            }
+            mma_commit(bar(kSFull, m));
+        };
+        while (good && walk.next()) {
+            const int n = walk.u1 - walk.u0, tiles = walk.tiles();
+            for (int m = 0; m < tiles && good; ++m) good = mbar_wait(bar(kQReady, m), segs[m]++ & 1, err, kErrWait);
+            if (!good || !(good = mbar_wait(bar(kKFull, kt % kStages), (kt / kStages) & 1, err, kErrWait))) break;
+            tc_fence_after();
+            for (int m = 0; m < tiles; ++m) scores(m, kt % kStages);
+            mma_commit(bar(kKEmpty, kt % kStages));
+            for (int i = 0; i < n && good; ++i, ++kt) {
+                const int stage = kt % kStages, next = (kt + 1) % kStages;
+                for (int m = 0; m < tiles && good; ++m) {
+                    if (m == 0 && !(good = mbar_wait(bar(kVFull, stage), (kt / kStages) & 1, err, kErrWait))) break;
+                    if (!(good = mbar_wait(bar(kPReady, m), done[m]++ & 1, err, kErrWait))) break;
+                    tc_fence_after();
+                    #pragma unroll
+                    for (int j = 0; j < kTile / 16; ++j) {
+                        mma_f16_ts(tmem + 256 + 128 * m, tmem + 128 * m + 8 * j,
+                                   smem_desc_sw128_kmajor(smem + L::kV + stage * L::kVStage + (j / 4) * (DP * 128)) + (j % 4) * 2,
+                                   id_pv, i > 0 || j > 0);
+                    }
+                    mma_commit(bar(kODone, m));
+                    if (m == tiles - 1) mma_commit(bar(kVEmpty, stage));
+                    if (i + 1 < n) {
+                        // (Over P, which the products just issued still read: products
+                        // of one thread run in the order of their issue.)
+                        if (m == 0 && !(good = mbar_wait(bar(kKFull, next), ((kt + 1) / kStages) & 1, err, kErrWait))) break;
+                        tc_fence_after();
+                        scores(m, next);
+                        if (m == tiles - 1) mma_commit(bar(kKEmpty, next));
+                    }
+                }
+            }
+        }
+    }
+    // Every product has been waited for by the softmax of its tile (kODone),
+    // or a wait ran out: then the issued ones are waited for here.
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kSoftWarps + kConvWarps) {
+        if (lane == 0) {
+            mma_commit(bar(kDrain, 0));
+            mbar_wait(bar(kDrain, 0), 0, err, kErrWait);
+        }
+        __syncwarp();
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+// Joins the partial results of split tasks: a warp takes one row at a time,
+// one entry's rows over eight blocks.
+template <typename T, int DP>
+__global__ void __launch_bounds__(256) kv_prompt_join_kernel(const AttnArgs a) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int entries = a.entry[0].x;
+    const int4 e = a.entry[1 + 2 * blockIdx.x];
+    const int task = a.entry[2 + 2 * blockIdx.x].x;
+    if (static_cast<int>(blockIdx.x) >= entries || e.x == 0) return;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int h = task % a.heads, count = e.x + 1;
+    constexpr int PER = DP / 32;  // elements of a lane
+    #pragma unroll 2
+    for (int i = 0; i < kRows / 64; ++i) {
+        const int r = blockIdx.y * (kRows / 8) + i * 8 + warp;
+        const int row = task / a.heads * kRows + r;
+        if (row >= e.w * a.group) continue;
+        const auto slot = [&](int c) { return static_cast<int64_t>(2 * (e.y + c) + (c == 0 ? 1 : 0)) * kRows + r; };
+        float top = -INFINITY, den = 0.0f, sum[PER] = {};
+        for (int c = 0; c < count; ++c) top = fmaxf(top, a.ml[slot(c)].x);
+        for (int c = 0; c < count; ++c) {
+            const float2 ml = a.ml[slot(c)];
+            const float f = join_factor(ml.x, top);
+            den = fmaf(ml.y, f, den);
+            const float* p = a.part + slot(c) * DP + PER * lane;
+            if constexpr (PER == 4) {
+                const float4 x = *reinterpret_cast<const float4*>(p);
+                sum[0] = fmaf(x.x, f, sum[0]), sum[1] = fmaf(x.y, f, sum[1]);
+                sum[2] = fmaf(x.z, f, sum[2]), sum[3] = fmaf(x.w, f, sum[3]);
+            } else {
+                const float2 x = *reinterpret_cast<const float2*>(p);
+                sum[0] = fmaf(x.x, f, sum[0]), sum[1] = fmaf(x.y, f, sum[1]);
+            }
+        }
+        const int tok = row / a.group, head = h * a.group + row - tok * a.group;
+        const float inv = inverse(den);
+        T* out = static_cast<T*>(a.out) + ((e.z + tok) * static_cast<int64_t>(a.heads * a.group) + head) * DP + PER * lane;
+        T o[PER];
+        #pragma unroll
+        for (int j = 0; j < PER; ++j) o[j] = from_f32<T>(sum[j] * inv);
+        if constexpr (PER == 4) {
+            *reinterpret_cast<uint2*>(out) = *reinterpret_cast<const uint2*>(o);
+        } else {
+            *reinterpret_cast<uint32_t*>(out) = *reinterpret_cast<const uint32_t*>(o);
+        }
+        if (lane == 0) store_lse(a, e.z + tok, head, den, top);
+    }
+}
+
+template <typename T, int DP>
+cudaError_t run_sized(AttnArgs a, void* ws, int64_t* ws_bytes, cudaStream_t stream) {
+    using L = Lay<DP>;
+    const int64_t grid = device_sm_count();
+    const int64_t entry_bytes = (1 + 2 * grid) * sizeof(int4), ml_bytes = 2 * grid * kRows * sizeof(float2);
+    if (ws_bytes != nullptr) {
+        *ws_bytes = entry_bytes + ml_bytes + 2 * grid * kRows * DP * sizeof(float);
+        return cudaSuccess;
+    }
+    static bool ready[64] = {};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev >= 64 || !__atomic_load_n(&ready[dev], __ATOMIC_RELAXED)) {
+        e = cudaFuncSetAttribute(kv_prompt_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kAlloc);
+        if (e != cudaSuccess) return e;
+        if (dev < 64) __atomic_store_n(&ready[dev], true, __ATOMIC_RELAXED);
+    }
+    const int64_t tasks = a.heads * (static_cast<int64_t>(a.tokens) * a.group / kRows + a.seqs);
+    a.by_task = tasks <= grid ? 1 : 0;
+    a.entries = static_cast<int>(a.by_task ? tasks : grid);
+    a.entry = static_cast<int4*>(ws);
+    a.ml = reinterpret_cast<float2*>(static_cast<char*>(ws) + entry_bytes);
+    a.part = reinterpret_cast<float*>(static_cast<char*>(ws) + entry_bytes + ml_bytes);
+    cudaLaunchAttribute attr[1];
+    cudaLaunchConfig_t cfg = pdl_config(dim3(static_cast<unsigned>(grid)), dim3(kPThreads), L::kAlloc, stream, attr);
+    e = cudaLaunchKernelEx(&cfg, kv_prompt_kernel<T, DP>, a);
+    if (e != cudaSuccess) return e;
+    cfg.gridDim = dim3(static_cast<unsigned>(a.entries), 8);
+    cfg.blockDim = dim3(256);
+    cfg.dynamicSmemBytes = 0;
+    return cudaLaunchKernelEx(&cfg, kv_prompt_join_kernel<T, DP>, a);
+}
+
+}  // namespace
+
+bool prompt_supported(popcornType_t type, int64_t dim) {
+    return (type == POPCORN_TYPE_F16 || type == POPCORN_TYPE_BF16) && (dim == 64 || dim == 128);
+}
+
+cudaError_t run_prompt(popcornType_t type, const AttnArgs& a, void* ws, int64_t* ws_bytes, cudaStream_t stream) {
+    if (type == POPCORN_TYPE_F16) {
+        return a.dim == 64 ? run_sized<__half, 64>(a, ws, ws_bytes, stream) : run_sized<__half, 128>(a, ws, ws_bytes, stream);
+    }
+    return a.dim == 64 ? run_sized<__nv_bfloat16, 64>(a, ws, ws_bytes, stream)
+                       : run_sized<__nv_bfloat16, 128>(a, ws, ws_bytes, stream);
+}
+
+cudaError_t kv_prompt_take_errors(unsigned int* bits) {
+    const unsigned int zero = 0;
+    cudaError_t e = cudaMemcpyFromSymbol(bits, g_prompt_err, sizeof(unsigned int));
+    if (e == cudaSuccess && *bits != 0) e = cudaMemcpyToSymbol(g_prompt_err, &zero, sizeof(unsigned int));
+    return e;
+}
+
+}  // namespace pcb

@@ -25,6 +25,8 @@
 //
 // Every wait is bounded (sm100.cuh); one that runs out sets error bit 0x8000
 // and ends the block.
+#include <type_traits>
+
 #include "kv_attention.cuh"
 #include "sm100.cuh"
 
@@ -91,6 +93,16 @@ __device__ __forceinline__ uint32_t as_f16(uint32_t biased) {  // halves 1024 + 
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Two scores times their factor, plus log2 of the value scale.
+__device__ __forceinline__ float2 scaled(uint32_t s0, uint32_t s1, float kf, float lv) {
+    return __ffma2_rn(make_float2(__uint_as_float(s0), __uint_as_float(s1)), make_float2(kf, kf), make_float2(lv, lv));
+}
+// -inf for tokens j, j + 1 outside [see0, see1).
+__device__ __forceinline__ void hide(float2& v, int j, int see0, int see1) {
+    if (j < see0 || j >= see1) v.x = -INFINITY;
+    if (j + 1 < see0 || j + 1 >= see1) v.y = -INFINITY;
 }
 
 // Walks a block's run segment by segment; every role walks the same way.
@@ -275,28 +287,39 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const AttnArgs 
                 const GroupScale* gs = ring + (ring_at % kScaleRing) * 8;
                 const int j0 = walk.see.lo + (walk.u0 + i) * kTile;
                 const bool whole = __all_sync(0xffffffffu, see0 <= j0 && j0 + kTile <= see1);
-                // --- maximum
+                // --- maximum; loops over 32 columns stay loops, for the
+                // instruction cache's sake, and load one round ahead.
+                uint32_t xa[32], xb[32];
                 float best = -INFINITY;
-                #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t x[32];
-                    tmem_ld_32x32b_x32(s_col + 32 * c, x);
-                    tmem_wait_ld();
+                const auto largest = [&](auto masked, const uint32_t (&x)[32], int c) {
                     #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const float kf = gs[2 * c + h].ks * fac, lv = gs[2 * c + h].lv;
-                        if (whole) {
-                            #pragma unroll
-                            for (int j = 0; j < 16; ++j) best = fmaxf(best, fmaf(__uint_as_float(x[16 * h + j]), kf, lv));
-                        } else {
-                            #pragma unroll
-                            for (int j = 0; j < 16; ++j) {
-                                const int k = j0 + 32 * c + 16 * h + j;
-                                if (k >= see0 && k < see1) best = fmaxf(best, fmaf(__uint_as_float(x[16 * h + j]), kf, lv));
-                            }
+                        float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                        #pragma unroll
+                        for (int j = 0; j < 16; j += 2) {
+                            float2 v = scaled(x[16 * h + j], x[16 * h + j + 1], kf, lv);
+                            if (decltype(masked)::value) hide(v, j0 + 32 * c + 16 * h + j, see0, see1);
+                            most[j / 2 % 4] = fmaxf(most[j / 2 % 4], fmaxf(v.x, v.y));
                         }
+                        best = fmaxf(best, fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])));
                     }
-                }
+                };
+                tmem_ld_32x32b_x32(s_col, xa);
+                tmem_wait_ld(xa);
+                const auto maximum = [&](auto masked) {
+                    #pragma unroll 1
+                    for (int c = 0; c < 4; c += 2) {
+                        tmem_ld_32x32b_x32(s_col + 32 * (c + 1), xb);
+                        largest(masked, xa, c);
+                        tmem_wait_ld(xb);
+                        tmem_ld_32x32b_x32(s_col + 32 * (c ^ 2), xa);  // the last round fetches the first columns again
+                        largest(masked, xb, c + 1);
+                        tmem_wait_ld(xa);
+                    }
+                };
+                if (whole) maximum(std::false_type{});
+                else maximum(std::true_type{});
                 const bool grow = best > top + kSlack;
                 if (__any_sync(0xffffffffu, grow)) {
                     const float now = fmaxf(top, best);
@@ -306,49 +329,51 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const AttnArgs 
                     if (i > 0) {
                         if (!(good = wait(kODone, m, steps_done - 1))) break;
                         tc_fence_after();
-                        #pragma unroll
+                        #pragma unroll 1
                         for (int c = 0; c < DP / 32; ++c) {
                             uint32_t x[32];
                             tmem_ld_32x32b_x32(o_col + 32 * c, x);
-                            tmem_wait_ld();
+                            tmem_wait_ld(x);
                             #pragma unroll
                             for (int j = 0; j < 32; ++j) x[j] = __float_as_uint(__uint_as_float(x[j]) * by);
                             tmem_st_32x32b_x32(o_col + 32 * c, x);
                         }
                     }
                 }
-                // --- probabilities, over the scores
+                // --- probabilities, over the scores (xa holds the first columns)
                 const float shift = kLift - (top == -INFINITY ? 0.0f : top);
-                #pragma unroll
-                for (int c2 = 0; c2 < 2; ++c2) {
-                    uint32_t w[32];
+                const auto weigh = [&](auto masked, const uint32_t (&x)[32], int c) {
+                    uint32_t w[16];
                     #pragma unroll
-                    for (int c1 = 0; c1 < 2; ++c1) {
-                        const int c = 2 * c2 + c1;
-                        uint32_t x[32];
-                        tmem_ld_32x32b_x32(s_col + 32 * c, x);
-                        tmem_wait_ld();
+                    for (int h = 0; h < 2; ++h) {
+                        const GroupScale g = gs[2 * c + h];
+                        const float kf = g.ks * fac, lv = g.lv + shift;
+                        float2 sum[2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
                         #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const GroupScale g = gs[2 * c + h];
-                            const float kf = g.ks * fac, lv = g.lv + shift;
-                            #pragma unroll
-                            for (int j = 0; j < 16; j += 2) {
-                                float p0 = exp2_fast(fmaf(__uint_as_float(x[16 * h + j]), kf, lv));
-                                float p1 = exp2_fast(fmaf(__uint_as_float(x[16 * h + j + 1]), kf, lv));
-                                if (!whole) {
-                                    const int k = j0 + 32 * c + 16 * h + j;
-                                    if (k < see0 || k >= see1) p0 = 0.0f;
-                                    if (k + 1 < see0 || k + 1 >= see1) p1 = 0.0f;
-                                }
-                                den = fmaf(p0, g.iv, den);
-                                den = fmaf(p1, g.iv, den);
-                                w[16 * c1 + 8 * h + j / 2] = pack_f16(p0, p1);
-                            }
+                        for (int j = 0; j < 16; j += 2) {
+                            float2 v = scaled(x[16 * h + j], x[16 * h + j + 1], kf, lv);
+                            if (decltype(masked)::value) hide(v, j0 + 32 * c + 16 * h + j, see0, see1);
+                            const float2 e = make_float2(exp2_fast(v.x), exp2_fast(v.y));
+                            sum[j / 2 % 2] = __fadd2_rn(sum[j / 2 % 2], e);
+                            w[8 * h + j / 2] = pack_f16(e.x, e.y);
                         }
+                        den = fmaf((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y), g.iv, den);
                     }
-                    tmem_st_32x32b_x32(s_col + 32 * c2, w);
-                }
+                    tmem_st_32x32b_x16(s_col + 16 * c, w);
+                };
+                const auto probabilities = [&](auto masked) {
+                    #pragma unroll 1
+                    for (int c = 0; c < 4; c += 2) {
+                        tmem_ld_32x32b_x32(s_col + 32 * (c + 1), xb);
+                        weigh(masked, xa, c);
+                        tmem_wait_ld(xb);
+                        if (c == 0) tmem_ld_32x32b_x32(s_col + 64, xa);
+                        weigh(masked, xb, c + 1);
+                        if (c == 0) tmem_wait_ld(xa);
+                    }
+                };
+                if (whole) probabilities(std::false_type{});
+                else probabilities(std::true_type{});
                 tmem_wait_st();
                 tc_fence_before();
                 mbar_arrive(bar(kPReady, m));
@@ -360,11 +385,11 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const AttnArgs 
             const int64_t slot = (2 * static_cast<int64_t>(blockIdx.x) + (walk.u0 > 0 ? 0 : 1)) * kRows + m * kTile + row;
             const float inv = inverse(den);
             T* out = static_cast<T*>(a.out) + ((walk.s.row0 + tok) * static_cast<int64_t>(a.heads * a.group) + head) * DP;
-            #pragma unroll
+            #pragma unroll 1
             for (int c = 0; c < DP / 32; ++c) {
                 uint32_t x[32];
                 tmem_ld_32x32b_x32(o_col + 32 * c, x);
-                tmem_wait_ld();
+                tmem_wait_ld(x);
                 if (!valid) continue;
                 if (walk.complete) {
                     #pragma unroll
@@ -392,58 +417,70 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const AttnArgs 
         }
     } else if (warp < kSoftWarps + kConvWarps) {
         // ----------------------------------------------------------- convert
-        constexpr int CK = DP / 16;                      // 16-byte pieces of a key row
-        constexpr int KN = kTile * CK / kConvThreads;    // pieces per thread and step
-        constexpr int RK = kConvThreads / CK;            // rows between a thread's pieces
-        constexpr int WV = DP / 4;                       // words of a value row
-        constexpr int VO = 16 * WV / kConvThreads;       // runs of 8 tokens (of one word) per thread and step
-        const int ct = tid - 32 * kSoftWarps;
-        const int krow = ct / CK, kpiece = ct % CK;
-        const int vword = ct % WV, voct = ct / WV;       // run voct + i * (kConvThreads / WV)
+        // A step's tokens are eight groups of 16, each inside one page; a warp
+        // has two of them, so that a group's address is the same for all lanes
+        // and every load is that address plus a constant of the lane.
+        constexpr int KN = 16 * DP / 16 / 32;   // 16-byte pieces of a group's keys per lane
+        constexpr int WV = DP / 4;              // words of a value row
+        constexpr int VO = 2 * WV / 32;         // runs of 8 tokens of a group's values per lane
+        const int cw = warp - kSoftWarps;
+        const int kpiece = lane % (DP / 16), krow = lane / (DP / 16);
+        const int vword = lane % WV, voct = lane / WV;
         const int page_mask = (1 << a.page_shift) - 1;
-        // The step's eight groups of 16 tokens: lane j < 8 of every warp looks up
-        // group j. -1: nothing there.
         struct Step {
             int h, j0, len;
-            int64_t seq;
+            int64_t table;  // of the sequence
         };
-        const auto look_up = [&](const Step& st) {
-            const int j = st.j0 + 16 * (lane & 7);
-            if (j >= st.len) return -1;
-            const int p = a.table[st.seq * a.table_pages + (j >> a.page_shift)];
-            if (p < 0 || p >= a.pages) {
-                if (lane < 8 && warp == kSoftWarps) atomicOr(err, kKvErrAttention);
-                return -1;
-            }
-            return p;
+        struct Groups {
+            int64_t block[2];   // page and head; -1: nothing there
+            float ks, vs;       // lane i < 2: scales of group i
         };
-        const auto block_of = [&](const Step& st, int pages, int group) -> int64_t {
-            const int p = __shfl_sync(0xffffffffu, pages, group);
-            if (p < 0) return -1;
-            const int j = st.j0 + 16 * group;
-            return (((static_cast<int64_t>(p) * a.heads + st.h) << a.page_shift) + (j & page_mask)) * DP;
-        };
-        uint4 kq[KN];
-        uint32_t vq[VO][8];
-        const auto load_k = [&](const Step& st, int pages) {
+        // Page indices are fetched two steps ahead of their use, scales one.
+        const auto fetch = [&](const Step& st, int (&pages)[2]) {
             #pragma unroll
-            for (int i = 0; i < KN; ++i) {
-                const int r = krow + i * RK;
-                const int64_t at = block_of(st, pages, r >> 4);
-                kq[i] = make_uint4(0u, 0u, 0u, 0u);
-                if (at >= 0) kq[i] = *reinterpret_cast<const uint4*>(a.k + at + (r & 15) * DP + 16 * kpiece);
+            for (int i = 0; i < 2; ++i) {
+                const int j = st.j0 + 16 * (2 * cw + i);
+                pages[i] = j < st.len ? a.table[st.table + (j >> a.page_shift)] : -1;
             }
         };
-        const auto load_v = [&](const Step& st, int pages) {
+        const auto look_up = [&](const Step& st, const int (&pages)[2], Groups& g) {
             #pragma unroll
-            for (int i = 0; i < VO; ++i) {
-                const int oct = voct + i * (kConvThreads / WV);
-                const int64_t at = block_of(st, pages, oct >> 1);
+            for (int i = 0; i < 2; ++i) {
+                const bool in = pages[i] >= 0 && pages[i] < a.pages;
+                g.block[i] = in ? static_cast<int64_t>(pages[i]) * a.heads + st.h : -1;
+                if (!in && lane == 0 && st.j0 + 16 * (2 * cw + i) < st.len) atomicOr(err, kKvErrAttention);
+            }
+            const int64_t mine = lane == 0 ? g.block[0] : g.block[1];
+            if (lane < 2 && mine >= 0) {
+                g.ks = a.ks[mine];
+                g.vs = a.vs[mine];
+            }
+        };
+        uint4 kq[2][KN];
+        uint32_t vq[2][VO][8];
+        const auto load_k = [&](const Step& st, const Groups& g) {
+            #pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int row = (st.j0 + 16 * (2 * cw + i)) & page_mask;
+                const int8_t* p = a.k + ((g.block[i] << a.page_shift) + row) * DP + 16 * lane;
                 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    vq[i][j] = 0u;
-                    if (at >= 0) {
-                        vq[i][j] = *reinterpret_cast<const uint32_t*>(a.v + at + (8 * (oct & 1) + j) * DP + 4 * vword);
+                for (int n = 0; n < KN; ++n) {
+                    kq[i][n] = make_uint4(0u, 0u, 0u, 0u);
+                    if (g.block[i] >= 0) kq[i][n] = *reinterpret_cast<const uint4*>(p + 512 * n);
+                }
+            }
+        };
+        const auto load_v = [&](const Step& st, const Groups& g) {
+            #pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int row = (st.j0 + 16 * (2 * cw + i)) & page_mask;
+                const int8_t* p = a.v + ((g.block[i] << a.page_shift) + row + 8 * voct) * DP + 4 * vword;
+                #pragma unroll
+                for (int n = 0; n < VO; ++n) {
+                    #pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        vq[i][n][j] = 0u;
+                        if (g.block[i] >= 0) vq[i][n][j] = *reinterpret_cast<const uint32_t*>(p + (8 * n + j) * DP);
                     }
                 }
             }
@@ -451,13 +488,13 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const AttnArgs 
         int kt = 0;  // steps of the block
         bool good = true;
         int left = 0;  // steps left in the segment
-        Step cur = {0, 0, 0, 0}, nxt;
+        Step cur = {0, 0, 0, 0}, nxt, after;  // this step, the next, the one after it
         const auto advance = [&](Step& st) -> bool {
             if (left == 0) {
                 if (!walk.next()) return false;
                 left = walk.u1 - walk.u0;
                 st.h = walk.task_in_tile;
-                st.seq = walk.b;
+                st.table = static_cast<int64_t>(walk.b) * a.table_pages;
                 st.len = min(walk.see.hi, walk.s.len);
                 st.j0 = walk.see.lo + walk.u0 * kTile;
             } else {
@@ -467,80 +504,94 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const AttnArgs 
             return true;
         };
         bool have = advance(cur);
-        int pages = -1, pages_next = -1;
+        Groups groups = {{-1, -1}, 0.0f, 0.0f}, groups_next = groups;
+        int pages[2];
+        nxt = cur;
+        bool have_next = false;
         if (have) {
-            pages = look_up(cur);
-            load_k(cur, pages);
+            fetch(cur, pages);
+            look_up(cur, pages, groups);
+            nxt = cur;
+            have_next = advance(nxt);
+            if (have_next) fetch(nxt, pages);
+            load_k(cur, groups);
+            load_v(cur, groups);
         }
         while (good && have) {
-            nxt = cur;
-            const bool have_next = advance(nxt);
+            if (have_next) look_up(nxt, pages, groups_next);
+            after = nxt;
+            const bool have_after = have_next && advance(after);
+            if (have_after) fetch(after, pages);
             const int stage = kt % kStages, turn = kt / kStages;
-            // Scales of the step's groups.
-            if (warp == kSoftWarps && lane < 8) {
+            if (lane < 2) {
                 GroupScale g = {0.0f, -INFINITY, 1.0f, 0.0f};
-                if (pages >= 0) {
-                    const int64_t at = static_cast<int64_t>(pages) * a.heads + cur.h;
-                    const float vs = a.vs[at];
-                    g.ks = a.ks[at];
-                    const bool tiny = fabsf(vs) < kKvSmallestScale;  // all-zero codes
-                    g.lv = tiny ? -80.0f : log2f(vs);
-                    g.iv = tiny ? 1.0f / kKvSmallestScale : fabsf(vs) <= 3.4028234663852886e38f ? 1.0f / vs : 1.0f;
+                if ((lane == 0 ? groups.block[0] : groups.block[1]) >= 0) {
+                    const bool tiny = fabsf(groups.vs) < kKvSmallestScale;  // all-zero codes
+                    g.ks = groups.ks;
+                    g.lv = tiny ? -80.0f : log2f(groups.vs);
+                    g.iv = tiny ? 1.0f / kKvSmallestScale
+                                : fabsf(groups.vs) <= 3.4028234663852886e38f ? 1.0f / groups.vs : 1.0f;
                 }
-                ring[(kt % kScaleRing) * 8 + lane] = g;
+                ring[(kt % kScaleRing) * 8 + 2 * cw + lane] = g;
             }
-            load_v(cur, pages);
-            if (have_next) pages_next = look_up(nxt);
             if (kt >= kStages && !(good = wait(kKEmpty, stage, turn - 1))) break;
             #pragma unroll
-            for (int i = 0; i < KN; ++i) {
-                const int r = krow + i * RK;
-                const uint32_t in[4] = {kq[i].x ^ 0x80808080u, kq[i].y ^ 0x80808080u, kq[i].z ^ 0x80808080u,
-                                        kq[i].w ^ 0x80808080u};
-                uint32_t lo[4], hi[4];
+            for (int i = 0; i < 2; ++i) {
                 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    lo[2 * j] = as_f16(__byte_perm(in[j], 0x64646464u, 0x4140));
-                    lo[2 * j + 1] = as_f16(__byte_perm(in[j], 0x64646464u, 0x4342));
-                    hi[2 * j] = as_f16(__byte_perm(in[2 + j], 0x64646464u, 0x4140));
-                    hi[2 * j + 1] = as_f16(__byte_perm(in[2 + j], 0x64646464u, 0x4342));
+                for (int n = 0; n < KN; ++n) {
+                    const uint4 q = kq[i][n];
+                    const uint32_t in[4] = {q.x ^ 0x80808080u, q.y ^ 0x80808080u, q.z ^ 0x80808080u, q.w ^ 0x80808080u};
+                    uint32_t lo[4], hi[4];
+                    #pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        lo[2 * j] = as_f16(__byte_perm(in[j], 0x64646464u, 0x4140));
+                        lo[2 * j + 1] = as_f16(__byte_perm(in[j], 0x64646464u, 0x4342));
+                        hi[2 * j] = as_f16(__byte_perm(in[2 + j], 0x64646464u, 0x4140));
+                        hi[2 * j + 1] = as_f16(__byte_perm(in[2 + j], 0x64646464u, 0x4342));
+                    }
+                    const int r = 16 * (2 * cw + i) + krow + n * (512 / DP);
+                    const uint32_t base = smem + L::kK + stage * L::kKStage + (kpiece / 4) * (kTile * 128) + r * 128;
+                    const uint32_t unit = 2 * (kpiece % 4);
+                    store_shared16(base + ((unit ^ (r & 7)) << 4), lo);
+                    store_shared16(base + (((unit + 1) ^ (r & 7)) << 4), hi);
                 }
-                const uint32_t base = smem + L::kK + stage * L::kKStage + (kpiece / 4) * (kTile * 128) + r * 128;
-                const uint32_t unit = 2 * (kpiece % 4);
-                store_shared16(base + (((unit) ^ (r & 7)) << 4), lo);
-                store_shared16(base + (((unit + 1) ^ (r & 7)) << 4), hi);
             }
             fence_async_shared();
             mbar_arrive(bar(kKFull, stage));
-            if (have_next) load_k(nxt, pages_next);
+            if (have_next) load_k(nxt, groups_next);
             if (kt >= kStages && !(good = wait(kVEmpty, stage, turn - 1))) break;
+            // V transposed: row d, 64 tokens to a 128-byte row. Lanes take a word's
+            // four bytes in different orders, so that eight lanes' stores fall into
+            // eight different 16-byte banks.
             #pragma unroll
-            for (int i = 0; i < VO; ++i) {
-                const int oct = voct + i * (kConvThreads / WV);
-                // V transposed: row d, 64 tokens to a 128-byte row. Lanes take the
-                // word's four bytes in different orders, so that eight lanes'
-                // stores fall into eight different 16-byte banks.
+            for (int i = 0; i < 2; ++i) {
                 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint32_t byte = (j + (vword >> 1)) & 3;
-                    const uint32_t sel = byte | (byte + 4) << 8;
-                    uint32_t w[4];
+                for (int n = 0; n < VO; ++n) {
+                    const int oct = 2 * (2 * cw + i) + voct + n;
                     #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const uint32_t x = __byte_perm(vq[i][2 * k], vq[i][2 * k + 1], sel);
-                        w[k] = as_f16((x & 0x00ff00ffu) ^ 0x64806480u);
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t byte = (j + (vword >> 1)) & 3;
+                        const uint32_t sel = byte | (byte + 4) << 8;
+                        uint32_t w[4];
+                        #pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const uint32_t x = __byte_perm(vq[i][n][2 * k], vq[i][n][2 * k + 1], sel);
+                            w[k] = as_f16((x & 0x00ff00ffu) ^ 0x64806480u);
+                        }
+                        const uint32_t d = 4 * vword + byte;
+                        store_shared16(smem + L::kV + stage * L::kVStage + (oct >> 3) * (DP * 128) + d * 128 +
+                                           (((oct & 7) ^ (d & 7)) << 4),
+                                       w);
                     }
-                    const uint32_t d = 4 * vword + byte;
-                    store_shared16(smem + L::kV + stage * L::kVStage + (oct >> 3) * (DP * 128) + d * 128 +
-                                       (((oct & 7) ^ (d & 7)) << 4),
-                                   w);
                 }
             }
             fence_async_shared();
             mbar_arrive(bar(kVFull, stage));
-            cur = nxt;
-            pages = pages_next;
+            if (have_next) load_v(nxt, groups_next);
+            nxt = after;
+            groups = groups_next;
             have = have_next;
+            have_next = have_after;
             ++kt;
         }
     } else if (lane == 0) {

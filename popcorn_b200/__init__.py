@@ -442,45 +442,30 @@ def dequantize(qweight, scale, out=None, stream=None, dtype=None):
 
 
 # ---------------------------------------------------------------------------
-# Serving operators (include/popcorn_serve.h).
+# Serving operators (include/popcorn_serve.h), through popcorn_b200/_serve.so:
+# it checks the tensors (ValueError), makes outputs and workspaces on the
+# current stream and calls the library, in a few us.
 # ---------------------------------------------------------------------------
-_TYPES = {}  # torch dtype -> popcornType_t, filled on first use
+_bound = None
 
 
-def _type_of(dtype, where: str) -> int:
-    if not _TYPES:
-        import torch
+def _binding():
+    global _bound
+    if _bound is None:
+        path = os.path.join(_HERE, "_serve.so")
+        if not os.path.exists(path):
+            raise OSError(f"popcorn_b200 binding not built: {path} (run `make -C popcorn_b200 python`)")
+        load_library()
+        import torch  # noqa: F401  (its libraries come first)
 
-        _TYPES.update({torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16})
-    try:
-        return _TYPES[dtype]
-    except KeyError:
-        raise ValueError(f"{where}: float32, float16 or bfloat16 wanted, got {dtype}") from None
+        from . import _serve
 
-
-def _want(ok: bool, where: str, what: str) -> None:
-    if not ok:
-        raise ValueError(f"{where}: {what}")
-
-
-def _stream_on(stream, device):
-    """The handle of `stream`, by default the current one of `device`. (torch.cuda.current_stream builds an object
-    for it, 3 us of a decode step's 8.)"""
-    if stream is None:
-        import torch
-
-        return torch._C._cuda_getCurrentRawStream(device.index)
-    return stream if isinstance(stream, int) else stream.cuda_stream
+        _bound = _serve
+    return _bound
 
 
-def _whole(t, shape, device, where: str, name: str):
-    """Device pointer of a contiguous int32 tensor of this shape."""
-    import torch
-
-    if t.dtype is not torch.int32 or t.shape != shape or not t.is_contiguous() or t.device != device:
-        raise ValueError(f"{where}: {name}: a contiguous int32 tensor {tuple(shape)} on {device} wanted, "
-                         f"got {t.dtype} {tuple(t.shape)} on {t.device}")
-    return t.data_ptr()
+def _handle(stream):
+    return stream if stream is None or isinstance(stream, int) else stream.cuda_stream
 
 
 class KvCache:
@@ -488,30 +473,31 @@ class KvCache:
     head [pages, heads], keys and values apart (a cached value is code * scale). ``page_size`` is a power of two from
     16 to 256, ``dim`` a multiple of 16 up to 256. Wraps the caller's tensors; :meth:`empty` makes them."""
 
-    __slots__ = ("k", "v", "k_scale", "v_scale", "pages", "heads", "page_size", "dim", "device", "_struct", "_ref",
-                 "_workspaces")
+    __slots__ = ("k", "v", "k_scale", "v_scale", "pages", "heads", "page_size", "dim", "device", "_struct", "_ref")
 
     def __init__(self, k, v, k_scale, v_scale):
         import torch
 
-        _want(k.dim() == 4 and k.shape == v.shape and k.dtype is v.dtype is torch.int8, "KvCache",
-              "k and v: int8 [pages, heads, page_size, dim]")
+        def want(ok, what):
+            if not ok:
+                raise ValueError(f"KvCache: {what}")
+
+        want(k.dim() == 4 and k.shape == v.shape and k.dtype is v.dtype is torch.int8,
+             "k and v: int8 [pages, heads, page_size, dim]")
         self.pages, self.heads, self.page_size, self.dim = k.shape
         for s in (k_scale, v_scale):
-            _want(s.shape == k.shape[:2] and s.dtype is torch.float32, "KvCache",
-                  "k_scale and v_scale: float32 [pages, heads]")
+            want(s.shape == k.shape[:2] and s.dtype is torch.float32, "k_scale and v_scale: float32 [pages, heads]")
         for t in (k, v, k_scale, v_scale):
-            _want(t.is_contiguous() and t.is_cuda and t.device == k.device, "KvCache",
-                  "contiguous CUDA tensors on one device")
-        _want(self.page_size in (16, 32, 64, 128, 256), "KvCache", "page_size: a power of two from 16 to 256")
-        _want(self.dim % 16 == 0 and 16 <= self.dim <= 256, "KvCache", "dim: a multiple of 16 from 16 to 256")
-        _want(self.pages > 0 and self.heads > 0, "KvCache", "at least one page and one head")
+            want(t.is_contiguous() and t.is_cuda and t.device == k.device, "contiguous CUDA tensors on one device")
+        want(self.page_size in (16, 32, 64, 128, 256), "page_size: a power of two from 16 to 256")
+        want(self.dim % 16 == 0 and 16 <= self.dim <= 256, "dim: a multiple of 16 from 16 to 256")
+        want(self.pages > 0 and self.heads > 0, "at least one page and one head")
+        want(k.data_ptr() % 16 == 0 and v.data_ptr() % 16 == 0, "k and v: 16-byte aligned")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.device = k.device.index
         self._struct = KvCacheStruct(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), self.pages,
                                      self.heads, self.page_size, self.dim)
         self._ref = ctypes.addressof(self._struct)
-        self.device = k.device
-        self._workspaces = {}  # sizes -> bytes of an attention call's workspace
 
     @classmethod
     def empty(cls, pages: int, heads: int, dim: int, page_size: int = 16, device="cuda"):
@@ -523,92 +509,34 @@ class KvCache:
         return cls(*codes, *scales)
 
 
-def _rows(t, shape, kind, device, where, name):
-    """Strides of the first two dimensions of [tokens, heads, dim] with dim contiguous."""
-    if t.shape != shape or t.dtype is not kind or t.device != device:
-        raise ValueError(f"{where}: {name}: {kind} {tuple(shape)} on {device} wanted, "
-                         f"got {t.dtype} {tuple(t.shape)} on {t.device}")
-    a, b, c = t.stride()
-    if c != 1:
-        raise ValueError(f"{where}: {name}: the last dimension must be contiguous")
-    return a, b
-
-
-def _batch(table, first, tokens, device, where):
-    if table.dim() != 2:
-        raise ValueError(f"{where}: table: [seqs, pages] wanted")
-    seqs, width = shape = table.shape
-    tp = _whole(table, shape, device, where, "table")
-    if first is not None:
-        return seqs, tp, width, _whole(first, (seqs + 1,), device, where, "first")
-    _want(tokens == seqs, where, f"{tokens} tokens for {seqs} sequences need `first`")
-    return seqs, tp, width, None
-
-
 def kv_append(cache: KvCache, k, v, table, start, first=None, q=None, cos=None, sin=None, interleaved: bool = False,
               q_out=None, stream=None):
-    """Append keys and values [tokens, heads, dim] to the sequences of ``table`` int32 [seqs, pages] behind the
-    ``start`` int32 [seqs] tokens that they hold, rotating keys (and queries ``q`` [tokens, q_heads, dim]) by the
-    tables ``cos``, ``sin`` f32 [positions, rot_dim / 2]. ``first`` int32 [seqs + 1]: each sequence's run of tokens
-    (None: one token each). Returns the rotated queries (``q_out``, or a new tensor), None without ``q``."""
-    import torch
-
-    where = "kv_append"
-    device, kind, dim = cache.device, k.dtype, cache.dim
-    shape = k.shape
-    tokens = shape[0]
-    _want(shape == (tokens, cache.heads, dim), where, f"k: [tokens, {cache.heads}, {dim}] wanted")
-    kt, kh = _rows(k, shape, kind, device, where, "k")
-    vt, vh = _rows(v, shape, kind, device, where, "v")
-    seqs, tp, width, fp = _batch(table, first, tokens, device, where)
-    sp = _whole(start, (seqs,), device, where, "start")
-    qp = op = None
-    qt = qh = q_heads = 0
-    if q is not None:
-        q_heads = q.shape[1]
-        shape = (tokens, q_heads, dim)
-        qt, qh = _rows(q, shape, kind, device, where, "q")
-        if q_out is None:
-            q_out = q.new_empty(shape)
-        else:
-            _rows(q_out, shape, kind, device, where, "q_out")
-            _want(q_out.is_contiguous(), where, "q_out must be contiguous")
-        qp, op = q.data_ptr(), q_out.data_ptr()
-    cp = np_ = None
-    positions = rot = 0
-    if cos is not None:
-        positions, rot = shape = cos.shape
-        for t in (cos, sin):
-            if t.shape != shape or t.dtype is not torch.float32 or not t.is_contiguous() or t.device != device:
-                raise ValueError(f"{where}: cos and sin: contiguous float32 [positions, rot_dim / 2] on {device}")
-        cp, np_, rot = cos.data_ptr(), sin.data_ptr(), 2 * rot
-    st = load_library().popcornKvAppend(cache._ref, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, _type_of(kind, where),
-                                        tp, width, fp, sp, seqs, tokens, op, qp, qt, qh, q_heads, cp, np_, positions,
-                                        rot, interleaved, _stream_on(stream, device))
-    _check(st, "popcornKvAppend")
+    """Append keys and values [tokens, heads, dim] (float32, float16 or bfloat16; dim contiguous) to the sequences of
+    ``table`` int32 [seqs, pages] behind the ``start`` int32 [seqs] tokens that they hold, rotating keys (and queries
+    ``q`` [tokens, q_heads, dim]) by the tables ``cos``, ``sin`` f32 [positions, rot_dim / 2]. ``first`` int32
+    [seqs + 1]: each sequence's run of tokens (None: one token each). Returns the rotated queries (``q_out``, or a new
+    tensor), None without ``q``."""
+    status, q_out = (_bound or _binding()).kv_append(cache._ref, cache.device, k, v, table, start, first, q, cos, sin,
+                                                     interleaved, q_out, _handle(stream))
+    _check(status, "popcornKvAppend")
     return q_out
 
 
 def kv_read(cache: KvCache, pages, dtype=None, k_out=None, v_out=None, stream=None):
     """The values (code * scale) of the pages listed in ``pages`` int32 [n]: (keys, values), each
     [n, heads, page_size, dim] in ``dtype`` (float32)."""
-    import torch
+    kind = TYPE_F32
+    if dtype is not None or k_out is not None:
+        import torch
 
-    where = "kv_read"
-    dtype = dtype or (k_out.dtype if k_out is not None else torch.float32)
-    n = pages.shape[0]
-    device = cache.device
-    shape = (n, cache.heads, cache.page_size, cache.dim)
-    if k_out is None:
-        k_out = cache.k_scale.new_empty(shape, dtype=dtype)
-    if v_out is None:
-        v_out = torch.empty_like(k_out)
-    for t in (k_out, v_out):
-        if t.shape != shape or t.dtype is not dtype or not t.is_contiguous() or t.device != device:
-            raise ValueError(f"{where}: outputs: contiguous {dtype} {shape} on {device}")
-    st = load_library().popcornKvRead(k_out.data_ptr(), v_out.data_ptr(), _type_of(dtype, where), cache._ref,
-                                      _whole(pages, (n,), device, where, "pages"), n, _stream_on(stream, device))
-    _check(st if n else POPCORN_SUCCESS, "popcornKvRead")
+        dtype = dtype or k_out.dtype
+        kinds = {torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}
+        if dtype not in kinds:
+            raise ValueError(f"kv_read: float32, float16 or bfloat16 wanted, got {dtype}")
+        kind = kinds[dtype]
+    status, k_out, v_out = (_bound or _binding()).kv_read(cache._ref, cache.device, pages, kind, k_out, v_out,
+                                                          _handle(stream))
+    _check(status, "popcornKvRead")
     return k_out, v_out
 
 
@@ -618,41 +546,9 @@ def kv_attention(cache: KvCache, q, table, length, first=None, max_tokens: int |
     [seqs] counts them, the queries' own included; sequence b's queries (``first`` as in :func:`kv_append`, at most
     ``max_tokens`` each) are its last positions. ``window`` > 0 limits a query to that many last positions, ``scale``
     is 1 / sqrt(dim) unless given, ``lse`` f32 [tokens, q_heads] takes the log of the softmax denominators."""
-    import torch
-
-    where = "kv_attention"
-    device, kind = cache.device, q.dtype
-    tokens, q_heads, dim = shape = q.shape
-    _want(dim == cache.dim and q_heads % cache.heads == 0, where,
-          f"q: {q_heads} heads of {dim} over a cache of {cache.heads} heads of {cache.dim}")
-    qt, qh = _rows(q, shape, kind, device, where, "q")
-    seqs, tp, width, fp = _batch(table, first, tokens, device, where)
-    lp = _whole(length, (seqs,), device, where, "length")
-    if out is None:
-        out = q.new_empty(shape)
-    else:
-        _rows(out, shape, kind, device, where, "out")
-        _want(out.is_contiguous(), where, "out must be contiguous")
-    ep = None
-    if lse is not None:
-        _want(lse.shape == (tokens, q_heads) and lse.dtype is torch.float32 and lse.is_contiguous() and
-              lse.device == device, where, f"lse: contiguous float32 [tokens, q_heads] on {device}")
-        ep = lse.data_ptr()
-    if max_tokens is None:
-        max_tokens = 1 if first is None else tokens
-    lib = load_library()
-    code = _type_of(kind, where)
-    sizes = (code, seqs, tokens, max_tokens, q_heads)
-    need = cache._workspaces.get(sizes)
-    if need is None:
-        need = lib.popcornKvAttentionWorkspace(cache._ref, *sizes)
-        if len(cache._workspaces) < 4096:
-            cache._workspaces[sizes] = need
-    ws = cache.k.new_empty(need)  # on the current stream, like the output
-    st = lib.popcornKvAttention(out.data_ptr(), ep, q.data_ptr(), qt, qh, code, cache._ref, tp, width, fp, lp, seqs,
-                                tokens, max_tokens, q_heads, causal, window, dim ** -0.5 if scale is None else scale,
-                                ws.data_ptr() if need else None, need, _stream_on(stream, device))
-    _check(st, "popcornKvAttention")
+    status, out = (_bound or _binding()).kv_attention(cache._ref, cache.device, q, table, length, first, max_tokens,
+                                                      causal, window, scale, out, lse, _handle(stream))
+    _check(status, "popcornKvAttention")
     return out
 
 
@@ -662,35 +558,7 @@ def moe(x, router, q_gate, s_gate, q_up, s_up, q_down, s_down, top_k: int, renor
     [E, K, F], f32 scales per output channel): each token's ``top_k`` experts by router f32 [E, K], weighted with
     their softmax probabilities (``renormalize``: divided by their sum). Returns out [M, K]; with ``routing``
     (out, experts int32 [M, top_k], weights f32 [M, top_k])."""
-    import torch
-
-    where = "moe"
-    device = x.device
-    (M, K), (E, F) = x.shape, s_gate.shape
-    f32, i8 = torch.float32, torch.int8
-    for name, t, shape, kind in (("x", x, (M, K), f32), ("router", router, (E, K), f32),
-                                 ("q_gate", q_gate, (E, F, K), i8), ("s_gate", s_gate, (E, F), f32),
-                                 ("q_up", q_up, (E, F, K), i8), ("s_up", s_up, (E, F), f32),
-                                 ("q_down", q_down, (E, K, F), i8), ("s_down", s_down, (E, K), f32)):
-        if t.shape != shape or t.dtype is not kind or not t.is_contiguous() or t.device != device:
-            raise ValueError(f"{where}: {name}: a contiguous {kind} {shape} on {device} wanted, "
-                             f"got {t.dtype} {tuple(t.shape)} on {t.device}")
-    _want(x.is_cuda, where, "CUDA tensors wanted")
-    if out is None:
-        out = torch.empty_like(x)
-    else:
-        _want(out.shape == (M, K) and out.dtype is f32 and out.is_contiguous() and out.device == device, where,
-              "out: contiguous float32 [M, K]")
-    experts = weights = None
-    if routing:
-        experts = x.new_empty((M, top_k), dtype=torch.int32)
-        weights = x.new_empty((M, top_k))
-    lib = load_library()
-    need = lib.popcornMoeWorkspace(M, K, F, E, top_k)
-    ws = q_gate.new_empty(need) if need else None  # on the current stream, like the output
-    st = lib.popcornMoe_i8f32(out.data_ptr(), _ptr_or_null(experts), _ptr_or_null(weights), x.data_ptr(),
-                              router.data_ptr(), q_gate.data_ptr(), s_gate.data_ptr(), q_up.data_ptr(),
-                              s_up.data_ptr(), q_down.data_ptr(), s_down.data_ptr(), M, K, F, E, top_k, renormalize,
-                              _ptr_or_null(ws), need, _stream_on(stream, device))
-    _check(st, "popcornMoe_i8f32")
+    status, out, experts, weights = (_bound or _binding()).moe(x, router, q_gate, s_gate, q_up, s_up, q_down, s_down,
+                                                               top_k, renormalize, out, routing, _handle(stream))
+    _check(status, "popcornMoe_i8f32")
     return (out, experts, weights) if routing else out

@@ -518,3 +518,39 @@ def test_side_streams_and_graphs(cuda):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want)
+
+
+def test_python_refusals(cuda):
+    torch = _torch()
+    z = lambda *shape, dtype=torch.float32: torch.zeros(shape, dtype=dtype, device=cuda)  # noqa: E731
+    cache = pc.KvCache.empty(4, 2, 64, 16, device=cuda)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=cuda)  # noqa: E731
+    k, q, table, start, first = z(3, 2, 64), z(3, 4, 64), torch.zeros((2, 2), dtype=torch.int32, device=cuda), i32(0, 0), i32(0, 1, 3)
+    cos = z(32, 32)
+    good = dict(k=k, v=k, table=table, start=start, first=first, q=q, cos=cos, sin=cos)
+    assert pc.kv_append(cache, **good).shape == q.shape
+    for name, bad in (("k", k.half()), ("k", k[:, :1]), ("k", k[0]), ("k", k.cpu()), ("k", k.double()), ("v", k[:2]),
+                      ("v", k.transpose(1, 2).contiguous().transpose(1, 2)), ("table", table.long()), ("table", table[0]),
+                      ("table", table.t()[:1]), ("start", start[:1]), ("start", start.cpu()), ("first", first[:2]),
+                      ("first", None), ("q", q[..., :32]), ("q", q.bfloat16()), ("cos", cos[0]), ("cos", cos.half()),
+                      ("sin", None), ("sin", cos[:5]), ("cos", cos[:, ::2]), ("q_out", q[:, :2]), ("q_out", q.half())):
+        with pytest.raises(ValueError, match="kv_append"):
+            pc.kv_append(cache, **{**good, name: bad})
+    with pytest.raises(pc.PopcornError):
+        pc.kv_append(cache, **{**good, "cos": z(32, 30), "sin": z(32, 30)})  # rot_dim 60
+    length = i32(1, 2)
+    good = dict(q=q, table=table, length=length, first=first)
+    assert pc.kv_attention(cache, **good).shape == q.shape
+    for name, bad in (("q", q[:, :3]), ("q", q[..., :32]), ("q", q.double()), ("q", q.cpu()), ("q", q[0]),
+                      ("table", table.long()), ("length", length[:1]), ("length", length.float()), ("first", None),
+                      ("out", q.half()), ("out", q[:, ::2]), ("lse", z(3, 5)), ("lse", z(4, 3).t())):
+        with pytest.raises(ValueError, match="kv_attention"):
+            pc.kv_attention(cache, **{**good, name: bad})
+    with pytest.raises(pc.PopcornError):
+        pc.kv_attention(cache, **good, max_tokens=0)
+    pages = i32(0, 1)
+    for kw in (dict(pages=pages.long()), dict(pages=pages.cpu()), dict(pages=pages[None]), dict(pages=pages, dtype=torch.int8),
+               dict(pages=pages, k_out=z(2, 2, 16, 32)), dict(pages=pages, v_out=z(2, 2, 16, 64, dtype=torch.float16))):
+        with pytest.raises(ValueError, match="kv_read"):
+            pc.kv_read(cache, **kw)
+    assert pc.kv_read(cache, pages[:0])[0].shape == (0, 2, 16, 64)

@@ -72,6 +72,22 @@ __device__ __forceinline__ void prefetch_l2_range(const void* p, int64_t bytes, 
                  : "memory");
 }
 
+// Asynchronous copies into shared memory: 16 bytes (the first `bytes` of them
+// from global memory, the rest zeros; a miss fetches 256 bytes into L2), or 4.
+// A thread's copies up to a commit are one group; wait_group<N> waits for all
+// but the last N groups.
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
+    asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait_group() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
 // Programmatic dependent launch, kernel side: let the next kernel of the
 // stream begin launching now, and wait for the previous kernel's writes.
 __device__ __forceinline__ void pdl_launch_dependents() {

@@ -11,9 +11,13 @@
 //    instructions and up to 8 NT query rows (the heads that share a key head,
 //    times the sequence's tokens) their N side, so that a few rows fill the
 //    instruction better than with queries as M. The operands of both products
-//    come straight from global memory in 16-byte loads: the sums over dim and
-//    over tokens may run in any order, so each lane takes whole 16-byte pieces
-//    and the other operand is permuted to match. No shared memory, no barrier.
+//    are read in 16-byte pieces: the sums over dim and over tokens may run in
+//    any order, so each lane takes whole pieces and the other operand is
+//    permuted to match.
+//  * Every warp streams its tiles through a ring of its own in shared memory by
+//    16-byte asynchronous copies, two to seven tiles ahead, without barriers.
+//    (Loads into registers kept 4 KB a warp in flight, 64 KB an SM: 102 us for
+//    64 ragged sequences, bf16, against X us.)
 //  * Scores: mma s8 x s8 -> s32 on the raw key codes; each query row is fixed
 //    point in signed base-256 digits (2 for f16 / bf16, 3 for f32), each
 //    digit one product, so the sums are exact integers. The accumulators
@@ -28,7 +32,7 @@
 //    in f32. For f32 each tile's product starts from zero and is added to the
 //    running sum by an ordinary f32 add: the tensor cores' accumulation
 //    truncates, which over hundreds of tiles costs more than f32 should lose.
-//  * Tasks of 16-token tiles, cut into equal runs over one wave of blocks
+//  * Tasks of 16-token tiles, cut over the workers of all SMs
 //    (kv_attention.cuh); split tasks are joined by kv_join_kernel.
 //
 // Sequences with more query rows than one tile of 16 go to the kernel of
@@ -47,7 +51,25 @@ constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr float kMagic = 12582912.0f;       // 1.5 2^23
 constexpr int kMagicBits = 0x4B400000;
-constexpr int kTaskUnits = 8;               // a task's fixed cost in tiles (its queries, its join)
+constexpr int kTaskUnits = 16;              // a task's fixed cost in tiles (its queries, its join)
+
+// d = c + a b with all of c the same register value: accumulators that begin at
+// a constant need no moves.
+__device__ __forceinline__ void mma_s8_16832_from(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, int c) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%10, %10, %10, %10};"
+        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(c));
+}
+__device__ __forceinline__ void mma_f16_16816_from(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1,
+                                                   float c) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%10, %10, %10, %10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c));
+}
 
 __device__ __forceinline__ void mma_f16_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile(
@@ -69,36 +91,6 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Cache codes are read once: no allocation in L1. CHECK: zeros unless ok.
-template <bool CHECK>
-__device__ __forceinline__ void load_codes(uint32_t (&w)[4], const int8_t* p, bool ok) {
-    if constexpr (CHECK) {
-        asm volatile(
-            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %5, 0;\n\t"
-            "mov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\tmov.b32 %3, 0;\n\t"
-            "@p ld.global.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];\n\t}"
-            : "=&r"(w[0]), "=&r"(w[1]), "=&r"(w[2]), "=&r"(w[3])
-            : "l"(p), "r"(static_cast<int>(ok)));
-    } else {
-        asm volatile("ld.global.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];"
-                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                     : "l"(p));
-    }
-}
-template <bool CHECK>
-__device__ __forceinline__ void load_codes(uint32_t (&w)[2], const int8_t* p, bool ok) {
-    if constexpr (CHECK) {
-        asm volatile(
-            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %3, 0;\n\t"
-            "mov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\t"
-            "@p ld.global.L1::no_allocate.v2.b32 {%0, %1}, [%2];\n\t}"
-            : "=&r"(w[0]), "=&r"(w[1])
-            : "l"(p), "r"(static_cast<int>(ok)));
-    } else {
-        asm volatile("ld.global.L1::no_allocate.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p));
-    }
-}
-
 // Two f16 of signed codes from the biased bytes (code + 128) that `sel` picks
 // out of w: byte u in the low mantissa byte of 1024 is 1024 + u.
 template <uint32_t SEL>
@@ -108,28 +100,49 @@ __device__ __forceinline__ uint32_t codes_f16(uint32_t w) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Query rows as the B operand of the score products: DIGITS words for each
-// 32-wide step's two halves, and each row's factor. Lane (g, t) = (lane / 4,
-// lane % 4) holds row g; its pieces are the 16-byte pieces t, t + 4, ... of
-// dim, the same ones that lane (., t) loads of a key.
+// A lane's part of a query row: lane (g, t) = (lane / 4, lane % 4) holds, of
+// row g, the 16-byte pieces t, t + 4, ... of dim that lane (., t) reads of a
+// key.
+template <typename T, int DP>
+struct Query {
+    T v[DP / 64][16];
+};
+template <typename T, int DP>
+__device__ __forceinline__ void load_query(Query<T, DP>& q, const T* row, bool valid, int dim, bool vec, int t) {
+    #pragma unroll
+    for (int c = 0; c < DP / 64; ++c) {
+        const int d0 = 16 * (t + 4 * c);
+        const bool in = valid && d0 < dim;
+        #pragma unroll
+        for (int w = 0; w < 16; w += 4) {
+            if (in && vec) {
+                if constexpr (sizeof(T) == 4) {
+                    *reinterpret_cast<float4*>(&q.v[c][w]) = *reinterpret_cast<const float4*>(row + d0 + w);
+                } else {
+                    *reinterpret_cast<uint2*>(&q.v[c][w]) = *reinterpret_cast<const uint2*>(row + d0 + w);
+                }
+            } else {
+                #pragma unroll
+                for (int j = 0; j < 4; ++j) q.v[c][w + j] = in ? row[d0 + w + j] : from_f32<T>(0.0f);
+            }
+        }
+    }
+}
+
+// The row as the B operand of the score products: DIGITS words for each
+// 32-wide step's two halves, and the row's factor.
 template <typename T, int DP, int DIGITS>
-__device__ __forceinline__ float query_digits(uint32_t (&qd)[DIGITS][DP / 16], const T* row, bool valid, int dim,
-                                              bool vec, int t) {
+__device__ __forceinline__ float query_digits(uint32_t (&qd)[DIGITS][DP / 16], const Query<T, DP>& q) {
     constexpr int PIECES = DP / 64;
     float m = 0.0f;
     bool bad = false;
     #pragma unroll
     for (int c = 0; c < PIECES; ++c) {
-        const int d0 = 16 * (t + 4 * c);
         #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            if (valid && d0 < dim) load4(row + d0 + 4 * w, vec, v);
-            #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                m = fmaxf(m, fabsf(v[j]));
-                bad = bad || !(fabsf(v[j]) <= 3.4028234663852886e38f);
-            }
+        for (int j = 0; j < 16; ++j) {
+            const float v = fabsf(to_f32(q.v[c][j]));
+            m = fmaxf(m, v);
+            bad = bad || !(v <= 3.4028234663852886e38f);
         }
     }
     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
@@ -154,14 +167,14 @@ __device__ __forceinline__ float query_digits(uint32_t (&qd)[DIGITS][DP / 16], c
     constexpr uint32_t BIAS = DIGITS == 2 ? 0x8080u : 0x808080u;
     #pragma unroll
     for (int c = 0; c < PIECES; ++c) {
-        const int d0 = 16 * (t + 4 * c);
         #pragma unroll
         for (int w = 0; w < 4; ++w) {
-            float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            if (valid && !nan && d0 < dim) load4(row + d0 + 4 * w, vec, v);
             uint32_t y[4];
             #pragma unroll
-            for (int j = 0; j < 4; ++j) y[j] = static_cast<uint32_t>(__float2int_rn(v[j] * up)) + BIAS;
+            for (int j = 0; j < 4; ++j) {
+                const float v = nan ? 0.0f : to_f32(q.v[c][4 * w + j]);
+                y[j] = static_cast<uint32_t>(__float2int_rn(v * up)) + BIAS;
+            }
             #pragma unroll
             for (int i = 0; i < DIGITS; ++i) {
                 const uint32_t sel = static_cast<uint32_t>(i | ((i + 4) << 4));
@@ -192,22 +205,58 @@ struct Traits<float> {
     static constexpr bool kFresh = true;
 };
 
+// A block of kv_rows_kernel is an SM's whole load: as many workers of four
+// warps as its registers hold, each with its own run and barrier, and each warp
+// with a ring of tiles in shared memory, 16 rows of keys and 16 of values a
+// tile. The rings take 192 KB, most of it in flight, which is what it takes to
+// stream at HBM's rate. (Workers as blocks of their own, three to an SM, left
+// holes in the registers where they met the blocks of another kernel: the
+// one that did not fit began when others ended, 69 us against 55 for 131075
+// tokens, f16.)
+template <typename T, int DP, int NT>
+struct Rows {
+    static constexpr int kWorkers = DP == 256 ? 2 : 3;
+    static constexpr int kTileBytes = 2 * 16 * DP;
+    static constexpr int kStages = (192 / kWorkers) * 1024 / (kWarps * kTileBytes);  // 3 to 8
+    static constexpr int kRing = kWarps * kStages * kTileBytes;                      // of a worker
+    static constexpr int kScales = kWorkers * kRing;                                 // [warp][stage] {ks, vs}
+    static constexpr int kBytes = kScales + kWorkers * kWarps * kStages * 8;
+    static_assert(kRing >= kWarps * 8 * NT * DP * 4, "the warps' sums take the ring's place");
+};
+
+__device__ __forceinline__ void load_shared(uint32_t (&w)[4], uint32_t addr) {
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                 : "r"(addr));
+}
+__device__ __forceinline__ void load_shared(uint32_t (&w)[2], uint32_t addr) {
+    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr));
+}
+
 // DP: dim rounded up to 64, 128 or 256; FULL: dim is DP.
 template <typename T, int DP, int NT, bool FULL>
-__global__ void __launch_bounds__(kThreads, Traits<T>::kFresh || NT == 2 || DP == 256 ? (DP == 256 ? 2 : 3) : 4)
-kv_rows_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__((kThreads * Rows<T, DP, NT>::kWorkers), 1) kv_rows_kernel(const AttnArgs a) {
+    using R = Rows<T, DP, NT>;
     constexpr int DIGITS = Traits<T>::kDigits;
     constexpr bool SPLIT = Traits<T>::kSplit, FRESH = Traits<T>::kFresh;
     constexpr int ROWS = 8 * NT;
-    constexpr int KP = DP / 64;                // 16-byte pieces of a key row per lane
+    constexpr int STAGES = R::kStages;
+    constexpr int CH = DP / 16;                // 16-byte pieces of a row
+    constexpr int KP = DP / 64;                // ... of a key row per lane
     constexpr int VW = DP == 64 ? 2 : 4;       // words per piece of a value row
     constexpr int VP = DP == 256 ? 2 : 1;      // pieces of a value row per lane
     constexpr int NJ = DP / 16;                // 16-wide steps of dim in the value product
-    __shared__ float s_ml[kWarps][ROWS][2];
-    __shared__ __align__(16) float s_o[kWarps][ROWS][DP];
+    constexpr int COPIES = CH / 2;             // 16-byte copies of a lane for 16 rows
+    __shared__ float s_mls[R::kWorkers][kWarps][ROWS][2];
+    extern __shared__ __align__(128) uint8_t s_ring[];
+    const int worker = threadIdx.x / kThreads;  // of the block
+    float (*const s_o)[ROWS][DP] = reinterpret_cast<float (*)[ROWS][DP]>(s_ring + worker * R::kRing);  // after a task's tiles
+    float (*const s_ml)[ROWS][2] = s_mls[worker];
+    const auto sync_worker = [&] { asm volatile("bar.sync %0, %1;" ::"r"(1 + worker), "n"(kThreads) : "memory"); };
 
+    const uint32_t smem_ring = static_cast<uint32_t>(__cvta_generic_to_shared(s_ring));
     const int dim = FULL ? DP : a.dim;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int tid = threadIdx.x % kThreads, lane = tid & 31, warp = tid >> 5;  // of the worker
     const int g = lane >> 2, t = lane & 3;
     pdl_launch_dependents();
     pdl_wait();
@@ -217,11 +266,11 @@ kv_rows_kernel(const AttnArgs a) {
         see = span_of(a, s, 0, s.rows - 1);
         return (see.hi - see.lo + 15) >> 4;
     };
-    const Run run = find_run<kThreads>(a.seqs, kTaskUnits + kWarps, [&](int b, int64_t& units, int64_t& tasks) {
+    const Run run = find_run<kThreads * R::kWorkers, R::kWorkers, true>(a.seqs, kWarps, kTaskUnits, [&](int b, int64_t& tiles, int64_t& tasks) {
         const Seq s = sequence(a, b, &g_attn_err);
         Span see;
         tasks = static_cast<int64_t>((s.rows * a.group + ROWS - 1) / ROWS) * a.heads;
-        units = tasks * (kTaskUnits + max(tiles_of(s, see), 1));
+        tiles = tasks * max(tiles_of(s, see), 1);
     });
     if (tid == 0) clear_entries(a, run);
     int64_t run0 = run.begin, from = run.from, task0 = run.task0;
@@ -232,7 +281,8 @@ kv_rows_kernel(const AttnArgs a) {
         Span see;
         const int seen_tiles = tiles_of(s, see), tiles = max(seen_tiles, 1);
         const int row_tiles = (s.rows * a.group + ROWS - 1) / ROWS;
-        const int each = kTaskUnits + tiles;
+        const int pieces = run.piece ? static_cast<int>(divide(tiles + run.piece - 1, run.piece)) : 1;
+        const int each = run.piece ? pieces : run.fixed + tiles;
         const int64_t units = static_cast<int64_t>(row_tiles) * a.heads * each;
         if (run0 >= from + units) {
             from += units;
@@ -240,12 +290,19 @@ kv_rows_kernel(const AttnArgs a) {
             ++b;
             continue;
         }
-        const int task = static_cast<int>((run0 - from) / each);
-        const int c0 = static_cast<int>((run0 - from) % each);
+        const int task = static_cast<int>(divide(run0 - from, each));
+        const int c0 = static_cast<int>(run0 - from - static_cast<int64_t>(task) * each);
         const int c1 = static_cast<int>(min(static_cast<int64_t>(each), c0 + (run.end - run0)));
         run0 += c1 - c0;
-        const int u0 = max(0, c0 - kTaskUnits), u1 = c1 - kTaskUnits;
-        if (u1 <= 0) continue;  // only the fixed cost fell into this run: the next block has it all
+        int u0, u1;
+        if (run.piece) {
+            u0 = static_cast<int>(divide(static_cast<int64_t>(tiles) * c0, pieces));
+            u1 = static_cast<int>(divide(static_cast<int64_t>(tiles) * c1, pieces));
+        } else {
+            u0 = max(0, c0 - run.fixed);
+            u1 = c1 - run.fixed;
+            if (u1 <= 0) continue;  // only the fixed cost fell into this run: the next worker has it all
+        }
         const int h = task % a.heads, rt = task / a.heads;
         const int row_end = s.rows * a.group;
 
@@ -254,55 +311,67 @@ kv_rows_kernel(const AttnArgs a) {
         const int all1 = a.causal ? s.len - s.rows + tok_lo + 1 : s.len;
         const int64_t all0 = a.window > 0 ? static_cast<int64_t>(s.len) - s.rows + tok_hi + 1 - a.window : 0;
 
+        // Query rows are asked for first; they arrive behind the page indices.
+        Query<T, DP> q[NT];
+        #pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const int r = rt * ROWS + 8 * n + g;
+            const int tok = r / a.group, hd = r - tok * a.group;
+            const T* row = static_cast<const T*>(a.q) + (s.row0 + tok) * a.q_tok +
+                           static_cast<int64_t>(h * a.group + hd) * a.q_head;
+            load_query<T, DP>(q[n], row, r < row_end, dim, a.q_vec != 0, t);
+        }
         const int32_t* table = a.table + static_cast<int64_t>(b) * a.table_pages;
         const int last = min(u1, seen_tiles);
         const int page_mask = (1 << a.page_shift) - 1;
         const auto page_of = [&](int tile) {
             return tile < last ? table[(see.lo + 16 * tile) >> a.page_shift] : 0;
         };
-        // This lane's pieces: keys of rows g, g + 8, values of rows 2 t, 2 t + 1
-        // and those eight further.
-        const int8_t* k_lane = a.k + g * dim + 16 * t;
-        const int8_t* v_lane = a.v + 2 * t * dim + 4 * VW * g;
-        uint32_t kr[2][KP][4], vr[4][VP][VW];
-        float ks = 0.0f, vs = 0.0f;
-        const auto load_k = [&](int tile, int page) {
-            const int64_t at = static_cast<int64_t>(page) * a.heads + h;
-            const int8_t* p = k_lane + ((at << a.page_shift) + ((see.lo + 16 * tile) & page_mask)) * dim;
-            #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                #pragma unroll
-                for (int c = 0; c < KP; ++c) {
-                    load_codes<!FULL>(kr[r][c], p + 8 * r * dim + 64 * c, 16 * (t + 4 * c) < dim);
-                }
-            }
-            ks = a.ks[at];
-        };
-        const auto load_v = [&](int tile, int page) {
-            const int64_t at = static_cast<int64_t>(page) * a.heads + h;
-            const int8_t* p = v_lane + ((at << a.page_shift) + ((see.lo + 16 * tile) & page_mask)) * dim;
-            #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                #pragma unroll
-                for (int c = 0; c < VP; ++c) {
-                    load_codes<!FULL>(vr[i][c], p + ((i & 1) + 8 * (i >> 1)) * dim + 32 * VW * c,
-                                      4 * VW * (g + 8 * c) < dim);
-                }
-            }
-            vs = a.vs[at];
-        };
         const auto checked = [&](int page, bool& ok) {
             ok = page >= 0 && page < a.pages;
             return ok ? page : 0;
         };
-
-        int tile = u0 + warp;
-        bool ok = true, ok_next = true;
-        int page = checked(page_of(tile), ok);
-        int page_next = page_of(tile + kWarps);
-        if (tile < last) {
-            load_k(tile, page);
-            load_v(tile, page);
+        // The ring: row r's piece c lies at c ^ 4 (r & 1) for keys, of which
+        // eight lanes read two rows' half, and at c ^ 2 (r / 2 % 4) for values, of
+        // which they read a quarter of rows 0, 2, 4, 6: both without conflicts.
+        // (At dim 64 keys need no swizzle and values keep two-way conflicts.)
+        const uint32_t ring = smem_ring + worker * R::kRing + warp * STAGES * R::kTileBytes;
+        const uint32_t scales = smem_ring + R::kScales + (worker * kWarps + warp) * STAGES * 8;
+        const int crow = lane / CH, cpiece = lane % CH;  // of this lane's first copy
+        const auto k_place = [&](int r, int c) { return DP == 64 ? c : c ^ (r & 1) << 2; };
+        const auto v_place = [&](int r, int c) { return DP == 64 ? c ^ (r >> 1 & 1) << 1 : c ^ (r >> 1 & 3) << 1; };
+        unsigned int valid = 0;  // bit s: the page of the tile in stage s is one
+        const auto copy = [&](int tile, int stage, int page) {
+            bool in;
+            page = checked(page, in);
+            valid = (valid & ~(1u << stage)) | static_cast<unsigned int>(in) << stage;
+            const int64_t at = static_cast<int64_t>(page) * a.heads + h;
+            const int64_t off = ((at << a.page_shift) + ((see.lo + 16 * tile) & page_mask)) * dim;
+            const uint32_t dst = ring + stage * R::kTileBytes;
+            #pragma unroll
+            for (int n = 0; n < COPIES; ++n) {
+                const int r = crow + n * (32 / CH);
+                const int64_t src = off + (FULL ? 16 * lane + 512 * n : r * dim + 16 * cpiece);
+                const int bytes = FULL || 16 * cpiece < dim ? 16 : 0;
+                cp_async16(dst + r * DP + 16 * k_place(r, cpiece), a.k + (bytes ? src : off), bytes);
+                cp_async16(dst + 16 * DP + r * DP + 16 * v_place(r, cpiece), a.v + (bytes ? src : off), bytes);
+            }
+            if (lane < 2) cp_async4(scales + 8 * stage + 4 * lane, (lane == 0 ? a.ks : a.vs) + at);
+        };
+        // Tiles u0 + warp, u0 + warp + kWarps, ...: the first STAGES - 1 go out now,
+        // their page indices together.
+        const int tile0 = u0 + warp;
+        int page_ahead;
+        {
+            int pages[STAGES];
+            #pragma unroll
+            for (int i = 0; i < STAGES; ++i) pages[i] = page_of(tile0 + i * kWarps);
+            #pragma unroll
+            for (int i = 0; i < STAGES - 1; ++i) {
+                if (tile0 + i * kWarps < last) copy(tile0 + i * kWarps, i, pages[i]);
+                cp_async_commit();
+            }
+            page_ahead = pages[STAGES - 1];
         }
         // --- query rows ------------------------------------------------------
         uint32_t qd[NT][DIGITS][DP / 16];
@@ -310,11 +379,7 @@ kv_rows_kernel(const AttnArgs a) {
         int see0[NT][2], see1[NT][2];  // visible tokens of rows 2 t, 2 t + 1
         #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            const int r = rt * ROWS + 8 * n + g;
-            const int tok = r / a.group, hd = r - tok * a.group;
-            const T* row = static_cast<const T*>(a.q) + (s.row0 + tok) * a.q_tok +
-                           static_cast<int64_t>(h * a.group + hd) * a.q_head;
-            const float f = query_digits<T, DP, DIGITS>(qd[n], row, r < row_end, dim, a.q_vec != 0, t) * a.scale_log2;
+            const float f = query_digits<T, DP, DIGITS>(qd[n], q[n]) * a.scale_log2;
             #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 fac[n][c] = __shfl_sync(0xffffffffu, f, 4 * (2 * t + c));
@@ -329,18 +394,29 @@ kv_rows_kernel(const AttnArgs a) {
         #pragma unroll
         for (int n = 0; n < NT; ++n) m[n][0] = m[n][1] = -INFINITY, l[n][0] = l[n][1] = 0.0f;
 
-        for (; tile < last; tile += kWarps) {
-            page_next = checked(page_next, ok_next);
-            const bool more = tile + kWarps < last;
+        int stage = 0;
+        for (int tile = tile0; tile < last; tile += kWarps) {
+            cp_async_wait_group<STAGES - 2>();
+            __syncwarp();
+            {
+                const int ahead = tile + (STAGES - 1) * kWarps;
+                if (ahead < last) copy(ahead, stage == 0 ? STAGES - 1 : stage - 1, page_ahead);
+                cp_async_commit();
+                page_ahead = page_of(ahead + kWarps);
+            }
+            const bool ok_now = valid >> stage & 1u;
+            const uint32_t at = ring + stage * R::kTileBytes;
+            uint32_t kr[2][KP][4];
+            #pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                #pragma unroll
+                for (int c = 0; c < KP; ++c) load_shared(kr[r][c], at + (g + 8 * r) * DP + 16 * k_place(g, t + 4 * c));
+            }
+            uint32_t sv[2];
+            load_shared(sv, scales + 8 * stage);
+            const float ks_now = __uint_as_float(sv[0]), vs = __uint_as_float(sv[1]);
 
             int sc[NT][DIGITS][4];
-            #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                #pragma unroll
-                for (int i = 0; i < DIGITS; ++i) {
-                    sc[n][i][0] = sc[n][i][1] = sc[n][i][2] = sc[n][i][3] = kMagicBits;
-                }
-            }
             #pragma unroll
             for (int step = 0; step < DP / 32; ++step) {
                 // Words of the step's two halves: pieces 2 i and 2 i + 1, or two
@@ -353,15 +429,12 @@ kv_rows_kernel(const AttnArgs a) {
                 for (int n = 0; n < NT; ++n) {
                     #pragma unroll
                     for (int i = 0; i < DIGITS; ++i) {
-                        mma_s8_16832(sc[n][i], ka, qd[n][i][4 * p0 + w0], qd[n][i][4 * p1 + w1]);
+                        const uint32_t b0 = qd[n][i][4 * p0 + w0], b1 = qd[n][i][4 * p1 + w1];
+                        if (step == 0) mma_s8_16832_from(sc[n][i], ka, b0, b1, kMagicBits);
+                        else mma_s8_16832(sc[n][i], ka, b0, b1);
                     }
                 }
             }
-            const float ks_now = ks;
-            const bool ok_now = ok;
-            const int page_after = page_of(tile + 2 * kWarps);
-            if (more) load_k(tile + kWarps, page_next);
-
             // vs = 2^ve vf with vf in [1, 2); scales below 2^-80 belong to
             // all-zero codes, non-finite ones pass through vf.
             const uint32_t vbits = __float_as_uint(vs);
@@ -437,6 +510,17 @@ kv_rows_kernel(const AttnArgs a) {
                     }
                 }
             }
+            uint32_t vr[4][VP][VW];
+            #pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int r = 2 * t + (i & 1) + 8 * (i >> 1);
+                #pragma unroll
+                for (int c = 0; c < VP; ++c) {
+                    const uint32_t row = at + 16 * DP + r * DP;
+                    if constexpr (DP == 64) load_shared(vr[i][c], row + 16 * v_place(r, g >> 1) + 8 * (g & 1));
+                    else load_shared(vr[i][c], row + 16 * v_place(r, g + 8 * c));
+                }
+            }
             #pragma unroll
             for (int c = 0; c < VP; ++c) {
                 #pragma unroll
@@ -457,8 +541,8 @@ kv_rows_kernel(const AttnArgs a) {
                         #pragma unroll
                         for (int n = 0; n < NT; ++n) {
                             if (FRESH) {
-                                float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                                mma_f16_16816(d, va[i], lo[n][0], lo[n][1]);
+                                float d[4];
+                                mma_f16_16816_from(d, va[i], lo[n][0], lo[n][1], 0.0f);
                                 mma_f16_16816(d, va[i], hi[n][0], hi[n][1]);
                                 #pragma unroll
                                 for (int c4 = 0; c4 < 4; ++c4) o[n][j][c4] += d[c4];
@@ -470,15 +554,13 @@ kv_rows_kernel(const AttnArgs a) {
                     }
                 }
             }
-            if (more) load_v(tile + kWarps, page_next);
             if (!ok_now && lane == 0) atomicOr(&g_attn_err, kKvErrAttention);
-            page = page_next;
-            ok = ok_next;
-            page_next = page_after;
+            stage = stage == STAGES - 1 ? 0 : stage + 1;
         }
+        cp_async_wait_group<0>();
 
         // --- join the warps --------------------------------------------------
-        __syncthreads();  // the previous task's results have been read
+        sync_worker();  // all tiles have been read
         #pragma unroll
         for (int n = 0; n < NT; ++n) {
             #pragma unroll
@@ -498,9 +580,9 @@ kv_rows_kernel(const AttnArgs a) {
                 }
             }
         }
-        __syncthreads();
+        sync_worker();
         const bool complete = u0 == 0 && u1 == tiles;
-        const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (u0 > 0 ? 0 : 1);
+        const int64_t slot = 2 * static_cast<int64_t>(run.worker) + (u0 > 0 ? 0 : 1);
         for (int i = tid; i < ROWS * (DP / 4); i += kThreads) {
             const int r = i / (DP / 4), d = 4 * (i % (DP / 4));
             const int row = rt * ROWS + r;
@@ -526,9 +608,11 @@ kv_rows_kernel(const AttnArgs a) {
             }
         }
         if (tid == 0 && u0 == 0 && (a.by_task || !complete)) {
-            const int owner = complete ? blockIdx.x : owner_of_last(run, from + static_cast<int64_t>(task + 1) * each);
-            put_entry(a, task0 + task, owner - blockIdx.x, s, task);
+            const int more = complete ? 0 : run.piece ? pieces - 1
+                                          : owner_of_last(run, from + static_cast<int64_t>(task + 1) * each) - run.worker;
+            put_entry(a, run, task0 + task, more, s, task);
         }
+        sync_worker();  // the ring is free again
     }
 }
 
@@ -615,20 +699,18 @@ __global__ void __launch_bounds__(kThreads) kv_join_kernel(const AttnArgs a) {
     store_row<T>(a, e.z + tk, h * a.group + row - tk * a.group, d, o, den, top, d == 0);
 }
 
-// Work blocks of kv_rows_kernel: one wave, as many as are resident at once.
+// Sets the kernels' shared memory once a device.
 template <typename T, int DP, int NT, bool FULL>
-cudaError_t rows_grid(int64_t* grid) {
-    static int resident = 0;
-    int per_sm = __atomic_load_n(&resident, __ATOMIC_RELAXED);
-    if (per_sm == 0) {
-        const cudaError_t e =
-            cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kv_rows_kernel<T, DP, NT, FULL>, kThreads, 0);
-        if (e != cudaSuccess) return e;
-        if (per_sm < 1) return cudaErrorInvalidConfiguration;
-        __atomic_store_n(&resident, per_sm, __ATOMIC_RELAXED);
-    }
-    *grid = static_cast<int64_t>(per_sm) * device_sm_count();
-    return cudaSuccess;
+cudaError_t rows_ready() {
+    constexpr int kDevices = 64;
+    static bool ready[kDevices] = {};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || (dev < kDevices && __atomic_load_n(&ready[dev], __ATOMIC_RELAXED))) return e;
+    e = cudaFuncSetAttribute(kv_rows_kernel<T, DP, NT, FULL>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             Rows<T, DP, NT>::kBytes);
+    if (e == cudaSuccess && dev < kDevices) __atomic_store_n(&ready[dev], true, __ATOMIC_RELAXED);
+    return e;
 }
 
 // Launches with the caller's workspace, or only says how many bytes it takes
@@ -636,9 +718,7 @@ cudaError_t rows_grid(int64_t* grid) {
 template <typename T, int DP, int NT, bool FULL>
 cudaError_t run_rows(AttnArgs a, int64_t tasks, void* ws, int64_t* ws_bytes, cudaStream_t stream) {
     constexpr int ROWS = 8 * NT;
-    int64_t grid = 0;
-    cudaError_t e = rows_grid<T, DP, NT, FULL>(&grid);
-    if (e != cudaSuccess) return e;
+    const int64_t blocks = device_sm_count(), grid = blocks * Rows<T, DP, NT>::kWorkers;
     const int64_t entry_bytes = (1 + 2 * grid) * sizeof(int4);
     const int64_t ml_bytes = 2 * grid * ROWS * sizeof(float2);
     if (ws_bytes != nullptr) {
@@ -650,11 +730,16 @@ cudaError_t run_rows(AttnArgs a, int64_t tasks, void* ws, int64_t* ws_bytes, cud
     a.entry = static_cast<int4*>(ws);
     a.ml = reinterpret_cast<float2*>(static_cast<char*>(ws) + entry_bytes);
     a.part = reinterpret_cast<float*>(static_cast<char*>(ws) + entry_bytes + ml_bytes);
+    cudaError_t e = rows_ready<T, DP, NT, FULL>();
+    if (e != cudaSuccess) return e;
     cudaLaunchAttribute attr[1];
-    cudaLaunchConfig_t cfg = pdl_config(dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, stream, attr);
+    cudaLaunchConfig_t cfg = pdl_config(dim3(static_cast<unsigned>(blocks)), dim3(kThreads * Rows<T, DP, NT>::kWorkers),
+                                        Rows<T, DP, NT>::kBytes, stream, attr);
     e = cudaLaunchKernelEx(&cfg, kv_rows_kernel<T, DP, NT, FULL>, a);
     if (e != cudaSuccess) return e;
     cfg.gridDim = dim3(static_cast<unsigned>(a.entries), ROWS);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = 0;
     return cudaLaunchKernelEx(&cfg, kv_join_kernel<T, DP, ROWS>, a);
 }
 

@@ -128,7 +128,7 @@ struct Walk {
     __device__ void tile_sizes() {
         see = span_of(a, s, rt * kRows / a.group, min(s.rows - 1, (rt * kRows + kRows - 1) / a.group));
         steps = max((see.hi - see.lo + kTile - 1) / kTile, 1);
-        each = kFixedUnits + steps;
+        each = run.fixed + steps;
     }
     __device__ bool next() {
         while (at < run.end) {
@@ -146,15 +146,15 @@ struct Walk {
                 if (++rt < row_tiles()) tile_sizes();
                 continue;
             }
-            task_in_tile = static_cast<int>((at - from) / each);
-            const int c0 = static_cast<int>((at - from) % each);
+            task_in_tile = static_cast<int>(divide(at - from, each));
+            const int c0 = static_cast<int>(at - from - static_cast<int64_t>(task_in_tile) * each);
             const int c1 = static_cast<int>(min(static_cast<int64_t>(each), c0 + (run.end - at)));
             at += c1 - c0;
-            u0 = max(0, c0 - kFixedUnits);
-            u1 = c1 - kFixedUnits;
+            u0 = max(0, c0 - run.fixed);
+            u1 = c1 - run.fixed;
             if (u1 <= 0) continue;
             complete = u0 == 0 && u1 == steps;
-            more = complete ? 0 : owner_of_last(run, from + static_cast<int64_t>(task_in_tile + 1) * each) - static_cast<int>(blockIdx.x);
+            more = complete ? 0 : owner_of_last(run, from + static_cast<int64_t>(task_in_tile + 1) * each) - run.worker;
             task_number = task0 + task_in_tile;
             return true;
         }
@@ -203,11 +203,11 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const AttnArgs 
         tmem_relinquish();
     }
     pdl_launch_dependents();
-    const Run run = find_run<kPThreads>(a.seqs, kFixedUnits + 1, [&](int b, int64_t& units, int64_t& tasks) {
+    const Run run = find_run<kPThreads, 1, false>(a.seqs, 1, kFixedUnits, [&](int b, int64_t& steps, int64_t& tasks) {
         const Seq s = sequence(a, b, &g_prompt_err);
         for (int r = 0; r < s.rows * a.group; r += kRows) {
             const Span see = span_of(a, s, r / a.group, min(s.rows - 1, (r + kRows - 1) / a.group));
-            units += static_cast<int64_t>(kFixedUnits + max((see.hi - see.lo + kTile - 1) / kTile, 1)) * a.heads;
+            steps += static_cast<int64_t>(max((see.hi - see.lo + kTile - 1) / kTile, 1)) * a.heads;
             tasks += a.heads;
         }
     });
@@ -411,7 +411,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const AttnArgs 
             if (valid && walk.complete) store_lse(a, walk.s.row0 + tok, head, den, top);
             if (valid && !walk.complete) a.ml[slot] = make_float2(top, den);
             if (tid == 0 && walk.u0 == 0 && (a.by_task || !walk.complete)) {
-                put_entry(a, walk.task_number, walk.more, walk.s, walk.rt * a.heads + walk.task_in_tile);
+                put_entry(a, run, walk.task_number, walk.more, walk.s, walk.rt * a.heads + walk.task_in_tile);
             }
             tc_fence_before();  // O has been read: the next segment's products may follow
         }

@@ -266,7 +266,8 @@ __global__ void __launch_bounds__((kThreads * Rows<T, DP, NT>::kWorkers), 1) kv_
         see = span_of(a, s, 0, s.rows - 1);
         return (see.hi - see.lo + 15) >> 4;
     };
-    const Run run = find_run<kThreads * R::kWorkers, R::kWorkers, true>(a.seqs, kWarps, kTaskUnits, [&](int b, int64_t& tiles, int64_t& tasks) {
+    // Worker g gridDim.x + blockIdx.x: the first ones of all blocks before the second.
+    const Run run = find_run<true>(a.seqs, worker * gridDim.x + blockIdx.x, R::kWorkers * gridDim.x, kWarps, kTaskUnits, [&](int b, int64_t& tiles, int64_t& tasks) {
         const Seq s = sequence(a, b, &g_attn_err);
         Span see;
         tasks = static_cast<int64_t>((s.rows * a.group + ROWS - 1) / ROWS) * a.heads;
@@ -311,7 +312,18 @@ __global__ void __launch_bounds__((kThreads * Rows<T, DP, NT>::kWorkers), 1) kv_
         const int all1 = a.causal ? s.len - s.rows + tok_lo + 1 : s.len;
         const int64_t all0 = a.window > 0 ? static_cast<int64_t>(s.len) - s.rows + tok_hi + 1 - a.window : 0;
 
-        // Query rows are asked for first; they arrive behind the page indices.
+        const int32_t* table = a.table + static_cast<int64_t>(b) * a.table_pages;
+        const int last = min(u1, seen_tiles);
+        const int page_mask = (1 << a.page_shift) - 1;
+        const auto page_of = [&](int tile) {
+            return tile < last ? table[(see.lo + 16 * tile) >> a.page_shift] : 0;
+        };
+        // Tiles u0 + warp, u0 + warp + kWarps, ...: the first tiles' page indices,
+        // then the query rows, are on their way while addresses are computed.
+        const int tile0 = u0 + warp;
+        int pages[STAGES];
+        #pragma unroll
+        for (int i = 0; i < STAGES; ++i) pages[i] = page_of(tile0 + i * kWarps);
         Query<T, DP> q[NT];
         #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -321,12 +333,6 @@ __global__ void __launch_bounds__((kThreads * Rows<T, DP, NT>::kWorkers), 1) kv_
                            static_cast<int64_t>(h * a.group + hd) * a.q_head;
             load_query<T, DP>(q[n], row, r < row_end, dim, a.q_vec != 0, t);
         }
-        const int32_t* table = a.table + static_cast<int64_t>(b) * a.table_pages;
-        const int last = min(u1, seen_tiles);
-        const int page_mask = (1 << a.page_shift) - 1;
-        const auto page_of = [&](int tile) {
-            return tile < last ? table[(see.lo + 16 * tile) >> a.page_shift] : 0;
-        };
         const auto checked = [&](int page, bool& ok) {
             ok = page >= 0 && page < a.pages;
             return ok ? page : 0;
@@ -358,21 +364,12 @@ __global__ void __launch_bounds__((kThreads * Rows<T, DP, NT>::kWorkers), 1) kv_
             }
             if (lane < 2) cp_async4(scales + 8 * stage + 4 * lane, (lane == 0 ? a.ks : a.vs) + at);
         };
-        // Tiles u0 + warp, u0 + warp + kWarps, ...: the first STAGES - 1 go out now,
-        // their page indices together.
-        const int tile0 = u0 + warp;
-        int page_ahead;
-        {
-            int pages[STAGES];
-            #pragma unroll
-            for (int i = 0; i < STAGES; ++i) pages[i] = page_of(tile0 + i * kWarps);
-            #pragma unroll
-            for (int i = 0; i < STAGES - 1; ++i) {
-                if (tile0 + i * kWarps < last) copy(tile0 + i * kWarps, i, pages[i]);
-                cp_async_commit();
-            }
-            page_ahead = pages[STAGES - 1];
+        #pragma unroll
+        for (int i = 0; i < STAGES - 1; ++i) {
+            if (tile0 + i * kWarps < last) copy(tile0 + i * kWarps, i, pages[i]);
+            cp_async_commit();
         }
+        int page_ahead = pages[STAGES - 1];
         // --- query rows ------------------------------------------------------
         uint32_t qd[NT][DIGITS][DP / 16];
         float fac[NT][2];

@@ -4,7 +4,7 @@
 // Work is a list of tasks (sequence, row tile, key head), in that order, each
 // a number of token tiles. The list is cut into equal runs, one per worker (a
 // group of warps), whatever the lengths are (they are on the device; every
-// block finds its workers' runs by a scan over them). A task that spans workers
+// warp finds its worker's run by a scan over them). A task that spans workers
 // leaves partial results (maximum, denominator, weighted sum), two slots per
 // worker: slot 0 for a task that an earlier worker began, slot 1 for one that a
 // later worker ends. They are joined in the workers' order.
@@ -113,116 +113,89 @@ __device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
     return a / b;
 }
 
-// Where a sequence's tasks begin in the scan over sequences: tiles or pieces
-// before it, tasks before it.
-template <int THREADS, class Add, class See>
-__device__ __forceinline__ void scan_sequences(int seqs, int64_t (&units)[THREADS / 32], int64_t (&tasks)[THREADS / 32],
-                                               int64_t& all_units, int64_t& all_tasks, const Add& add, const See& see) {
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    all_units = all_tasks = 0;
-    for (int base = 0; base < seqs; base += THREADS) {
-        int64_t mine = 0, mine_tasks = 0;
-        if (base + tid < seqs) add(base + tid, mine, mine_tasks);
-        int64_t x = mine, y = mine_tasks;
-        #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int64_t u = __shfl_up_sync(0xffffffffu, x, o), w = __shfl_up_sync(0xffffffffu, y, o);
-            if (lane >= o) x += u, y += w;
-        }
-        __syncthreads();  // the sums before have been read
-        if (lane == 31) units[warp] = x, tasks[warp] = y;
-        __syncthreads();
-        int64_t before = all_units, before_tasks = all_tasks;
-        #pragma unroll
-        for (int w = 0; w < THREADS / 32; ++w) {
-            if (w < warp) before += units[w], before_tasks += tasks[w];
-            all_units += units[w], all_tasks += tasks[w];
-        }
-        see(base + tid, base + THREADS >= seqs, before + x - mine, mine, before_tasks + y - mine_tasks, mine_tasks);
-    }
-}
-
 // share(b, tiles, tasks): what sequence b adds to the list. A worker gets at
 // least `least` tiles (while there are that many). Where workers get many
 // tiles, a task's fixed cost counts as `fixed` of them. PIECES: all tasks of a
 // sequence have the same number of tiles, and few tasks are cut into pieces.
-template <int THREADS, int GROUPS, bool PIECES, class Share>
-__device__ Run find_run(int seqs, int least, int fixed, const Share& share) {
-    __shared__ int64_t s_units[THREADS / 32], s_tasks[THREADS / 32], s_from[GROUPS], s_task0[GROUPS];
-    __shared__ int s_b[GROUPS];
-    const int group = threadIdx.x / (THREADS / GROUPS);
-    const int64_t workers = static_cast<int64_t>(GROUPS) * gridDim.x;
-    Run run = {};
-    int64_t begins[GROUPS];
-    const auto cut = [&](int64_t units, int64_t by) {
-        run.total = units;
-        run.each = divide(units, by);
-        run.extra = units - run.each * by;
+//
+// Every warp does it for itself, a lane for each 32nd of the sequences: two
+// memory latencies and a scan by shuffles, no barrier (at a few sequences, where
+// it counts, a scan by the whole block took 2.7 us of a 9 us kernel).
+template <bool PIECES, class Share>
+__device__ Run find_run(int seqs, int worker, int64_t workers, int least, int fixed, const Share& share) {
+    const int lane = threadIdx.x & 31;
+    const int per = (seqs + 31) >> 5, b0 = lane * per, b1 = min(seqs, b0 + per);
+    const auto scan = [&](int64_t x) {  // inclusive
         #pragma unroll
-        for (int g = 0; g < GROUPS; ++g) {
-            const int64_t me = static_cast<int64_t>(g) * gridDim.x + blockIdx.x;
-            const bool on = me < by;
-            begins[g] = on ? me * run.each + min(me, run.extra) : units;
-            if (g == group) {
-                run.worker = static_cast<int>(me);
-                run.begin = begins[g];
-                run.end = on ? run.begin + run.each + (me < run.extra) : units;
-            }
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t u = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += u;
         }
+        return x;
     };
-    const auto plan = [&](int64_t tiles, int64_t tasks) {
-        run.tasks = tasks;
-        if (PIECES && 4 * tasks <= workers) {
-            const int64_t free = workers - tasks;  // rounding up costs a task at most one piece
-            run.piece = max(static_cast<int64_t>(least), divide(tiles + free - 1, free));
-            return;
-        }
-        run.fixed = tiles >= 4LL * fixed * workers ? fixed : 0;
-        cut(tiles + run.fixed * tasks, max(int64_t{1}, min(workers, divide(tiles, least))));
-    };
-    const auto found = [&](int b, int64_t from, int64_t units, int64_t task0) {
-        #pragma unroll
-        for (int g = 0; g < GROUPS; ++g) {
-            if (begins[g] >= from && begins[g] < from + units) s_b[g] = b, s_from[g] = from, s_task0[g] = task0;
-        }
-    };
-    int64_t tiles, tasks;
-    scan_sequences<THREADS>(seqs, s_units, s_tasks, tiles, tasks, share,
-                            [&](int b, bool last, int64_t from, int64_t mine, int64_t task0, int64_t mine_tasks) {
-                                // One chunk holds every sequence: this scan is all it takes.
-                                if (seqs > THREADS) return;
-                                int64_t all = 0, all_tasks = 0;
-                                for (int w = 0; w < THREADS / 32; ++w) all += s_units[w], all_tasks += s_tasks[w];
-                                plan(all, all_tasks);
-                                if (run.piece == 0) found(b, from + run.fixed * task0, mine + run.fixed * mine_tasks, task0);
-                            });
-    if (seqs > THREADS) plan(tiles, tasks);
-    if (run.piece != 0) {
-        // Pieces: their number in all, then (or at once) whose this worker's is.
-        const auto pieces = [&](int b, int64_t& units, int64_t& mine_tasks) {
-            int64_t t = 0;
-            share(b, t, mine_tasks);
-            units = mine_tasks > 0 ? mine_tasks * divide(divide(t, mine_tasks) + run.piece - 1, run.piece) : 0;
-        };
-        #pragma unroll
-        for (int g = 0; g < GROUPS; ++g) begins[g] = static_cast<int64_t>(g) * gridDim.x + blockIdx.x;
-        run.worker = static_cast<int>(static_cast<int64_t>(group) * gridDim.x + blockIdx.x);
-        int64_t count = 0;
-        scan_sequences<THREADS>(seqs, s_units, s_tasks, count, tasks, pieces,
-                                [&](int b, bool last, int64_t from, int64_t mine, int64_t task0, int64_t mine_tasks) {
-                                    found(b, from, mine, task0);
-                                });
-        run.total = count;
-        run.begin = min(static_cast<int64_t>(run.worker), count);
-        run.end = min(run.begin + 1, count);
-    } else if (seqs > THREADS) {
-        scan_sequences<THREADS>(seqs, s_units, s_tasks, tiles, tasks, share,
-                                [&](int b, bool last, int64_t from, int64_t mine, int64_t task0, int64_t mine_tasks) {
-                                    found(b, from + run.fixed * task0, mine + run.fixed * mine_tasks, task0);
-                                });
+    int64_t mine = 0, mine_tasks = 0;
+    #pragma unroll 4
+    for (int b = b0; b < b1; ++b) {
+        int64_t t = 0, k = 0;
+        share(b, t, k);
+        mine += t, mine_tasks += k;
     }
-    __syncthreads();
-    run.b = s_b[group], run.from = s_from[group], run.task0 = s_task0[group];
+    int64_t units = scan(mine);
+    const int64_t tasks = scan(mine_tasks), tiles = __shfl_sync(0xffffffffu, units, 31);
+    Run run = {};
+    run.worker = worker;
+    run.tasks = __shfl_sync(0xffffffffu, tasks, 31);
+    int64_t task0 = tasks - mine_tasks, from = units - mine;
+    if (PIECES && 4 * run.tasks <= workers) {
+        const int64_t free = workers - run.tasks;  // rounding up costs a task at most one piece
+        run.piece = max(static_cast<int64_t>(least), divide(tiles + free - 1, free));
+    } else {
+        run.fixed = tiles >= 4LL * fixed * workers ? fixed : 0;
+    }
+    const auto units_of = [&](int64_t t, int64_t k) {
+        if (run.piece == 0) return t + run.fixed * k;
+        return k > 0 ? k * divide(divide(t, k) + run.piece - 1, run.piece) : 0;
+    };
+    if (run.piece != 0) {
+        mine = 0;
+        for (int b = b0; b < b1; ++b) {
+            int64_t t = 0, k = 0;
+            share(b, t, k);
+            mine += units_of(t, k);
+        }
+        units = scan(mine);
+        from = units - mine;
+        run.total = __shfl_sync(0xffffffffu, units, 31);
+        run.begin = min(static_cast<int64_t>(worker), run.total);
+        run.end = min(run.begin + 1, run.total);
+    } else {
+        from += run.fixed * task0;
+        mine += run.fixed * mine_tasks;
+        run.total = tiles + run.fixed * run.tasks;
+        const int64_t by = max(int64_t{1}, min(workers, divide(tiles, least)));
+        run.each = divide(run.total, by);
+        run.extra = run.total - run.each * by;
+        run.begin = worker < by ? worker * run.each + min(static_cast<int64_t>(worker), run.extra) : run.total;
+        run.end = worker < by ? run.begin + run.each + (worker < run.extra) : run.total;
+    }
+    // The lane whose sequences hold the first unit walks through them.
+    int b = b0;
+    const bool here = run.begin >= from && run.begin < from + mine;
+    if (here) {
+        for (; b < b1 - 1; ++b) {
+            int64_t t = 0, k = 0;
+            share(b, t, k);
+            t = units_of(t, k);
+            if (run.begin < from + t) break;
+            from += t;
+            task0 += k;
+        }
+    }
+    const unsigned int who = __ballot_sync(0xffffffffu, here);
+    const int src = who ? __ffs(who) - 1 : 0;  // (none: an empty run)
+    run.b = __shfl_sync(0xffffffffu, b, src);
+    run.from = __shfl_sync(0xffffffffu, from, src);
+    run.task0 = __shfl_sync(0xffffffffu, task0, src);
     return run;
 }
 

@@ -203,7 +203,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const AttnArgs 
         tmem_relinquish();
     }
     pdl_launch_dependents();
-    const Run run = find_run<kPThreads, 1, false>(a.seqs, 1, kFixedUnits, [&](int b, int64_t& steps, int64_t& tasks) {
+    const Run run = find_run<false>(a.seqs, blockIdx.x, gridDim.x, 1, kFixedUnits, [&](int b, int64_t& steps, int64_t& tasks) {
         const Seq s = sequence(a, b, &g_prompt_err);
         for (int r = 0; r < s.rows * a.group; r += kRows) {
             const Span see = span_of(a, s, r / a.group, min(s.rows - 1, (r + kRows - 1) / a.group));

@@ -51,7 +51,7 @@ constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr float kMagic = 12582912.0f;       // 1.5 2^23
 constexpr int kMagicBits = 0x4B400000;
-constexpr int kTaskUnits = 16;              // a task's fixed cost in tiles (its queries, its join)
+constexpr int kTaskUnits = 24;             // a task's fixed cost in tiles (5 us: its queries, its first tiles, its join)
 
 // d = c + a b with all of c the same register value: accumulators that begin at
 // a constant need no moves.

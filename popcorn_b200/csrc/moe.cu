@@ -28,7 +28,6 @@
 #include "common.cuh"
 #include "mma_frag.cuh"
 #include "popcorn_serve.h"
-#include "sm100.cuh"
 
 namespace pcb {
 namespace {
@@ -60,19 +59,8 @@ struct MoeArgs {
     float* hs;         // [M top][fp / 32] their units
     float* h;          // [M top][F] hidden values (plain kernels only)
     int M, K, F, E, top, renorm, kp, fp;
-    int split;         // blocks that share 16 output channels of the down product
+    int rows;          // output channels of a tile of the down product
 };
-
-__device__ __forceinline__ uint4 load_stream(const int8_t* p, bool ok) {
-    uint4 v;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %5, 0;\n\t"
-        "mov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\tmov.b32 %3, 0;\n\t"
-        "@p ld.global.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];\n\t}"
-        : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w)
-        : "l"(p), "r"(static_cast<int>(ok)));
-    return v;
-}
 
 // Fixed point of values up to m in magnitude: 2^s brings m to [2^29, 2^30)
 // (as two factors, since s goes up to 149, where the unit 2^-s is f32's
@@ -249,12 +237,12 @@ __device__ void pick_experts(const MoeArgs& a, int m, Routing& r, int lane) {
 }
 
 // The block's lists from the picks in r.pick.
-template <int NP>
+template <int NP, int THREADS>
 __device__ void list_jobs(const MoeArgs& a, Routing& r) {
     const int tid = threadIdx.x;
-    if (tid < kMoeExperts) r.tokens[tid][0] = r.tokens[tid][1] = 0;
+    for (int e = tid; e < a.E; e += THREADS) r.tokens[e][0] = r.tokens[e][1] = 0;
     __syncthreads();
-    for (int i = tid; i < a.M * a.top; i += kMoeThreads) {
+    for (int i = tid; i < a.M * a.top; i += THREADS) {
         const int m = i / a.top;
         atomicOr(&r.tokens[r.pick[i]][m >> 5], 1u << (m & 31));
     }
@@ -284,7 +272,7 @@ __device__ void list_jobs(const MoeArgs& a, Routing& r) {
         if (tid == 0) r.jobs = jobs;
     }
     __syncthreads();
-    for (int i = tid; i < a.M * a.top; i += kMoeThreads) {
+    for (int i = tid; i < a.M * a.top; i += THREADS) {
         const int m = i / a.top, e = r.pick[i];
         const unsigned int below = (1u << (m & 31)) - 1u;
         const int rank = m < 32 ? __popc(r.tokens[e][0] & below) : __popc(r.tokens[e][0]) + __popc(r.tokens[e][1] & below);
@@ -294,12 +282,13 @@ __device__ void list_jobs(const MoeArgs& a, Routing& r) {
     __syncthreads();
 }
 
+template <int THREADS>
 __device__ void route_tokens(const MoeArgs& a, Routing& r) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for (int m = warp; m < a.M; m += kMoeWarps) pick_experts(a, m, r, lane);
+    for (int m = warp; m < a.M; m += THREADS / 32) pick_experts(a, m, r, lane);
     __syncthreads();
     if (blockIdx.x == 0) {
-        for (int i = threadIdx.x; i < a.M * a.top; i += kMoeThreads) {
+        for (int i = threadIdx.x; i < a.M * a.top; i += THREADS) {
             a.experts[i] = r.pick[i];
             a.weights[i] = r.weight[i];
         }
@@ -309,36 +298,103 @@ __device__ void route_tokens(const MoeArgs& a, Routing& r) {
 // ------------------------------------------------------------- gate and up
 // An item is a job's 32 rows of both matrices: two tiles of 16 rows each, of
 // which rows 0-7 and 8-15 are runs of eight (the columns that share a unit in
-// the next product). Warps take every eighth window; a window's loads are
-// issued as soon as the one before has been multiplied, across items too, so
-// that they are in flight while the item's sums are joined.
+// the next product). A block is an SM's whole load, three workers of four warps,
+// each with its own items and barrier; a warp has a quarter of the windows and
+// streams them, from one item into the next, through a ring of its own in
+// shared memory (4 KB a window) by asynchronous copies: 144 KB an SM in flight.
+// (Loads into registers with two or three blocks an SM kept at most 96 KB in
+// flight and reached 4.5 TB/s.)
+constexpr int kUpWarps = 4, kUpThreads = 32 * kUpWarps, kUpWorkers = 3;
 template <int NP>
-__global__ void __launch_bounds__(kMoeThreads, NP == 1 ? 3 : 2) up_kernel(const MoeArgs a) {
+struct Up {
+    static constexpr int kStages = NP == 4 ? 3 : 4;
+    static constexpr int kParities = NP == 1 ? 2 : 1;   // sums of an item may wait while the next is multiplied
+    static constexpr int kWindow = 64 * 64;             // [gate runs 0-3, up runs 0-3][8 rows][64 bytes]
+    static constexpr int kRing = kUpWorkers * kUpWarps * kStages * kWindow;
+    static constexpr int kBytes = kRing;
+};
+
+__device__ __forceinline__ uint4 load_shared16(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+    return v;
+}
+
+template <int NP>
+__global__ void __launch_bounds__(kUpWorkers* kUpThreads, 1) up_kernel(const MoeArgs a) {
+    using U = Up<NP>;
+    constexpr int STAGES = U::kStages, THREADS = kUpWorkers * kUpThreads;
+    extern __shared__ __align__(128) uint8_t s_ring[];
     __shared__ Routing r;
-    __shared__ int sums[2][4][16][8 * NP + 1];  // item parity; [gate 0, gate 1, up 0, up 1][row][token, digit]
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    __shared__ int s_sums[kUpWorkers][U::kParities][4][16][8 * NP + 1];  // [gate 0, gate 1, up 0, up 1][row][token, digit]
+    const int worker = threadIdx.x / kUpThreads;
+    const int tid = threadIdx.x % kUpThreads, lane = tid & 31, warp = tid >> 5;  // of the worker
     const int g = lane >> 2, t = lane & 3;
+    const auto sync_worker = [&] { asm volatile("bar.sync %0, %1;" ::"r"(1 + worker), "n"(kUpThreads) : "memory"); };
+    auto& sums = s_sums[worker];
     pdl_launch_dependents();
-    for (int i = tid; i < 2 * 4 * 16 * (8 * NP + 1); i += kMoeThreads) (&sums[0][0][0][0])[i] = 0;
+    for (int i = threadIdx.x; i < static_cast<int>(sizeof(s_sums) / 4); i += THREADS) (&s_sums[0][0][0][0][0])[i] = 0;
     pdl_wait();
-    route_tokens(a, r);
-    list_jobs<NP>(a, r);
+    route_tokens<THREADS>(a, r);
+    list_jobs<NP, THREADS>(a, r);
 
     const int halves = a.fp / 32, windows = (a.K + 63) / 64;
     const int items = r.jobs * halves;
-    const int8_t *gate[4], *up[4], *xd[NP];
-    bool on[NP];
-    uint4 q[4][2], b[NP];
-    const auto setup = [&](int item) {
+    const int w_begin = warp * windows / kUpWarps, w_end = (warp + 1) * windows / kUpWarps;
+    const int first = worker * gridDim.x + blockIdx.x, stride = kUpWorkers * gridDim.x;
+    const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(s_ring)) +
+                          (worker * kUpWarps + warp) * STAGES * U::kWindow;
+
+    // The copying side: item, window and this lane's rows of the item.
+    int c_item = first, c_w = w_begin, c_stage = 0;
+    const int8_t *gate = nullptr, *up = nullptr;  // row of run 0
+    int64_t step[4] = {0, 0, 0, 0};               // bytes from there to the row of run i
+    const auto rows_of = [&](int item) {
         const Job job = job_of(r, item / halves);
         const int h = item % halves;
+        const int f = h / 2 * 64 + 8 * (h & 1) + g;
+        const int64_t at = (static_cast<int64_t>(job.expert) * a.F + min(f, a.F - 1)) * a.K;
+        gate = a.qg + at + 16 * t;
+        up = a.qu + at + 16 * t;
         #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int f = min(h / 2 * 64 + 16 * i + 8 * (h & 1) + g, a.F - 1);
-            const int64_t at = (static_cast<int64_t>(job.expert) * a.F + f) * a.K + 16 * t;
-            gate[i] = a.qg + at;
-            up[i] = a.qu + at;
+        for (int i = 1; i < 4; ++i) step[i] = static_cast<int64_t>(min(f + 16 * i, a.F - 1) - min(f, a.F - 1)) * a.K;
+    };
+    const auto copy_next = [&] {
+        if (c_item < items && w_begin < w_end) {
+            const int bytes = 64 * c_w + 16 * t < a.K ? 16 : 0;
+            const int64_t at = bytes ? 64 * c_w : 0;
+            const uint32_t dst = ring + c_stage * U::kWindow + 16 * lane;
+            #pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                cp_async16(dst + 512 * i, gate + step[i] + at, bytes);
+                cp_async16(dst + 2048 + 512 * i, up + step[i] + at, bytes);
+            }
+            if (++c_w == w_end) {
+                c_w = w_begin;
+                c_item += stride;
+                if (c_item < items) rows_of(c_item);
+            }
         }
+        cp_async_commit();
+        c_stage = c_stage == STAGES - 1 ? 0 : c_stage + 1;
+    };
+    if (first < items) rows_of(first);
+    #pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i) copy_next();
+
+    int parity = 0, stage = 0;
+    for (int item = first; item < items; item += stride) {
+        const Job job = job_of(r, item / halves);
+        const int8_t* xd[NP];
+        bool on[NP];
+        uint4 b[NP];
+        const auto load_b = [&](int w) {
+            #pragma unroll
+            for (int n = 0; n < NP; ++n) {
+                b[n] = make_uint4(0u, 0u, 0u, 0u);
+                if (on[n]) b[n] = *reinterpret_cast<const uint4*>(xd[n] + 64 * w);
+            }
+        };
         #pragma unroll
         for (int n = 0; n < NP; ++n) {
             const int j = 2 * n + (g >> 2);
@@ -346,45 +402,30 @@ __global__ void __launch_bounds__(kMoeThreads, NP == 1 ? 3 : 2) up_kernel(const 
             const int m = on[n] ? r.token[job.pos + j] : 0;
             xd[n] = a.xd + (static_cast<int64_t>(m) * 4 + (g & 3)) * a.kp + 16 * t;
         }
-    };
-    const auto load = [&](int w) {
-        const bool in = 64 * w + 16 * t < a.K;
-        #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            q[i >> 1][i & 1] = load_stream(gate[i] + 64 * w, in);
-            q[2 + (i >> 1)][i & 1] = load_stream(up[i] + 64 * w, in);
-        }
-        #pragma unroll
-        for (int n = 0; n < NP; ++n) {
-            b[n] = make_uint4(0u, 0u, 0u, 0u);
-            if (on[n]) b[n] = *reinterpret_cast<const uint4*>(xd[n] + 64 * w);
-        }
-    };
-    int parity = 0;
-    if (static_cast<int>(blockIdx.x) < items) {
-        setup(blockIdx.x);
-        if (warp < windows) load(warp);
-    }
-    for (int item = blockIdx.x; item < items; item += gridDim.x, parity ^= 1) {
+        if (w_begin < w_end) load_b(w_begin);
         int acc[NP][4][4] = {};
-        for (int w = warp; w < windows; w += kMoeWarps) {
+        for (int w = w_begin; w < w_end; ++w) {
+            cp_async_wait_group<STAGES - 2>();
+            __syncwarp();
+            copy_next();
+            const uint32_t at = ring + stage * U::kWindow + 16 * lane;
+            stage = stage == STAGES - 1 ? 0 : stage + 1;
+            uint4 now[NP];
             #pragma unroll
-            for (int n = 0; n < NP; ++n) {
+            for (int n = 0; n < NP; ++n) now[n] = b[n];
+            if (w + 1 < w_end) load_b(w + 1);
+            #pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint4 q0 = load_shared16(at + 1024 * i), q1 = load_shared16(at + 1024 * i + 512);
+                const uint32_t lo[4] = {q0.x, q1.x, q0.y, q1.y}, hi[4] = {q0.z, q1.z, q0.w, q1.w};
                 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t lo[4] = {q[i][0].x, q[i][1].x, q[i][0].y, q[i][1].y};
-                    const uint32_t hi[4] = {q[i][0].z, q[i][1].z, q[i][0].w, q[i][1].w};
-                    mma_s8_16832(acc[n][i], lo, b[n].x, b[n].y);
-                    mma_s8_16832(acc[n][i], hi, b[n].z, b[n].w);
+                for (int n = 0; n < NP; ++n) {
+                    mma_s8_16832(acc[n][i], lo, now[n].x, now[n].y);
+                    mma_s8_16832(acc[n][i], hi, now[n].z, now[n].w);
                 }
             }
-            if (w + kMoeWarps < windows) load(w + kMoeWarps);
         }
-        const int next = item + gridDim.x;
-        if (next < items) {
-            setup(next);
-            if (warp < windows) load(warp);
-        }
+        if (U::kParities == 1) sync_worker();  // the sums before have been taken
         #pragma unroll
         for (int n = 0; n < NP; ++n) {
             #pragma unroll
@@ -395,13 +436,12 @@ __global__ void __launch_bounds__(kMoeThreads, NP == 1 ? 3 : 2) up_kernel(const 
                 }
             }
         }
-        __syncthreads();
-        // Warp j: the job's token j; lane: one of the 32 rows. Sums are set back
-        // to zero as they are read; the other parity's barrier comes before the
-        // next use of this one's.
-        const Job job = job_of(r, item / halves);
-        if (warp < job.count) {
-            const int m = r.token[job.pos + warp];
+        sync_worker();
+        // Warp j: the job's tokens j, j + 4; lane: one of the 32 rows. Sums are set
+        // back to zero as they are read; a barrier of the next item comes before
+        // their next use.
+        for (int j = warp; j < job.count; j += kUpWarps) {
+            const int m = r.token[job.pos + j];
             const int h2 = item % halves;
             const int run = lane >> 3, f = h2 / 2 * 64 + 16 * run + 8 * (h2 & 1) + (lane & 7);
             const int tile = run >> 1, row = 8 * (run & 1) + (lane & 7);
@@ -409,7 +449,7 @@ __global__ void __launch_bounds__(kMoeThreads, NP == 1 ? 3 : 2) up_kernel(const 
             const int64_t at = static_cast<int64_t>(job.expert) * a.F + min(f, a.F - 1);
             const float sg = a.sg[at], su = a.su[at];
             const auto dot = [&](int (&s)[16][8 * NP + 1]) {
-                int* d = &s[row][4 * warp];
+                int* d = &s[row][4 * j];
                 const double v = ((static_cast<double>(d[3]) * 256.0 + d[2]) * 256.0 + d[1]) * 256.0 + d[0];
                 d[0] = d[1] = d[2] = d[3] = 0;
                 return static_cast<float>(v);
@@ -420,145 +460,182 @@ __global__ void __launch_bounds__(kMoeThreads, NP == 1 ? 3 : 2) up_kernel(const 
             const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(h))));
             const Fixed fx = fixed_for(top, bad);
             const uint32_t y = bad ? 0u : digits_of(h, fx);
-            const int64_t pair = r.pair[job.pos + warp];
+            const int64_t pair = r.pair[job.pos + j];
             int8_t* hd = a.hd + pair * 4 * a.fp + f;
             #pragma unroll
             for (int i = 0; i < 4; ++i) hd[static_cast<int64_t>(i) * a.fp] = static_cast<int8_t>(y >> (8 * i));
             if (lane == 0) a.hs[pair * halves + h2] = fx.unit;
         }
+        if (U::kParities == 2) parity ^= 1;
     }
+    cp_async_wait_group<0>();
 }
 
 // -------------------------------------------------------------------- down
-// A cluster of blocks owns output channels 16 x .. 16 x + 15 and its warps
-// share the (job, window) list in equal runs. Four windows' loads go out at
-// once; a step's exact integer sums join in f32 with the step's unit. At the
-// end of a job a warp adds its result, weighted, to its own sums per token;
-// warps, then blocks, are added in order at the end.
-template <int NP>
-__global__ void __launch_bounds__(kMoeThreads, 2) down_kernel(const MoeArgs a) {
-    extern __shared__ float outs[];  // [warp][token][16]
+// A block is an SM's whole load, 16 warps, and owns `rows` (at most 16, the M
+// side) output channels at a time: 14 for 2048 channels, twice 14 for 4096. Its
+// warps share the (job, window) list of a tile in equal runs, so that no other
+// block is needed for a token's sum over its experts; they stream it, from one
+// tile into the next, through rings in shared memory, four windows (4 KB) a
+// stage. A step's exact integer sums join in f32 with the step's unit. At the
+// end of a job a warp adds its result, weighted, to its own sums per token; the
+// warps' are added in order at the end of the tile.
+constexpr int kDownWarps = 16, kDownThreads = 32 * kDownWarps;
+constexpr int kDownWindows = 4, kDownStage = kDownWindows * 16 * 64;
+constexpr int down_stages(int tokens) { return tokens <= 16 ? 3 : 2; }  // what the sums leave room for
+
+template <int NP, int STAGES>
+__global__ void __launch_bounds__(kDownThreads, 1) down_kernel(const MoeArgs a) {
+    extern __shared__ __align__(128) uint8_t s_raw[];
+    float* const outs = reinterpret_cast<float*>(s_raw + kDownWarps * STAGES * kDownStage);  // [warp][token][16]
     __shared__ Routing r;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = lane >> 2, t = lane & 3;
     pdl_launch_dependents();
-    for (int i = tid; i < kMoeWarps * a.M * 16; i += kMoeThreads) outs[i] = 0.0f;
+    for (int i = tid; i < kDownWarps * a.M * 16; i += kDownThreads) outs[i] = 0.0f;
     pdl_wait();
-    for (int i = tid; i < a.M * a.top; i += kMoeThreads) {
+    for (int i = tid; i < a.M * a.top; i += kDownThreads) {
         r.pick[i] = static_cast<short>(a.experts[i]);
         r.weight[i] = a.weights[i];
     }
     __syncthreads();
-    list_jobs<NP>(a, r);
+    list_jobs<NP, kDownThreads>(a, r);
 
-    const int rank = blockIdx.x % a.split;
-    const int n0 = blockIdx.x / a.split * 16;
-    const int windows = a.fp / 64;
+    const int windows = a.fp / 64, tiles = (a.K + a.rows - 1) / a.rows;
     const int64_t units = static_cast<int64_t>(r.jobs) * windows;
-    const int who = rank * kMoeWarps + warp, all = a.split * kMoeWarps;
-    int u = static_cast<int>(units * who / all);
-    const int u_end = static_cast<int>(units * (who + 1) / all);
-    float* mine = outs + warp * a.M * 16;
-    while (u < u_end) {
-        const int w_begin = u % windows;
-        const Job job = job_of(r, u / windows);
-        const int w_end = min(windows, w_begin + (u_end - u));
-        u += w_end - w_begin;
-        const int8_t* rows[2];
-        float scale[2];
-        #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int64_t n = static_cast<int64_t>(job.expert) * a.K + min(n0 + 8 * j + g, a.K - 1);
-            rows[j] = a.qd + n * a.F + 16 * t;
-            scale[j] = a.sd[n];
-        }
-        const int8_t* hd[NP];
-        const float* hs[NP];
-        bool on[NP];
-        #pragma unroll
-        for (int n = 0; n < NP; ++n) {
-            // This lane's column of the B operand, and the token of its result columns.
-            const int j = 2 * n + (g >> 2), jr = min(2 * n + (t >> 1), job.count - 1);
-            on[n] = j < job.count;
-            hd[n] = a.hd + (static_cast<int64_t>(r.pair[job.pos + (on[n] ? j : 0)]) * 4 + (g & 3)) * a.fp + 16 * t;
-            hs[n] = a.hs + static_cast<int64_t>(r.pair[job.pos + jr]) * (2 * windows);
-        }
-        float acc[NP][4] = {};
-        constexpr int AHEAD = NP == 4 ? 2 : 4;
-        for (int w0 = w_begin; w0 < w_end; w0 += AHEAD) {
-            uint4 q[AHEAD][2], b[AHEAD][NP];
-            float2 unit[AHEAD][NP];
+    const int u_begin = static_cast<int>(units * warp / kDownWarps), u_end = static_cast<int>(units * (warp + 1) / kDownWarps);
+    const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(s_raw)) + warp * STAGES * kDownStage;
+    float* const mine = outs + warp * a.M * 16;
+
+    // The copying side: a stage is up to four windows of one job.
+    int c_tile = blockIdx.x, c_u = u_begin, c_stage = 0;
+    const auto copy_next = [&] {
+        if (c_tile < tiles && c_u < u_end) {
+            const int job_i = c_u / windows, w = c_u - job_i * windows;
+            const int count = min(min(kDownWindows, windows - w), u_end - c_u);
+            const int n0 = c_tile * a.rows, n_end = min(a.K, n0 + a.rows);
+            const int64_t expert = static_cast<int64_t>(job_of(r, job_i).expert) * a.K;
+            const uint32_t dst = ring + c_stage * kDownStage + 16 * lane;
             #pragma unroll
-            for (int k = 0; k < AHEAD; ++k) {
-                const int w = w0 + k;
-                const bool in = w < w_end && 64 * w + 16 * t < a.F;
+            for (int j = 0; j < 2; ++j) {
+                const int n = n0 + 8 * j + g;
+                const int8_t* row = a.qd + (expert + min(n, a.K - 1)) * a.F;
                 #pragma unroll
-                for (int j = 0; j < 2; ++j) q[k][j] = load_stream(rows[j] + 64 * w, in);
+                for (int k = 0; k < kDownWindows; ++k) {
+                    const int col = 64 * (w + k) + 16 * t;
+                    const int bytes = n < n_end && k < count && col < a.F ? 16 : 0;
+                    cp_async16(dst + 1024 * k + 512 * j, row + (bytes ? col : 0), bytes);
+                }
+            }
+            c_u += count;
+            if (c_u == u_end) {
+                c_u = u_begin;
+                c_tile += gridDim.x;
+            }
+        }
+        cp_async_commit();
+        c_stage = c_stage == STAGES - 1 ? 0 : c_stage + 1;
+    };
+    #pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i) copy_next();
+
+    int stage = 0;
+    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+        const int n0 = tile * a.rows, n_end = min(a.K, n0 + a.rows);
+        for (int u = u_begin; u < u_end;) {
+            const int w_begin = u % windows;
+            const Job job = job_of(r, u / windows);
+            const int w_end = min(windows, w_begin + (u_end - u));
+            u += w_end - w_begin;
+            float scale[2];
+            #pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                scale[j] = a.sd[static_cast<int64_t>(job.expert) * a.K + min(n0 + 8 * j + g, n_end - 1)];
+            }
+            const int8_t* hd[NP];
+            const float* hs[NP];
+            bool on[NP];
+            #pragma unroll
+            for (int n = 0; n < NP; ++n) {
+                // This lane's column of the B operand, and the token of its result columns.
+                const int j = 2 * n + (g >> 2), jr = min(2 * n + (t >> 1), job.count - 1);
+                on[n] = j < job.count;
+                hd[n] = a.hd + (static_cast<int64_t>(r.pair[job.pos + (on[n] ? j : 0)]) * 4 + (g & 3)) * a.fp + 16 * t;
+                hs[n] = a.hs + static_cast<int64_t>(r.pair[job.pos + jr]) * (2 * windows);
+            }
+            uint4 b[kDownWindows][NP];
+            float2 unit[kDownWindows][NP];
+            const auto load_b = [&](int w0) {
                 #pragma unroll
-                for (int n = 0; n < NP; ++n) {
-                    b[k][n] = make_uint4(0u, 0u, 0u, 0u);
-                    unit[k][n] = make_float2(0.0f, 0.0f);
-                    if (w < w_end) {
-                        if (on[n]) b[k][n] = *reinterpret_cast<const uint4*>(hd[n] + 64 * w);
-                        unit[k][n] = *reinterpret_cast<const float2*>(hs[n] + 2 * w);
+                for (int k = 0; k < kDownWindows; ++k) {
+                    #pragma unroll
+                    for (int n = 0; n < NP; ++n) {
+                        b[k][n] = make_uint4(0u, 0u, 0u, 0u);
+                        unit[k][n] = make_float2(0.0f, 0.0f);
+                        if (w0 + k < w_end) {
+                            if (on[n]) b[k][n] = *reinterpret_cast<const uint4*>(hd[n] + 64 * (w0 + k));
+                            unit[k][n] = *reinterpret_cast<const float2*>(hs[n] + 2 * (w0 + k));
+                        }
+                    }
+                }
+            };
+            if (NP == 1) load_b(w_begin);
+            float acc[NP][4] = {};
+            for (int w0 = w_begin; w0 < w_end; w0 += kDownWindows) {
+                if (NP > 1) load_b(w0);  // (too many registers to hold a stage ahead)
+                cp_async_wait_group<STAGES - 2>();
+                __syncwarp();
+                copy_next();
+                const uint32_t at = ring + stage * kDownStage + 16 * lane;
+                stage = stage == STAGES - 1 ? 0 : stage + 1;
+                #pragma unroll
+                for (int k = 0; k < kDownWindows; ++k) {
+                    const uint4 q0 = load_shared16(at + 1024 * k), q1 = load_shared16(at + 1024 * k + 512);
+                    const uint32_t lo[4] = {q0.x, q1.x, q0.y, q1.y}, hi[4] = {q0.z, q1.z, q0.w, q1.w};
+                    #pragma unroll
+                    for (int n = 0; n < NP; ++n) {
+                        int d[2][4];
+                        #pragma unroll
+                        for (int c = 0; c < 4; ++c) d[0][c] = d[1][c] = kMagicBits;
+                        mma_s8_16832(d[0], lo, b[k][n].x, b[k][n].y);
+                        mma_s8_16832(d[1], hi, b[k][n].z, b[k][n].w);
+                        #pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            acc[n][c] = fmaf(__int_as_float(d[0][c]) - kMagic, unit[k][n].x, acc[n][c]);
+                            acc[n][c] = fmaf(__int_as_float(d[1][c]) - kMagic, unit[k][n].y, acc[n][c]);
+                        }
+                    }
+                }
+                if (NP == 1 && w0 + kDownWindows < w_end) load_b(w0 + kDownWindows);
+            }
+            #pragma unroll
+            for (int n = 0; n < NP; ++n) {
+                // Lane (g, t) has digits 2 (t % 2) and 2 (t % 2) + 1 of token t / 2.
+                const int j = 2 * n + (t >> 1);
+                #pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    float v = fmaf(acc[n][2 * i + 1], 256.0f, acc[n][2 * i]);
+                    v = fmaf(__shfl_xor_sync(0xffffffffu, v, 1), (t & 1) ? 0.0f : 65536.0f, v);
+                    if (j < job.count && !(t & 1)) {
+                        mine[r.token[job.pos + j] * 16 + 8 * i + g] += v * scale[i] * r.weight[r.pair[job.pos + j]];
                     }
                 }
             }
+        }
+        __syncthreads();
+        for (int i = tid; i < a.M * 16; i += kDownThreads) {
+            const int m = i / 16, n = n0 + i % 16;
+            float v = 0.0f;
             #pragma unroll
-            for (int k = 0; k < AHEAD; ++k) {
-                const uint32_t lo[4] = {q[k][0].x, q[k][1].x, q[k][0].y, q[k][1].y};
-                const uint32_t hi[4] = {q[k][0].z, q[k][1].z, q[k][0].w, q[k][1].w};
-                #pragma unroll
-                for (int n = 0; n < NP; ++n) {
-                    int d[2][4];
-                    #pragma unroll
-                    for (int c = 0; c < 4; ++c) d[0][c] = d[1][c] = kMagicBits;
-                    mma_s8_16832(d[0], lo, b[k][n].x, b[k][n].y);
-                    mma_s8_16832(d[1], hi, b[k][n].z, b[k][n].w);
-                    #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        acc[n][c] = fmaf(__int_as_float(d[0][c]) - kMagic, unit[k][n].x, acc[n][c]);
-                        acc[n][c] = fmaf(__int_as_float(d[1][c]) - kMagic, unit[k][n].y, acc[n][c]);
-                    }
-                }
+            for (int w = 0; w < kDownWarps; ++w) {
+                v += outs[w * a.M * 16 + i];
+                outs[w * a.M * 16 + i] = 0.0f;
             }
+            if (n < n_end) a.out[static_cast<int64_t>(m) * a.K + n] = v;
         }
-        #pragma unroll
-        for (int n = 0; n < NP; ++n) {
-            // Lane (g, t) has digits 2 (t % 2) and 2 (t % 2) + 1 of token t / 2.
-            const int j = 2 * n + (t >> 1);
-            #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                float v = fmaf(acc[n][2 * i + 1], 256.0f, acc[n][2 * i]);
-                v = fmaf(__shfl_xor_sync(0xffffffffu, v, 1), (t & 1) ? 0.0f : 65536.0f, v);
-                if (j < job.count && !(t & 1)) {
-                    mine[r.token[job.pos + j] * 16 + 8 * i + g] += v * scale[i] * r.weight[r.pair[job.pos + j]];
-                }
-            }
-        }
+        __syncthreads();
     }
-    __syncthreads();
-    for (int i = tid; i < a.M * 16; i += kMoeThreads) {
-        float v = 0.0f;
-        #pragma unroll
-        for (int w = 0; w < kMoeWarps; ++w) v += outs[w * a.M * 16 + i];
-        outs[i] = v;  // (only this thread reads or writes place i of any warp)
-    }
-    sm100::cluster_sync();
-    for (int i = rank * kMoeThreads + tid; i < a.M * 16; i += a.split * kMoeThreads) {
-        const int m = i / 16, n = n0 + i % 16;
-        float v = 0.0f;
-        for (int c = 0; c < a.split; ++c) {
-            float x;
-            asm volatile("ld.shared::cluster.f32 %0, [%1];"
-                         : "=f"(x)
-                         : "r"(sm100::mapa_shared(sm100::smem_addr(outs + i), c))
-                         : "memory");
-            v += x;
-        }
-        if (n < a.K) a.out[static_cast<int64_t>(m) * a.K + n] = v;
-    }
-    sm100::cluster_sync();  // no block leaves while another reads its sums
+    cp_async_wait_group<0>();
 }
 
 // --------------------------------------------------- any sizes and alignment
@@ -567,7 +644,7 @@ __global__ void __launch_bounds__(kMoeThreads) plain_up_kernel(const MoeArgs a) 
     __shared__ Routing r;
     pdl_launch_dependents();
     pdl_wait();
-    route_tokens(a, r);
+    route_tokens<kMoeThreads>(a, r);
     const int lane = threadIdx.x & 31;
     const int64_t total = static_cast<int64_t>(a.M) * a.top * a.F;
     for (int64_t i = blockIdx.x * kMoeWarps + (threadIdx.x >> 5); i < total; i += gridDim.x * kMoeWarps) {
@@ -646,28 +723,35 @@ int64_t lay_out(MoeArgs& a, char* ws, int64_t M, bool tensor, bool own_picks) {
     return at;
 }
 
+template <int NP, int STAGES>
+cudaError_t run_down(const MoeArgs& a, int blocks, cudaStream_t stream) {
+    const int bytes = kDownWarps * (STAGES * kDownStage + a.M * 16 * static_cast<int>(sizeof(float)));
+    const cudaError_t e =
+        cudaFuncSetAttribute(down_kernel<NP, STAGES>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return e;
+    cudaLaunchAttribute attr[1];
+    const cudaLaunchConfig_t cfg =
+        pdl_config(dim3(static_cast<unsigned>(blocks)), dim3(kDownThreads), static_cast<size_t>(bytes), stream, attr);
+    return cudaLaunchKernelEx(&cfg, down_kernel<NP, STAGES>, a);
+}
+
 template <int NP>
 cudaError_t run_tensor(MoeArgs a, cudaStream_t stream) {
     const int64_t sms = device_sm_count();
-    cudaLaunchAttribute attr[2];
-    // Items of the chosen experts are dealt out to one wave of blocks.
-    const int64_t jobs = a.M * a.top;  // at most
-    const int64_t items = jobs * (a.fp / 32), wave = (NP == 1 ? 3 : 2) * sms;
-    cudaLaunchConfig_t cfg =
-        pdl_config(dim3(static_cast<unsigned>(items < wave ? items : wave)), dim3(kMoeThreads), 0, stream, attr);
-    cudaError_t e = cudaLaunchKernelEx(&cfg, up_kernel<NP>, a);
+    cudaError_t e = cudaFuncSetAttribute(up_kernel<NP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Up<NP>::kBytes);
     if (e != cudaSuccess) return e;
-    // Enough blocks for three on every SM, at most a cluster of eight.
-    const int64_t tiles = ceil_div(a.K, 16);
-    a.split = 1;
-    while (a.split < 8 && tiles * a.split < 3 * sms) a.split *= 2;
-    cfg.gridDim = dim3(static_cast<unsigned>(tiles * a.split));
-    cfg.dynamicSmemBytes = static_cast<size_t>(kMoeWarps) * a.M * 16 * sizeof(float);
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = a.split;
-    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-    cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, down_kernel<NP>, a);
+    cudaLaunchAttribute attr[1];
+    const int64_t items = static_cast<int64_t>(a.M) * a.top * (a.fp / 32);  // at most
+    const cudaLaunchConfig_t cfg = pdl_config(dim3(static_cast<unsigned>(items < sms ? items : sms)),
+                                              dim3(kUpWorkers * kUpThreads), Up<NP>::kBytes, stream, attr);
+    e = cudaLaunchKernelEx(&cfg, up_kernel<NP>, a);
+    if (e != cudaSuccess) return e;
+    // Down: as many tiles for every SM, as few as 16 rows allow.
+    const int64_t rounds = ceil_div(a.K, 16 * sms);
+    a.rows = static_cast<int>(ceil_div(a.K, rounds * sms));
+    const int64_t tiles = ceil_div(a.K, a.rows);
+    const int blocks = static_cast<int>(tiles < sms ? tiles : sms);
+    return down_stages(a.M) == 3 ? run_down<NP, 3>(a, blocks, stream) : run_down<NP, 2>(a, blocks, stream);
 }
 
 cudaError_t run_pass(const MoeArgs& a, bool tensor, cudaStream_t stream) {

@@ -53,15 +53,7 @@ constexpr float kMagic = 12582912.0f;       // 1.5 2^23
 constexpr int kMagicBits = 0x4B400000;
 constexpr int kTaskUnits = 24;             // a task's fixed cost in tiles (5 us: its queries, its first tiles, its join)
 
-// d = c + a b with all of c the same register value: accumulators that begin at
-// a constant need no moves.
-__device__ __forceinline__ void mma_s8_16832_from(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, int c) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-        "{%10, %10, %10, %10};"
-        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(c));
-}
+// d = c + a b with all of c the same value (mma_frag.cuh has the s8 form).
 __device__ __forceinline__ void mma_f16_16816_from(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1,
                                                    float c) {
     asm volatile(
@@ -105,7 +97,7 @@ __device__ __forceinline__ uint32_t codes_f16(uint32_t w) {
 // key.
 template <typename T, int DP>
 struct Query {
-    T v[DP / 64][16];
+    alignas(16) T v[DP / 64][16];
 };
 template <typename T, int DP>
 __device__ __forceinline__ void load_query(Query<T, DP>& q, const T* row, bool valid, int dim, bool vec, int t) {

@@ -696,7 +696,7 @@ __global__ void __launch_bounds__(256) kv_prompt_join_kernel(const AttnArgs a) {
         const int tok = row / a.group, head = h * a.group + row - tok * a.group;
         const float inv = inverse(den);
         T* out = static_cast<T*>(a.out) + ((e.z + tok) * static_cast<int64_t>(a.heads * a.group) + head) * DP + PER * lane;
-        T o[PER];
+        alignas(8) T o[PER];
         #pragma unroll
         for (int j = 0; j < PER; ++j) o[j] = from_f32<T>(sum[j] * inv);
         if constexpr (PER == 4) {

@@ -24,6 +24,7 @@
 // 64 w + 16 t + 8 s + i (t < 4, i < 8), which are the columns of step s of
 // window w in the next product.
 #include <cmath>
+#include <cstdlib>
 
 #include "common.cuh"
 #include "mma_frag.cuh"
@@ -299,19 +300,19 @@ __device__ void route_tokens(const MoeArgs& a, Routing& r) {
 // An item is a job's 32 rows of both matrices: two tiles of 16 rows each, of
 // which rows 0-7 and 8-15 are runs of eight (the columns that share a unit in
 // the next product). A block is an SM's whole load, three workers of four warps,
-// each with its own items and barrier; a warp has a quarter of the windows and
-// streams them, from one item into the next, through a ring of its own in
-// shared memory (4 KB a window) by asynchronous copies: 144 KB an SM in flight.
-// (Loads into registers with two or three blocks an SM kept at most 96 KB in
-// flight and reached 4.5 TB/s.)
+// each with its own items and barrier; a warp has one of the four tiles and
+// streams its rows, from one item into the next, through a ring of its own in
+// shared memory by asynchronous copies, 256 bytes of each row (4 KB) a stage:
+// 144 KB an SM in flight. (Loads into registers with two or three blocks an SM
+// kept at most 96 KB in flight, X us for the 11008-row case; warps that shared
+// the rows and had a quarter of the columns each read 64 bytes a row at a time, Y us.)
 constexpr int kUpWarps = 4, kUpThreads = 32 * kUpWarps, kUpWorkers = 3;
+constexpr int kWindows = 4, kStageBytes = kWindows * 16 * 64;  // a stage: [window][16 rows][64 bytes]
 template <int NP>
 struct Up {
     static constexpr int kStages = NP == 4 ? 3 : 4;
-    static constexpr int kParities = NP == 1 ? 2 : 1;   // sums of an item may wait while the next is multiplied
-    static constexpr int kWindow = 64 * 64;             // [gate runs 0-3, up runs 0-3][8 rows][64 bytes]
-    static constexpr int kRing = kUpWorkers * kUpWarps * kStages * kWindow;
-    static constexpr int kBytes = kRing;
+    static constexpr int kParities = NP == 1 ? 2 : 1;  // an item's sums may wait while the next is multiplied
+    static constexpr int kBytes = kUpWorkers * kUpWarps * kStages * kStageBytes;
 };
 
 __device__ __forceinline__ uint4 load_shared16(uint32_t addr) {
@@ -322,55 +323,50 @@ __device__ __forceinline__ uint4 load_shared16(uint32_t addr) {
 
 template <int NP>
 __global__ void __launch_bounds__(kUpWorkers* kUpThreads, 1) up_kernel(const MoeArgs a) {
-    using U = Up<NP>;
-    constexpr int STAGES = U::kStages, THREADS = kUpWorkers * kUpThreads;
+    constexpr int STAGES = Up<NP>::kStages, THREADS = kUpWorkers * kUpThreads;
     extern __shared__ __align__(128) uint8_t s_ring[];
     __shared__ Routing r;
-    __shared__ int s_sums[kUpWorkers][U::kParities][4][16][8 * NP + 1];  // [gate 0, gate 1, up 0, up 1][row][token, digit]
+    __shared__ __align__(16) int s_sums[kUpWorkers][Up<NP>::kParities][4][16][8 * NP];  // [item parity][gate 0, gate 1, up 0, up 1][row][token, digit]
     const int worker = threadIdx.x / kUpThreads;
     const int tid = threadIdx.x % kUpThreads, lane = tid & 31, warp = tid >> 5;  // of the worker
     const int g = lane >> 2, t = lane & 3;
     const auto sync_worker = [&] { asm volatile("bar.sync %0, %1;" ::"r"(1 + worker), "n"(kUpThreads) : "memory"); };
     auto& sums = s_sums[worker];
     pdl_launch_dependents();
-    for (int i = threadIdx.x; i < static_cast<int>(sizeof(s_sums) / 4); i += THREADS) (&s_sums[0][0][0][0][0])[i] = 0;
     pdl_wait();
     route_tokens<THREADS>(a, r);
     list_jobs<NP, THREADS>(a, r);
 
     const int halves = a.fp / 32, windows = (a.K + 63) / 64;
     const int items = r.jobs * halves;
-    const int w_begin = warp * windows / kUpWarps, w_end = (warp + 1) * windows / kUpWarps;
     const int first = worker * gridDim.x + blockIdx.x, stride = kUpWorkers * gridDim.x;
     const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(s_ring)) +
-                          (worker * kUpWarps + warp) * STAGES * U::kWindow;
+                          (worker * kUpWarps + warp) * STAGES * kStageBytes;
+    const int8_t* const codes = (warp & 2 ? a.qu : a.qg) + 16 * t;
 
-    // The copying side: item, window and this lane's rows of the item.
-    int c_item = first, c_w = w_begin, c_stage = 0;
-    const int8_t *gate = nullptr, *up = nullptr;  // row of run 0
-    int64_t step[4] = {0, 0, 0, 0};               // bytes from there to the row of run i
+    // The copying side: item, window and this lane's rows g and g + 8.
+    int c_item = first, c_w = 0, c_stage = 0;
+    const int8_t *row0 = nullptr, *row1 = nullptr;
     const auto rows_of = [&](int item) {
-        const Job job = job_of(r, item / halves);
         const int h = item % halves;
-        const int f = h / 2 * 64 + 8 * (h & 1) + g;
-        const int64_t at = (static_cast<int64_t>(job.expert) * a.F + min(f, a.F - 1)) * a.K;
-        gate = a.qg + at + 16 * t;
-        up = a.qu + at + 16 * t;
-        #pragma unroll
-        for (int i = 1; i < 4; ++i) step[i] = static_cast<int64_t>(min(f + 16 * i, a.F - 1) - min(f, a.F - 1)) * a.K;
+        const int f = h / 2 * 64 + 32 * (warp & 1) + 8 * (h & 1) + g;
+        const int64_t at = static_cast<int64_t>(job_of(r, item / halves).expert) * a.F;
+        row0 = codes + (at + min(f, a.F - 1)) * a.K;
+        row1 = codes + (at + min(f + 16, a.F - 1)) * a.K;
     };
     const auto copy_next = [&] {
-        if (c_item < items && w_begin < w_end) {
-            const int bytes = 64 * c_w + 16 * t < a.K ? 16 : 0;
-            const int64_t at = bytes ? 64 * c_w : 0;
-            const uint32_t dst = ring + c_stage * U::kWindow + 16 * lane;
+        if (c_item < items) {
+            const uint32_t dst = ring + c_stage * kStageBytes + 16 * lane;
             #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                cp_async16(dst + 512 * i, gate + step[i] + at, bytes);
-                cp_async16(dst + 2048 + 512 * i, up + step[i] + at, bytes);
+            for (int k = 0; k < kWindows; ++k) {
+                const int col = 64 * (c_w + k);
+                const int bytes = col + 16 * t < a.K ? 16 : 0;
+                cp_async16(dst + 1024 * k, row0 + (bytes ? col : 0), bytes);
+                cp_async16(dst + 1024 * k + 512, row1 + (bytes ? col : 0), bytes);
             }
-            if (++c_w == w_end) {
-                c_w = w_begin;
+            c_w += kWindows;
+            if (c_w >= windows) {
+                c_w = 0;
                 c_item += stride;
                 if (c_item < items) rows_of(c_item);
             }
@@ -383,16 +379,19 @@ __global__ void __launch_bounds__(kUpWorkers* kUpThreads, 1) up_kernel(const Moe
     for (int i = 0; i < STAGES - 1; ++i) copy_next();
 
     int parity = 0, stage = 0;
-    for (int item = first; item < items; item += stride) {
+    for (int item = first; item < items; item += stride, parity ^= Up<NP>::kParities - 1) {
         const Job job = job_of(r, item / halves);
         const int8_t* xd[NP];
         bool on[NP];
-        uint4 b[NP];
-        const auto load_b = [&](int w) {
+        uint4 b[kWindows][NP];
+        const auto load_b = [&](int w0) {
             #pragma unroll
-            for (int n = 0; n < NP; ++n) {
-                b[n] = make_uint4(0u, 0u, 0u, 0u);
-                if (on[n]) b[n] = *reinterpret_cast<const uint4*>(xd[n] + 64 * w);
+            for (int k = 0; k < kWindows; ++k) {
+                #pragma unroll
+                for (int n = 0; n < NP; ++n) {
+                    b[k][n] = make_uint4(0u, 0u, 0u, 0u);
+                    if (on[n] && w0 + k < windows) b[k][n] = *reinterpret_cast<const uint4*>(xd[n] + 64 * (w0 + k));
+                }
             }
         };
         #pragma unroll
@@ -402,44 +401,38 @@ __global__ void __launch_bounds__(kUpWorkers* kUpThreads, 1) up_kernel(const Moe
             const int m = on[n] ? r.token[job.pos + j] : 0;
             xd[n] = a.xd + (static_cast<int64_t>(m) * 4 + (g & 3)) * a.kp + 16 * t;
         }
-        if (w_begin < w_end) load_b(w_begin);
-        int acc[NP][4][4] = {};
-        for (int w = w_begin; w < w_end; ++w) {
+        if (NP <= 2) load_b(0);
+        int acc[NP][4] = {};
+        for (int w0 = 0; w0 < windows; w0 += kWindows) {
+            if (NP > 2) load_b(w0);  // (too many registers to hold a stage ahead)
             cp_async_wait_group<STAGES - 2>();
             __syncwarp();
             copy_next();
-            const uint32_t at = ring + stage * U::kWindow + 16 * lane;
+            const uint32_t at = ring + stage * kStageBytes + 16 * lane;
             stage = stage == STAGES - 1 ? 0 : stage + 1;
-            uint4 now[NP];
             #pragma unroll
-            for (int n = 0; n < NP; ++n) now[n] = b[n];
-            if (w + 1 < w_end) load_b(w + 1);
-            #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint4 q0 = load_shared16(at + 1024 * i), q1 = load_shared16(at + 1024 * i + 512);
+            for (int k = 0; k < kWindows; ++k) {
+                const uint4 q0 = load_shared16(at + 1024 * k), q1 = load_shared16(at + 1024 * k + 512);
                 const uint32_t lo[4] = {q0.x, q1.x, q0.y, q1.y}, hi[4] = {q0.z, q1.z, q0.w, q1.w};
                 #pragma unroll
                 for (int n = 0; n < NP; ++n) {
-                    mma_s8_16832(acc[n][i], lo, now[n].x, now[n].y);
-                    mma_s8_16832(acc[n][i], hi, now[n].z, now[n].w);
+                    mma_s8_16832(acc[n], lo, b[k][n].x, b[k][n].y);
+                    mma_s8_16832(acc[n], hi, b[k][n].z, b[k][n].w);
                 }
             }
+            if (NP <= 2 && w0 + kWindows < windows) load_b(w0 + kWindows);
         }
-        if (U::kParities == 1) sync_worker();  // the sums before have been taken
+        if (Up<NP>::kParities == 1) sync_worker();  // the sums before have been taken
         #pragma unroll
         for (int n = 0; n < NP; ++n) {
             #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    atomicAdd(&sums[parity][i][g + 8 * (c >> 1)][8 * n + 2 * t + (c & 1)], acc[n][i][c]);
-                }
+            for (int c = 0; c < 4; c += 2) {
+                *reinterpret_cast<int2*>(&sums[parity][warp][g + 4 * c][8 * n + 2 * t]) = make_int2(acc[n][c], acc[n][c + 1]);
             }
         }
         sync_worker();
-        // Warp j: the job's tokens j, j + 4; lane: one of the 32 rows. Sums are set
-        // back to zero as they are read; a barrier of the next item comes before
-        // their next use.
+        // Warp j: the job's tokens j, j + 4; lane: one of the 32 rows. (A
+        // barrier of the next item comes before these sums are written again.)
         for (int j = warp; j < job.count; j += kUpWarps) {
             const int m = r.token[job.pos + j];
             const int h2 = item % halves;
@@ -448,11 +441,9 @@ __global__ void __launch_bounds__(kUpWorkers* kUpThreads, 1) up_kernel(const Moe
             const float unit = a.xs[m];
             const int64_t at = static_cast<int64_t>(job.expert) * a.F + min(f, a.F - 1);
             const float sg = a.sg[at], su = a.su[at];
-            const auto dot = [&](int (&s)[16][8 * NP + 1]) {
-                int* d = &s[row][4 * j];
-                const double v = ((static_cast<double>(d[3]) * 256.0 + d[2]) * 256.0 + d[1]) * 256.0 + d[0];
-                d[0] = d[1] = d[2] = d[3] = 0;
-                return static_cast<float>(v);
+            const auto dot = [&](const int (&s)[16][8 * NP]) {
+                const int4 d = *reinterpret_cast<const int4*>(&s[row][4 * j]);
+                return static_cast<float>(((static_cast<double>(d.w) * 256.0 + d.z) * 256.0 + d.y) * 256.0 + d.x);
             };
             const float gv = dot(sums[parity][tile]) * unit * sg, uv = dot(sums[parity][2 + tile]) * unit * su;
             const float h = f < a.F ? gv / (1.0f + expf(-gv)) * uv : 0.0f;
@@ -466,7 +457,6 @@ __global__ void __launch_bounds__(kUpWorkers* kUpThreads, 1) up_kernel(const Moe
             for (int i = 0; i < 4; ++i) hd[static_cast<int64_t>(i) * a.fp] = static_cast<int8_t>(y >> (8 * i));
             if (lane == 0) a.hs[pair * halves + h2] = fx.unit;
         }
-        if (U::kParities == 2) parity ^= 1;
     }
     cp_async_wait_group<0>();
 }
@@ -481,13 +471,12 @@ __global__ void __launch_bounds__(kUpWorkers* kUpThreads, 1) up_kernel(const Moe
 // end of a job a warp adds its result, weighted, to its own sums per token; the
 // warps' are added in order at the end of the tile.
 constexpr int kDownWarps = 16, kDownThreads = 32 * kDownWarps;
-constexpr int kDownWindows = 4, kDownStage = kDownWindows * 16 * 64;
 constexpr int down_stages(int tokens) { return tokens <= 16 ? 3 : 2; }  // what the sums leave room for
 
 template <int NP, int STAGES>
 __global__ void __launch_bounds__(kDownThreads, 1) down_kernel(const MoeArgs a) {
     extern __shared__ __align__(128) uint8_t s_raw[];
-    float* const outs = reinterpret_cast<float*>(s_raw + kDownWarps * STAGES * kDownStage);  // [warp][token][16]
+    float* const outs = reinterpret_cast<float*>(s_raw + kDownWarps * STAGES * kStageBytes);  // [warp][token][16]
     __shared__ Routing r;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = lane >> 2, t = lane & 3;
@@ -504,7 +493,7 @@ __global__ void __launch_bounds__(kDownThreads, 1) down_kernel(const MoeArgs a) 
     const int windows = a.fp / 64, tiles = (a.K + a.rows - 1) / a.rows;
     const int64_t units = static_cast<int64_t>(r.jobs) * windows;
     const int u_begin = static_cast<int>(units * warp / kDownWarps), u_end = static_cast<int>(units * (warp + 1) / kDownWarps);
-    const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(s_raw)) + warp * STAGES * kDownStage;
+    const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(s_raw)) + warp * STAGES * kStageBytes;
     float* const mine = outs + warp * a.M * 16;
 
     // The copying side: a stage is up to four windows of one job.
@@ -512,16 +501,16 @@ __global__ void __launch_bounds__(kDownThreads, 1) down_kernel(const MoeArgs a) 
     const auto copy_next = [&] {
         if (c_tile < tiles && c_u < u_end) {
             const int job_i = c_u / windows, w = c_u - job_i * windows;
-            const int count = min(min(kDownWindows, windows - w), u_end - c_u);
+            const int count = min(min(kWindows, windows - w), u_end - c_u);
             const int n0 = c_tile * a.rows, n_end = min(a.K, n0 + a.rows);
             const int64_t expert = static_cast<int64_t>(job_of(r, job_i).expert) * a.K;
-            const uint32_t dst = ring + c_stage * kDownStage + 16 * lane;
+            const uint32_t dst = ring + c_stage * kStageBytes + 16 * lane;
             #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const int n = n0 + 8 * j + g;
                 const int8_t* row = a.qd + (expert + min(n, a.K - 1)) * a.F;
                 #pragma unroll
-                for (int k = 0; k < kDownWindows; ++k) {
+                for (int k = 0; k < kWindows; ++k) {
                     const int col = 64 * (w + k) + 16 * t;
                     const int bytes = n < n_end && k < count && col < a.F ? 16 : 0;
                     cp_async16(dst + 1024 * k + 512 * j, row + (bytes ? col : 0), bytes);
@@ -563,11 +552,11 @@ __global__ void __launch_bounds__(kDownThreads, 1) down_kernel(const MoeArgs a) 
                 hd[n] = a.hd + (static_cast<int64_t>(r.pair[job.pos + (on[n] ? j : 0)]) * 4 + (g & 3)) * a.fp + 16 * t;
                 hs[n] = a.hs + static_cast<int64_t>(r.pair[job.pos + jr]) * (2 * windows);
             }
-            uint4 b[kDownWindows][NP];
-            float2 unit[kDownWindows][NP];
+            uint4 b[kWindows][NP];
+            float2 unit[kWindows][NP];
             const auto load_b = [&](int w0) {
                 #pragma unroll
-                for (int k = 0; k < kDownWindows; ++k) {
+                for (int k = 0; k < kWindows; ++k) {
                     #pragma unroll
                     for (int n = 0; n < NP; ++n) {
                         b[k][n] = make_uint4(0u, 0u, 0u, 0u);
@@ -581,24 +570,22 @@ __global__ void __launch_bounds__(kDownThreads, 1) down_kernel(const MoeArgs a) 
             };
             if (NP == 1) load_b(w_begin);
             float acc[NP][4] = {};
-            for (int w0 = w_begin; w0 < w_end; w0 += kDownWindows) {
+            for (int w0 = w_begin; w0 < w_end; w0 += kWindows) {
                 if (NP > 1) load_b(w0);  // (too many registers to hold a stage ahead)
                 cp_async_wait_group<STAGES - 2>();
                 __syncwarp();
                 copy_next();
-                const uint32_t at = ring + stage * kDownStage + 16 * lane;
+                const uint32_t at = ring + stage * kStageBytes + 16 * lane;
                 stage = stage == STAGES - 1 ? 0 : stage + 1;
                 #pragma unroll
-                for (int k = 0; k < kDownWindows; ++k) {
+                for (int k = 0; k < kWindows; ++k) {
                     const uint4 q0 = load_shared16(at + 1024 * k), q1 = load_shared16(at + 1024 * k + 512);
                     const uint32_t lo[4] = {q0.x, q1.x, q0.y, q1.y}, hi[4] = {q0.z, q1.z, q0.w, q1.w};
                     #pragma unroll
                     for (int n = 0; n < NP; ++n) {
                         int d[2][4];
-                        #pragma unroll
-                        for (int c = 0; c < 4; ++c) d[0][c] = d[1][c] = kMagicBits;
-                        mma_s8_16832(d[0], lo, b[k][n].x, b[k][n].y);
-                        mma_s8_16832(d[1], hi, b[k][n].z, b[k][n].w);
+                        mma_s8_16832_from(d[0], lo, b[k][n].x, b[k][n].y, kMagicBits);
+                        mma_s8_16832_from(d[1], hi, b[k][n].z, b[k][n].w, kMagicBits);
                         #pragma unroll
                         for (int c = 0; c < 4; ++c) {
                             acc[n][c] = fmaf(__int_as_float(d[0][c]) - kMagic, unit[k][n].x, acc[n][c]);
@@ -606,7 +593,7 @@ __global__ void __launch_bounds__(kDownThreads, 1) down_kernel(const MoeArgs a) 
                         }
                     }
                 }
-                if (NP == 1 && w0 + kDownWindows < w_end) load_b(w0 + kDownWindows);
+                if (NP == 1 && w0 + kWindows < w_end) load_b(w0 + kWindows);
             }
             #pragma unroll
             for (int n = 0; n < NP; ++n) {
@@ -725,7 +712,7 @@ int64_t lay_out(MoeArgs& a, char* ws, int64_t M, bool tensor, bool own_picks) {
 
 template <int NP, int STAGES>
 cudaError_t run_down(const MoeArgs& a, int blocks, cudaStream_t stream) {
-    const int bytes = kDownWarps * (STAGES * kDownStage + a.M * 16 * static_cast<int>(sizeof(float)));
+    const int bytes = kDownWarps * (STAGES * kStageBytes + a.M * 16 * static_cast<int>(sizeof(float)));
     const cudaError_t e =
         cudaFuncSetAttribute(down_kernel<NP, STAGES>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != cudaSuccess) return e;
@@ -767,6 +754,7 @@ cudaError_t run_pass(const MoeArgs& a, bool tensor, cudaStream_t stream) {
     }
     // Tokens an expert has to take at a time: by how many pick it on average.
     if (a.M <= 2) return run_tensor<1>(a, stream);
+    if (getenv("NP1")) return run_tensor<1>(a, stream);
     if (a.M <= 4 || a.M * a.top <= 2 * a.E) return run_tensor<2>(a, stream);
     return run_tensor<4>(a, stream);
 }

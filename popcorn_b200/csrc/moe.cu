@@ -24,7 +24,6 @@
 // 64 w + 16 t + 8 s + i (t < 4, i < 8), which are the columns of step s of
 // window w in the next product.
 #include <cmath>
-#include <cstdlib>
 
 #include "common.cuh"
 #include "mma_frag.cuh"
@@ -35,6 +34,9 @@ namespace {
 
 constexpr int kMoeThreads = 256;
 constexpr int kMoeWarps = kMoeThreads / 32;
+constexpr int kWindows = 4;       // windows of a stage: 256 columns of 16 rows
+constexpr int kColumns = 64 * kWindows;
+constexpr int kStageBytes = 16 * kColumns;  // [window][16 rows][64 bytes]
 constexpr int kMoeTokens = 64;    // tokens of one pass
 constexpr int kMoeExperts = 256;
 constexpr int kMoeTop = 16;
@@ -57,7 +59,7 @@ struct MoeArgs {
     int8_t* xd;        // [M][4][kp] digits of x
     float* xs;         // [M] its unit
     int8_t* hd;        // [M top][4][fp] digits of the hidden values
-    float* hs;         // [M top][fp / 32] their units
+    float* hs;         // [M top][fp / 32] their units (kp, fp: K, F rounded up to whole stages)
     float* h;          // [M top][F] hidden values (plain kernels only)
     int M, K, F, E, top, renorm, kp, fp;
     int rows;          // output channels of a tile of the down product
@@ -127,6 +129,13 @@ __global__ void __launch_bounds__(128) route_kernel(const MoeArgs a) {
             }
         }
         if (tid == 0) a.xs[m] = f.unit;
+        // Units of the padding of this token's hidden values (its digits meet codes
+        // that are zeros and may be anything).
+        const int used = (a.F + 63) / 64 * 2, all = a.fp / 32;
+        for (int i = tid; i < a.top * (all - used); i += 128) {
+            const int j = i / (all - used);
+            a.hs[(static_cast<int64_t>(m) * a.top + j) * all + used + i - j * (all - used)] = 0.0f;
+        }
         return;
     }
     const float* w = a.router + static_cast<int64_t>(e) * a.K;
@@ -307,7 +316,6 @@ __device__ void route_tokens(const MoeArgs& a, Routing& r) {
 // kept at most 96 KB in flight, X us for the 11008-row case; warps that shared
 // the rows and had a quarter of the columns each read 64 bytes a row at a time, Y us.)
 constexpr int kUpWarps = 4, kUpThreads = 32 * kUpWarps, kUpWorkers = 3;
-constexpr int kWindows = 4, kStageBytes = kWindows * 16 * 64;  // a stage: [window][16 rows][64 bytes]
 template <int NP>
 struct Up {
     static constexpr int kStages = NP == 4 ? 3 : 4;
@@ -319,6 +327,26 @@ __device__ __forceinline__ uint4 load_shared16(uint32_t addr) {
     uint4 v;
     asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
     return v;
+}
+
+// One stage: this lane's pieces of two rows (of `bytes0`, `bytes1` = 16, or 0
+// for rows that are not there) from column `col` on, zeros past `end`.
+__device__ __forceinline__ void copy_stage(uint32_t dst, const int8_t* row0, const int8_t* row1, int bytes0, int bytes1,
+                                           int col, int t, int end) {
+    if (col + kColumns <= end) {
+        #pragma unroll
+        for (int k = 0; k < kWindows; ++k) {
+            cp_async16(dst + 1024 * k, row0 + col + 64 * k, bytes0);
+            cp_async16(dst + 1024 * k + 512, row1 + col + 64 * k, bytes1);
+        }
+    } else {
+        #pragma unroll
+        for (int k = 0; k < kWindows; ++k) {
+            const bool in = col + 64 * k + 16 * t < end;
+            cp_async16(dst + 1024 * k, row0 + (in ? col + 64 * k : 0), in ? bytes0 : 0);
+            cp_async16(dst + 1024 * k + 512, row1 + (in ? col + 64 * k : 0), in ? bytes1 : 0);
+        }
+    }
 }
 
 template <int NP>
@@ -337,15 +365,15 @@ __global__ void __launch_bounds__(kUpWorkers* kUpThreads, 1) up_kernel(const Moe
     route_tokens<THREADS>(a, r);
     list_jobs<NP, THREADS>(a, r);
 
-    const int halves = a.fp / 32, windows = (a.K + 63) / 64;
+    const int halves = (a.F + 63) / 64 * 2, stages = a.kp / kColumns;
     const int items = r.jobs * halves;
     const int first = worker * gridDim.x + blockIdx.x, stride = kUpWorkers * gridDim.x;
     const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(s_ring)) +
-                          (worker * kUpWarps + warp) * STAGES * kStageBytes;
+                          (worker * kUpWarps + warp) * STAGES * kStageBytes + 16 * lane;
     const int8_t* const codes = (warp & 2 ? a.qu : a.qg) + 16 * t;
 
-    // The copying side: item, window and this lane's rows g and g + 8.
-    int c_item = first, c_w = 0, c_stage = 0;
+    // The copying side: item, stage of it and this lane's rows g and g + 8.
+    int c_item = first, c_s = 0, c_slot = 0;
     const int8_t *row0 = nullptr, *row1 = nullptr;
     const auto rows_of = [&](int item) {
         const int h = item % halves;
@@ -356,60 +384,48 @@ __global__ void __launch_bounds__(kUpWorkers* kUpThreads, 1) up_kernel(const Moe
     };
     const auto copy_next = [&] {
         if (c_item < items) {
-            const uint32_t dst = ring + c_stage * kStageBytes + 16 * lane;
-            #pragma unroll
-            for (int k = 0; k < kWindows; ++k) {
-                const int col = 64 * (c_w + k);
-                const int bytes = col + 16 * t < a.K ? 16 : 0;
-                cp_async16(dst + 1024 * k, row0 + (bytes ? col : 0), bytes);
-                cp_async16(dst + 1024 * k + 512, row1 + (bytes ? col : 0), bytes);
-            }
-            c_w += kWindows;
-            if (c_w >= windows) {
-                c_w = 0;
+            copy_stage(ring + c_slot * kStageBytes, row0, row1, 16, 16, c_s * kColumns, t, a.K);
+            if (++c_s == stages) {
+                c_s = 0;
                 c_item += stride;
                 if (c_item < items) rows_of(c_item);
             }
         }
         cp_async_commit();
-        c_stage = c_stage == STAGES - 1 ? 0 : c_stage + 1;
+        c_slot = c_slot == STAGES - 1 ? 0 : c_slot + 1;
     };
     if (first < items) rows_of(first);
     #pragma unroll
     for (int i = 0; i < STAGES - 1; ++i) copy_next();
 
-    int parity = 0, stage = 0;
+    int parity = 0, slot = 0;
     for (int item = first; item < items; item += stride, parity ^= Up<NP>::kParities - 1) {
         const Job job = job_of(r, item / halves);
+        // This lane's column of the B operand: a digit of a token. (Columns of
+        // tokens that the job does not have repeat its last one and are not used.)
         const int8_t* xd[NP];
-        bool on[NP];
+        #pragma unroll
+        for (int n = 0; n < NP; ++n) {
+            const int m = r.token[job.pos + min(2 * n + (g >> 2), job.count - 1)];
+            xd[n] = a.xd + (static_cast<int64_t>(m) * 4 + (g & 3)) * a.kp + 16 * t;
+        }
         uint4 b[kWindows][NP];
-        const auto load_b = [&](int w0) {
+        const auto load_b = [&](int st) {
             #pragma unroll
             for (int k = 0; k < kWindows; ++k) {
                 #pragma unroll
-                for (int n = 0; n < NP; ++n) {
-                    b[k][n] = make_uint4(0u, 0u, 0u, 0u);
-                    if (on[n] && w0 + k < windows) b[k][n] = *reinterpret_cast<const uint4*>(xd[n] + 64 * (w0 + k));
-                }
+                for (int n = 0; n < NP; ++n) b[k][n] = *reinterpret_cast<const uint4*>(xd[n] + kColumns * st + 64 * k);
             }
         };
-        #pragma unroll
-        for (int n = 0; n < NP; ++n) {
-            const int j = 2 * n + (g >> 2);
-            on[n] = j < job.count;
-            const int m = on[n] ? r.token[job.pos + j] : 0;
-            xd[n] = a.xd + (static_cast<int64_t>(m) * 4 + (g & 3)) * a.kp + 16 * t;
-        }
         if (NP <= 2) load_b(0);
         int acc[NP][4] = {};
-        for (int w0 = 0; w0 < windows; w0 += kWindows) {
-            if (NP > 2) load_b(w0);  // (too many registers to hold a stage ahead)
+        for (int st = 0; st < stages; ++st) {
+            if (NP > 2) load_b(st);  // (too many registers to hold a stage ahead)
             cp_async_wait_group<STAGES - 2>();
             __syncwarp();
             copy_next();
-            const uint32_t at = ring + stage * kStageBytes + 16 * lane;
-            stage = stage == STAGES - 1 ? 0 : stage + 1;
+            const uint32_t at = ring + slot * kStageBytes;
+            slot = slot == STAGES - 1 ? 0 : slot + 1;
             #pragma unroll
             for (int k = 0; k < kWindows; ++k) {
                 const uint4 q0 = load_shared16(at + 1024 * k), q1 = load_shared16(at + 1024 * k + 512);
@@ -420,7 +436,7 @@ __global__ void __launch_bounds__(kUpWorkers* kUpThreads, 1) up_kernel(const Moe
                     mma_s8_16832(acc[n], hi, b[k][n].z, b[k][n].w);
                 }
             }
-            if (NP <= 2 && w0 + kWindows < windows) load_b(w0 + kWindows);
+            if (NP <= 2 && st + 1 < stages) load_b(st + 1);
         }
         if (Up<NP>::kParities == 1) sync_worker();  // the sums before have been taken
         #pragma unroll
@@ -455,7 +471,7 @@ __global__ void __launch_bounds__(kUpWorkers* kUpThreads, 1) up_kernel(const Moe
             int8_t* hd = a.hd + pair * 4 * a.fp + f;
             #pragma unroll
             for (int i = 0; i < 4; ++i) hd[static_cast<int64_t>(i) * a.fp] = static_cast<int8_t>(y >> (8 * i));
-            if (lane == 0) a.hs[pair * halves + h2] = fx.unit;
+            if (lane == 0) a.hs[pair * (a.fp / 32) + h2] = fx.unit;
         }
     }
     cp_async_wait_group<0>();
@@ -464,10 +480,9 @@ __global__ void __launch_bounds__(kUpWorkers* kUpThreads, 1) up_kernel(const Moe
 // -------------------------------------------------------------------- down
 // A block is an SM's whole load, 16 warps, and owns `rows` (at most 16, the M
 // side) output channels at a time: 14 for 2048 channels, twice 14 for 4096. Its
-// warps share the (job, window) list of a tile in equal runs, so that no other
+// warps share the (job, stage) list of a tile in equal runs, so that no other
 // block is needed for a token's sum over its experts; they stream it, from one
-// tile into the next, through rings in shared memory, four windows (4 KB) a
-// stage. A step's exact integer sums join in f32 with the step's unit. At the
+// tile into the next, through rings in shared memory. A step's exact integer sums join in f32 with the step's unit. At the
 // end of a job a warp adds its result, weighted, to its own sums per token; the
 // warps' are added in order at the end of the tile.
 constexpr int kDownWarps = 16, kDownThreads = 32 * kDownWarps;
@@ -490,93 +505,95 @@ __global__ void __launch_bounds__(kDownThreads, 1) down_kernel(const MoeArgs a) 
     __syncthreads();
     list_jobs<NP, kDownThreads>(a, r);
 
-    const int windows = a.fp / 64, tiles = (a.K + a.rows - 1) / a.rows;
-    const int64_t units = static_cast<int64_t>(r.jobs) * windows;
-    const int u_begin = static_cast<int>(units * warp / kDownWarps), u_end = static_cast<int>(units * (warp + 1) / kDownWarps);
-    const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(s_raw)) + warp * STAGES * kStageBytes;
+    const int stages = a.fp / kColumns, tiles = (a.K + a.rows - 1) / a.rows;
+    const int units = r.jobs * stages;  // under 2^18
+    const int u_begin = units * warp / kDownWarps, u_end = units * (warp + 1) / kDownWarps;
+    const uint32_t ring =
+        static_cast<uint32_t>(__cvta_generic_to_shared(s_raw)) + warp * STAGES * kStageBytes + 16 * lane;
     float* const mine = outs + warp * a.M * 16;
 
-    // The copying side: a stage is up to four windows of one job.
-    int c_tile = blockIdx.x, c_u = u_begin, c_stage = 0;
+    // The copying side: tile, job, stage of it, this lane's rows g and g + 8.
+    int c_tile = blockIdx.x, c_left = u_end - u_begin, c_job = u_begin / stages, c_s = u_begin % stages, c_slot = 0;
+    int bytes0 = 0, bytes1 = 0;
+    const int8_t *row0 = nullptr, *row1 = nullptr;
+    const auto rows_of = [&] {
+        const int n0 = c_tile * a.rows, n_end = min(a.K, n0 + a.rows);
+        const int64_t at = static_cast<int64_t>(job_of(r, c_job).expert) * a.K;
+        bytes0 = n0 + g < n_end ? 16 : 0;
+        bytes1 = n0 + 8 + g < n_end ? 16 : 0;
+        row0 = a.qd + (at + min(n0 + g, a.K - 1)) * a.F + 16 * t;
+        row1 = a.qd + (at + min(n0 + 8 + g, a.K - 1)) * a.F + 16 * t;
+    };
     const auto copy_next = [&] {
-        if (c_tile < tiles && c_u < u_end) {
-            const int job_i = c_u / windows, w = c_u - job_i * windows;
-            const int count = min(min(kWindows, windows - w), u_end - c_u);
-            const int n0 = c_tile * a.rows, n_end = min(a.K, n0 + a.rows);
-            const int64_t expert = static_cast<int64_t>(job_of(r, job_i).expert) * a.K;
-            const uint32_t dst = ring + c_stage * kStageBytes + 16 * lane;
-            #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int n = n0 + 8 * j + g;
-                const int8_t* row = a.qd + (expert + min(n, a.K - 1)) * a.F;
-                #pragma unroll
-                for (int k = 0; k < kWindows; ++k) {
-                    const int col = 64 * (w + k) + 16 * t;
-                    const int bytes = n < n_end && k < count && col < a.F ? 16 : 0;
-                    cp_async16(dst + 1024 * k + 512 * j, row + (bytes ? col : 0), bytes);
-                }
-            }
-            c_u += count;
-            if (c_u == u_end) {
-                c_u = u_begin;
+        if (c_left > 0) {
+            copy_stage(ring + c_slot * kStageBytes, row0, row1, bytes0, bytes1, c_s * kColumns, t, a.F);
+            --c_left;
+            ++c_s;
+            if (c_left == 0) {
                 c_tile += gridDim.x;
+                c_job = u_begin / stages, c_s = u_begin % stages;
+                if (c_tile < tiles) c_left = u_end - u_begin, rows_of();
+            } else if (c_s == stages) {
+                c_s = 0;
+                ++c_job;
+                rows_of();
             }
         }
         cp_async_commit();
-        c_stage = c_stage == STAGES - 1 ? 0 : c_stage + 1;
+        c_slot = c_slot == STAGES - 1 ? 0 : c_slot + 1;
     };
+    if (c_left > 0) rows_of();
     #pragma unroll
     for (int i = 0; i < STAGES - 1; ++i) copy_next();
 
-    int stage = 0;
+    int slot = 0;
     for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
         const int n0 = tile * a.rows, n_end = min(a.K, n0 + a.rows);
         for (int u = u_begin; u < u_end;) {
-            const int w_begin = u % windows;
-            const Job job = job_of(r, u / windows);
-            const int w_end = min(windows, w_begin + (u_end - u));
-            u += w_end - w_begin;
+            const int s_begin = u % stages;
+            const Job job = job_of(r, u / stages);
+            const int s_end = min(stages, s_begin + (u_end - u));
+            u += s_end - s_begin;
             float scale[2];
             #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 scale[j] = a.sd[static_cast<int64_t>(job.expert) * a.K + min(n0 + 8 * j + g, n_end - 1)];
             }
+            // This lane's column of the B operand, and the token of its result
+            // columns (columns of tokens that the job does not have are not used).
             const int8_t* hd[NP];
             const float* hs[NP];
-            bool on[NP];
             #pragma unroll
             for (int n = 0; n < NP; ++n) {
-                // This lane's column of the B operand, and the token of its result columns.
-                const int j = 2 * n + (g >> 2), jr = min(2 * n + (t >> 1), job.count - 1);
-                on[n] = j < job.count;
-                hd[n] = a.hd + (static_cast<int64_t>(r.pair[job.pos + (on[n] ? j : 0)]) * 4 + (g & 3)) * a.fp + 16 * t;
-                hs[n] = a.hs + static_cast<int64_t>(r.pair[job.pos + jr]) * (2 * windows);
+                const int j = min(2 * n + (g >> 2), job.count - 1), jr = min(2 * n + (t >> 1), job.count - 1);
+                hd[n] = a.hd + (static_cast<int64_t>(r.pair[job.pos + j]) * 4 + (g & 3)) * a.fp + 16 * t;
+                hs[n] = a.hs + static_cast<int64_t>(r.pair[job.pos + jr]) * (a.fp / 32);
             }
             uint4 b[kWindows][NP];
             float2 unit[kWindows][NP];
-            const auto load_b = [&](int w0) {
+            const auto load_b = [&](int st) {
                 #pragma unroll
-                for (int k = 0; k < kWindows; ++k) {
+                for (int n = 0; n < NP; ++n) {
                     #pragma unroll
-                    for (int n = 0; n < NP; ++n) {
-                        b[k][n] = make_uint4(0u, 0u, 0u, 0u);
-                        unit[k][n] = make_float2(0.0f, 0.0f);
-                        if (w0 + k < w_end) {
-                            if (on[n]) b[k][n] = *reinterpret_cast<const uint4*>(hd[n] + 64 * (w0 + k));
-                            unit[k][n] = *reinterpret_cast<const float2*>(hs[n] + 2 * (w0 + k));
-                        }
+                    for (int k = 0; k < kWindows; ++k) {
+                        b[k][n] = *reinterpret_cast<const uint4*>(hd[n] + kColumns * st + 64 * k);
+                    }
+                    #pragma unroll
+                    for (int k = 0; k < kWindows; k += 2) {
+                        const float4 x = *reinterpret_cast<const float4*>(hs[n] + 2 * kWindows * st + 2 * k);
+                        unit[k][n] = make_float2(x.x, x.y), unit[k + 1][n] = make_float2(x.z, x.w);
                     }
                 }
             };
-            if (NP == 1) load_b(w_begin);
-            float acc[NP][4] = {};
-            for (int w0 = w_begin; w0 < w_end; w0 += kWindows) {
-                if (NP > 1) load_b(w0);  // (too many registers to hold a stage ahead)
+            if (NP == 1) load_b(s_begin);
+            float2 acc2[NP][2] = {};
+            for (int st = s_begin; st < s_end; ++st) {
+                if (NP > 1) load_b(st);  // (too many registers to hold a stage ahead)
                 cp_async_wait_group<STAGES - 2>();
                 __syncwarp();
                 copy_next();
-                const uint32_t at = ring + stage * kStageBytes + 16 * lane;
-                stage = stage == STAGES - 1 ? 0 : stage + 1;
+                const uint32_t at = ring + slot * kStageBytes;
+                slot = slot == STAGES - 1 ? 0 : slot + 1;
                 #pragma unroll
                 for (int k = 0; k < kWindows; ++k) {
                     const uint4 q0 = load_shared16(at + 1024 * k), q1 = load_shared16(at + 1024 * k + 512);
@@ -587,13 +604,23 @@ __global__ void __launch_bounds__(kDownThreads, 1) down_kernel(const MoeArgs a) 
                         mma_s8_16832_from(d[0], lo, b[k][n].x, b[k][n].y, kMagicBits);
                         mma_s8_16832_from(d[1], hi, b[k][n].z, b[k][n].w, kMagicBits);
                         #pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            acc[n][c] = fmaf(__int_as_float(d[0][c]) - kMagic, unit[k][n].x, acc[n][c]);
-                            acc[n][c] = fmaf(__int_as_float(d[1][c]) - kMagic, unit[k][n].y, acc[n][c]);
+                        for (int h = 0; h < 2; ++h) {
+                            const float by = h == 0 ? unit[k][n].x : unit[k][n].y;
+                            #pragma unroll
+                            for (int c = 0; c < 2; ++c) {
+                                const float2 x = __fadd2_rn(make_float2(__int_as_float(d[h][2 * c]), __int_as_float(d[h][2 * c + 1])),
+                                                            make_float2(-kMagic, -kMagic));
+                                acc2[n][c] = __ffma2_rn(x, make_float2(by, by), acc2[n][c]);
+                            }
                         }
                     }
                 }
-                if (NP == 1 && w0 + kWindows < w_end) load_b(w0 + kWindows);
+                if (NP == 1 && st + 1 < s_end) load_b(st + 1);
+            }
+            float acc[NP][4];
+            #pragma unroll
+            for (int n = 0; n < NP; ++n) {
+                acc[n][0] = acc2[n][0].x, acc[n][1] = acc2[n][0].y, acc[n][2] = acc2[n][1].x, acc[n][3] = acc2[n][1].y;
             }
             #pragma unroll
             for (int n = 0; n < NP; ++n) {
@@ -728,7 +755,7 @@ cudaError_t run_tensor(MoeArgs a, cudaStream_t stream) {
     cudaError_t e = cudaFuncSetAttribute(up_kernel<NP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Up<NP>::kBytes);
     if (e != cudaSuccess) return e;
     cudaLaunchAttribute attr[1];
-    const int64_t items = static_cast<int64_t>(a.M) * a.top * (a.fp / 32);  // at most
+    const int64_t items = static_cast<int64_t>(a.M) * a.top * ((a.F + 63) / 64 * 2);  // at most
     const cudaLaunchConfig_t cfg = pdl_config(dim3(static_cast<unsigned>(items < sms ? items : sms)),
                                               dim3(kUpWorkers * kUpThreads), Up<NP>::kBytes, stream, attr);
     e = cudaLaunchKernelEx(&cfg, up_kernel<NP>, a);
@@ -754,7 +781,6 @@ cudaError_t run_pass(const MoeArgs& a, bool tensor, cudaStream_t stream) {
     }
     // Tokens an expert has to take at a time: by how many pick it on average.
     if (a.M <= 2) return run_tensor<1>(a, stream);
-    if (getenv("NP1")) return run_tensor<1>(a, stream);
     if (a.M <= 4 || a.M * a.top <= 2 * a.E) return run_tensor<2>(a, stream);
     return run_tensor<4>(a, stream);
 }
@@ -766,7 +792,7 @@ extern "C" int64_t popcornMoeWorkspace(int64_t M, int64_t K, int64_t F, int64_t 
     if (M <= 0 || K <= 0 || F <= 0 || E <= 0 || top_k <= 0 || !pcb::sizes_supported(M, K, F, E, top_k)) return 0;
     pcb::MoeArgs a = {};
     a.K = static_cast<int>(K), a.F = static_cast<int>(F), a.E = static_cast<int>(E), a.top = static_cast<int>(top_k);
-    a.kp = static_cast<int>(pcb::round_up(K, 64)), a.fp = static_cast<int>(pcb::round_up(F, 64));
+    a.kp = static_cast<int>(pcb::round_up(K, pcb::kColumns)), a.fp = static_cast<int>(pcb::round_up(F, pcb::kColumns));
     const int64_t m = M < pcb::kMoeTokens ? M : pcb::kMoeTokens;
     // (Either kind of kernel: the sizes do not say how the codes are aligned.)
     const int64_t plain = pcb::lay_out(a, nullptr, m, false, true);
@@ -800,7 +826,7 @@ extern "C" popcornStatus_t popcornMoe_i8f32(float* out, int32_t* experts, float*
     a.router = router, a.qg = q_gate, a.sg = s_gate, a.qu = q_up, a.su = s_up, a.qd = q_down, a.sd = s_down;
     a.K = static_cast<int>(K), a.F = static_cast<int>(F), a.E = static_cast<int>(E), a.top = static_cast<int>(top_k);
     a.renorm = renormalize;
-    a.kp = static_cast<int>(pcb::round_up(K, 64)), a.fp = static_cast<int>(pcb::round_up(F, 64));
+    a.kp = static_cast<int>(pcb::round_up(K, pcb::kColumns)), a.fp = static_cast<int>(pcb::round_up(F, pcb::kColumns));
     cudaError_t e = cudaSuccess;
     for (int64_t m = 0; m < M && e == cudaSuccess; m += pcb::kMoeTokens) {
         a.M = static_cast<int>(M - m < pcb::kMoeTokens ? M - m : pcb::kMoeTokens);

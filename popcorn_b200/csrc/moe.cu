@@ -32,6 +32,7 @@
 namespace pcb {
 namespace {
 
+constexpr int kDownWarps = 16, kDownThreads = 32 * kDownWarps;
 constexpr int kMoeThreads = 256;
 constexpr int kMoeWarps = kMoeThreads / 32;
 constexpr int kWindows = 4;       // windows of a stage: 256 columns of 16 rows
@@ -84,79 +85,103 @@ __device__ __forceinline__ uint32_t digits_of(float v, const Fixed& f) {
 __device__ __forceinline__ bool not_finite(float v) { return !(fabsf(v) <= 3.4028234663852886e38f); }
 
 // ------------------------------------------------------------------ routing
-// Block e < E: logits of expert e for tokens 8 y .. 8 y + 7. Blocks behind
-// them (y = 0): the digits of one token each.
-__global__ void __launch_bounds__(128) route_kernel(const MoeArgs a) {
-    __shared__ float part[4][8];
-    __shared__ int s_bad;
+// Block e < E: logits of expert e for tokens 8 y .. 8 y + 7; the router's row is
+// read before the kernel waits for the one ahead. Blocks behind them (y = 0):
+// the digits of one token each.
+constexpr int kRouteThreads = 256, kRouteWarps = kRouteThreads / 32;
+__global__ void __launch_bounds__(kRouteThreads) route_kernel(const MoeArgs a) {
+    constexpr int HELD = 4;  // float4 pieces of the router's row per thread: 4096 columns
+    __shared__ float part[kRouteWarps][8];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     pdl_launch_dependents();
     const int e = blockIdx.x;
-    if (e < a.E && blockIdx.y == 0 && tid < 4) {
-        prefetch_l2_range(a.router + static_cast<int64_t>(e) * a.K, 4LL * a.K, tid, 4);
+    const bool vec =
+        a.K % 4 == 0 && ((reinterpret_cast<uintptr_t>(a.router) | reinterpret_cast<uintptr_t>(a.x)) & 15u) == 0;
+    const float* w = a.router + static_cast<int64_t>(e) * a.K;
+    float4 held[HELD];
+    if (e < a.E && vec) {
+        #pragma unroll
+        for (int i = 0; i < HELD; ++i) {
+            const int k = 4 * (tid + i * kRouteThreads);
+            held[i] = k < a.K ? *reinterpret_cast<const float4*>(w + k) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
     }
     pdl_wait();
     if (e >= a.E) {
         const int m = e - a.E;
         if (blockIdx.y != 0 || a.xd == nullptr) return;
         const float* x = a.x + static_cast<int64_t>(m) * a.K;
+        // Four columns at a time, the first ones held between maximum and digits.
+        const auto four = [&](int k) {
+            if (k >= a.K) return make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            return vec ? *reinterpret_cast<const float4*>(x + k) : make_float4(x[k], x[k + 1], x[k + 2], x[k + 3]);
+        };
         float top = 0.0f;
         bool bad = false;
-        for (int k = tid; k < a.K; k += 128) {
-            const float v = x[k];
-            top = fmaxf(top, fabsf(v));
-            bad = bad || not_finite(v);
-        }
-        if (tid == 0) s_bad = 0;
+        const auto look = [&](const float4& v) {
+            top = fmaxf(fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
+            bad = bad || not_finite(v.x) || not_finite(v.y) || not_finite(v.z) || not_finite(v.w);
+        };
+        #pragma unroll
+        for (int i = 0; i < HELD; ++i) held[i] = four(4 * (tid + i * kRouteThreads));
+        #pragma unroll
+        for (int i = 0; i < HELD; ++i) look(held[i]);
+        for (int k = 4 * (tid + HELD * kRouteThreads); k < a.K; k += 4 * kRouteThreads) look(four(k));
         top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
         if (lane == 0) part[warp][0] = top;
-        __syncthreads();
-        if (bad) s_bad = 1;
-        __syncthreads();
+        const bool any_bad = __syncthreads_or(bad) != 0;
         #pragma unroll
-        for (int w = 0; w < 4; ++w) top = fmaxf(top, part[w][0]);
-        const Fixed f = fixed_for(top, s_bad != 0);
+        for (int i = 0; i < kRouteWarps; ++i) top = fmaxf(top, part[i][0]);
+        const Fixed f = fixed_for(top, any_bad);
         int8_t* d = a.xd + static_cast<int64_t>(m) * 4 * a.kp;
-        for (int k = 4 * tid; k < a.kp; k += 512) {
-            uint32_t y[4];
-            #pragma unroll
-            for (int j = 0; j < 4; ++j) y[j] = k < a.K && f.up != 0.0f ? digits_of(x[k + j], f) : 0u;
+        const auto put = [&](int k, const float4& v) {
+            if (k >= a.kp) return;
+            const uint32_t y[4] = {any_bad ? 0u : digits_of(v.x, f), any_bad ? 0u : digits_of(v.y, f),
+                                   any_bad ? 0u : digits_of(v.z, f), any_bad ? 0u : digits_of(v.w, f)};
             #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const uint32_t sel = static_cast<uint32_t>(i | ((i + 4) << 4));
                 *reinterpret_cast<uint32_t*>(d + static_cast<int64_t>(i) * a.kp + k) =
                     __byte_perm(__byte_perm(y[0], y[1], sel), __byte_perm(y[2], y[3], sel), 0x5410);
             }
-        }
+        };
+        #pragma unroll
+        for (int i = 0; i < HELD; ++i) put(4 * (tid + i * kRouteThreads), held[i]);
+        for (int k = 4 * (tid + HELD * kRouteThreads); k < a.kp; k += 4 * kRouteThreads) put(k, four(k));
         if (tid == 0) a.xs[m] = f.unit;
         // Units of the padding of this token's hidden values (its digits meet codes
         // that are zeros and may be anything).
         const int used = (a.F + 63) / 64 * 2, all = a.fp / 32;
-        for (int i = tid; i < a.top * (all - used); i += 128) {
+        for (int i = tid; i < a.top * (all - used); i += kRouteThreads) {
             const int j = i / (all - used);
             a.hs[(static_cast<int64_t>(m) * a.top + j) * all + used + i - j * (all - used)] = 0.0f;
         }
         return;
     }
-    const float* w = a.router + static_cast<int64_t>(e) * a.K;
     const int m0 = blockIdx.y * 8;
     const int n = min(8, a.M - m0);
     const float* x = a.x + static_cast<int64_t>(m0) * a.K;
     float acc[8] = {};
-    if (a.K % 4 == 0 && ((reinterpret_cast<uintptr_t>(a.router) | reinterpret_cast<uintptr_t>(a.x)) & 15u) == 0) {
-        #pragma unroll 4
-        for (int k = 4 * tid; k < a.K; k += 512) {
-            const float4 r = *reinterpret_cast<const float4*>(w + k);
-            #pragma unroll
-            for (int m = 0; m < 8; ++m) {
-                if (m < n) {
-                    const float4 v = *reinterpret_cast<const float4*>(x + static_cast<int64_t>(m) * a.K + k);
-                    acc[m] = fmaf(r.x, v.x, fmaf(r.y, v.y, fmaf(r.z, v.z, fmaf(r.w, v.w, acc[m]))));
-                }
+    const auto add = [&](int k, const float4& q) {
+        #pragma unroll
+        for (int m = 0; m < 8; ++m) {
+            if (m < n) {
+                const float4 v = *reinterpret_cast<const float4*>(x + static_cast<int64_t>(m) * a.K + k);
+                acc[m] = fmaf(q.x, v.x, fmaf(q.y, v.y, fmaf(q.z, v.z, fmaf(q.w, v.w, acc[m]))));
             }
         }
+    };
+    if (vec) {
+        #pragma unroll
+        for (int i = 0; i < HELD; ++i) {
+            const int k = 4 * (tid + i * kRouteThreads);
+            if (k < a.K) add(k, held[i]);
+        }
+        for (int k = 4 * (tid + HELD * kRouteThreads); k < a.K; k += 4 * kRouteThreads) {
+            add(k, *reinterpret_cast<const float4*>(w + k));
+        }
     } else {
-        for (int k = tid; k < a.K; k += 128) {
+        for (int k = tid; k < a.K; k += kRouteThreads) {
             #pragma unroll
             for (int m = 0; m < 8; ++m) {
                 if (m < n) acc[m] = fmaf(w[k], x[static_cast<int64_t>(m) * a.K + k], acc[m]);
@@ -165,13 +190,18 @@ __global__ void __launch_bounds__(128) route_kernel(const MoeArgs a) {
     }
     #pragma unroll
     for (int m = 0; m < 8; ++m) {
-        #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) acc[m] += __shfl_xor_sync(0xffffffffu, acc[m], o);
-        if (lane == 0) part[warp][m] = acc[m];
+        if (m < n) {
+            #pragma unroll
+            for (int o = 16; o > 0; o >>= 1) acc[m] += __shfl_xor_sync(0xffffffffu, acc[m], o);
+            if (lane == 0) part[warp][m] = acc[m];
+        }
     }
     __syncthreads();
     if (tid < n) {
-        a.logits[static_cast<int64_t>(m0 + tid) * a.E + e] = part[0][tid] + part[1][tid] + part[2][tid] + part[3][tid];
+        float z = 0.0f;
+        #pragma unroll
+        for (int i = 0; i < kRouteWarps; ++i) z += part[i][tid];
+        a.logits[static_cast<int64_t>(m0 + tid) * a.E + e] = z;
     }
 }
 
@@ -313,8 +343,9 @@ __device__ void route_tokens(const MoeArgs& a, Routing& r) {
 // streams its rows, from one item into the next, through a ring of its own in
 // shared memory by asynchronous copies, 256 bytes of each row (4 KB) a stage:
 // 144 KB an SM in flight. (Loads into registers with two or three blocks an SM
-// kept at most 96 KB in flight, X us for the 11008-row case; warps that shared
-// the rows and had a quarter of the columns each read 64 bytes a row at a time, Y us.)
+// kept at most 96 KB in flight; warps that shared
+// the rows and had a quarter of the columns each read 64 bytes a row at a time:
+// 38 us against 34 for the two experts of 11008 rows.)
 constexpr int kUpWarps = 4, kUpThreads = 32 * kUpWarps, kUpWorkers = 3;
 template <int NP>
 struct Up {
@@ -485,7 +516,6 @@ __global__ void __launch_bounds__(kUpWorkers* kUpThreads, 1) up_kernel(const Moe
 // tile into the next, through rings in shared memory. A step's exact integer sums join in f32 with the step's unit. At the
 // end of a job a warp adds its result, weighted, to its own sums per token; the
 // warps' are added in order at the end of the tile.
-constexpr int kDownWarps = 16, kDownThreads = 32 * kDownWarps;
 constexpr int down_stages(int tokens) { return tokens <= 16 ? 3 : 2; }  // what the sums leave room for
 
 template <int NP, int STAGES>
@@ -755,14 +785,13 @@ cudaError_t run_tensor(MoeArgs a, cudaStream_t stream) {
     cudaError_t e = cudaFuncSetAttribute(up_kernel<NP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Up<NP>::kBytes);
     if (e != cudaSuccess) return e;
     cudaLaunchAttribute attr[1];
+    // Down: as many tiles for every SM, as few as 16 rows allow.
+    a.rows = static_cast<int>(ceil_div(a.K, ceil_div(a.K, 16 * sms) * sms));
     const int64_t items = static_cast<int64_t>(a.M) * a.top * ((a.F + 63) / 64 * 2);  // at most
     const cudaLaunchConfig_t cfg = pdl_config(dim3(static_cast<unsigned>(items < sms ? items : sms)),
                                               dim3(kUpWorkers * kUpThreads), Up<NP>::kBytes, stream, attr);
     e = cudaLaunchKernelEx(&cfg, up_kernel<NP>, a);
     if (e != cudaSuccess) return e;
-    // Down: as many tiles for every SM, as few as 16 rows allow.
-    const int64_t rounds = ceil_div(a.K, 16 * sms);
-    a.rows = static_cast<int>(ceil_div(a.K, rounds * sms));
     const int64_t tiles = ceil_div(a.K, a.rows);
     const int blocks = static_cast<int>(tiles < sms ? tiles : sms);
     return down_stages(a.M) == 3 ? run_down<NP, 3>(a, blocks, stream) : run_down<NP, 2>(a, blocks, stream);
@@ -770,7 +799,8 @@ cudaError_t run_tensor(MoeArgs a, cudaStream_t stream) {
 
 cudaError_t run_pass(const MoeArgs& a, bool tensor, cudaStream_t stream) {
     cudaLaunchAttribute attr[1];
-    cudaLaunchConfig_t cfg = pdl_config(dim3(a.E + (tensor ? a.M : 0), (a.M + 7) / 8), dim3(128), 0, stream, attr);
+    cudaLaunchConfig_t cfg = pdl_config(dim3(a.E + (tensor ? a.M : 0), (a.M + 7) / 8), dim3(kRouteThreads), 0,
+                                        stream, attr);
     cudaError_t e = cudaLaunchKernelEx(&cfg, route_kernel, a);
     if (e != cudaSuccess) return e;
     if (!tensor) {

@@ -17,11 +17,16 @@
 //       memory, f32 sums in tensor memory
 //
 // Warps 0-3 and 4-7 are the softmax of the two tiles (a thread owns a row, so
-// maxima and sums need no exchange), 8-11 convert codes, one thread of warp 12
-// issues the products: while one tile's softmax runs, the tensor cores work on
-// the other's. The maximum moves only when a score exceeds it by 2^8 (then the
-// thread rescales O in tensor memory), as in kv_attention.cu, whose scaling
-// conventions, work split and partial results these are.
+// maxima and sums need no exchange), 8-14 convert codes, and one thread of warp
+// 15 issues the products: while one tile's softmax runs, the tensor cores work
+// on the other's. (Issued by the softmax's own threads the products held them
+// up, 2000 cycles a step: the queue is short.) Codes come into shared memory by
+// asynchronous copies, so that all loops here are short ones: 16 warps in four
+// roles live on one instruction cache, and with the conversion unrolled over
+// registers they waited for it more than for anything else. The maximum moves
+// only when a score exceeds it by 2^8 (then the thread rescales O in tensor
+// memory), as in kv_attention.cu, whose scaling conventions, work split and
+// partial results these are.
 //
 // Every wait is bounded (sm100.cuh); one that runs out sets error bit 0x8000
 // and ends the block.
@@ -40,9 +45,9 @@ constexpr unsigned int kErrWait = 0x8000u;
 
 constexpr int kTile = 128;          // rows of a tile, tokens of a step
 constexpr int kRows = 2 * kTile;    // rows of a task
-constexpr int kSoftWarps = 8, kConvWarps = 4;
-constexpr int kPThreads = 32 * (kSoftWarps + kConvWarps + 1);
+constexpr int kSoftWarps = 8, kConvWarps = 7, kIssue = kSoftWarps + kConvWarps;
 constexpr int kConvThreads = 32 * kConvWarps;
+constexpr int kPThreads = 32 * (kIssue + 1);
 constexpr int kStages = 2;
 constexpr int kScaleRing = 4;
 constexpr int kFixedUnits = 2;      // a task's fixed cost in steps
@@ -58,7 +63,9 @@ struct Lay {  // shared memory, bytes; operand tiles in 128-byte swizzled rows
     static constexpr int kQ = 0;
     static constexpr int kK = kQ + 2 * kQTile;
     static constexpr int kV = kK + kStages * kKStage;
-    static constexpr int kScales = kV + kStages * kVStage;  // [ring][8] {ks, log2 vs, 1 / vs}
+    static constexpr int kRawK = kV + kStages * kVStage;    // codes of a step as they are
+    static constexpr int kRawV = kRawK + kTile * DP;
+    static constexpr int kScales = kRawV + kTile * DP;      // [ring][8] {ks, log2 vs, 1 / vs}
     static constexpr int kBytes = kScales + kScaleRing * 8 * 16;
     static constexpr int kAlloc = kBytes + 1024;            // the tiles start on 1024 bytes
 };
@@ -82,6 +89,17 @@ __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy
 __device__ __forceinline__ void store_shared16(uint32_t addr, const uint32_t (&v)[4]) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3])
                  : "memory");
+}
+
+__device__ __forceinline__ uint4 load_shared16(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+    return v;
+}
+__device__ __forceinline__ uint32_t load_shared4(uint32_t addr) {
+    uint32_t v;
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(addr));
+    return v;
 }
 
 __device__ __forceinline__ uint32_t as_f16(uint32_t biased) {  // halves 1024 + code + 128
@@ -198,11 +216,10 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const AttnArgs 
     // after may start only when it has been taken: neither can hold columns
     // that the other waits for.
     pdl_wait();
-    if (warp == kSoftWarps + kConvWarps) {
+    if (warp == kIssue) {
         tmem_alloc(smem_addr(&s_tmem), 512);
         tmem_relinquish();
     }
-    pdl_launch_dependents();
     const Run run = find_run<false>(a.seqs, blockIdx.x, gridDim.x, 1, kFixedUnits, [&](int b, int64_t& steps, int64_t& tasks) {
         const Seq s = sequence(a, b, &g_prompt_err);
         for (int r = 0; r < s.rows * a.group; r += kRows) {
@@ -215,6 +232,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const AttnArgs 
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    pdl_launch_dependents();
     const uint32_t tmem = s_tmem;
     // Columns: S and P of the two tiles at 0 and 128, O at 256 and 384.
 
@@ -226,12 +244,12 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const AttnArgs 
         const uint32_t lanes = tmem + (static_cast<uint32_t>(warp & 3) << 21);  // this warp's 32 lanes
         const uint32_t s_col = lanes + 128 * m, o_col = lanes + 256 + 128 * m;
         int steps_done = 0;                         // of this tile, over all segments
-        int ring_at = 0;                            // steps of the block, both tiles
+        int kt = 0;                                 // steps of the block, both tiles
         bool good = true;
         while (good && walk.next()) {
             const int n = walk.u1 - walk.u0;
             if (m >= walk.tiles()) {
-                ring_at += n;
+                kt += n;
                 continue;
             }
             const int r = walk.rt * kRows + m * kTile + row;
@@ -281,10 +299,10 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const AttnArgs 
             if (!valid) see0 = 0, see1 = INT32_MAX;  // (never stored: no reason to mask)
             if (see1 <= see0) fac = 0.0f;
             float top = -INFINITY, den = 0.0f;
-            for (int i = 0; i < n; ++i, ++steps_done, ++ring_at) {
+            for (int i = 0; i < n; ++i, ++steps_done, ++kt) {
                 if (!(good = wait(kSFull, m, steps_done))) break;
                 tc_fence_after();
-                const GroupScale* gs = ring + (ring_at % kScaleRing) * 8;
+                const GroupScale* gs = ring + (kt % kScaleRing) * 8;
                 const int j0 = walk.see.lo + (walk.u0 + i) * kTile;
                 const bool whole = __all_sync(0xffffffffu, see0 <= j0 && j0 + kTile <= see1);
                 // --- maximum; loops over 32 columns stay loops, for the
@@ -415,80 +433,23 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const AttnArgs 
             }
             tc_fence_before();  // O has been read: the next segment's products may follow
         }
-    } else if (warp < kSoftWarps + kConvWarps) {
+    } else if (warp < kIssue) {
         // ----------------------------------------------------------- convert
-        // A step's tokens are eight groups of 16, each inside one page; a warp
-        // has two of them, so that a group's address is the same for all lanes
-        // and every load is that address plus a constant of the lane.
-        constexpr int KN = 16 * DP / 16 / 32;   // 16-byte pieces of a group's keys per lane
-        constexpr int WV = DP / 4;              // words of a value row
-        constexpr int VO = 2 * WV / 32;         // runs of 8 tokens of a group's values per lane
-        const int cw = warp - kSoftWarps;
-        const int kpiece = lane % (DP / 16), krow = lane / (DP / 16);
-        const int vword = lane % WV, voct = lane / WV;
+        // A step's tokens are eight groups of 16, each inside one page. The first
+        // warp's lanes 0-7 look after a group each: its page index is fetched two
+        // steps ahead, its codes' offset and its scales one.
+        constexpr int CH = DP / 16;  // 16-byte pieces of a row
+        constexpr int WV = DP / 4;   // words of a row
+        __shared__ int64_t s_offset[2][8];  // step parity; -1: nothing there
+        const int ct = tid - 32 * kSoftWarps;
+        const bool scout = ct < 8;
         const int page_mask = (1 << a.page_shift) - 1;
+        const auto sync_conv = [&] { asm volatile("bar.sync 1, %0;" ::"n"(kConvThreads) : "memory"); };
         struct Step {
             int h, j0, len;
             int64_t table;  // of the sequence
         };
-        struct Groups {
-            int64_t block[2];   // page and head; -1: nothing there
-            float ks, vs;       // lane i < 2: scales of group i
-        };
-        // Page indices are fetched two steps ahead of their use, scales one.
-        const auto fetch = [&](const Step& st, int (&pages)[2]) {
-            #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int j = st.j0 + 16 * (2 * cw + i);
-                pages[i] = j < st.len ? a.table[st.table + (j >> a.page_shift)] : -1;
-            }
-        };
-        const auto look_up = [&](const Step& st, const int (&pages)[2], Groups& g) {
-            #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const bool in = pages[i] >= 0 && pages[i] < a.pages;
-                g.block[i] = in ? static_cast<int64_t>(pages[i]) * a.heads + st.h : -1;
-                if (!in && lane == 0 && st.j0 + 16 * (2 * cw + i) < st.len) atomicOr(err, kKvErrAttention);
-            }
-            const int64_t mine = lane == 0 ? g.block[0] : g.block[1];
-            if (lane < 2 && mine >= 0) {
-                g.ks = a.ks[mine];
-                g.vs = a.vs[mine];
-            }
-        };
-        uint4 kq[2][KN];
-        uint32_t vq[2][VO][8];
-        const auto load_k = [&](const Step& st, const Groups& g) {
-            #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int row = (st.j0 + 16 * (2 * cw + i)) & page_mask;
-                const int8_t* p = a.k + ((g.block[i] << a.page_shift) + row) * DP + 16 * lane;
-                #pragma unroll
-                for (int n = 0; n < KN; ++n) {
-                    kq[i][n] = make_uint4(0u, 0u, 0u, 0u);
-                    if (g.block[i] >= 0) kq[i][n] = *reinterpret_cast<const uint4*>(p + 512 * n);
-                }
-            }
-        };
-        const auto load_v = [&](const Step& st, const Groups& g) {
-            #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int row = (st.j0 + 16 * (2 * cw + i)) & page_mask;
-                const int8_t* p = a.v + ((g.block[i] << a.page_shift) + row + 8 * voct) * DP + 4 * vword;
-                #pragma unroll
-                for (int n = 0; n < VO; ++n) {
-                    #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        vq[i][n][j] = 0u;
-                        if (g.block[i] >= 0) vq[i][n][j] = *reinterpret_cast<const uint32_t*>(p + (8 * n + j) * DP);
-                    }
-                }
-            }
-        };
-        int kt = 0;  // steps of the block
-        bool good = true;
         int left = 0;  // steps left in the segment
-        Step cur = {0, 0, 0, 0}, nxt, after;  // this step, the next, the one after it
         const auto advance = [&](Step& st) -> bool {
             if (left == 0) {
                 if (!walk.next()) return false;
@@ -503,124 +464,156 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const AttnArgs 
             --left;
             return true;
         };
+        int page = -1;
+        float ks = 0.0f, vs = 0.0f;
+        bool there = false;
+        const auto fetch = [&](const Step& st) {
+            const int j = st.j0 + 16 * ct;
+            return j < st.len ? a.table[st.table + (j >> a.page_shift)] : -1;
+        };
+        const auto look_up = [&](const Step& st, int parity) {
+            const int j = st.j0 + 16 * ct;
+            there = page >= 0 && page < a.pages;
+            if (!there && j < st.len) atomicOr(err, kKvErrAttention);
+            const int64_t block = static_cast<int64_t>(page) * a.heads + st.h;
+            s_offset[parity][ct] = there ? ((block << a.page_shift) + (j & page_mask)) * DP : -1;
+            if (there) ks = a.ks[block], vs = a.vs[block];
+        };
+        // A step's keys or values into their place in shared memory.
+        const auto copy = [&](const int8_t* from, int raw_at, int parity) {
+            #pragma unroll 2
+            for (int i = ct; i < kTile * CH; i += kConvThreads) {
+                const int group = i / (16 * CH);
+                const int64_t off = s_offset[parity][group];
+                cp_async16(smem + raw_at + 16 * i, from + (off < 0 ? 0 : off + 16 * (i % (16 * CH))), off < 0 ? 0 : 16);
+            }
+            cp_async_commit();
+        };
+        Step cur = {0, 0, 0, 0}, nxt, after;  // this step, the next, the one after it
+        int kt = 0;                           // steps of the block
+        bool good = true;
         bool have = advance(cur);
-        Groups groups = {{-1, -1}, 0.0f, 0.0f}, groups_next = groups;
-        int pages[2];
         nxt = cur;
-        bool have_next = false;
+        bool have_next = have && advance(nxt);
         if (have) {
-            fetch(cur, pages);
-            look_up(cur, pages, groups);
-            nxt = cur;
-            have_next = advance(nxt);
-            if (have_next) fetch(nxt, pages);
-            load_k(cur, groups);
-            load_v(cur, groups);
+            if (scout) {
+                page = fetch(cur);
+                look_up(cur, 0);
+                page = have_next ? fetch(nxt) : -1;
+            }
+            sync_conv();
+            copy(a.k, L::kRawK, 0);
+            copy(a.v, L::kRawV, 0);
+            cp_async_wait_group<1>();
+            sync_conv();
         }
-        while (good && have) {
-            if (have_next) look_up(nxt, pages, groups_next);
+        // (When a wait runs out the warps go on through their joint barriers, only
+        // without the work between them.)
+        while (have) {
             after = nxt;
             const bool have_after = have_next && advance(after);
-            if (have_after) fetch(after, pages);
-            const int stage = kt % kStages, turn = kt / kStages;
-            if (lane < 2) {
+            const int stage = kt % kStages, turn = kt / kStages - 1, parity = (kt + 1) & 1;
+            if (good && kt >= kStages) good = wait(kKEmpty, stage, turn);
+            if (scout) {
                 GroupScale g = {0.0f, -INFINITY, 1.0f, 0.0f};
-                if ((lane == 0 ? groups.block[0] : groups.block[1]) >= 0) {
-                    const bool tiny = fabsf(groups.vs) < kKvSmallestScale;  // all-zero codes
-                    g.ks = groups.ks;
-                    g.lv = tiny ? -80.0f : log2f(groups.vs);
+                if (there) {
+                    const bool tiny = fabsf(vs) < kKvSmallestScale;  // all-zero codes
+                    g.ks = ks;
+                    g.lv = tiny ? -80.0f : __log2f(vs);
                     g.iv = tiny ? 1.0f / kKvSmallestScale
-                                : fabsf(groups.vs) <= 3.4028234663852886e38f ? 1.0f / groups.vs : 1.0f;
+                                : fabsf(vs) <= 3.4028234663852886e38f ? __fdividef(1.0f, vs) : 1.0f;
                 }
-                ring[(kt % kScaleRing) * 8 + 2 * cw + lane] = g;
+                ring[(kt % kScaleRing) * 8 + ct] = g;
+                if (have_next) look_up(nxt, parity);
+                page = have_after ? fetch(after) : -1;
             }
-            if (kt >= kStages && !(good = wait(kKEmpty, stage, turn - 1))) break;
-            #pragma unroll
-            for (int i = 0; i < 2; ++i) {
+            #pragma unroll 2
+            for (int i = ct; good && i < kTile * CH; i += kConvThreads) {
+                const uint4 x = load_shared16(smem + L::kRawK + 16 * i);
+                const uint32_t in[4] = {x.x ^ 0x80808080u, x.y ^ 0x80808080u, x.z ^ 0x80808080u, x.w ^ 0x80808080u};
+                uint32_t lo[4], hi[4];
                 #pragma unroll
-                for (int n = 0; n < KN; ++n) {
-                    const uint4 q = kq[i][n];
-                    const uint32_t in[4] = {q.x ^ 0x80808080u, q.y ^ 0x80808080u, q.z ^ 0x80808080u, q.w ^ 0x80808080u};
-                    uint32_t lo[4], hi[4];
-                    #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        lo[2 * j] = as_f16(__byte_perm(in[j], 0x64646464u, 0x4140));
-                        lo[2 * j + 1] = as_f16(__byte_perm(in[j], 0x64646464u, 0x4342));
-                        hi[2 * j] = as_f16(__byte_perm(in[2 + j], 0x64646464u, 0x4140));
-                        hi[2 * j + 1] = as_f16(__byte_perm(in[2 + j], 0x64646464u, 0x4342));
-                    }
-                    const int r = 16 * (2 * cw + i) + krow + n * (512 / DP);
-                    const uint32_t base = smem + L::kK + stage * L::kKStage + (kpiece / 4) * (kTile * 128) + r * 128;
-                    const uint32_t unit = 2 * (kpiece % 4);
-                    store_shared16(base + ((unit ^ (r & 7)) << 4), lo);
-                    store_shared16(base + (((unit + 1) ^ (r & 7)) << 4), hi);
+                for (int j = 0; j < 2; ++j) {
+                    lo[2 * j] = as_f16(__byte_perm(in[j], 0x64646464u, 0x4140));
+                    lo[2 * j + 1] = as_f16(__byte_perm(in[j], 0x64646464u, 0x4342));
+                    hi[2 * j] = as_f16(__byte_perm(in[2 + j], 0x64646464u, 0x4140));
+                    hi[2 * j + 1] = as_f16(__byte_perm(in[2 + j], 0x64646464u, 0x4342));
                 }
+                const int r = i / CH, piece = i % CH;
+                const uint32_t base = smem + L::kK + stage * L::kKStage + (piece / 4) * (kTile * 128) + r * 128;
+                const uint32_t unit = 2 * (piece % 4);
+                store_shared16(base + ((unit ^ (r & 7)) << 4), lo);
+                store_shared16(base + (((unit + 1) ^ (r & 7)) << 4), hi);
             }
             fence_async_shared();
-            mbar_arrive(bar(kKFull, stage));
-            if (have_next) load_k(nxt, groups_next);
-            if (kt >= kStages && !(good = wait(kVEmpty, stage, turn - 1))) break;
+            if (good) mbar_arrive(bar(kKFull, stage));
+            cp_async_wait_group<0>();
+            sync_conv();  // raw keys are free, raw values there
+            if (have_next) copy(a.k, L::kRawK, parity);
+            if (good && kt >= kStages) good = wait(kVEmpty, stage, turn);
             // V transposed: row d, 64 tokens to a 128-byte row. Lanes take a word's
             // four bytes in different orders, so that eight lanes' stores fall into
             // eight different 16-byte banks.
-            #pragma unroll
-            for (int i = 0; i < 2; ++i) {
+            #pragma unroll 1
+            for (int i = ct; good && i < 16 * WV; i += kConvThreads) {
+                const int word = i % WV, oct = i / WV;
+                uint32_t q[8];
                 #pragma unroll
-                for (int n = 0; n < VO; ++n) {
-                    const int oct = 2 * (2 * cw + i) + voct + n;
+                for (int j = 0; j < 8; ++j) q[j] = load_shared4(smem + L::kRawV + (8 * oct + j) * DP + 4 * word);
+                #pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t byte = (j + (word >> 1)) & 3;
+                    const uint32_t sel = byte | (byte + 4) << 8;
+                    uint32_t w[4];
                     #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const uint32_t byte = (j + (vword >> 1)) & 3;
-                        const uint32_t sel = byte | (byte + 4) << 8;
-                        uint32_t w[4];
-                        #pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const uint32_t x = __byte_perm(vq[i][n][2 * k], vq[i][n][2 * k + 1], sel);
-                            w[k] = as_f16((x & 0x00ff00ffu) ^ 0x64806480u);
-                        }
-                        const uint32_t d = 4 * vword + byte;
-                        store_shared16(smem + L::kV + stage * L::kVStage + (oct >> 3) * (DP * 128) + d * 128 +
-                                           (((oct & 7) ^ (d & 7)) << 4),
-                                       w);
+                    for (int k = 0; k < 4; ++k) {
+                        const uint32_t x = __byte_perm(q[2 * k], q[2 * k + 1], sel);
+                        w[k] = as_f16((x & 0x00ff00ffu) ^ 0x64806480u);
                     }
+                    const uint32_t d = 4 * word + byte;
+                    store_shared16(smem + L::kV + stage * L::kVStage + (oct >> 3) * (DP * 128) + d * 128 +
+                                       (((oct & 7) ^ (d & 7)) << 4),
+                                   w);
                 }
             }
             fence_async_shared();
-            mbar_arrive(bar(kVFull, stage));
-            if (have_next) load_v(nxt, groups_next);
+            if (good) mbar_arrive(bar(kVFull, stage));
+            cp_async_wait_group<0>();
+            sync_conv();  // raw values are free, the next raw keys there
+            if (have_next) copy(a.v, L::kRawV, parity);
             nxt = after;
-            groups = groups_next;
             have = have_next;
             have_next = have_after;
             ++kt;
         }
+        cp_async_wait_group<0>();
     } else if (lane == 0) {
         // ------------------------------------------------------------- issue
         constexpr uint32_t id_qk = idesc_f16_f32(kTile, kTile), id_pv = idesc_f16_f32(kTile, DP);
         int kt = 0, segs[2] = {0, 0}, done[2] = {0, 0};
         bool good = true;
+        const auto arrived = [&](int which, int i, int turn) { return mbar_wait(bar(which, i), turn & 1, err, kErrWait); };
         const auto scores = [&](int m, int stage) {
             #pragma unroll
             for (int j = 0; j < DP / 16; ++j) {
                 const uint32_t off = (j / 4) * (kTile * 128);
-                mma_f16_ss(tmem + 128 * m,
-                           smem_desc_sw128_kmajor(smem + L::kQ + m * L::kQTile + off) + (j % 4) * 2,
+                mma_f16_ss(tmem + 128 * m, smem_desc_sw128_kmajor(smem + L::kQ + m * L::kQTile + off) + (j % 4) * 2,
                            smem_desc_sw128_kmajor(smem + L::kK + stage * L::kKStage + off) + (j % 4) * 2, id_qk, j > 0);
             }
             mma_commit(bar(kSFull, m));
         };
         while (good && walk.next()) {
             const int n = walk.u1 - walk.u0, tiles = walk.tiles();
-            for (int m = 0; m < tiles && good; ++m) good = mbar_wait(bar(kQReady, m), segs[m]++ & 1, err, kErrWait);
-            if (!good || !(good = mbar_wait(bar(kKFull, kt % kStages), (kt / kStages) & 1, err, kErrWait))) break;
+            for (int m = 0; m < tiles && good; ++m) good = arrived(kQReady, m, segs[m]++);
+            if (!good || !(good = arrived(kKFull, kt % kStages, kt / kStages))) break;
             tc_fence_after();
             for (int m = 0; m < tiles; ++m) scores(m, kt % kStages);
             mma_commit(bar(kKEmpty, kt % kStages));
             for (int i = 0; i < n && good; ++i, ++kt) {
                 const int stage = kt % kStages, next = (kt + 1) % kStages;
                 for (int m = 0; m < tiles && good; ++m) {
-                    if (m == 0 && !(good = mbar_wait(bar(kVFull, stage), (kt / kStages) & 1, err, kErrWait))) break;
-                    if (!(good = mbar_wait(bar(kPReady, m), done[m]++ & 1, err, kErrWait))) break;
+                    if (m == 0 && !(good = arrived(kVFull, stage, kt / kStages))) break;
+                    if (!(good = arrived(kPReady, m, done[m]++))) break;
                     tc_fence_after();
                     #pragma unroll
                     for (int j = 0; j < kTile / 16; ++j) {
@@ -631,9 +624,9 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const AttnArgs 
                     mma_commit(bar(kODone, m));
                     if (m == tiles - 1) mma_commit(bar(kVEmpty, stage));
                     if (i + 1 < n) {
-                        // (Over P, which the products just issued still read: products
-                        // of one thread run in the order of their issue.)
-                        if (m == 0 && !(good = mbar_wait(bar(kKFull, next), ((kt + 1) / kStages) & 1, err, kErrWait))) break;
+                        // Over P, so the products that read it have to be done.
+                        if (!(good = arrived(kODone, m, done[m] - 1))) break;
+                        if (m == 0 && !(good = arrived(kKFull, next, (kt + 1) / kStages))) break;
                         tc_fence_after();
                         scores(m, next);
                         if (m == tiles - 1) mma_commit(bar(kKEmpty, next));
@@ -641,18 +634,14 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const AttnArgs 
                 }
             }
         }
+        // Nothing is in flight any more, or a wait ran out: then it is waited for here.
+        mma_commit(bar(kDrain, 0));
+        mbar_wait(bar(kDrain, 0), 0, err, kErrWait);
     }
-    // Every product has been waited for by the softmax of its tile (kODone),
-    // or a wait ran out: then the issued ones are waited for here.
     __syncwarp();
     tc_fence_before();
     __syncthreads();
-    if (warp == kSoftWarps + kConvWarps) {
-        if (lane == 0) {
-            mma_commit(bar(kDrain, 0));
-            mbar_wait(bar(kDrain, 0), 0, err, kErrWait);
-        }
-        __syncwarp();
+    if (warp == kIssue) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }

@@ -70,6 +70,9 @@ struct Lay {  // shared memory, bytes; operand tiles in 128-byte swizzled rows
     static constexpr int kAlloc = kBytes + 1024;            // the tiles start on 1024 bytes
 };
 
+template <typename T>
+using Pair = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
+
 struct GroupScale {
     float ks, lv, iv, pad;
 };
@@ -259,32 +262,37 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const AttnArgs 
             // --- the query row: a power of two brings its largest element to [2^9, 2^10)
             float fac;
             {
+                // (held whole: one memory latency)
                 const T* q = static_cast<const T*>(a.q) + (walk.s.row0 + tok) * a.q_tok + head * a.q_head;
-                float top = 0.0f;
-                bool bad = false;
-                #pragma unroll 4
-                for (int d = 0; d < DP; d += 4) {
-                    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                    if (valid) load4(q + d, a.q_vec != 0, v);
+                Pair<T> x[DP / 2];
+                #pragma unroll
+                for (int d = 0; d < DP / 2; ++d) x[d].x = x[d].y = from_f32<T>(0.0f);
+                if (valid && a.q_vec != 0) {
                     #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        top = fmaxf(top, fabsf(v[j]));
-                        bad = bad || !(fabsf(v[j]) <= 3.4028234663852886e38f);
+                    for (int d = 0; d < DP / 2; d += 2) {
+                        *reinterpret_cast<uint2*>(&x[d]) = *reinterpret_cast<const uint2*>(q + 2 * d);
                     }
+                } else if (valid) {
+                    #pragma unroll
+                    for (int d = 0; d < DP / 2; ++d) x[d].x = q[2 * d], x[d].y = q[2 * d + 1];
                 }
+                Pair<T> most = __habs2(x[0]);
+                #pragma unroll
+                for (int d = 1; d < DP / 2; ++d) most = __hmax2_nan(most, __habs2(x[d]));
+                const T largest_q = __hmax_nan(most.x, most.y);
+                const float top = to_f32(largest_q);
+                const bool bad = !(top <= 3.4028234663852886e38f);
                 const int e = max(-126, min(120, 9 + 127 - static_cast<int>(__float_as_uint(top) >> 23)));
                 const float up = bad ? 0.0f : __int_as_float((127 + e) << 23);
                 const uint32_t base = smem + L::kQ + m * L::kQTile + row * 128;
-                #pragma unroll 4
+                #pragma unroll
                 for (int d = 0; d < DP; d += 8) {
-                    float v[8] = {};
-                    if (valid && !bad) {
-                        load4(q + d, a.q_vec != 0, reinterpret_cast<float(&)[4]>(v[0]));
-                        load4(q + d + 4, a.q_vec != 0, reinterpret_cast<float(&)[4]>(v[4]));
-                    }
                     uint32_t w[4];
                     #pragma unroll
-                    for (int j = 0; j < 4; ++j) w[j] = pack_f16(v[2 * j] * up, v[2 * j + 1] * up);
+                    for (int j = 0; j < 4; ++j) {
+                        const Pair<T> v = x[d / 2 + j];
+                        w[j] = bad ? 0u : pack_f16(to_f32(v.x) * up, to_f32(v.y) * up);
+                    }
                     store_shared16(base + (d / 64) * (kTile * 128) + ((((d % 64) / 8) ^ (row & 7)) << 4), w);
                 }
                 fac = bad ? __int_as_float(0x7fffffff) : __int_as_float((127 - e) << 23) * a.scale_log2;
@@ -647,8 +655,9 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const AttnArgs 
     }
 }
 
-// Joins the partial results of split tasks: a warp takes one row at a time,
-// one entry's rows over eight blocks.
+// Joins the partial results of split tasks. The rows of an entry are shared
+// out over gridDim.y blocks, a warp takes one row at a time. 32 parts at a time:
+// first their maxima and denominators, a lane each, then their sums.
 template <typename T, int DP>
 __global__ void __launch_bounds__(256) kv_prompt_join_kernel(const AttnArgs a) {
     pdl_launch_dependents();
@@ -660,26 +669,41 @@ __global__ void __launch_bounds__(256) kv_prompt_join_kernel(const AttnArgs a) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int h = task % a.heads, count = e.x + 1;
     constexpr int PER = DP / 32;  // elements of a lane
-    #pragma unroll 2
-    for (int i = 0; i < kRows / 64; ++i) {
-        const int r = blockIdx.y * (kRows / 8) + i * 8 + warp;
+    const int rows = kRows / gridDim.y;
+    #pragma unroll 1
+    for (int i = warp; i < rows; i += 8) {
+        const int r = blockIdx.y * rows + i;
         const int row = task / a.heads * kRows + r;
         if (row >= e.w * a.group) continue;
         const auto slot = [&](int c) { return static_cast<int64_t>(2 * (e.y + c) + (c == 0 ? 1 : 0)) * kRows + r; };
         float top = -INFINITY, den = 0.0f, sum[PER] = {};
-        for (int c = 0; c < count; ++c) top = fmaxf(top, a.ml[slot(c)].x);
-        for (int c = 0; c < count; ++c) {
-            const float2 ml = a.ml[slot(c)];
+        for (int c0 = 0; c0 < count; c0 += 32) {
+            const int n = min(32, count - c0);
+            const float2 ml = lane < n ? a.ml[slot(c0 + lane)] : make_float2(-INFINITY, 0.0f);
+            float now = fmaxf(top, ml.x);
+            #pragma unroll
+            for (int o = 16; o > 0; o >>= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, o));
+            if (c0 > 0) {
+                const float by = join_factor(top, now);
+                den *= by;
+                #pragma unroll
+                for (int j = 0; j < PER; ++j) sum[j] *= by;
+            }
+            top = now;
             const float f = join_factor(ml.x, top);
-            den = fmaf(ml.y, f, den);
-            const float* p = a.part + slot(c) * DP + PER * lane;
-            if constexpr (PER == 4) {
-                const float4 x = *reinterpret_cast<const float4*>(p);
-                sum[0] = fmaf(x.x, f, sum[0]), sum[1] = fmaf(x.y, f, sum[1]);
-                sum[2] = fmaf(x.z, f, sum[2]), sum[3] = fmaf(x.w, f, sum[3]);
-            } else {
-                const float2 x = *reinterpret_cast<const float2*>(p);
-                sum[0] = fmaf(x.x, f, sum[0]), sum[1] = fmaf(x.y, f, sum[1]);
+            #pragma unroll 8
+            for (int c = 0; c < n; ++c) {
+                const float fc = __shfl_sync(0xffffffffu, f, c);
+                den = fmaf(__shfl_sync(0xffffffffu, ml.y, c), fc, den);
+                const float* p = a.part + slot(c0 + c) * DP + PER * lane;
+                if constexpr (PER == 4) {
+                    const float4 x = *reinterpret_cast<const float4*>(p);
+                    sum[0] = fmaf(x.x, fc, sum[0]), sum[1] = fmaf(x.y, fc, sum[1]);
+                    sum[2] = fmaf(x.z, fc, sum[2]), sum[3] = fmaf(x.w, fc, sum[3]);
+                } else {
+                    const float2 x = *reinterpret_cast<const float2*>(p);
+                    sum[0] = fmaf(x.x, fc, sum[0]), sum[1] = fmaf(x.y, fc, sum[1]);
+                }
             }
         }
         const int tok = row / a.group, head = h * a.group + row - tok * a.group;
@@ -725,7 +749,8 @@ cudaError_t run_sized(AttnArgs a, void* ws, int64_t* ws_bytes, cudaStream_t stre
     cudaLaunchConfig_t cfg = pdl_config(dim3(static_cast<unsigned>(grid)), dim3(kPThreads), L::kAlloc, stream, attr);
     e = cudaLaunchKernelEx(&cfg, kv_prompt_kernel<T, DP>, a);
     if (e != cudaSuccess) return e;
-    cfg.gridDim = dim3(static_cast<unsigned>(a.entries), 8);
+    // As many blocks as fit at a time, a row to a warp where there are few entries.
+    cfg.gridDim = dim3(static_cast<unsigned>(a.entries), 8 * a.entries <= 2 * grid ? 32 : 8);
     cfg.blockDim = dim3(256);
     cfg.dynamicSmemBytes = 0;
     return cudaLaunchKernelEx(&cfg, kv_prompt_join_kernel<T, DP>, a);

@@ -39,6 +39,8 @@
 // kv_prompt.cu where it takes their type and dim.
 #include <type_traits>
 
+#include <algorithm>
+
 #include "kv_attention.cuh"
 #include "mma_frag.cuh"
 
@@ -764,13 +766,17 @@ cudaError_t run_rows_typed(popcornType_t type, const AttnArgs& a, int64_t max_to
 }
 
 // Launches the kernel, or the two, that the sizes ask for; with ws_bytes only
-// says how much workspace they take. Sequences of up to 16 query rows go to
-// kv_rows_kernel and longer ones to the prompt kernel, each of which skips the
-// other's; where all sequences have max_tokens queries only one is launched.
+// says how much workspace they take, for any block table if a.table_pages is 0.
+// Sequences of less than kPromptRows query rows go to kv_rows_kernel and others
+// to the prompt kernel, each of which skips the other's; where all sequences have
+// max_tokens queries only one is launched, and in small calls kv_rows_kernel
+// takes them all.
 cudaError_t run_typed(popcornType_t type, AttnArgs a, int64_t max_tokens, void* ws, int64_t* ws_bytes,
                       cudaStream_t stream) {
     a.min_rows = 1, a.max_rows = INT32_MAX;
-    if (max_tokens * a.group < kPromptRows || !prompt_supported(type, a.dim)) {
+    const int64_t tasks = a.heads * (static_cast<int64_t>(a.tokens) * a.group / 16 + a.seqs);
+    const bool small = tasks <= device_sm_count() && tasks * (a.table_pages << a.page_shift) <= kFewTokens;
+    if (max_tokens * a.group < kPromptRows || !prompt_supported(type, a.dim) || (small && a.table_pages > 0)) {
         return run_rows_typed(type, a, max_tokens, ws, ws_bytes, stream);
     }
     const bool both = a.tokens != max_tokens * a.seqs;
@@ -778,12 +784,13 @@ cudaError_t run_typed(popcornType_t type, AttnArgs a, int64_t max_tokens, void* 
     AttnArgs rows = a;
     rows.max_rows = kPromptRows - 1;
     a.min_rows = kPromptRows;
-    int64_t bytes = 0, more = 0;
     cudaError_t e = cudaSuccess;
     if (ws_bytes != nullptr) {
-        e = run_prompt(type, a, nullptr, &bytes, stream);
-        if (e == cudaSuccess && both && few > 0) e = run_rows_typed(type, rows, few, nullptr, &more, stream);
-        *ws_bytes = bytes > more ? bytes : more;
+        int64_t prompt = 0, beside = 0, alone = 0;
+        e = run_prompt(type, a, nullptr, &prompt, stream);
+        if (e == cudaSuccess && both && few > 0) e = run_rows_typed(type, rows, few, nullptr, &beside, stream);
+        if (e == cudaSuccess && small) e = run_rows_typed(type, rows, max_tokens, nullptr, &alone, stream);
+        *ws_bytes = std::max({prompt, beside, alone});
         return e;
     }
     e = run_prompt(type, a, ws, nullptr, stream);

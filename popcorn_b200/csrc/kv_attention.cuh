@@ -42,9 +42,17 @@ struct AttnArgs {
 };
 
 // The kernel for many query rows of one sequence (16-bit types, dim 64 or
-// 128): from this many on it is the faster one. Launches, or says how many
-// bytes of workspace it takes.
-constexpr int kPromptRows = 17;
+// 128): from this many on it is the faster one (bf16, dim 128, 8 key heads, 32
+// and 48 rows, it against kv_rows_kernel: 99 and 100 us against 73 and 102 for 4
+// sequences of 16,000 tokens, 112 and 113 against 82 and 115 for 32 of 2000)
+// unless the whole call is small (kFewTokens). Launches, or says how many bytes
+// of workspace it takes.
+constexpr int kPromptRows = 48;
+// A call is small where its rows make no more tasks of kv_rows_kernel than there
+// are SMs, and these have no more than this many tokens together, by the size of
+// the block table: 8 heads, 96 rows of one sequence: 20 us against 24 over 2000
+// tokens, 53 against 42 over 16,000 (768,000 together).
+constexpr int64_t kFewTokens = 1 << 19;
 bool prompt_supported(popcornType_t type, int64_t dim);
 cudaError_t run_prompt(popcornType_t type, const AttnArgs& a, void* ws, int64_t* ws_bytes, cudaStream_t stream);
 cudaError_t kv_prompt_take_errors(unsigned int* bits);

@@ -554,3 +554,43 @@ def test_python_refusals(cuda):
         with pytest.raises(ValueError, match="kv_read"):
             pc.kv_read(cache, **kw)
     assert pc.kv_read(cache, pages[:0])[0].shape == (0, 2, 16, 64)
+
+
+PROMPTS = [
+    # heads, group, dim, page, lengths, queries, causal, window
+    (1, 1, 64, 16, [300], [257], True, 0),
+    (2, 1, 128, 32, [130, 48, 5], [47, 48, 5], True, 0),            # rows on both sides of the kernels' border
+    (2, 4, 128, 16, [700, 90, 12, 0], [100, 12, 1, 0], True, 0),
+    (1, 8, 128, 64, [2000], [70], True, 0),
+    (3, 5, 64, 16, [31, 200, 0, 2], [40, 9, 20, 3], True, 0),       # more queries than tokens: rows that see nothing
+    (2, 4, 64, 16, [333, 1000], [50, 130], True, 64),
+    (2, 3, 128, 128, [200, 650], [70, 65], True, 1),
+    (1, 2, 128, 16, [150, 129], [50, 129], False, 30),
+    (1, 3, 64, 32, [777, 130], [20, 300], False, 0),
+    (4, 2, 128, 256, [1025, 511], [256, 1], True, 0),
+]
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("case", range(len(PROMPTS)))
+def test_prompts_against_64_bits(cuda, kind, wide, case):
+    """Small calls, and the same ones with a block table that could hold long sequences."""
+    torch = _torch()
+    heads, group, dim, page, length, new, causal, window = PROMPTS[case]
+    rng = _rng("prompts", case)
+    table, pages = _pages(rng, [(n + page - 1) // page for n in length])
+    c = Cache(rng, pages, heads, page, dim, cuda)
+    if wide:
+        table = np.concatenate([table, np.full((len(length), (1 << 19) // page), -9, np.int32)], 1)
+    q = _cast(rng.standard_normal((sum(new), heads * group, dim)) * 1.5, kind)
+    up = lambda a: torch.from_numpy(np.ascontiguousarray(a)).to(cuda)  # noqa: E731
+    lse = torch.zeros((sum(new), heads * group), device=cuda)
+    call = lambda most, lse=None: pc.kv_attention(c.dev, q.to(cuda), up(table), up(np.int32(length)),  # noqa: E731
+                                                  first=up(_first(new)), max_tokens=most, causal=causal,
+                                                  window=window, lse=lse)
+    got = call(max(new), lse)
+    assert torch.equal(got, call(max(new)))
+    assert pc.device_errors() == 0
+    _check(c, _f32(q).astype(np.float64), _f32(got).astype(np.float64), lse.cpu().numpy().astype(np.float64), table, length, new,
+           group, causal, window, dim ** -0.5, kind)

@@ -23,6 +23,7 @@
 // hidden values' one for each 32 rows that an item covers: columns
 // 64 w + 16 t + 8 s + i (t < 4, i < 8), which are the columns of step s of
 // window w in the next product.
+#include <algorithm>
 #include <cmath>
 
 #include "common.cuh"
@@ -33,6 +34,7 @@ namespace pcb {
 namespace {
 
 constexpr int kDownWarps = 16, kDownThreads = 32 * kDownWarps;
+constexpr int kDownShared = 208 * 1024;  // dynamic shared memory beside the routing lists
 constexpr int kMoeThreads = 256;
 constexpr int kMoeWarps = kMoeThreads / 32;
 constexpr int kWindows = 4;       // windows of a stage: 256 columns of 16 rows
@@ -360,22 +362,25 @@ __device__ __forceinline__ uint4 load_shared16(uint32_t addr) {
     return v;
 }
 
-// One stage: this lane's pieces of two rows (of `bytes0`, `bytes1` = 16, or 0
-// for rows that are not there) from column `col` on, zeros past `end`.
-__device__ __forceinline__ void copy_stage(uint32_t dst, const int8_t* row0, const int8_t* row1, int bytes0, int bytes1,
+// One stage: this lane's pieces of its rows, one of every eight (of `bytes` 16,
+// or 0 for rows that are not there), from column `col` on, zeros past `end`.
+template <int GROUPS, int WIDE>
+__device__ __forceinline__ void copy_stage(uint32_t dst, const int8_t* const (&rows)[GROUPS], const int (&bytes)[GROUPS],
                                            int col, int t, int end) {
-    if (col + kColumns <= end) {
+    if (col + 64 * WIDE <= end) {
         #pragma unroll
-        for (int k = 0; k < kWindows; ++k) {
-            cp_async16(dst + 1024 * k, row0 + col + 64 * k, bytes0);
-            cp_async16(dst + 1024 * k + 512, row1 + col + 64 * k, bytes1);
+        for (int k = 0; k < WIDE; ++k) {
+            #pragma unroll
+            for (int i = 0; i < GROUPS; ++i) cp_async16(dst + 512 * (GROUPS * k + i), rows[i] + col + 64 * k, bytes[i]);
         }
     } else {
         #pragma unroll
-        for (int k = 0; k < kWindows; ++k) {
+        for (int k = 0; k < WIDE; ++k) {
             const bool in = col + 64 * k + 16 * t < end;
-            cp_async16(dst + 1024 * k, row0 + (in ? col + 64 * k : 0), in ? bytes0 : 0);
-            cp_async16(dst + 1024 * k + 512, row1 + (in ? col + 64 * k : 0), in ? bytes1 : 0);
+            #pragma unroll
+            for (int i = 0; i < GROUPS; ++i) {
+                cp_async16(dst + 512 * (GROUPS * k + i), rows[i] + (in ? col + 64 * k : 0), in ? bytes[i] : 0);
+            }
         }
     }
 }
@@ -405,17 +410,18 @@ __global__ void __launch_bounds__(kUpWorkers* kUpThreads, 1) up_kernel(const Moe
 
     // The copying side: item, stage of it and this lane's rows g and g + 8.
     int c_item = first, c_s = 0, c_slot = 0;
-    const int8_t *row0 = nullptr, *row1 = nullptr;
+    const int8_t* rows[2] = {};
+    const int bytes[2] = {16, 16};
     const auto rows_of = [&](int item) {
         const int h = item % halves;
         const int f = h / 2 * 64 + 32 * (warp & 1) + 8 * (h & 1) + g;
         const int64_t at = static_cast<int64_t>(job_of(r, item / halves).expert) * a.F;
-        row0 = codes + (at + min(f, a.F - 1)) * a.K;
-        row1 = codes + (at + min(f + 16, a.F - 1)) * a.K;
+        rows[0] = codes + (at + min(f, a.F - 1)) * a.K;
+        rows[1] = codes + (at + min(f + 16, a.F - 1)) * a.K;
     };
     const auto copy_next = [&] {
         if (c_item < items) {
-            copy_stage(ring + c_slot * kStageBytes, row0, row1, 16, 16, c_s * kColumns, t, a.K);
+            copy_stage<2, kWindows>(ring + c_slot * kStageBytes, rows, bytes, c_s * kColumns, t, a.K);
             if (++c_s == stages) {
                 c_s = 0;
                 c_item += stride;
@@ -509,24 +515,44 @@ __global__ void __launch_bounds__(kUpWorkers* kUpThreads, 1) up_kernel(const Moe
 }
 
 // -------------------------------------------------------------------- down
-// A block is an SM's whole load, 16 warps, and owns `rows` (at most 16, the M
-// side) output channels at a time: 14 for 2048 channels, twice 14 for 4096. Its
-// warps share the (job, stage) list of a tile in equal runs, so that no other
-// block is needed for a token's sum over its experts; they stream it, from one
-// tile into the next, through rings in shared memory. A step's exact integer sums join in f32 with the step's unit. At the
-// end of a job a warp adds its result, weighted, to its own sums per token; the
-// warps' are added in order at the end of the tile.
-constexpr int down_stages(int tokens) { return tokens <= 16 ? 3 : 2; }  // what the sums leave room for
+// A block is an SM's whole load, 16 warps, and owns `rows` (at most 8 GROUPS)
+// output channels at a time: 14 for 2048 channels, 18 for 2560. Its warps share
+// the (job, stage) list of a tile in equal runs, so that no other block is needed
+// for a token's sum over its experts; they stream it, from one tile into the
+// next, through rings in shared memory. A step's exact integer sums join in f32
+// with the step's unit. At the end of a job a warp adds its result, weighted, to
+// its own sums per token; the warps' are added in order at the end of the tile.
+//
+// Every tile reads all digits of the hidden values (4 bytes a value, from L2), so
+// with several tokens to an expert a tile has up to 32 rows, two M sides that
+// share them: 2560 channels as 18 rows a tile instead of twice 9 took 55 us
+// instead of 71 (24 picks among 24 experts of 5056), 197 instead of 380 (25
+// tokens that all pick all 8 experts of 6448), 4096 as 28 instead of twice 14 43
+// instead of 49 (72 picks among 64 of 1088). One token's are few: it stays with
+// the 16-row tiles, whose copies take 256 bytes of a row at a time.
+template <int NP, int GROUPS>
+struct Down {
+    static constexpr int kRows = 8 * GROUPS;
+    static constexpr int kTiles = (GROUPS + 1) / 2;           // M sides
+    static constexpr int kWide = GROUPS == 2 && NP < 4 ? 4 : 2;  // windows of a stage, what registers allow
+    static constexpr int kCols = 64 * kWide;
+    static constexpr int kBytes = 512 * GROUPS * kWide;       // of a stage: [window][row][64 bytes]
+    static constexpr int bytes(int stages, int tokens) {      // of shared memory
+        return kDownWarps * (stages * kBytes + tokens * kRows * static_cast<int>(sizeof(float)));
+    }
+};
 
-template <int NP, int STAGES>
+template <int NP, int GROUPS, int STAGES>
 __global__ void __launch_bounds__(kDownThreads, 1) down_kernel(const MoeArgs a) {
+    using D = Down<NP, GROUPS>;
+    constexpr int TILES = D::kTiles, WIDE = D::kWide, ROWS = D::kRows;
     extern __shared__ __align__(128) uint8_t s_raw[];
-    float* const outs = reinterpret_cast<float*>(s_raw + kDownWarps * STAGES * kStageBytes);  // [warp][token][16]
+    float* const outs = reinterpret_cast<float*>(s_raw + kDownWarps * STAGES * D::kBytes);  // [warp][token][ROWS]
     __shared__ Routing r;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = lane >> 2, t = lane & 3;
     pdl_launch_dependents();
-    for (int i = tid; i < kDownWarps * a.M * 16; i += kDownThreads) outs[i] = 0.0f;
+    for (int i = tid; i < kDownWarps * a.M * ROWS; i += kDownThreads) outs[i] = 0.0f;
     pdl_wait();
     for (int i = tid; i < a.M * a.top; i += kDownThreads) {
         r.pick[i] = static_cast<short>(a.experts[i]);
@@ -535,28 +561,28 @@ __global__ void __launch_bounds__(kDownThreads, 1) down_kernel(const MoeArgs a) 
     __syncthreads();
     list_jobs<NP, kDownThreads>(a, r);
 
-    const int stages = a.fp / kColumns, tiles = (a.K + a.rows - 1) / a.rows;
-    const int units = r.jobs * stages;  // under 2^18
+    const int stages = a.fp / D::kCols, tiles = (a.K + a.rows - 1) / a.rows;
+    const int units = r.jobs * stages;  // under 2^19
     const int u_begin = units * warp / kDownWarps, u_end = units * (warp + 1) / kDownWarps;
-    const uint32_t ring =
-        static_cast<uint32_t>(__cvta_generic_to_shared(s_raw)) + warp * STAGES * kStageBytes + 16 * lane;
-    float* const mine = outs + warp * a.M * 16;
+    const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(s_raw)) + warp * STAGES * D::kBytes + 16 * lane;
+    float* const mine = outs + warp * a.M * ROWS;
 
-    // The copying side: tile, job, stage of it, this lane's rows g and g + 8.
+    // The copying side: tile, job, stage of it, this lane's rows g, g + 8, ...
     int c_tile = blockIdx.x, c_left = u_end - u_begin, c_job = u_begin / stages, c_s = u_begin % stages, c_slot = 0;
-    int bytes0 = 0, bytes1 = 0;
-    const int8_t *row0 = nullptr, *row1 = nullptr;
+    int bytes[GROUPS] = {};
+    const int8_t* rows[GROUPS] = {};
     const auto rows_of = [&] {
         const int n0 = c_tile * a.rows, n_end = min(a.K, n0 + a.rows);
         const int64_t at = static_cast<int64_t>(job_of(r, c_job).expert) * a.K;
-        bytes0 = n0 + g < n_end ? 16 : 0;
-        bytes1 = n0 + 8 + g < n_end ? 16 : 0;
-        row0 = a.qd + (at + min(n0 + g, a.K - 1)) * a.F + 16 * t;
-        row1 = a.qd + (at + min(n0 + 8 + g, a.K - 1)) * a.F + 16 * t;
+        #pragma unroll
+        for (int i = 0; i < GROUPS; ++i) {
+            bytes[i] = n0 + 8 * i + g < n_end ? 16 : 0;
+            rows[i] = a.qd + (at + min(n0 + 8 * i + g, a.K - 1)) * a.F + 16 * t;
+        }
     };
     const auto copy_next = [&] {
         if (c_left > 0) {
-            copy_stage(ring + c_slot * kStageBytes, row0, row1, bytes0, bytes1, c_s * kColumns, t, a.F);
+            copy_stage<GROUPS, WIDE>(ring + c_slot * D::kBytes, rows, bytes, c_s * D::kCols, t, a.F);
             --c_left;
             ++c_s;
             if (c_left == 0) {
@@ -584,11 +610,6 @@ __global__ void __launch_bounds__(kDownThreads, 1) down_kernel(const MoeArgs a) 
             const Job job = job_of(r, u / stages);
             const int s_end = min(stages, s_begin + (u_end - u));
             u += s_end - s_begin;
-            float scale[2];
-            #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                scale[j] = a.sd[static_cast<int64_t>(job.expert) * a.K + min(n0 + 8 * j + g, n_end - 1)];
-            }
             // This lane's column of the B operand, and the token of its result
             // columns (columns of tokens that the job does not have are not used).
             const int8_t* hd[NP];
@@ -599,81 +620,88 @@ __global__ void __launch_bounds__(kDownThreads, 1) down_kernel(const MoeArgs a) 
                 hd[n] = a.hd + (static_cast<int64_t>(r.pair[job.pos + j]) * 4 + (g & 3)) * a.fp + 16 * t;
                 hs[n] = a.hs + static_cast<int64_t>(r.pair[job.pos + jr]) * (a.fp / 32);
             }
-            uint4 b[kWindows][NP];
-            float2 unit[kWindows][NP];
+            float scale[GROUPS];
+            #pragma unroll
+            for (int i = 0; i < GROUPS; ++i) {
+                scale[i] = a.sd[static_cast<int64_t>(job.expert) * a.K + min(n0 + 8 * i + g, n_end - 1)];
+            }
+            uint4 b[WIDE][NP];
+            float2 unit[WIDE][NP];
             const auto load_b = [&](int st) {
                 #pragma unroll
                 for (int n = 0; n < NP; ++n) {
                     #pragma unroll
-                    for (int k = 0; k < kWindows; ++k) {
-                        b[k][n] = *reinterpret_cast<const uint4*>(hd[n] + kColumns * st + 64 * k);
+                    for (int k = 0; k < WIDE; ++k) {
+                        b[k][n] = *reinterpret_cast<const uint4*>(hd[n] + D::kCols * st + 64 * k);
                     }
                     #pragma unroll
-                    for (int k = 0; k < kWindows; k += 2) {
-                        const float4 x = *reinterpret_cast<const float4*>(hs[n] + 2 * kWindows * st + 2 * k);
+                    for (int k = 0; k < WIDE; k += 2) {
+                        const float4 x = *reinterpret_cast<const float4*>(hs[n] + 2 * WIDE * st + 2 * k);
                         unit[k][n] = make_float2(x.x, x.y), unit[k + 1][n] = make_float2(x.z, x.w);
                     }
                 }
             };
             if (NP == 1) load_b(s_begin);
-            float2 acc2[NP][2] = {};
+            float2 acc2[TILES][NP][2] = {};
             for (int st = s_begin; st < s_end; ++st) {
                 if (NP > 1) load_b(st);  // (too many registers to hold a stage ahead)
                 cp_async_wait_group<STAGES - 2>();
                 __syncwarp();
                 copy_next();
-                const uint32_t at = ring + slot * kStageBytes;
+                const uint32_t at = ring + slot * D::kBytes;
                 slot = slot == STAGES - 1 ? 0 : slot + 1;
                 #pragma unroll
-                for (int k = 0; k < kWindows; ++k) {
-                    const uint4 q0 = load_shared16(at + 1024 * k), q1 = load_shared16(at + 1024 * k + 512);
-                    const uint32_t lo[4] = {q0.x, q1.x, q0.y, q1.y}, hi[4] = {q0.z, q1.z, q0.w, q1.w};
+                for (int k = 0; k < WIDE; ++k) {
                     #pragma unroll
-                    for (int n = 0; n < NP; ++n) {
-                        int d[2][4];
-                        mma_s8_16832_from(d[0], lo, b[k][n].x, b[k][n].y, kMagicBits);
-                        mma_s8_16832_from(d[1], hi, b[k][n].z, b[k][n].w, kMagicBits);
+                    for (int i = 0; i < TILES; ++i) {
+                        const uint32_t from = at + 512 * (GROUPS * k + 2 * i);
+                        const uint4 q0 = load_shared16(from);
+                        const uint4 q1 = 2 * i + 1 < GROUPS ? load_shared16(from + 512) : make_uint4(0, 0, 0, 0);
+                        const uint32_t lo[4] = {q0.x, q1.x, q0.y, q1.y}, hi[4] = {q0.z, q1.z, q0.w, q1.w};
                         #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const float by = h == 0 ? unit[k][n].x : unit[k][n].y;
+                        for (int n = 0; n < NP; ++n) {
+                            int d[2][4];
+                            mma_s8_16832_from(d[0], lo, b[k][n].x, b[k][n].y, kMagicBits);
+                            mma_s8_16832_from(d[1], hi, b[k][n].z, b[k][n].w, kMagicBits);
                             #pragma unroll
-                            for (int c = 0; c < 2; ++c) {
-                                const float2 x = __fadd2_rn(make_float2(__int_as_float(d[h][2 * c]), __int_as_float(d[h][2 * c + 1])),
-                                                            make_float2(-kMagic, -kMagic));
-                                acc2[n][c] = __ffma2_rn(x, make_float2(by, by), acc2[n][c]);
+                            for (int h = 0; h < 2; ++h) {
+                                const float by = h == 0 ? unit[k][n].x : unit[k][n].y;
+                                #pragma unroll
+                                for (int c = 0; c < 2; ++c) {
+                                    if (2 * i + c >= GROUPS) continue;
+                                    const float2 x = __fadd2_rn(make_float2(__int_as_float(d[h][2 * c]), __int_as_float(d[h][2 * c + 1])),
+                                                                make_float2(-kMagic, -kMagic));
+                                    acc2[i][n][c] = __ffma2_rn(x, make_float2(by, by), acc2[i][n][c]);
+                                }
                             }
                         }
                     }
                 }
                 if (NP == 1 && st + 1 < s_end) load_b(st + 1);
             }
-            float acc[NP][4];
-            #pragma unroll
-            for (int n = 0; n < NP; ++n) {
-                acc[n][0] = acc2[n][0].x, acc[n][1] = acc2[n][0].y, acc[n][2] = acc2[n][1].x, acc[n][3] = acc2[n][1].y;
-            }
             #pragma unroll
             for (int n = 0; n < NP; ++n) {
                 // Lane (g, t) has digits 2 (t % 2) and 2 (t % 2) + 1 of token t / 2.
                 const int j = 2 * n + (t >> 1);
                 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    float v = fmaf(acc[n][2 * i + 1], 256.0f, acc[n][2 * i]);
+                for (int i = 0; i < GROUPS; ++i) {
+                    const float2 d = acc2[i / 2][n][i % 2];
+                    float v = fmaf(d.y, 256.0f, d.x);
                     v = fmaf(__shfl_xor_sync(0xffffffffu, v, 1), (t & 1) ? 0.0f : 65536.0f, v);
                     if (j < job.count && !(t & 1)) {
-                        mine[r.token[job.pos + j] * 16 + 8 * i + g] += v * scale[i] * r.weight[r.pair[job.pos + j]];
+                        mine[r.token[job.pos + j] * ROWS + 8 * i + g] += v * scale[i] * r.weight[r.pair[job.pos + j]];
                     }
                 }
             }
         }
         __syncthreads();
-        for (int i = tid; i < a.M * 16; i += kDownThreads) {
-            const int m = i / 16, n = n0 + i % 16;
+        for (int i = tid; i < a.M * ROWS; i += kDownThreads) {
+            const int m = i / ROWS, n = n0 + i % ROWS;
             float v = 0.0f;
             #pragma unroll
             for (int w = 0; w < kDownWarps; ++w) {
-                v += outs[w * a.M * 16 + i];
-                outs[w * a.M * 16 + i] = 0.0f;
+                v += outs[w * a.M * ROWS + i];
+                outs[w * a.M * ROWS + i] = 0.0f;
             }
             if (n < n_end) a.out[static_cast<int64_t>(m) * a.K + n] = v;
         }
@@ -767,34 +795,70 @@ int64_t lay_out(MoeArgs& a, char* ws, int64_t M, bool tensor, bool own_picks) {
     return at;
 }
 
-template <int NP, int STAGES>
+// Lets a kernel have that much shared memory, once for each device and size.
+template <class Kernel>
+cudaError_t allow_shared(Kernel kernel, int bytes, int (&allowed)[64]) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 64 && __atomic_load_n(&allowed[dev], __ATOMIC_RELAXED) >= bytes) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && dev < 64) __atomic_store_n(&allowed[dev], bytes, __ATOMIC_RELAXED);
+    return e;
+}
+
+template <int NP, int GROUPS, int STAGES>
 cudaError_t run_down(const MoeArgs& a, int blocks, cudaStream_t stream) {
-    const int bytes = kDownWarps * (STAGES * kStageBytes + a.M * 16 * static_cast<int>(sizeof(float)));
-    const cudaError_t e =
-        cudaFuncSetAttribute(down_kernel<NP, STAGES>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    const int bytes = Down<NP, GROUPS>::bytes(STAGES, a.M);
+    static int allowed[64] = {};  // per device
+    const cudaError_t e = allow_shared(down_kernel<NP, GROUPS, STAGES>, bytes, allowed);
     if (e != cudaSuccess) return e;
     cudaLaunchAttribute attr[1];
     const cudaLaunchConfig_t cfg =
         pdl_config(dim3(static_cast<unsigned>(blocks)), dim3(kDownThreads), static_cast<size_t>(bytes), stream, attr);
-    return cudaLaunchKernelEx(&cfg, down_kernel<NP, STAGES>, a);
+    return cudaLaunchKernelEx(&cfg, down_kernel<NP, GROUPS, STAGES>, a);
+}
+
+// As many tiles for every SM, as few as `most` rows a tile allow.
+int tile_rows(int K, int most, int64_t sms) { return static_cast<int>(ceil_div(K, ceil_div(K, most * sms) * sms)); }
+
+template <int NP>
+cudaError_t run_down_sized(MoeArgs a, cudaStream_t stream) {
+    const int64_t sms = device_sm_count();
+    a.rows = tile_rows(a.K, 16, sms);
+    const auto blocks = [&] { return static_cast<int>(std::min(ceil_div(a.K, a.rows), sms)); };
+    if constexpr (NP > 1) {
+        const int rows = tile_rows(a.K, 32, sms);
+        MoeArgs wide = a;
+        wide.rows = rows;
+        const int at = static_cast<int>(std::min(ceil_div(a.K, rows), sms));
+        if (rows > 24 && Down<NP, 4>::bytes(2, a.M) <= kDownShared) {
+            return Down<NP, 4>::bytes(3, a.M) <= kDownShared ? run_down<NP, 4, 3>(wide, at, stream)
+                                                         : run_down<NP, 4, 2>(wide, at, stream);
+        }
+        if (rows > 16 && rows <= 24 && Down<NP, 3>::bytes(3, a.M) <= kDownShared) {
+            return Down<NP, 3>::bytes(4, a.M) <= kDownShared ? run_down<NP, 3, 4>(wide, at, stream)
+                                                         : run_down<NP, 3, 3>(wide, at, stream);
+        }
+    }
+    constexpr int HALF = Down<NP, 2>::kWide == 4 ? 1 : 2;  // stages of half the size
+    return Down<NP, 2>::bytes(3 * HALF, a.M) <= kDownShared ? run_down<NP, 2, 3 * HALF>(a, blocks(), stream)
+                                                            : run_down<NP, 2, 2 * HALF>(a, blocks(), stream);
 }
 
 template <int NP>
 cudaError_t run_tensor(MoeArgs a, cudaStream_t stream) {
     const int64_t sms = device_sm_count();
-    cudaError_t e = cudaFuncSetAttribute(up_kernel<NP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Up<NP>::kBytes);
+    static int allowed[64] = {};  // per device
+    cudaError_t e = allow_shared(up_kernel<NP>, Up<NP>::kBytes, allowed);
     if (e != cudaSuccess) return e;
     cudaLaunchAttribute attr[1];
-    // Down: as many tiles for every SM, as few as 16 rows allow.
-    a.rows = static_cast<int>(ceil_div(a.K, ceil_div(a.K, 16 * sms) * sms));
     const int64_t items = static_cast<int64_t>(a.M) * a.top * ((a.F + 63) / 64 * 2);  // at most
     const cudaLaunchConfig_t cfg = pdl_config(dim3(static_cast<unsigned>(items < sms ? items : sms)),
                                               dim3(kUpWorkers * kUpThreads), Up<NP>::kBytes, stream, attr);
     e = cudaLaunchKernelEx(&cfg, up_kernel<NP>, a);
     if (e != cudaSuccess) return e;
-    const int64_t tiles = ceil_div(a.K, a.rows);
-    const int blocks = static_cast<int>(tiles < sms ? tiles : sms);
-    return down_stages(a.M) == 3 ? run_down<NP, 3>(a, blocks, stream) : run_down<NP, 2>(a, blocks, stream);
+    return run_down_sized<NP>(a, stream);
 }
 
 cudaError_t run_pass(const MoeArgs& a, bool tensor, cudaStream_t stream) {

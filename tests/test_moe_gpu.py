@@ -199,3 +199,19 @@ def test_moe_refusals(cuda):
             pc.moe(*args, top_k=top)
     with pytest.raises(ValueError):
         pc.moe(*args, top_k=2, out=torch.zeros((2, 63), device=cuda))
+
+
+@pytest.mark.parametrize("M, K, F, E, top", [
+    # wide hidden sizes: more than 16 output channels to an SM, by tokens of a pass and tokens of an expert
+    (3, 2560, 272, 4, 2), (8, 2560, 48, 16, 2), (12, 2560, 80, 3, 2), (33, 2560, 64, 4, 2), (57, 2544, 32, 30, 1),
+    (2, 4096, 80, 4, 2), (3, 4096, 320, 4, 2), (9, 4096, 64, 8, 1), (20, 4096, 64, 4, 3), (41, 4096, 48, 2, 1),
+    (60, 4096, 48, 8, 4), (5, 5120, 48, 4, 2), (64, 5120, 32, 64, 2), (6, 9488, 32, 2, 1),
+])
+def test_moe_wide_hidden_sizes(cuda, M, K, F, E, top):
+    layer = _layer(M, K, F, E, 900 + M)
+    want, tol, experts, weights, dz = _reference(layer, top, True)
+    out, got_experts, got_weights = _call(layer, top, True, cuda)
+    np.testing.assert_array_equal(got_experts, experts)
+    assert (np.abs(got_weights - weights) <= (4 * dz.max(1, keepdims=True) + 2.0 ** -20) * weights).all()
+    assert (np.abs(out - want) <= tol).all(), (np.abs(out - want) / tol).max()
+    np.testing.assert_array_equal(_call(layer, top, True, cuda, routing=False), out)

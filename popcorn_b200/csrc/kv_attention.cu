@@ -37,9 +37,8 @@
 //
 // Sequences with more query rows than one tile of 16 go to the kernel of
 // kv_prompt.cu where it takes their type and dim.
-#include <type_traits>
-
 #include <algorithm>
+#include <type_traits>
 
 #include "kv_attention.cuh"
 #include "mma_frag.cuh"
@@ -866,8 +865,11 @@ extern "C" popcornStatus_t popcornKvAttention(void* out, float* lse, const void*
     const int64_t four = 4 * pcb::kv_type_size(type);
     a.q_vec = reinterpret_cast<uintptr_t>(q) % four == 0 && q_token_stride % 4 == 0 && q_head_stride % 4 == 0;
 
+    // A caller's workspace has the size that the query gives, for any block table.
     int64_t need = 0;
-    cudaError_t e = pcb::run_typed(type, a, max_tokens, nullptr, &need, stream);
+    pcb::AttnArgs sizes = a;
+    if (workspace != nullptr) sizes.table_pages = 0;
+    cudaError_t e = pcb::run_typed(type, sizes, max_tokens, nullptr, &need, stream);
     if (e != cudaSuccess) return pcb::record_cuda(e);
     void* ws = workspace;
     if (workspace == nullptr) {

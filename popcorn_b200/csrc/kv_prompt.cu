@@ -655,10 +655,11 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const AttnArgs 
     }
 }
 
-// Joins the partial results of split tasks. The rows of an entry are shared
-// out over gridDim.y blocks, a warp takes one row at a time. 32 parts at a time:
-// first their maxima and denominators, a lane each, then their sums.
-template <typename T, int DP>
+// Joins the partial results of split tasks, LANES lanes a row: 8 where there are
+// entries for all SMs (all their rows at a time, four to a warp; one after the
+// other they took 20 us of a 254 us prompt), 32 where there are few. LANES parts
+// at a time: first their maxima and denominators, a lane each, then their sums.
+template <typename T, int DP, int LANES>
 __global__ void __launch_bounds__(256) kv_prompt_join_kernel(const AttnArgs a) {
     pdl_launch_dependents();
     pdl_wait();
@@ -666,59 +667,62 @@ __global__ void __launch_bounds__(256) kv_prompt_join_kernel(const AttnArgs a) {
     const int4 e = a.entry[1 + 2 * blockIdx.x];
     const int task = a.entry[2 + 2 * blockIdx.x].x;
     if (static_cast<int>(blockIdx.x) >= entries || e.x == 0) return;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    constexpr int VEC = DP / LANES < 4 ? DP / LANES : 4, PIECES = DP / LANES / VEC;
+    using Piece = std::conditional_t<VEC == 4, float4, float2>;
+    const int l = threadIdx.x % LANES;
+    const int r = (blockIdx.y * 256 + threadIdx.x) / LANES;
     const int h = task % a.heads, count = e.x + 1;
-    constexpr int PER = DP / 32;  // elements of a lane
-    const int rows = kRows / gridDim.y;
-    #pragma unroll 1
-    for (int i = warp; i < rows; i += 8) {
-        const int r = blockIdx.y * rows + i;
-        const int row = task / a.heads * kRows + r;
-        if (row >= e.w * a.group) continue;
-        const auto slot = [&](int c) { return static_cast<int64_t>(2 * (e.y + c) + (c == 0 ? 1 : 0)) * kRows + r; };
-        float top = -INFINITY, den = 0.0f, sum[PER] = {};
-        for (int c0 = 0; c0 < count; c0 += 32) {
-            const int n = min(32, count - c0);
-            const float2 ml = lane < n ? a.ml[slot(c0 + lane)] : make_float2(-INFINITY, 0.0f);
-            float now = fmaxf(top, ml.x);
-            #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, o));
-            if (c0 > 0) {
-                const float by = join_factor(top, now);
-                den *= by;
-                #pragma unroll
-                for (int j = 0; j < PER; ++j) sum[j] *= by;
-            }
-            top = now;
-            const float f = join_factor(ml.x, top);
-            #pragma unroll 8
-            for (int c = 0; c < n; ++c) {
-                const float fc = __shfl_sync(0xffffffffu, f, c);
-                den = fmaf(__shfl_sync(0xffffffffu, ml.y, c), fc, den);
-                const float* p = a.part + slot(c0 + c) * DP + PER * lane;
-                if constexpr (PER == 4) {
-                    const float4 x = *reinterpret_cast<const float4*>(p);
-                    sum[0] = fmaf(x.x, fc, sum[0]), sum[1] = fmaf(x.y, fc, sum[1]);
-                    sum[2] = fmaf(x.z, fc, sum[2]), sum[3] = fmaf(x.w, fc, sum[3]);
-                } else {
-                    const float2 x = *reinterpret_cast<const float2*>(p);
-                    sum[0] = fmaf(x.x, fc, sum[0]), sum[1] = fmaf(x.y, fc, sum[1]);
-                }
-            }
-        }
-        const int tok = row / a.group, head = h * a.group + row - tok * a.group;
-        const float inv = inverse(den);
-        T* out = static_cast<T*>(a.out) + ((e.z + tok) * static_cast<int64_t>(a.heads * a.group) + head) * DP + PER * lane;
-        alignas(8) T o[PER];
+    const int row = task / a.heads * kRows + r;
+    const bool there = row < e.w * a.group;
+    const auto slot = [&](int c) { return static_cast<int64_t>(2 * (e.y + c) + (c == 0 ? 1 : 0)) * kRows + r; };
+    float top = -INFINITY, den = 0.0f, sum[PIECES][VEC] = {};
+    for (int c0 = 0; c0 < count; c0 += LANES) {
+        const int n = min(LANES, count - c0);
+        const float2 ml = there && l < n ? a.ml[slot(c0 + l)] : make_float2(-INFINITY, 0.0f);
+        float now = fmaxf(top, ml.x);
         #pragma unroll
-        for (int j = 0; j < PER; ++j) o[j] = from_f32<T>(sum[j] * inv);
-        if constexpr (PER == 4) {
-            *reinterpret_cast<uint2*>(out) = *reinterpret_cast<const uint2*>(o);
-        } else {
-            *reinterpret_cast<uint32_t*>(out) = *reinterpret_cast<const uint32_t*>(o);
+        for (int o = LANES / 2; o > 0; o >>= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, o));
+        if (c0 > 0) {
+            const float by = join_factor(top, now);
+            den *= by;
+            #pragma unroll
+            for (int i = 0; i < PIECES; ++i) {
+                #pragma unroll
+                for (int j = 0; j < VEC; ++j) sum[i][j] *= by;
+            }
         }
-        if (lane == 0) store_lse(a, e.z + tok, head, den, top);
+        top = now;
+        const float f = join_factor(ml.x, top);
+        #pragma unroll 4
+        for (int c = 0; c < n; ++c) {
+            const float fc = __shfl_sync(0xffffffffu, f, c, LANES);
+            den = fmaf(__shfl_sync(0xffffffffu, ml.y, c, LANES), fc, den);
+            if (!there) continue;
+            const float* p = a.part + slot(c0 + c) * DP + VEC * l;
+            #pragma unroll
+            for (int i = 0; i < PIECES; ++i) {
+                const Piece x = *reinterpret_cast<const Piece*>(p + LANES * VEC * i);
+                #pragma unroll
+                for (int j = 0; j < VEC; ++j) sum[i][j] = fmaf(reinterpret_cast<const float*>(&x)[j], fc, sum[i][j]);
+            }
+        }
     }
+    if (!there) return;
+    const int tok = row / a.group, head = h * a.group + row - tok * a.group;
+    const float inv = inverse(den);
+    T* out = static_cast<T*>(a.out) + ((e.z + tok) * static_cast<int64_t>(a.heads * a.group) + head) * DP + VEC * l;
+    #pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+        alignas(8) T o[VEC];
+        #pragma unroll
+        for (int j = 0; j < VEC; ++j) o[j] = from_f32<T>(sum[i][j] * inv);
+        if constexpr (VEC == 4) {
+            *reinterpret_cast<uint2*>(out + LANES * VEC * i) = *reinterpret_cast<const uint2*>(o);
+        } else {
+            *reinterpret_cast<uint32_t*>(out + LANES * VEC * i) = *reinterpret_cast<const uint32_t*>(o);
+        }
+    }
+    if (l == 0) store_lse(a, e.z + tok, head, den, top);
 }
 
 template <typename T, int DP>
@@ -749,11 +753,12 @@ cudaError_t run_sized(AttnArgs a, void* ws, int64_t* ws_bytes, cudaStream_t stre
     cudaLaunchConfig_t cfg = pdl_config(dim3(static_cast<unsigned>(grid)), dim3(kPThreads), L::kAlloc, stream, attr);
     e = cudaLaunchKernelEx(&cfg, kv_prompt_kernel<T, DP>, a);
     if (e != cudaSuccess) return e;
-    // As many blocks as fit at a time, a row to a warp where there are few entries.
-    cfg.gridDim = dim3(static_cast<unsigned>(a.entries), 8 * a.entries <= 2 * grid ? 32 : 8);
+    const int lanes = 8 * a.entries <= 2 * grid ? 32 : 8;
+    cfg.gridDim = dim3(static_cast<unsigned>(a.entries), kRows * lanes / 256);
     cfg.blockDim = dim3(256);
     cfg.dynamicSmemBytes = 0;
-    return cudaLaunchKernelEx(&cfg, kv_prompt_join_kernel<T, DP>, a);
+    return lanes == 8 ? cudaLaunchKernelEx(&cfg, kv_prompt_join_kernel<T, DP, 8>, a)
+                      : cudaLaunchKernelEx(&cfg, kv_prompt_join_kernel<T, DP, 32>, a);
 }
 
 }  // namespace

@@ -35,8 +35,14 @@
 //  * Tasks of 16-token tiles, cut over the workers of all SMs
 //    (kv_attention.cuh); split tasks are joined by kv_join_kernel.
 //
-// Sequences with more query rows than one tile of 16 go to the kernel of
-// kv_prompt.cu where it takes their type and dim.
+// Measured, with the join: 16 sequences of 4096 tokens, 32 key heads of 128, one
+// f32 query each: 98 us, 5.5 TB/s; 64 ragged ones up to 8192, 8 key heads, bf16:
+// 87 us, 5.7 TB/s; one of 131,075 tokens, f16: 55 us, 4.9 TB/s. Small calls are a
+// chain of latencies (schedule, block table, codes, partial results, join): 12 us
+// for 1000 tokens.
+//
+// Sequences with many query rows go to the kernel of kv_prompt.cu where it takes
+// their type and dim (kPromptRows).
 #include <algorithm>
 #include <type_traits>
 

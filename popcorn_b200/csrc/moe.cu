@@ -9,8 +9,12 @@
 //  2. up_kernel: every block picks the experts itself from the logits (a few
 //     KB, cheaper than a launch), then walks over (chosen expert, 32 rows of
 //     gate and of up) items and writes silu(g) u as fixed point.
-//  3. down_kernel: a block owns 16 output channels and goes through all chosen
-//     experts, so that a token's sum over its experts needs no other block.
+//  3. down_kernel: a block owns up to 32 output channels at a time and goes
+//     through all chosen experts, so that a token's sum over its experts needs no
+//     other block.
+// Measured: one token, 2 of 16 experts of 4096 x 11008: 56 us, 4.9 TB/s (up 34,
+// down 21, both at the rate of a plain copy but for their ends); 16 tokens, 6 of
+// 64 experts of 2048 x 1424 each: 99 us, 4.5 TB/s.
 //
 // Products. mma s8 x s8 -> s32 with the codes as they are: 16 weight rows are
 // the M side; the eight columns of the N side are two tokens times the four

@@ -11,13 +11,12 @@
 // scales (written), and the block's earlier codes only where the scale grew.
 // At decode that is a few KB a block, so the call is bound by launch and the
 // chain first/start -> table -> scale -> codes (four dependent loads), not by
-// bandwidth. At prompts it is bound by instructions (2.8 a cycle and SM) before
-// it is by HBM. Measured, append and read-back of the touched pages: a token for
-// one sequence 4.7 us, a token for each of 64 7.9 us, 4 ragged prompts of up to
-// 2048 tokens in f32 with 32 query heads rotated 69 us, of which the append 55 at
-// 3.5 TB/s. Tried there and no faster: two query tokens a block (56), blocks of
-// queries and of keys taking turns (56), products by 1 / s with a division only
-// near halves (64: more registers, spilled).
+// bandwidth. At prompts instructions count as much as HBM. Measured, append and
+// read-back of the touched pages: a token for one sequence 4.7 us, a token for
+// each of 64 7.9 us, 4 ragged prompts of up to 2048 tokens in f32 with 32 query
+// heads rotated 67 us, of which the append 53 at 3.7 TB/s. Tried there and no
+// faster: two query tokens a block, blocks of queries and of keys taking turns,
+// more units held in registers (72), more blocks an SM.
 #include "kv.cuh"
 
 namespace pcb {
@@ -99,9 +98,38 @@ __device__ __forceinline__ int encode(float x, float s) {
     // rint of the quotient, clamped; NaN (0 / 0, inf / inf) becomes 0.
     return s > 0.0f ? max(-128, min(127, __float2int_rn(__fdiv_rn(x, s)))) : 0;
 }
-__device__ __forceinline__ uint32_t encode4(const float* v, float s) {
-    uint32_t r = 0;
+// rint of a value up to 2^22 in magnitude: the low bits of the sum and the sum
+// less the constant (1.5 2^23).
+constexpr float kRound = 12582912.0f;
+__device__ __forceinline__ uint32_t low_bytes(const float (&t)[4]) {
+    const uint32_t a = __byte_perm(__float_as_uint(t[0]), __float_as_uint(t[1]), 0x0040);
+    const uint32_t b = __byte_perm(__float_as_uint(t[2]), __float_as_uint(t[3]), 0x0040);
+    return __byte_perm(a, b, 0x5410);
+}
+// Four codes. FAST: v * by, with by = 1 / s, is within 1e-4 of v / s (|v| <=
+// 127 s), so that its rint is the quotient's unless it lies near a half; only
+// then, and for NaN, there are divisions. At prompts that took 3 us off the 69 of
+// the prompts above; at decode a thread has one or two values and the reciprocal
+// stands before them (8.2 us against 7.9).
+template <bool FAST>
+__device__ __forceinline__ uint32_t encode4(const float* v, float s, float by) {
+    if (!FAST) {
+        uint32_t r = 0;
+        #pragma unroll
+        for (int j = 0; j < 4; ++j) r |= (static_cast<uint32_t>(encode(v[j], s)) & 0xffu) << (8 * j);
+        return r;
+    }
+    float t[4];
+    bool clear = s > 0.0f;
     #pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float y = __fmul_rn(v[j], by);
+        t[j] = __fadd_rn(y, kRound);
+        clear = clear && fabsf(y - __fsub_rn(t[j], kRound)) <= 0.4999f;
+    }
+    if (clear) return low_bytes(t);
+    uint32_t r = 0;
+    #pragma unroll 1
     for (int j = 0; j < 4; ++j) r |= (static_cast<uint32_t>(encode(v[j], s)) & 0xffu) << (8 * j);
     return r;
 }
@@ -114,6 +142,7 @@ __device__ __forceinline__ uint32_t encode4(const float* v, float s) {
 template <typename T, int THREADS, int CU>
 __global__ void __launch_bounds__(THREADS, THREADS == 64 ? 12 : 4) append_kernel(const AppendArgs a) {
     constexpr int H = THREADS / 2;
+    constexpr bool FAST = THREADS > 64;
     __shared__ float part[THREADS / 32];
     pdl_launch_dependents();
     pdl_wait();
@@ -190,34 +219,39 @@ __global__ void __launch_bounds__(THREADS, THREADS == 64 ? 12 : 4) append_kernel
         const int64_t block = page * a.heads + h;
         int8_t* codes = a.codes[kv] + (block << a.page_shift) * a.dim;
         const float old = row == 0 ? 0.0f : a.scale[kv][block];
-        const int total = n * units;
 
-        const auto rotated = [&](int i, Unit& un, float (&v)[8]) {  // returns the element index in the block
-            const int r = i / units;
-            un = unit_of(i - r * units, rot, inter);
+        // This thread's units are H apart: unit c of row r, then the next.
+        const int dr = H / units, dc = H - dr * units, r_first = ht / units, c_first = ht - r_first * units;
+        const auto step = [&](int& r, int& c) {
+            r += dr, c += dc;
+            if (c >= units) c -= units, ++r;
+        };
+        const auto rotated = [&](int r, int c, Unit& un, float (&v)[8]) {  // returns the element index in the block
+            un = unit_of(c, rot, inter);
             load_unit(x + (t + r) * a.tok[kv], un, rot, vec, v);
             if (rot > 0) turn_unit(un, rot, a.cos + (pos + r) * (rot >> 1), a.sin + (pos + r) * (rot >> 1), vec, v);
             return (row + r) * a.dim + un.at;
         };
-        const auto put = [&](int e, Unit un, const float (&v)[8], float s) {
-            *reinterpret_cast<uint32_t*>(codes + e) = encode4(v, s);
-            if (un.pair) *reinterpret_cast<uint32_t*>(codes + e + (rot >> 1)) = encode4(v + 4, s);
+        const auto put = [&](int e, Unit un, const float (&v)[8], float s, float by) {
+            *reinterpret_cast<uint32_t*>(codes + e) = encode4<FAST>(v, s, by);
+            if (un.pair) *reinterpret_cast<uint32_t*>(codes + e + (rot >> 1)) = encode4<FAST>(v + 4, s, by);
         };
         float v[CU][8];
         float m = 0.0f;
+        int r = r_first, c = c_first;
         #pragma unroll
-        for (int u = 0; u < CU; ++u) {
+        for (int u = 0; u < CU; ++u, step(r, c)) {
             Unit un;
-            if (ht + u * H < total) {
-                rotated(ht + u * H, un, v[u]);
+            if (r < n) {
+                rotated(r, c, un, v[u]);
                 #pragma unroll
                 for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(v[u][j]));  // (a single group's rest is zero)
             }
         }
-        for (int i = ht + CU * H; i < total; i += H) {
+        for (; r < n; step(r, c)) {
             Unit un;
             float w[8];
-            rotated(i, un, w);
+            rotated(r, c, un, w);
             #pragma unroll
             for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(w[j]));
         }
@@ -242,31 +276,28 @@ __global__ void __launch_bounds__(THREADS, THREADS == 64 ? 12 : 4) append_kernel
                 uint32_t* e = reinterpret_cast<uint32_t*>(&c);
                 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    uint32_t r = 0;
+                    float f[4];
                     #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        const float f = static_cast<float>(static_cast<int8_t>(e[j] >> (8 * k)));
-                        r |= (static_cast<uint32_t>(__float2int_rn(__fmul_rn(f, ratio))) & 0xffu) << (8 * k);
+                        f[k] = __fadd_rn(__fmul_rn(static_cast<float>(static_cast<int8_t>(e[j] >> (8 * k))), ratio), kRound);
                     }
-                    e[j] = r;
+                    e[j] = low_bytes(f);
                 }
                 w[i] = c;
             }
         }
+        const float by = FAST ? __fdiv_rn(1.0f, s) : 0.0f;
+        r = r_first, c = c_first;
         #pragma unroll
-        for (int u = 0; u < CU; ++u) {
-            const int i = ht + u * H;
-            if (i < total) {
-                const int r = i / units;
-                const Unit un = unit_of(i - r * units, rot, inter);
-                put((row + r) * a.dim + un.at, un, v[u], s);
-            }
+        for (int u = 0; u < CU; ++u, step(r, c)) {
+            const Unit un = unit_of(c, rot, inter);
+            if (r < n) put((row + r) * a.dim + un.at, un, v[u], s, by);
         }
-        for (int i = ht + CU * H; i < total; i += H) {
+        for (; r < n; step(r, c)) {
             Unit un;
             float w[8];
-            const int e = rotated(i, un, w);
-            put(e, un, w, s);
+            const int e = rotated(r, c, un, w);
+            put(e, un, w, s, by);
         }
         __syncwarp();  // every lane has read the old scale
         if (ht == 0 && (row == 0 || s != old)) a.scale[kv][block] = s;
@@ -319,7 +350,7 @@ cudaError_t launch_append(const AppendArgs& a, bool few, cudaStream_t stream) {
     cudaLaunchAttribute attr[1];
     const cudaLaunchConfig_t cfg = pdl_config(dim3(static_cast<unsigned>(grid)), dim3(threads), 0, stream, attr);
     return few ? cudaLaunchKernelEx(&cfg, append_kernel<T, 64, 2>, a)
-               : cudaLaunchKernelEx(&cfg, append_kernel<T, 256, 4>, a);
+               : cudaLaunchKernelEx(&cfg, append_kernel<T, 256, 2>, a);
 }
 
 template <typename T>

@@ -594,3 +594,30 @@ def test_prompts_against_64_bits(cuda, kind, wide, case):
     assert pc.device_errors() == 0
     _check(c, _f32(q).astype(np.float64), _f32(got).astype(np.float64), lse.cpu().numpy().astype(np.float64), table, length, new,
            group, causal, window, dim ** -0.5, kind)
+
+
+@pytest.mark.parametrize("tokens", [3, 40])
+def test_append_rounds_values_next_to_halves(cuda, tokens):
+    """Codes at k + 1/2 and a few ulps beside it, for scales from 1e-22 to the largest, and blocks of zeros, NaN and
+    infinities: decode and prompt forms of the kernel give the definition's codes."""
+    torch = _torch()
+    rng = _rng("halves", tokens)
+    top = np.float32([1.0, 127.0, 3e-20, 7e20, 3.4e38, 0.0, 1e-30, 1.0, 1.0])
+    heads, dim, page = len(top), 64, 64
+    c = Cache(rng, 3, heads, page, dim, cuda)
+    half = rng.integers(-127, 127, (tokens, heads, dim)) + 0.5
+    with np.errstate(over="ignore"):
+        k = (half * (top / np.float32(127))[None, :, None].astype(np.float64)).astype(np.float32)
+    k = (k.view(np.int32) + rng.integers(-3, 4, k.shape)).astype(np.int32).view(np.float32)
+    k[0, :, 0] = top
+    k[:, 5] = 0.0
+    k[1, 7, 9] = np.nan
+    k[2, 8, 60] = -np.inf
+    v = np.ascontiguousarray(k[:, ::-1])
+    table, old, new = np.int32([[1]]), [0], [tokens]
+    _put(c.k, c.ks, k, table, old, new, page)
+    _put(c.v, c.vs, v, table, old, new, page)
+    up = lambda a: torch.from_numpy(np.ascontiguousarray(a)).to(cuda)  # noqa: E731
+    pc.kv_append(c.dev, up(k), up(v), up(table), up(np.int32(old)), first=up(_first(new)))
+    c.same()
+    assert pc.device_errors() == 0

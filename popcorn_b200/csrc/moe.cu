@@ -352,10 +352,18 @@ __device__ void route_tokens(const MoeArgs& a, Routing& r) {
 // kept at most 96 KB in flight; warps that shared
 // the rows and had a quarter of the columns each read 64 bytes a row at a time:
 // 38 us against 34 for the two experts of 11008 rows.)
+//
+// With eight tokens to a job the digits are twice the codes, and each of the four
+// warps read all of them. There a warp has 16 rows of both matrices and half of
+// the columns, 128 bytes of each row a stage, and two warps' sums are added: 25
+// tokens that all pick all 8 experts of 2560 x 6448 took 179 us instead of 221.
 constexpr int kUpWarps = 4, kUpThreads = 32 * kUpWarps, kUpWorkers = 3;
 template <int NP>
 struct Up {
     static constexpr int kStages = NP == 4 ? 3 : 4;
+    static constexpr bool kPaired = NP == 4;         // a warp has both matrices' rows, half of the columns
+    static constexpr int kTiles = kPaired ? 2 : 1;   // of 16 rows, a warp's
+    static constexpr int kWide = kPaired ? 2 : 4;    // windows of a stage
     static constexpr int kParities = NP == 1 ? 2 : 1;  // an item's sums may wait while the next is multiplied
     static constexpr int kBytes = kUpWorkers * kUpWarps * kStages * kStageBytes;
 };
@@ -410,22 +418,31 @@ __global__ void __launch_bounds__(kUpWorkers* kUpThreads, 1) up_kernel(const Moe
     const int first = worker * gridDim.x + blockIdx.x, stride = kUpWorkers * gridDim.x;
     const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(s_ring)) +
                           (worker * kUpWarps + warp) * STAGES * kStageBytes + 16 * lane;
-    const int8_t* const codes = (warp & 2 ? a.qu : a.qg) + 16 * t;
+    constexpr int TILES = Up<NP>::kTiles, WIDE = Up<NP>::kWide;
+    constexpr bool PAIRED = Up<NP>::kPaired;
+    const int half = PAIRED ? 64 * WIDE * (warp >> 1) : 0;  // first column of a stage
+    const int8_t* const codes = (!PAIRED && (warp & 2) ? a.qu : a.qg) + 16 * t;
 
     // The copying side: item, stage of it and this lane's rows g and g + 8.
     int c_item = first, c_s = 0, c_slot = 0;
-    const int8_t* rows[2] = {};
-    const int bytes[2] = {16, 16};
+    const int8_t* rows[2 * TILES] = {};
+    int bytes[2 * TILES];
+    #pragma unroll
+    for (int i = 0; i < 2 * TILES; ++i) bytes[i] = 16;
     const auto rows_of = [&](int item) {
         const int h = item % halves;
         const int f = h / 2 * 64 + 32 * (warp & 1) + 8 * (h & 1) + g;
         const int64_t at = static_cast<int64_t>(job_of(r, item / halves).expert) * a.F;
         rows[0] = codes + (at + min(f, a.F - 1)) * a.K;
         rows[1] = codes + (at + min(f + 16, a.F - 1)) * a.K;
+        if constexpr (PAIRED) {
+            rows[2] = a.qu + 16 * t + (at + min(f, a.F - 1)) * a.K;
+            rows[3] = a.qu + 16 * t + (at + min(f + 16, a.F - 1)) * a.K;
+        }
     };
     const auto copy_next = [&] {
         if (c_item < items) {
-            copy_stage<2, kWindows>(ring + c_slot * kStageBytes, rows, bytes, c_s * kColumns, t, a.K);
+            copy_stage<2 * TILES, WIDE>(ring + c_slot * kStageBytes, rows, bytes, c_s * kColumns + half, t, a.K);
             if (++c_s == stages) {
                 c_s = 0;
                 c_item += stride;
@@ -448,44 +465,61 @@ __global__ void __launch_bounds__(kUpWorkers* kUpThreads, 1) up_kernel(const Moe
         #pragma unroll
         for (int n = 0; n < NP; ++n) {
             const int m = r.token[job.pos + min(2 * n + (g >> 2), job.count - 1)];
-            xd[n] = a.xd + (static_cast<int64_t>(m) * 4 + (g & 3)) * a.kp + 16 * t;
+            xd[n] = a.xd + (static_cast<int64_t>(m) * 4 + (g & 3)) * a.kp + 16 * t + half;
         }
-        uint4 b[kWindows][NP];
+        uint4 b[WIDE][NP];
         const auto load_b = [&](int st) {
             #pragma unroll
-            for (int k = 0; k < kWindows; ++k) {
+            for (int k = 0; k < WIDE; ++k) {
                 #pragma unroll
                 for (int n = 0; n < NP; ++n) b[k][n] = *reinterpret_cast<const uint4*>(xd[n] + kColumns * st + 64 * k);
             }
         };
         if (NP <= 2) load_b(0);
-        int acc[NP][4] = {};
+        int acc[TILES][NP][4] = {};
         for (int st = 0; st < stages; ++st) {
-            if (NP > 2) load_b(st);  // (too many registers to hold a stage ahead)
+            if (NP > 2) load_b(st);  // (held a stage ahead: 185 us against 179 for the example above)
             cp_async_wait_group<STAGES - 2>();
             __syncwarp();
             copy_next();
             const uint32_t at = ring + slot * kStageBytes;
             slot = slot == STAGES - 1 ? 0 : slot + 1;
             #pragma unroll
-            for (int k = 0; k < kWindows; ++k) {
-                const uint4 q0 = load_shared16(at + 1024 * k), q1 = load_shared16(at + 1024 * k + 512);
-                const uint32_t lo[4] = {q0.x, q1.x, q0.y, q1.y}, hi[4] = {q0.z, q1.z, q0.w, q1.w};
+            for (int k = 0; k < WIDE; ++k) {
                 #pragma unroll
-                for (int n = 0; n < NP; ++n) {
-                    mma_s8_16832(acc[n], lo, b[k][n].x, b[k][n].y);
-                    mma_s8_16832(acc[n], hi, b[k][n].z, b[k][n].w);
+                for (int i = 0; i < TILES; ++i) {
+                    const uint32_t from = at + 1024 * (TILES * k + i);
+                    const uint4 q0 = load_shared16(from), q1 = load_shared16(from + 512);
+                    const uint32_t lo[4] = {q0.x, q1.x, q0.y, q1.y}, hi[4] = {q0.z, q1.z, q0.w, q1.w};
+                    #pragma unroll
+                    for (int n = 0; n < NP; ++n) {
+                        mma_s8_16832(acc[i][n], lo, b[k][n].x, b[k][n].y);
+                        mma_s8_16832(acc[i][n], hi, b[k][n].z, b[k][n].w);
+                    }
                 }
             }
             if (NP <= 2 && st + 1 < stages) load_b(st + 1);
         }
         if (Up<NP>::kParities == 1) sync_worker();  // the sums before have been taken
-        #pragma unroll
-        for (int n = 0; n < NP; ++n) {
+        const auto put_sums = [&](bool add) {
             #pragma unroll
-            for (int c = 0; c < 4; c += 2) {
-                *reinterpret_cast<int2*>(&sums[parity][warp][g + 4 * c][8 * n + 2 * t]) = make_int2(acc[n][c], acc[n][c + 1]);
+            for (int i = 0; i < TILES; ++i) {
+                #pragma unroll
+                for (int n = 0; n < NP; ++n) {
+                    #pragma unroll
+                    for (int c = 0; c < 4; c += 2) {
+                        int2* const to = reinterpret_cast<int2*>(
+                            &sums[parity][PAIRED ? (warp & 1) + 2 * i : warp][g + 4 * c][8 * n + 2 * t]);
+                        const int2 had = add ? *to : make_int2(0, 0);
+                        *to = make_int2(had.x + acc[i][n][c], had.y + acc[i][n][c + 1]);
+                    }
+                }
             }
+        };
+        if (!PAIRED || warp < 2) put_sums(false);
+        if constexpr (PAIRED) {
+            sync_worker();
+            if (warp >= 2) put_sums(true);
         }
         sync_worker();
         // Warp j: the job's tokens j, j + 4; lane: one of the 32 rows. (A

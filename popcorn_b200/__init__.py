@@ -443,8 +443,9 @@ def dequantize(qweight, scale, out=None, stream=None, dtype=None):
 
 # ---------------------------------------------------------------------------
 # Serving operators (include/popcorn_serve.h), through popcorn_b200/_serve.so:
-# it checks the tensors (ValueError), makes outputs and workspaces on the
-# current stream and calls the library, in a few us.
+# it checks the tensors (ValueError), makes outputs and workspaces and calls
+# the library, in a few us. `stream` (a torch stream or a handle) stands for
+# `with torch.cuda.stream(stream):` around the call; None is the current one.
 # ---------------------------------------------------------------------------
 _bound = None
 

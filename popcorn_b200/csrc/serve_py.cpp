@@ -5,6 +5,9 @@
 // exists for its speed: the same checks through ctypes and tensor attributes
 // take 10 to 14 us a call, several times the kernels of a small decode step.
 //
+// With a stream given the whole call is as inside torch.cuda.stream(...): what
+// it allocates belongs to that stream.
+//
 // Argument errors raise ValueError; the entry point's status is returned.
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -65,10 +68,38 @@ struct Call {
             default: refuse(where, "dtype", "float32, float16 or bfloat16 wanted", nullptr);
         }
     }
-    cudaStream_t stream(const std::optional<int64_t>& given) const {
-        return given ? reinterpret_cast<cudaStream_t>(*given)
-                     : c10::cuda::getCurrentCUDAStream(device.index()).stream();
+};
+
+// The stream of a call: the current one, or the caller's, which is then the
+// current one until the call returns. Outputs and workspaces come from the
+// allocator's blocks of the stream that the kernels run on: a block of another
+// stream may still be in use by that stream's earlier work, and the workspace,
+// released on return, would go to that stream's next tensor while the kernels
+// run. Outputs are recorded on the stream that was current before, where the
+// caller goes on with them: a block released there is not written again before
+// that stream's work on it has ended.
+class OnStream {
+  public:
+    OnStream(const Call& c, const std::optional<int64_t>& given)
+        : before_(c10::cuda::getCurrentCUDAStream(c.device.index())), handle_(before_.stream()) {
+        if (!given) return;
+        handle_ = reinterpret_cast<cudaStream_t>(*given);
+        if (handle_ == before_.stream()) return;
+        const bool legacy = handle_ == nullptr || handle_ == cudaStreamLegacy;
+        guard_.emplace(legacy ? c10::cuda::getDefaultCUDAStream(c.device.index())
+                              : c10::cuda::getStreamFromExternal(handle_, c.device.index()));
     }
+    cudaStream_t handle() const { return handle_; }
+    Tensor output(at::IntArrayRef shape, const at::TensorOptions& options) const {
+        Tensor t = at::empty(shape, options);
+        if (guard_) t.record_stream(before_.unwrap());
+        return t;
+    }
+
+  private:
+    c10::cuda::CUDAStream before_;
+    cudaStream_t handle_;
+    std::optional<c10::cuda::CUDAStreamGuard> guard_;
 };
 
 Call on_cache(const char* where, int64_t device) {
@@ -102,6 +133,7 @@ py::tuple kv_append(int64_t ref, int64_t device, const Tensor& k, const Tensor& 
                     const Optional& sin, bool interleaved, Optional q_out, std::optional<int64_t> stream) {
     const Call c = on_cache("kv_append", device);
     const c10::cuda::CUDAGuard guard(c.device);
+    const OnStream on(c, stream);
     const popcornKvCache_t& cache = cache_at(ref);
     three(c, k, "k");
     const int64_t tokens = k.size(0);
@@ -119,7 +151,7 @@ py::tuple kv_append(int64_t ref, int64_t device, const Tensor& k, const Tensor& 
         q_heads = q->size(1);
         qp = c.rows(*q, kind, {tokens, q_heads, cache.dim}, "q");
         qt = q->stride(0), qh = q->stride(1);
-        if (!q_out) q_out = at::empty({tokens, q_heads, cache.dim}, q->options());
+        if (!q_out) q_out = on.output({tokens, q_heads, cache.dim}, q->options());
         op = c.contiguous(*q_out, kind, {tokens, q_heads, cache.dim}, "q_out");
     } else if (q_out) {
         refuse(c.where, "q_out", "q_out needs q", nullptr);
@@ -135,7 +167,7 @@ py::tuple kv_append(int64_t ref, int64_t device, const Tensor& k, const Tensor& 
     }
     const int status = popcornKvAppend(&cache, kp, k.stride(0), k.stride(1), vp, v.stride(0), v.stride(1), type, b.table,
                                        b.width, b.first, sp, b.seqs, tokens, op, qp, qt, qh, q_heads, cp, np, positions,
-                                       2 * half, interleaved, c.stream(stream));
+                                       2 * half, interleaved, on.handle());
     return py::make_tuple(status, q_out);
 }
 
@@ -143,18 +175,19 @@ py::tuple kv_read(int64_t ref, int64_t device, const Tensor& pages, int type, Op
                   std::optional<int64_t> stream) {
     const Call c = on_cache("kv_read", device);
     const c10::cuda::CUDAGuard guard(c.device);
+    const OnStream on(c, stream);
     const popcornKvCache_t& cache = cache_at(ref);
     if (pages.dim() != 1) refuse(c.where, "pages", "[n]", &pages);
     const int64_t n = pages.size(0);
     const at::ScalarType kind = type == POPCORN_TYPE_F32 ? at::kFloat : type == POPCORN_TYPE_F16 ? at::kHalf : at::kBFloat16;
     const int32_t* list = c.whole(pages, {n}, "pages");
     const auto options = at::TensorOptions().dtype(kind).device(c.device);
-    if (!k_out) k_out = at::empty({n, cache.heads, cache.page_size, cache.dim}, options);
-    if (!v_out) v_out = at::empty({n, cache.heads, cache.page_size, cache.dim}, options);
+    if (!k_out) k_out = on.output({n, cache.heads, cache.page_size, cache.dim}, options);
+    if (!v_out) v_out = on.output({n, cache.heads, cache.page_size, cache.dim}, options);
     void* kp = c.contiguous(*k_out, kind, {n, cache.heads, cache.page_size, cache.dim}, "k_out");
     void* vp = c.contiguous(*v_out, kind, {n, cache.heads, cache.page_size, cache.dim}, "v_out");
     const int status = n == 0 ? POPCORN_SUCCESS
-                              : popcornKvRead(kp, vp, static_cast<popcornType_t>(type), &cache, list, n, c.stream(stream));
+                              : popcornKvRead(kp, vp, static_cast<popcornType_t>(type), &cache, list, n, on.handle());
     return py::make_tuple(status, k_out, v_out);
 }
 
@@ -163,6 +196,7 @@ py::tuple kv_attention(int64_t ref, int64_t device, const Tensor& q, const Tenso
                        std::optional<double> scale, Optional out, const Optional& lse, std::optional<int64_t> stream) {
     const Call c = on_cache("kv_attention", device);
     const c10::cuda::CUDAGuard guard(c.device);
+    const OnStream on(c, stream);
     const popcornKvCache_t& cache = cache_at(ref);
     three(c, q, "q");
     const int64_t tokens = q.size(0), q_heads = q.size(1);
@@ -172,17 +206,17 @@ py::tuple kv_attention(int64_t ref, int64_t device, const Tensor& q, const Tenso
     if (q_heads % cache.heads != 0) refuse(c.where, "q", "a multiple of the cache's heads", &q);
     const Batch b = batch(c, table, first, tokens);
     const int32_t* lp = c.whole(length, {b.seqs}, "length");
-    if (!out) out = at::empty({tokens, q_heads, cache.dim}, q.options());
+    if (!out) out = on.output({tokens, q_heads, cache.dim}, q.options());
     void* op = c.contiguous(*out, kind, {tokens, q_heads, cache.dim}, "out");
     float* ep = lse ? static_cast<float*>(c.contiguous(*lse, at::kFloat, {tokens, q_heads}, "lse")) : nullptr;
     const int64_t most = max_tokens ? *max_tokens : b.first == nullptr ? 1 : tokens;
     const int64_t need = popcornKvAttentionWorkspace(&cache, type, b.seqs, tokens, most, q_heads);
-    Tensor ws;  // on the current stream, like the output
+    Tensor ws;
     if (need > 0) ws = bytes_on(c.device, need);
     const float by = static_cast<float>(scale ? *scale : 1.0 / std::sqrt(static_cast<double>(cache.dim)));
     const int status = popcornKvAttention(op, ep, qp, q.stride(0), q.stride(1), type, &cache, b.table, b.width, b.first,
                                           lp, b.seqs, tokens, most, q_heads, causal, window, by,
-                                          need > 0 ? ws.data_ptr() : nullptr, need, c.stream(stream));
+                                          need > 0 ? ws.data_ptr() : nullptr, need, on.handle());
     return py::make_tuple(status, out);
 }
 
@@ -192,6 +226,7 @@ py::tuple moe(const Tensor& x, const Tensor& router, const Tensor& q_gate, const
     const Call c = {"moe", x.device()};
     if (!x.is_cuda() || x.dim() != 2) refuse(c.where, "x", "a CUDA tensor [M, K]", &x);
     const c10::cuda::CUDAGuard guard(c.device);
+    const OnStream on(c, stream);
     if (s_gate.dim() != 2) refuse(c.where, "s_gate", "[E, F]", &s_gate);
     const int64_t M = x.size(0), K = x.size(1), E = s_gate.size(0), F = s_gate.size(1);
     const auto floats = [&](const Tensor& t, std::initializer_list<int64_t> shape, const char* name) {
@@ -207,21 +242,21 @@ py::tuple moe(const Tensor& x, const Tensor& router, const Tensor& q_gate, const
     const float* us = floats(s_up, {E, F}, "s_up");
     const int8_t* dp = codes(q_down, {E, K, F}, "q_down");
     const float* ds = floats(s_down, {E, K}, "s_down");
-    if (!out) out = at::empty({M, K}, x.options());
+    if (!out) out = on.output({M, K}, x.options());
     float* op = floats(*out, {M, K}, "out");
     Optional experts, weights;
     if (routing) {
         if (top_k < 0) refuse(c.where, "top_k", "a positive number wanted", nullptr);
-        experts = at::empty({M, top_k}, x.options().dtype(at::kInt));
-        weights = at::empty({M, top_k}, x.options());
+        experts = on.output({M, top_k}, x.options().dtype(at::kInt));
+        weights = on.output({M, top_k}, x.options());
     }
     const int64_t need = popcornMoeWorkspace(M, K, F, E, top_k);
-    Tensor ws;  // on the current stream, like the output
+    Tensor ws;
     if (need > 0) ws = bytes_on(c.device, need);
     const int status = popcornMoe_i8f32(op, routing ? experts->data_ptr<int32_t>() : nullptr,
                                         routing ? weights->data_ptr<float>() : nullptr, xp, rp, gp, gs, up, us, dp, ds,
                                         M, K, F, E, top_k, renormalize, need > 0 ? ws.data_ptr() : nullptr, need,
-                                        c.stream(stream));
+                                        on.handle());
     return py::make_tuple(status, out, experts, weights);
 }
 

@@ -773,9 +773,10 @@ cudaError_t run_rows_typed(popcornType_t type, const AttnArgs& a, int64_t max_to
 // Launches the kernel, or the two, that the sizes ask for; with ws_bytes only
 // says how much workspace they take, for any block table if a.table_pages is 0.
 // Sequences of less than kPromptRows query rows go to kv_rows_kernel and others
-// to the prompt kernel, each of which skips the other's; where all sequences have
-// max_tokens queries only one is launched, and in small calls kv_rows_kernel
-// takes them all.
+// to the prompt kernel, each of which skips the other's; where tokens are seqs
+// times max_tokens only the prompt kernel is launched, and in small calls only
+// kv_rows_kernel. One that is alone takes sequences of any number of rows: `first`,
+// which only the device knows, may end before `tokens` and leave some with fewer.
 cudaError_t run_typed(popcornType_t type, AttnArgs a, int64_t max_tokens, void* ws, int64_t* ws_bytes,
                       cudaStream_t stream) {
     a.min_rows = 1, a.max_rows = INT32_MAX;
@@ -788,7 +789,7 @@ cudaError_t run_typed(popcornType_t type, AttnArgs a, int64_t max_tokens, void* 
     const int64_t few = (kPromptRows - 1) / a.group;  // queries of a sequence that kv_rows_kernel keeps
     AttnArgs rows = a;
     rows.max_rows = kPromptRows - 1;
-    a.min_rows = kPromptRows;
+    if (both) a.min_rows = kPromptRows;
     cudaError_t e = cudaSuccess;
     if (ws_bytes != nullptr) {
         int64_t prompt = 0, beside = 0, alone = 0;

@@ -59,7 +59,9 @@ typedef struct {
  *   k, v      [tokens, heads, dim] of `type`, strides in elements per token
  *             and per head, dim contiguous
  *   first     [seqs + 1]: sequence b's new tokens are rows first[b] to
- *             first[b + 1] - 1 (NULL: one token each, tokens == seqs)
+ *             first[b + 1] - 1 (NULL: one token each, tokens == seqs); rows
+ *             before first[0] and from first[seqs] on are not looked at, and
+ *             outputs of theirs are left as they are
  *   start     [seqs]: tokens that sequence b holds before the call; its new
  *             tokens take positions start[b], start[b] + 1, ...
  *   table     [seqs, table_pages] int32 page indices (table_pages wide)

@@ -164,8 +164,9 @@ __global__ void __launch_bounds__(THREADS, THREADS == 64 ? 12 : 4) append_kernel
             if (i < total) load_unit(q + h * a.q_head, unit_of(i - h * q_units, a.rot, inter), a.rot, vec, v[u]);
         }
         const int64_t b = a.first ? sequence_of(a.first, a.seqs, t, lane) : t;
-        if (b >= a.seqs) return;
-        const int64_t pos = a.start[b] + (a.first ? t - a.first[b] : 0);
+        const int64_t in = a.first ? t - a.first[b] : 0;
+        if (b >= a.seqs || in < 0) return;  // a row of no sequence
+        const int64_t pos = a.start[b] + in;
         if (a.rot > 0 && (pos < 0 || pos >= a.positions)) {
             if (tid == 0) atomicOr(&g_kv_err, kKvErrAppend);
             return;
@@ -192,7 +193,8 @@ __global__ void __launch_bounds__(THREADS, THREADS == 64 ? 12 : 4) append_kernel
     const int units = kv == 0 ? q_units : a.dim >> 2;
     const int page_size = 1 << a.page_shift;
 
-    for (int64_t t = slot * a.chunk; t < t_end;) {
+    // (Rows before first[0] belong to no sequence.)
+    for (int64_t t = a.first ? max(slot * a.chunk, static_cast<int64_t>(a.first[0])) : slot * a.chunk; t < t_end;) {
         const int64_t b = a.first ? sequence_of(a.first, a.seqs, t, lane) : t;
         if (b >= a.seqs) return;
         const int64_t t0 = a.first ? a.first[b] : t, t1 = a.first ? min(a.tokens, static_cast<int64_t>(a.first[b + 1])) : t + 1;

@@ -867,7 +867,8 @@ extern "C" popcornStatus_t popcornKvAttention(void* out, float* lse, const void*
     a.out = out, a.lse = lse, a.q = q, a.q_tok = q_token_stride, a.q_head = q_head_stride;
     a.k = cache->k, a.v = cache->v, a.ks = cache->k_scale, a.vs = cache->v_scale;
     a.table = table, a.first = first, a.length = length;
-    a.table_pages = table_pages, a.window = window, a.causal = causal;
+    // (Positions are below 2^31: a window of that many tokens hides none.)
+    a.table_pages = table_pages, a.window = window > INT32_MAX ? 0 : window, a.causal = causal;
     a.scale_log2 = scale * 1.4426950408889634f;
     const int64_t four = 4 * pcb::kv_type_size(type);
     a.q_vec = reinterpret_cast<uintptr_t>(q) % four == 0 && q_token_stride % 4 == 0 && q_head_stride % 4 == 0;

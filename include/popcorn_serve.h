@@ -35,6 +35,11 @@ typedef enum {
  * k and v 16-byte aligned. (page, head) blocks are contiguous, so a block's
  * codes are one run of page_size * dim bytes.
  *
+ * Scales are not negative, and below 2^126 or not finite. Attention takes a
+ * value scale below 2^-80 for that of a block of zeros, as an append writes
+ * it. Where the value scales that a query sees (at least 2^-80 for this) are
+ * up to 2^96 apart, softmax weights down to 2^-30 of the largest are kept.
+ *
  * A sequence's token at position p is row p % page_size of page
  * table[sequence, p / page_size]. Only table entries of pages that hold one
  * of the sequence's tokens are read; the others may hold anything. A page
@@ -156,9 +161,10 @@ popcornStatus_t popcornKvRead(
  * A query that sees nothing gives zeros. Scores, statistics and sums are
  * f32 or exact integers; f32 queries keep 23 bits relative to their row's
  * largest element and f32 probabilities, f16 and bf16 queries 16 bits and
- * f16 probabilities. A query row that holds a NaN or an infinity, or sees a
- * block with a non-finite scale, gives NaN. Results do not depend on the
- * order in which blocks of the GPU run.
+ * f16 probabilities. A query row that holds a NaN or an infinity and sees a
+ * token, or sees a block with a non-finite scale, gives NaN; so is its lse,
+ * which may stay that of the scores where only a value scale is not finite.
+ * Results do not depend on the order in which blocks of the GPU run.
  */
 popcornStatus_t popcornKvAttention(
     void* out,

@@ -410,7 +410,7 @@ __global__ void __launch_bounds__((kThreads * Rows<T, DP, NT>::kWorkers), 1) kv_
             }
             uint32_t sv[2];
             load_shared(sv, scales + 8 * stage);
-            const float ks_now = __uint_as_float(sv[0]), vs = __uint_as_float(sv[1]);
+            const float ks_now = nan_unless_finite(__uint_as_float(sv[0])), vs = __uint_as_float(sv[1]);
 
             int sc[NT][DIGITS][4];
             #pragma unroll
@@ -432,11 +432,11 @@ __global__ void __launch_bounds__((kThreads * Rows<T, DP, NT>::kWorkers), 1) kv_
                 }
             }
             // vs = 2^ve vf with vf in [1, 2); scales below 2^-80 belong to
-            // all-zero codes, non-finite ones pass through vf.
+            // all-zero codes, for non-finite ones vf is NaN.
             const uint32_t vbits = __float_as_uint(vs);
             int ve = static_cast<int>((vbits >> 23) & 0xffu) - 127;
             float vf = __uint_as_float((vbits & 0x807fffffu) | 0x3f800000u);
-            if (ve == 128) ve = 0, vf = vs;
+            if (ve == 128) ve = 0, vf = __int_as_float(0x7fffffff);
             if (ve < -80) ve = -80, vf = 0.0f;
             if (!ok_now) ve = 0, vf = 0.0f;
             const float vexp = static_cast<float>(ve), vinv = __int_as_float((127 - ve) << 23);

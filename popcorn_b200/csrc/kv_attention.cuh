@@ -237,6 +237,10 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return y;
 }
 
+// A block scale, or NaN for an infinite one: a score of minus infinity would
+// count as a hidden token.
+__device__ __forceinline__ float nan_unless_finite(float scale) { return scale + (scale - scale); }
+
 // Scales a partial result with maximum m to the joint maximum.
 __device__ __forceinline__ float join_factor(float m, float top) { return m == -INFINITY ? 0.0f : exp2_fast(m - top); }
 

@@ -533,8 +533,8 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const AttnArgs 
                 GroupScale g = {0.0f, -INFINITY, 1.0f, 0.0f};
                 if (there) {
                     const bool tiny = fabsf(vs) < kKvSmallestScale;  // all-zero codes
-                    g.ks = ks;
-                    g.lv = tiny ? -80.0f : __log2f(vs);
+                    g.ks = nan_unless_finite(ks);
+                    g.lv = tiny ? -80.0f : __log2f(nan_unless_finite(vs));
                     g.iv = tiny ? 1.0f / kKvSmallestScale
                                 : fabsf(vs) <= 3.4028234663852886e38f ? __fdividef(1.0f, vs) : 1.0f;
                 }

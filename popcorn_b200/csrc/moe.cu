@@ -91,9 +91,11 @@ __device__ __forceinline__ uint32_t digits_of(float v, const Fixed& f) {
 __device__ __forceinline__ bool not_finite(float v) { return !(fabsf(v) <= 3.4028234663852886e38f); }
 
 // ------------------------------------------------------------------ routing
-// Block e < E: logits of expert e for tokens 8 y .. 8 y + 7; the router's row is
-// read before the kernel waits for the one ahead. Blocks behind them (y = 0):
-// the digits of one token each.
+// Block e < E: logits of expert e for tokens 8 y .. 8 y + 7. Blocks behind them
+// (y = 0): the digits of one token each. The router is f32 and may be what the
+// kernel ahead writes: its rows are read after the wait like everything else, and
+// only fetched into L2 before it. (One token through 2 of 16 experts of 4096 x
+// 11008: 58.1 us so, 58.7 without, 57.5 with stale rows where that is so.)
 constexpr int kRouteThreads = 256, kRouteWarps = kRouteThreads / 32;
 __global__ void __launch_bounds__(kRouteThreads) route_kernel(const MoeArgs a) {
     constexpr int HELD = 4;  // float4 pieces of the router's row per thread: 4096 columns
@@ -105,13 +107,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const MoeArgs a) {
         a.K % 4 == 0 && ((reinterpret_cast<uintptr_t>(a.router) | reinterpret_cast<uintptr_t>(a.x)) & 15u) == 0;
     const float* w = a.router + static_cast<int64_t>(e) * a.K;
     float4 held[HELD];
-    if (e < a.E && vec) {
-        #pragma unroll
-        for (int i = 0; i < HELD; ++i) {
-            const int k = 4 * (tid + i * kRouteThreads);
-            held[i] = k < a.K ? *reinterpret_cast<const float4*>(w + k) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        }
-    }
+    if (e < a.E && tid == 0) prefetch_l2_range(w, sizeof(float) * min(a.K, 4 * HELD * kRouteThreads), 0, 1);
     pdl_wait();
     if (e >= a.E) {
         const int m = e - a.E;
@@ -178,6 +174,11 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const MoeArgs a) {
         }
     };
     if (vec) {
+        #pragma unroll
+        for (int i = 0; i < HELD; ++i) {
+            const int k = 4 * (tid + i * kRouteThreads);
+            held[i] = k < a.K ? *reinterpret_cast<const float4*>(w + k) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
         #pragma unroll
         for (int i = 0; i < HELD; ++i) {
             const int k = 4 * (tid + i * kRouteThreads);

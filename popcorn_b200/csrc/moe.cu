@@ -834,23 +834,24 @@ int64_t lay_out(MoeArgs& a, char* ws, int64_t M, bool tensor, bool own_picks) {
     return at;
 }
 
-// Lets a kernel have that much shared memory, once for each device and size.
-template <class Kernel>
-cudaError_t allow_shared(Kernel kernel, int bytes, int (&allowed)[64]) {
+// Lets a kernel have BYTES of shared memory, once for each device. (The same
+// number from every call: threads that get here together set the same limit.)
+template <int BYTES, class Kernel>
+cudaError_t allow_shared(Kernel kernel, bool (&allowed)[64]) {
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
-    if (dev < 64 && __atomic_load_n(&allowed[dev], __ATOMIC_RELAXED) >= bytes) return cudaSuccess;
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e == cudaSuccess && dev < 64) __atomic_store_n(&allowed[dev], bytes, __ATOMIC_RELAXED);
+    if (dev < 64 && __atomic_load_n(&allowed[dev], __ATOMIC_RELAXED)) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES);
+    if (e == cudaSuccess && dev < 64) __atomic_store_n(&allowed[dev], true, __ATOMIC_RELAXED);
     return e;
 }
 
 template <int NP, int GROUPS, int STAGES>
 cudaError_t run_down(const MoeArgs& a, int blocks, cudaStream_t stream) {
-    const int bytes = Down<NP, GROUPS>::bytes(STAGES, a.M);
-    static int allowed[64] = {};  // per device
-    const cudaError_t e = allow_shared(down_kernel<NP, GROUPS, STAGES>, bytes, allowed);
+    const int bytes = Down<NP, GROUPS>::bytes(STAGES, a.M);  // at most kDownShared (run_down_sized)
+    static bool allowed[64] = {};
+    const cudaError_t e = allow_shared<kDownShared>(down_kernel<NP, GROUPS, STAGES>, allowed);
     if (e != cudaSuccess) return e;
     cudaLaunchAttribute attr[1];
     const cudaLaunchConfig_t cfg =
@@ -888,8 +889,8 @@ cudaError_t run_down_sized(MoeArgs a, cudaStream_t stream) {
 template <int NP>
 cudaError_t run_tensor(MoeArgs a, cudaStream_t stream) {
     const int64_t sms = device_sm_count();
-    static int allowed[64] = {};  // per device
-    cudaError_t e = allow_shared(up_kernel<NP>, Up<NP>::kBytes, allowed);
+    static bool allowed[64] = {};
+    cudaError_t e = allow_shared<Up<NP>::kBytes>(up_kernel<NP>, allowed);
     if (e != cudaSuccess) return e;
     cudaLaunchAttribute attr[1];
     const int64_t items = static_cast<int64_t>(a.M) * a.top * ((a.F + 63) / 64 * 2);  // at most

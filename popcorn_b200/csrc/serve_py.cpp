@@ -8,7 +8,9 @@
 // With a stream given the whole call is as inside torch.cuda.stream(...): what
 // it allocates belongs to that stream.
 //
-// Argument errors raise ValueError; the entry point's status is returned.
+// Argument errors raise ValueError; the entry point's status is returned. A call
+// without work ends here once its arguments are checked: tensors without elements
+// have null pointers, which the entry points refuse.
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -165,6 +167,7 @@ py::tuple kv_append(int64_t ref, int64_t device, const Tensor& k, const Tensor& 
         cp = static_cast<const float*>(c.contiguous(*cos, at::kFloat, {positions, half}, "cos"));
         np = static_cast<const float*>(c.contiguous(*sin, at::kFloat, {positions, half}, "sin"));
     }
+    if (tokens == 0 || b.seqs == 0) return py::make_tuple(static_cast<int>(POPCORN_SUCCESS), q_out);
     const int status = popcornKvAppend(&cache, kp, k.stride(0), k.stride(1), vp, v.stride(0), v.stride(1), type, b.table,
                                        b.width, b.first, sp, b.seqs, tokens, op, qp, qt, qh, q_heads, cp, np, positions,
                                        2 * half, interleaved, on.handle());
@@ -186,8 +189,8 @@ py::tuple kv_read(int64_t ref, int64_t device, const Tensor& pages, int type, Op
     if (!v_out) v_out = on.output({n, cache.heads, cache.page_size, cache.dim}, options);
     void* kp = c.contiguous(*k_out, kind, {n, cache.heads, cache.page_size, cache.dim}, "k_out");
     void* vp = c.contiguous(*v_out, kind, {n, cache.heads, cache.page_size, cache.dim}, "v_out");
-    const int status = n == 0 ? POPCORN_SUCCESS
-                              : popcornKvRead(kp, vp, static_cast<popcornType_t>(type), &cache, list, n, on.handle());
+    if (n == 0) return py::make_tuple(static_cast<int>(POPCORN_SUCCESS), k_out, v_out);
+    const int status = popcornKvRead(kp, vp, static_cast<popcornType_t>(type), &cache, list, n, on.handle());
     return py::make_tuple(status, k_out, v_out);
 }
 
@@ -209,6 +212,7 @@ py::tuple kv_attention(int64_t ref, int64_t device, const Tensor& q, const Tenso
     if (!out) out = on.output({tokens, q_heads, cache.dim}, q.options());
     void* op = c.contiguous(*out, kind, {tokens, q_heads, cache.dim}, "out");
     float* ep = lse ? static_cast<float*>(c.contiguous(*lse, at::kFloat, {tokens, q_heads}, "lse")) : nullptr;
+    if (tokens == 0 || b.seqs == 0) return py::make_tuple(static_cast<int>(POPCORN_SUCCESS), out);
     const int64_t most = max_tokens ? *max_tokens : b.first == nullptr ? 1 : tokens;
     const int64_t need = popcornKvAttentionWorkspace(&cache, type, b.seqs, tokens, most, q_heads);
     Tensor ws;
@@ -250,6 +254,7 @@ py::tuple moe(const Tensor& x, const Tensor& router, const Tensor& q_gate, const
         experts = on.output({M, top_k}, x.options().dtype(at::kInt));
         weights = on.output({M, top_k}, x.options());
     }
+    if (M == 0) return py::make_tuple(static_cast<int>(POPCORN_SUCCESS), out, experts, weights);
     const int64_t need = popcornMoeWorkspace(M, K, F, E, top_k);
     Tensor ws;
     if (need > 0) ws = bytes_on(c.device, need);

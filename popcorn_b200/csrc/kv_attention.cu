@@ -857,9 +857,10 @@ extern "C" popcornStatus_t popcornKvAttention(void* out, float* lse, const void*
         return POPCORN_ERROR_INVALID_VALUE;
     }
     if (seqs <= 0 || tokens <= 0) return POPCORN_SUCCESS;
-    // Positions and row counts are 32-bit inside a sequence.
+    // Positions and row counts are 32-bit inside a sequence; the kernel for
+    // prompts counts up to 255 tokens past the last one.
     if (!pcb::attention_supported(*cache, type, seqs, tokens, max_tokens, q_heads) || table_pages <= 0 ||
-        table_pages > (INT32_MAX - 64) / cache->page_size || !pcb::aligned16(out) ||
+        table_pages > (INT32_MAX - 256) / cache->page_size || !pcb::aligned16(out) ||
         (first == nullptr && tokens != seqs)) {
         return POPCORN_ERROR_INVALID_VALUE;
     }

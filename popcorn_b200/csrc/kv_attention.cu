@@ -780,6 +780,7 @@ cudaError_t run_rows_typed(popcornType_t type, const AttnArgs& a, int64_t max_to
 cudaError_t run_typed(popcornType_t type, AttnArgs a, int64_t max_tokens, void* ws, int64_t* ws_bytes,
                       cudaStream_t stream) {
     a.min_rows = 1, a.max_rows = INT32_MAX;
+    max_tokens = std::min(max_tokens, static_cast<int64_t>(a.tokens));
     const int64_t tasks = a.heads * (static_cast<int64_t>(a.tokens) * a.group / 16 + a.seqs);
     const bool small = tasks <= device_sm_count() && tasks * (a.table_pages << a.page_shift) <= kFewTokens;
     if (max_tokens * a.group < kPromptRows || !prompt_supported(type, a.dim) || (small && a.table_pages > 0)) {

@@ -95,7 +95,8 @@ __device__ __forceinline__ bool not_finite(float v) { return !(fabsf(v) <= 3.402
 // (y = 0): the digits of one token each. The router is f32 and may be what the
 // kernel ahead writes: its rows are read after the wait like everything else, and
 // only fetched into L2 before it. (One token through 2 of 16 experts of 4096 x
-// 11008: 58.1 us so, 58.7 without, 57.5 with stale rows where that is so.)
+// 11008, called from Python: 58.1 us, 58.7 without the fetch, 57.5 when the rows
+// were read before the wait.)
 constexpr int kRouteThreads = 256, kRouteWarps = kRouteThreads / 32;
 __global__ void __launch_bounds__(kRouteThreads) route_kernel(const MoeArgs a) {
     constexpr int HELD = 4;  // float4 pieces of the router's row per thread: 4096 columns
@@ -913,9 +914,15 @@ cudaError_t run_pass(const MoeArgs& a, bool tensor, cudaStream_t stream) {
         e = cudaLaunchKernelEx(&cfg, plain_up_kernel, a);
         return e != cudaSuccess ? e : cudaLaunchKernelEx(&cfg, plain_down_kernel, a);
     }
-    // Tokens an expert has to take at a time: by how many pick it on average.
+    // Tokens of a job: two, four or eight. One or two tokens rarely share an expert
+    // (2 tokens, 2 of 16 experts of 4096 x 11008: 92 us with two, 103 with four). A
+    // job of eight costs more than one of four and pays where most experts have more
+    // than four tokens: 24, 32 and 40 tokens, 2 of 16 experts of 4096 x 5504, 201,
+    // 243 and 293 us with four, 228, 250 and 258 with eight; 11, 32 and 64 tokens, 6
+    // of 64 of 2048 x 1424, 84, 133 and 200 against 104, 149 and 189; 4 and 5 tokens
+    // on all of 8 of 2560 x 2576, 52 and 69 against 66 and 67.
     if (a.M <= 2) return run_tensor<1>(a, stream);
-    if (a.M <= 4 || a.M * a.top <= 2 * a.E) return run_tensor<2>(a, stream);
+    if (a.M * a.top <= 4 * a.E) return run_tensor<2>(a, stream);
     return run_tensor<4>(a, stream);
 }
 

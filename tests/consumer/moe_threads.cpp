@@ -65,7 +65,7 @@ void __cudaRegisterVar(void**, char*, char*, const char*, int, size_t, int, int)
 
 int main(int argc, char** argv) {
     if (argc != 6) return 2;
-    const int64_t K = std::atol(argv[1]), F = 64, E = 4, top = 2;
+    const int64_t K = std::atol(argv[1]), F = 64, E = 2, top = 2;
     const int64_t many = std::atol(argv[2]), few = std::atol(argv[3]);
     const int from = std::atoi(argv[4]), kernels = std::atoi(argv[5]);
     char* const p = reinterpret_cast<char*>(0x10000);  // never dereferenced

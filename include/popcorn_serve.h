@@ -160,8 +160,8 @@ popcornStatus_t popcornKvRead(
  *
  * A query that sees nothing gives zeros. Scores, statistics and sums are
  * f32 or exact integers; f32 queries keep 23 bits relative to their row's
- * largest element and f32 probabilities, f16 and bf16 queries 16 bits and
- * f16 probabilities. A query row that holds a NaN or an infinity and sees a
+ * largest element, f16 and bf16 queries 16 bits; probabilities keep 22 bits,
+ * those of bf16 queries 11. A query row that holds a NaN or an infinity and sees a
  * token, or sees a block with a non-finite scale, gives NaN; so is its lse,
  * which may stay that of the scores where only a value scale is not finite.
  * Results do not depend on the order in which blocks of the GPU run.

@@ -42,11 +42,13 @@ struct AttnArgs {
 };
 
 // The kernel for many query rows of one sequence (16-bit types, dim 64 or
-// 128): from this many on it is the faster one (bf16, dim 128, 8 key heads, 32
-// and 48 rows, it against kv_rows_kernel: 99 and 100 us against 73 and 102 for 4
-// sequences of 16,000 tokens, 112 and 113 against 82 and 115 for 32 of 2000)
-// unless the whole call is small (kFewTokens). Launches, or says how many bytes
-// of workspace it takes.
+// 128): from this many on it is the faster one (8 key heads of 128, 32, 48 and 64
+// rows, it against kv_rows_kernel: 4 sequences of 16,000 tokens 94, 95 and 101 us
+// against 73, 101 and 118 in bf16, 108, 109 and 114 against 83, 117 and 134 in f16;
+// 32 of 2000 103, 104 and 106 against 82, 113 and 141, and 121, 122 and 124 against
+// 89, 124 and 155; at dim 64 the two meet at 64 rows: 84, 84 and 84 against 56, 76
+// and 94 in bf16) unless the whole call is small (kFewTokens). Launches, or says
+// how many bytes of workspace it takes.
 constexpr int kPromptRows = 48;
 // A call is small where its rows make no more tasks of kv_rows_kernel than there
 // are SMs, and these have no more than this many tokens together, by the size of

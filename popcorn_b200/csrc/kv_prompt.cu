@@ -12,7 +12,9 @@
 //       of two, exact for f16, and for bf16 down to 2^-24 of the row's largest
 //       element), key codes as f16 (exact), f32 sums in tensor memory
 //   P = exp2(S ks f + log2(vs) - m): the block scales are constant over 16
-//       tokens at least; f16, written over S in tensor memory
+//       tokens at least; written over S in tensor memory, for bf16 as one f16 (an
+//       eighth of the outputs' own rounding), for f16 as two, the leading 11 bits
+//       and the rest, each with a product of its own
 //   O += P V: value codes as f16 (exact), transposed on the way into shared
 //       memory, f32 sums in tensor memory
 //
@@ -29,11 +31,14 @@
 // partial results these are.
 //
 // Measured, with the join: two sequences of 1024 new and 4000 cached tokens, 32
-// query heads on 8 of 128, bf16: 244 us, 621 TFLOP/s. The conversion sets the
-// pace, 5000 cycles a step, with the softmax close behind (3700 and a wait for the
-// scores). Tried and slower: an eighth converting warp (the softmax's registers
-// spill, 294 us; with registers shared out by setmaxnreg 267 us), warps apart for
-// keys and values (341 us).
+// query heads on 8 of 128: bf16 246 us, 616 TFLOP/s, f16 290 us. (With one f16 for
+// a probability f16 took 246 us too, but its results were 2.8e-4 off those in 64
+// bits, where rounding to f16 alone makes 2.1e-4, as much as kv_rows_kernel gives.)
+// For bf16 the conversion sets the pace, 5000 cycles a step, with the softmax close
+// behind (3700 and a wait for the scores); for f16 the softmax does. Tried and
+// slower in bf16: an eighth converting warp (the softmax's registers spill, 294 us;
+// with registers shared out by setmaxnreg 267 us), warps apart for keys and values
+// (341 us).
 //
 // Every wait is bounded (sm100.cuh); one that runs out sets error bit 0x8000
 // and ends the block.
@@ -79,6 +84,9 @@ struct Lay {  // shared memory, bytes; operand tiles in 128-byte swizzled rows
 
 template <typename T>
 using Pair = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
+// Probabilities as two f16: the leading bits and the rest.
+template <typename T>
+constexpr bool kSplit = std::is_same_v<T, __half>;
 
 struct GroupScale {
     float ks, lv, iv, pad;
@@ -127,6 +135,9 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
 __device__ __forceinline__ float2 scaled(uint32_t s0, uint32_t s1, float kf, float lv) {
     return __ffma2_rn(make_float2(__uint_as_float(s0), __uint_as_float(s1)), make_float2(kf, kf), make_float2(lv, lv));
 }
+// The leading 11 bits of x: exact in f16 (from 2^-14 on), and so is x less them in
+// f32.
+__device__ __forceinline__ float high_bits(float x) { return __uint_as_float(__float_as_uint(x) & 0xffffe000u); }
 // -inf for tokens j, j + 1 outside [see0, see1).
 __device__ __forceinline__ void hide(float2& v, int j, int see0, int see1) {
     if (j < see0 || j >= see1) v.x = -INFINITY;
@@ -376,7 +387,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const AttnArgs 
                 // --- probabilities, over the scores (xa holds the first columns)
                 const float shift = kLift - (top == -INFINITY ? 0.0f : top);
                 const auto weigh = [&](auto masked, const uint32_t (&x)[32], int c) {
-                    uint32_t w[16];
+                    uint32_t w[16];  // split: the high words of 16 tokens, then their rests
                     #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const GroupScale g = gs[2 * c + h];
@@ -388,11 +399,19 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const AttnArgs 
                             if (decltype(masked)::value) hide(v, j0 + 32 * c + 16 * h + j, see0, see1);
                             const float2 e = make_float2(exp2_fast(v.x), exp2_fast(v.y));
                             sum[j / 2 % 2] = __fadd2_rn(sum[j / 2 % 2], e);
-                            w[8 * h + j / 2] = pack_f16(e.x, e.y);
+                            if constexpr (kSplit<T>) {
+                                const float2 hi = make_float2(high_bits(e.x), high_bits(e.y));
+                                const float2 rest = __ffma2_rn(hi, make_float2(-1.0f, -1.0f), e);
+                                w[j / 2] = pack_f16(hi.x, hi.y);
+                                w[8 + j / 2] = pack_f16(rest.x, rest.y);
+                            } else {
+                                w[8 * h + j / 2] = pack_f16(e.x, e.y);
+                            }
                         }
                         den = fmaf((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y), g.iv, den);
+                        if constexpr (kSplit<T>) tmem_st_32x32b_x16(s_col + 32 * c + 16 * h, w);
                     }
-                    tmem_st_32x32b_x16(s_col + 16 * c, w);
+                    if constexpr (!kSplit<T>) tmem_st_32x32b_x16(s_col + 16 * c, w);
                 };
                 const auto probabilities = [&](auto masked) {
                     #pragma unroll 1
@@ -632,9 +651,10 @@ __global__ void __launch_bounds__(kPThreads, 1) kv_prompt_kernel(const AttnArgs 
                     tc_fence_after();
                     #pragma unroll
                     for (int j = 0; j < kTile / 16; ++j) {
-                        mma_f16_ts(tmem + 256 + 128 * m, tmem + 128 * m + 8 * j,
-                                   smem_desc_sw128_kmajor(smem + L::kV + stage * L::kVStage + (j / 4) * (DP * 128)) + (j % 4) * 2,
-                                   id_pv, i > 0 || j > 0);
+                        const uint64_t v = smem_desc_sw128_kmajor(smem + L::kV + stage * L::kVStage + (j / 4) * (DP * 128)) + (j % 4) * 2;
+                        const uint32_t p = tmem + 128 * m + (kSplit<T> ? 16 : 8) * j;
+                        mma_f16_ts(tmem + 256 + 128 * m, p, v, id_pv, i > 0 || j > 0);
+                        if constexpr (kSplit<T>) mma_f16_ts(tmem + 256 + 128 * m, p + 8, v, id_pv, 1);
                     }
                     mma_commit(bar(kODone, m));
                     if (m == tiles - 1) mma_commit(bar(kVEmpty, stage));

@@ -164,7 +164,10 @@ popcornStatus_t popcornKvRead(
  * those of bf16 queries 11. A query row that holds a NaN or an infinity and sees a
  * token, or sees a block with a non-finite scale, gives NaN; so is its lse,
  * which may stay that of the scores where only a value scale is not finite.
- * Results do not depend on the order in which blocks of the GPU run.
+ * Results do not depend on the order in which blocks of the GPU run. The cut of
+ * the work and, for 16-bit types, the kernel are chosen by the sizes given, the
+ * width of the block table among them: calls of other sizes may differ in the
+ * last bits for the same tokens.
  */
 popcornStatus_t popcornKvAttention(
     void* out,

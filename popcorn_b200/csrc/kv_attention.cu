@@ -35,11 +35,13 @@
 //  * Tasks of 16-token tiles, cut over the workers of all SMs
 //    (kv_attention.cuh); split tasks are joined by kv_join_kernel.
 //
-// Measured, with the join: 16 sequences of 4096 tokens, 32 key heads of 128, one
-// f32 query each: 98 us, 5.5 TB/s; 64 ragged ones up to 8192, 8 key heads, bf16:
-// 87 us, 5.7 TB/s; one of 131,075 tokens, f16: 55 us, 4.9 TB/s. Small calls are a
-// chain of latencies (schedule, block table, codes, partial results, join): 12 us
-// for 1000 tokens.
+// Measured, with the join, in a graph: 16 sequences of 4096 tokens, 32 key heads of
+// 128, one f32 query each: 99 us, 5.4 TB/s; 64 ragged ones up to 8192, 8 key heads,
+// bf16: 87 us, 5.7 TB/s; one of 131,075 tokens, f16: 55 us, 4.9 TB/s. Small calls
+// are a chain of latencies (schedule, block table, codes, partial results, join):
+// 12 us for 1000 tokens. Ragged batches of short sequences are far from HBM's rate:
+// below 4 kTaskUnits tiles a worker the runs are equal in tiles, however many tasks
+// they hold (64 sequences up to 512, 32 heads, f16: 204 us, floor 21).
 //
 // Sequences with many query rows go to the kernel of kv_prompt.cu where it takes
 // their type and dim (kPromptRows).
@@ -741,7 +743,12 @@ cudaError_t run_rows(AttnArgs a, int64_t tasks, void* ws, int64_t* ws_bytes, cud
 
 template <typename T>
 cudaError_t run_attention(const AttnArgs& a, int64_t max_tokens, void* ws, int64_t* ws_bytes, cudaStream_t stream) {
-    // Tasks of at most 8 or 16 query rows; an upper bound of their number.
+    // Tasks of at most 8 or 16 query rows; an upper bound of their number. Two
+    // sides of 8 read the codes once for 16 rows and pay where they come from HBM:
+    // 64 sequences of 4000 tokens, 8 key heads of 128, 16 rows, bf16: 154 us against
+    // 171 with one side, 16 sequences with 32 rows 76 against 82. With less work one
+    // side is the faster: 16 sequences with 16 rows 48 against 52, one of 1000 tokens
+    // 10.5 against 13.2.
     const bool two = !Traits<T>::kFresh && a.dim <= 128 && max_tokens * a.group > 8;
     const int rows = two ? 16 : 8;
     const int64_t tasks = a.heads * (static_cast<int64_t>(a.tokens) * a.group / rows + a.seqs);

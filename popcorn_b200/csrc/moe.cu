@@ -12,18 +12,20 @@
 //  3. down_kernel: a block owns up to 32 output channels at a time and goes
 //     through all chosen experts, so that a token's sum over its experts needs no
 //     other block.
-// Measured: one token, 2 of 16 experts of 4096 x 11008: 56 us, 4.9 TB/s (up 34,
-// down 21, both at the rate of a plain copy but for their ends); 16 tokens, 6 of
-// 64 experts of 2048 x 1424 each: 99 us, 4.5 TB/s.
+// Measured in a graph: one token, 2 of 16 experts of 4096 x 11008: 56 us, 4.8 TB/s;
+// 16 tokens, 6 of 64 experts of 2048 x 1424 each: 99 us, 4.5 TB/s. By themselves,
+// with cold caches, the kernels read at 5.0 (up, 37 us) and 4.0 TB/s (down, 23 us)
+// and at 4.7 (63 us) and 4.0 TB/s (41 us): their starts, the ends of their blocks
+// and, in down, the wait for the first codes are inside.
 //
 // Products. mma s8 x s8 -> s32 with the codes as they are: 16 weight rows are
 // the M side; the eight columns of the N side are two tokens times the four
 // balanced base-256 digits of 30-bit fixed point. Sums are exact integers and
-// join in double or f32, so the result's error is f32 rounding. The operands
-// come from global memory in 16-byte loads without shared memory: columns of
-// the product may be taken in any order, so lane (g, t) = (lane / 4, lane % 4)
-// takes piece t of each 64-column window, the words of which feed two 32-deep
-// steps. The activations' fixed point has one power of two per token, the
+// join in double or f32, so the result's error is f32 rounding. Codes come through
+// rings of shared memory that each warp fills by asynchronous copies and reads
+// alone; digits are read in 16-byte loads from L2. Columns of the product may be
+// taken in any order, so lane (g, t) = (lane / 4, lane % 4) takes piece t of each
+// 64-column window of both, the words of which feed two 32-deep steps. The activations' fixed point has one power of two per token, the
 // hidden values' one for each 32 rows that an item covers: columns
 // 64 w + 16 t + 8 s + i (t < 4, i < 8), which are the columns of step s of
 // window w in the next product.

@@ -25,10 +25,10 @@
 // rings of shared memory that each warp fills by asynchronous copies and reads
 // alone; digits are read in 16-byte loads from L2. Columns of the product may be
 // taken in any order, so lane (g, t) = (lane / 4, lane % 4) takes piece t of each
-// 64-column window of both, the words of which feed two 32-deep steps. The activations' fixed point has one power of two per token, the
-// hidden values' one for each 32 rows that an item covers: columns
-// 64 w + 16 t + 8 s + i (t < 4, i < 8), which are the columns of step s of
-// window w in the next product.
+// 64-column window of both, the words of which feed two 32-deep steps. The
+// activations' fixed point has one power of two per token, the hidden values' one
+// for each 32 rows that an item covers: columns 64 w + 16 t + 8 s + i (t < 4, i < 8),
+// which are the columns of step s of window w in the next product.
 #include <algorithm>
 #include <cmath>
 
